@@ -37,7 +37,7 @@ enum {
   LH_ERR_WORKSPACE = 5/* workspace too small                              */
 };
 
-enum { LH_DTYPE_BF16 = 0, LH_DTYPE_F32 = 1 };
+enum { LH_DTYPE_BF16 = 0, LH_DTYPE_F32 = 1, LH_DTYPE_E4M3 = 2 /* rms_norm output only */ };
 
 /* Message for the last non-zero return on this thread ("" if none). */
 const char* lh_last_error(void);
@@ -213,6 +213,37 @@ int lh_rope_apply(const void* xq, const void* xk, void* oq, void* ok, const floa
  * scorer's q->k and k->q passes); pass NULL for all three to skip it. */
 int lh_simple_gla_fwd(const void* q, const void* k, const void* v, const float* g, void* o, const void* q2,
                       const void* k2, void* o2, int dtype, int B, int T, int H, int D, float scale, void* stream);
+
+/* Root-mean-square norm with the residual's addition (model harness: the block
+ * computes x + branch and then norms it, PATCH:700-737 context).
+ *   x         (N, D) x_dtype
+ *   residual  (N, D) r_dtype, or NULL (then h is not written and the norm is x's)
+ *   weight    (D) w_dtype
+ *   h         (N, D) r_dtype out: x + residual, rounded once
+ *   y         (N, D) y_dtype out: h * rstd * weight, rstd = (mean(h^2) + eps)^-1/2
+ *             of the stored h
+ *   rstd      (N) fp32 out, may be NULL
+ * y_dtype LH_DTYPE_E4M3: t = h * weight, a = max(|t|, 2^-100) over the row
+ * (group 0) or over each 128 columns (group 128); y = e4m3(448 t / a) and
+ * scale = a * rstd / 448, (N) or (N, ceil(D / 128)) fp32.
+ * The float types are bf16 and fp32 in any combination.  D % 8 == 0,
+ * D <= 16384; pointers 16-byte aligned. */
+int lh_rms_norm_fwd(const void* x, int x_dtype, const void* residual, int r_dtype, const void* weight, int w_dtype,
+                    long long N, int D, float eps, void* y, int y_dtype, float* scale, int group, void* h,
+                    float* rstd, void* stream);
+
+/* Bytes of workspace lh_rms_norm_bwd needs. */
+size_t lh_rms_norm_bwd_workspace_size(long long N, int D);
+
+/* Backward of lh_rms_norm_fwd (float outputs).
+ *   dy (N, D) dy_dtype; dh (N, D) h_dtype upstream gradient of h, may be NULL
+ *   h  (N, D) h_dtype: the forward's h (x itself where it had no residual)
+ *   dx (N, D) dx_dtype out; dres (N, D) h_dtype out, may be NULL (same values)
+ *   dw (D) w_dtype out: sum over rows of dy * h * rstd, summed in a fixed order
+ *   workspace >= lh_rms_norm_bwd_workspace_size bytes, 16-byte aligned */
+int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h, int h_dtype, const void* weight,
+                    int w_dtype, const float* rstd, long long N, int D, void* dx, int dx_dtype, void* dres, void* dw,
+                    void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

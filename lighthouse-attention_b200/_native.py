@@ -49,6 +49,12 @@ _SIGS = {
     "lh_unpool_bwd": (ctypes.c_int, [_VP] * 4 + [ctypes.c_int] * 8 + [_VP] * 4),
     "lh_rope_apply": (ctypes.c_int, [_VP] * 5 + [ctypes.c_int] * 6 + [_VP]),
     "lh_simple_gla_fwd": (ctypes.c_int, [_VP] * 8 + [ctypes.c_int] * 5 + [ctypes.c_float, _VP]),
+    "lh_rms_norm_fwd": (ctypes.c_int, [_VP, ctypes.c_int] * 3 + [ctypes.c_longlong, ctypes.c_int, ctypes.c_float, _VP,
+                                                                ctypes.c_int, _VP, ctypes.c_int] + [_VP] * 3),
+    "lh_rms_norm_bwd_workspace_size": (ctypes.c_size_t, [ctypes.c_longlong, ctypes.c_int]),
+    "lh_rms_norm_bwd": (ctypes.c_int, [_VP, ctypes.c_int, _VP, _VP, ctypes.c_int, _VP, ctypes.c_int, _VP,
+                                       ctypes.c_longlong, ctypes.c_int, _VP, ctypes.c_int] + [_VP] * 3
+                        + [ctypes.c_size_t, _VP]),
 }
 
 
@@ -309,3 +315,88 @@ def simple_gla_fwd(q, k, v, g, scale: float, q2=None, k2=None):
     _check(load().lh_simple_gla_fwd(_ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(o), _ptr(q2), _ptr(k2), _ptr(o2),
                                     LH_DTYPE[q.dtype], B, T, H, D, scale, _stream()))
     return o if q2 is None else (o, o2)
+
+
+# --------------------------------------------------------------------------- norm
+def _on_one_device(what: str, *ts) -> torch.device:
+    """All tensors are CUDA tensors of one device, which is returned."""
+    _require_cuda(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) != 1:
+        raise ValueError(f"{what}: tensors on different devices: {sorted(map(str, devs))}")
+    return devs.pop()
+
+
+def _dense16(t):
+    """t as a contiguous tensor whose first element is 16-byte aligned."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _norm_check(what, x, residual, weight):
+    if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1] or (
+            residual is not None and residual.shape != x.shape):
+        raise LighthouseShapeError(f"{what}: x and residual (..., D) and weight (D) must agree")
+    for t in (x, residual, weight):
+        if t is not None and t.dtype not in LH_DTYPE:
+            raise ValueError(f"{what}: bf16 and fp32 tensors only, got {t.dtype}")
+    D = x.shape[-1]
+    if D % 8 or not 8 <= D <= 16384:
+        raise LighthouseShapeError(f"{what}: D must be a multiple of 8 and at most 16384, got {D}")
+
+
+def rms_norm_fwd(x, residual, weight, eps: float, out_dtype, group: int = 0, with_rstd: bool = True):
+    """RMS norm of h = x + residual ((..., D), residual may be None) -> (y, scale, h, rstd).
+
+    out_dtype torch.float8_e4m3fn gives y in 8 bits and scale (..., 1), or
+    (..., ceil(D / 128)) with group 128; scale is None otherwise.  h is None
+    without a residual, rstd (rows) fp32 is None unless asked for."""
+    _norm_check("rms_norm", x, residual, weight)
+    fp8 = out_dtype == torch.float8_e4m3fn
+    if not fp8 and out_dtype not in LH_DTYPE:
+        raise ValueError(f"rms_norm: out_dtype must be bf16, fp32 or float8_e4m3fn, got {out_dtype}")
+    if group not in ((0, 128) if fp8 else (0,)):
+        raise ValueError("rms_norm: scales per row (group 0) or per 128 columns (group 128)")
+    dev = _on_one_device("rms_norm", x, residual, weight)
+    D = x.shape[-1]
+    N = x.numel() // D
+    y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    n_groups = (D + 127) // 128 if group else 1
+    scale = torch.empty(*x.shape[:-1], n_groups, dtype=torch.float32, device=dev) if fp8 else None
+    h = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=dev)
+    rstd = torch.empty(N, dtype=torch.float32, device=dev) if with_rstd else None
+    if N:
+        with torch.cuda.device(dev):
+            x, weight = _dense16(x), _dense16(weight)
+            residual = None if residual is None else _dense16(residual)
+            _check(load().lh_rms_norm_fwd(_ptr(x), LH_DTYPE[x.dtype], _ptr(residual),
+                                          0 if residual is None else LH_DTYPE[residual.dtype], _ptr(weight),
+                                          LH_DTYPE[weight.dtype], N, D, eps, _ptr(y), 2 if fp8 else LH_DTYPE[out_dtype],
+                                          _ptr(scale), group, _ptr(h), _ptr(rstd), _stream()))
+    return y, scale, h, rstd
+
+
+def rms_norm_bwd(dy, dh, h, weight, rstd, dx_dtype, with_dres: bool):
+    """Backward of rms_norm_fwd: (dx, dres, dw); dh may be None, dres is None unless asked for."""
+    _norm_check("rms_norm_bwd", h, dy, weight)
+    if dx_dtype not in LH_DTYPE or (dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype)):
+        raise LighthouseShapeError("rms_norm_bwd: dh must have the shape and type of h")
+    dev = _on_one_device("rms_norm_bwd", dy, dh, h, weight, rstd)
+    D = h.shape[-1]
+    N = h.numel() // D
+    if rstd.dtype != torch.float32 or rstd.numel() != N:
+        raise LighthouseShapeError("rms_norm_bwd: rstd must be fp32, one per row")
+    dx = torch.empty(h.shape, dtype=dx_dtype, device=dev)
+    dres = torch.empty(h.shape, dtype=h.dtype, device=dev) if with_dres else None
+    if not N:
+        return dx, dres, torch.zeros_like(weight)
+    dw = torch.empty(D, dtype=weight.dtype, device=dev)
+    with torch.cuda.device(dev):
+        dy, h, weight, rstd = _dense16(dy), _dense16(h), _dense16(weight), rstd.contiguous()
+        dh = None if dh is None else _dense16(dh)
+        ws_bytes = int(load().lh_rms_norm_bwd_workspace_size(N, D))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _check(load().lh_rms_norm_bwd(_ptr(dy), LH_DTYPE[dy.dtype], _ptr(dh), _ptr(h), LH_DTYPE[h.dtype], _ptr(weight),
+                                      LH_DTYPE[weight.dtype], _ptr(rstd), N, D, _ptr(dx), LH_DTYPE[dx_dtype], _ptr(dres),
+                                      _ptr(dw), _ptr(ws), ws_bytes, _stream()))
+    return dx, dres, dw

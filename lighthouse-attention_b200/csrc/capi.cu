@@ -72,6 +72,12 @@ int attn_bwd_noalloc(const void*, const void*, const void*, const void*, const f
 int attn_bwd(const void*, const void*, const void*, const void*, const float*, const void*, int, int, int, int,
              int, int, float, void*, void*, void*, void*, size_t, cudaStream_t);
 
+int rms_norm_fwd(const void*, int, const void*, int, const void*, int, long long, int, float, void*, int, float*, int,
+                 void*, float*, cudaStream_t);
+size_t rms_norm_bwd_workspace_size(long long, int);
+int rms_norm_bwd(const void*, int, const void*, const void*, int, const void*, int, const float*, long long, int, void*,
+                 int, void*, void*, void*, cudaStream_t);
+
 }  // namespace lh
 
 using namespace lh;
@@ -265,6 +271,49 @@ int lh_simple_gla_fwd(const void* q, const void* k, const void* v, const float* 
   LH_REQUIRE(B > 0 && T > 0 && H > 0 && B <= 32767 && H <= 65535, LH_ERR_SHAPE, "gla: bad shape");
   LH_ARCH();
   return simple_gla_fwd(q, k, o, q2, k2, o2, v, g, B, T, H, scale, S_(stream));
+}
+
+static bool float_dtype(int d) { return d == LH_DTYPE_BF16 || d == LH_DTYPE_F32; }
+
+int lh_rms_norm_fwd(const void* x, int x_dtype, const void* residual, int r_dtype, const void* weight, int w_dtype,
+                    long long N, int D, float eps, void* y, int y_dtype, float* scale, int group, void* h, float* rstd,
+                    void* stream) {
+  g_err[0] = 0;
+  LH_REQUIRE(x && weight && y && (!residual || h), LH_ERR_ARG, "rms_norm: null pointer");
+  LH_REQUIRE(float_dtype(x_dtype) && float_dtype(w_dtype) && (!residual || float_dtype(r_dtype)) &&
+                 (float_dtype(y_dtype) || y_dtype == LH_DTYPE_E4M3), LH_ERR_ARG, "rms_norm: bad dtype");
+  LH_REQUIRE(y_dtype != LH_DTYPE_E4M3 || (scale && (group == 0 || group == 128)), LH_ERR_ARG,
+             "rms_norm: an 8-bit output needs its scales, one per row (group 0) or per 128 columns (group 128)");
+  LH_REQUIRE(N > 0 && N < (1ll << 31) && D > 0, LH_ERR_SHAPE, "rms_norm: bad shape");
+  LH_REQUIRE(D % 8 == 0 && D <= 16384, LH_ERR_SHAPE, "rms_norm: D must be a multiple of 8 and at most 16384, got %d", D);
+  LH_REQUIRE(!(((uintptr_t)x | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)y | (uintptr_t)(residual ? h : nullptr)) & 15) &&
+                 !(((uintptr_t)scale | (uintptr_t)rstd) & 3), LH_ERR_ARG, "rms_norm: pointers must be 16-byte aligned");
+  LH_ARCH();
+  return rms_norm_fwd(x, x_dtype, residual, r_dtype, weight, w_dtype, N, D, eps, y, y_dtype, scale, group, h, rstd,
+                      S_(stream));
+}
+
+size_t lh_rms_norm_bwd_workspace_size(long long N, int D) {
+  return N > 0 && D > 0 ? rms_norm_bwd_workspace_size(N, D) : 0;
+}
+
+int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h, int h_dtype, const void* weight,
+                    int w_dtype, const float* rstd, long long N, int D, void* dx, int dx_dtype, void* dres, void* dw,
+                    void* ws, size_t ws_bytes, void* stream) {
+  g_err[0] = 0;
+  LH_REQUIRE(dy && h && weight && rstd && dx && dw, LH_ERR_ARG, "rms_norm_bwd: null pointer");
+  LH_REQUIRE(float_dtype(dy_dtype) && float_dtype(h_dtype) && float_dtype(w_dtype) && float_dtype(dx_dtype), LH_ERR_ARG,
+             "rms_norm_bwd: bad dtype");
+  LH_REQUIRE(N > 0 && N < (1ll << 31) && D > 0, LH_ERR_SHAPE, "rms_norm_bwd: bad shape");
+  LH_REQUIRE(D % 8 == 0 && D <= 16384, LH_ERR_SHAPE, "rms_norm_bwd: D must be a multiple of 8 and at most 16384, got %d", D);
+  LH_REQUIRE(ws_bytes >= rms_norm_bwd_workspace_size(N, D), LH_ERR_WORKSPACE,
+             "rms_norm_bwd: workspace of %zu bytes is smaller than the %zu needed", ws_bytes,
+             rms_norm_bwd_workspace_size(N, D));
+  LH_REQUIRE(ws && !(((uintptr_t)dy | (uintptr_t)dh | (uintptr_t)h | (uintptr_t)weight | (uintptr_t)dx | (uintptr_t)dres |
+                      (uintptr_t)ws) & 15) && !(((uintptr_t)rstd | (uintptr_t)dw) & 3), LH_ERR_ARG,
+             "rms_norm_bwd: pointers must be 16-byte aligned");
+  LH_ARCH();
+  return rms_norm_bwd(dy, dy_dtype, dh, h, h_dtype, weight, w_dtype, rstd, N, D, dx, dx_dtype, dres, dw, ws, S_(stream));
 }
 
 }  // extern "C"

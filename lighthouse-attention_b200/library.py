@@ -198,4 +198,85 @@ def _(q, k, v, g, scale, q2, k2):
     return q.new_empty(q.shape), q.new_empty(q.shape)
 
 
+# --------------------------------------------------------------------------- norm
+@torch.library.custom_op(f"{NS}::rms_norm", mutates_args=())
+def rms_norm(x: Tensor, weight: Tensor, eps: float, out_dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    """y = x * rstd * weight in out_dtype and rstd (rows) fp32."""
+    y, _, _, rstd = _native.rms_norm_fwd(x, None, weight, eps, out_dtype)
+    return y, rstd
+
+
+@rms_norm.register_fake
+def _(x, weight, eps, out_dtype):
+    return x.new_empty(x.shape, dtype=out_dtype), x.new_empty(x.numel() // x.shape[-1], dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NS}::add_rms_norm", mutates_args=())
+def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float,
+                 out_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    """h = x + residual in the residual's type, y = h * rstd * weight in out_dtype, rstd (rows) fp32."""
+    y, _, h, rstd = _native.rms_norm_fwd(x, residual, weight, eps, out_dtype)
+    return y, h, rstd
+
+
+@add_rms_norm.register_fake
+def _(x, residual, weight, eps, out_dtype):
+    return (x.new_empty(x.shape, dtype=out_dtype), x.new_empty(x.shape, dtype=residual.dtype),
+            x.new_empty(x.numel() // x.shape[-1], dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{NS}::rms_norm_bwd", mutates_args=())
+def rms_norm_bwd(dy: Tensor, h: Tensor, weight: Tensor, rstd: Tensor) -> tuple[Tensor, Tensor]:
+    """Backward of rms_norm: dx in x's type, dw in weight's."""
+    dx, _, dw = _native.rms_norm_bwd(dy, None, h, weight, rstd, h.dtype, False)
+    return dx, dw
+
+
+@rms_norm_bwd.register_fake
+def _(dy, h, weight, rstd):
+    return h.new_empty(h.shape), weight.new_empty(weight.shape)
+
+
+@torch.library.custom_op(f"{NS}::add_rms_norm_bwd", mutates_args=())
+def add_rms_norm_bwd(dy: Tensor, dh: Tensor | None, h: Tensor, weight: Tensor, rstd: Tensor,
+                     dx_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    """Backward of add_rms_norm: dx in x's type, dresidual in h's, dw in weight's."""
+    return _native.rms_norm_bwd(dy, dh, h, weight, rstd, dx_dtype, True)
+
+
+@add_rms_norm_bwd.register_fake
+def _(dy, dh, h, weight, rstd, dx_dtype):
+    return h.new_empty(h.shape, dtype=dx_dtype), h.new_empty(h.shape), weight.new_empty(weight.shape)
+
+
+def _scale_shape(x, group):
+    return (*x.shape[:-1], (x.shape[-1] + 127) // 128 if group else 1)
+
+
+@torch.library.custom_op(f"{NS}::rms_norm_fp8", mutates_args=())
+def rms_norm_fp8(x: Tensor, weight: Tensor, eps: float, group: int) -> tuple[Tensor, Tensor]:
+    """RMS norm in float8_e4m3fn and its fp32 scales (..., 1) or (..., ceil(D / 128))."""
+    y, scale, _, _ = _native.rms_norm_fwd(x, None, weight, eps, torch.float8_e4m3fn, group, with_rstd=False)
+    return y, scale
+
+
+@rms_norm_fp8.register_fake
+def _(x, weight, eps, group):
+    return x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(_scale_shape(x, group), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NS}::add_rms_norm_fp8", mutates_args=())
+def add_rms_norm_fp8(x: Tensor, residual: Tensor, weight: Tensor, eps: float,
+                     group: int) -> tuple[Tensor, Tensor, Tensor]:
+    """rms_norm_fp8 of h = x + residual; returns the codes, the scales and h."""
+    y, scale, h, _ = _native.rms_norm_fwd(x, residual, weight, eps, torch.float8_e4m3fn, group, with_rstd=False)
+    return y, scale, h
+
+
+@add_rms_norm_fp8.register_fake
+def _(x, residual, weight, eps, group):
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(_scale_shape(x, group), dtype=torch.float32),
+            x.new_empty(x.shape, dtype=residual.dtype))
+
+
 ops = torch.ops.lighthouse_b200
