@@ -7,6 +7,7 @@ that with importlib).  Modules:
   lighthouse_selection       drop-in for the reference module of the same name
   lighthouse_selection_cuda  drop-in for the reference module of the same name
   norm                       RMS norm with the residual's addition; output in 8 bits with scales
+  losses                     cross entropy and distillation of an output projection, without its logits
   cp                         context-parallel layer (NCCL all-gather of selected K/V)
   _native                    ctypes binding of liblighthouse_b200.so (include/lighthouse_b200.h)
 """
@@ -17,4 +18,5 @@ from .lighthouse_selection import (DialatedLighthouseNormScorer, DialatedLightho
                                    LighthouseLocal, compute_output_indices_selection, lighthouse_attention,
                                    scatter_to_base_sequence)
 from .lighthouse_selection_cuda import LighthouseSelectionQkKqChunkedTopkNvrtc  # noqa: F401
+from .losses import linear_cross_entropy, linear_distillation  # noqa: F401
 from .norm import add_rms_norm, add_rms_norm_fp8, rms_norm, rms_norm_fp8  # noqa: F401

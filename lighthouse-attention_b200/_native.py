@@ -55,7 +55,18 @@ _SIGS = {
     "lh_rms_norm_bwd": (ctypes.c_int, [_VP, ctypes.c_int, _VP, _VP, ctypes.c_int, _VP, ctypes.c_int, _VP,
                                        ctypes.c_longlong, ctypes.c_int, _VP, ctypes.c_int] + [_VP] * 3
                         + [ctypes.c_size_t, _VP]),
+    "lh_linear_loss_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 4),
+    "lh_linear_xent_fwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int64] + [ctypes.c_int] * 4 + [_VP] * 6
+                           + [ctypes.c_size_t, _VP]),
+    "lh_linear_xent_bwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int] * 3 + [_VP] * 5 + [ctypes.c_int] + [_VP] * 3
+                           + [ctypes.c_size_t, _VP]),
+    "lh_linear_distill_fwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int, _VP] + [ctypes.c_int] * 4
+                              + [ctypes.c_float, ctypes.c_int] + [_VP] * 8 + [ctypes.c_size_t, _VP]),
+    "lh_linear_distill_bwd": (ctypes.c_int, [_VP] * 2 + [ctypes.c_int] * 4 + [ctypes.c_float] + [_VP] * 7
+                              + [ctypes.c_int] + [_VP] * 3 + [ctypes.c_size_t, _VP]),
 }
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def lib_path() -> pathlib.Path:
@@ -400,3 +411,128 @@ def rms_norm_bwd(dy, dh, h, weight, rstd, dx_dtype, with_dres: bool):
                                       LH_DTYPE[weight.dtype], _ptr(rstd), N, D, _ptr(dx), LH_DTYPE[dx_dtype], _ptr(dres),
                                       _ptr(dw), _ptr(ws), ws_bytes, _stream()))
     return dx, dres, dw
+
+
+# --------------------------------------------------------------------------- losses of an output projection
+def _loss_check(what, hidden, weight, reduction=None):
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
+        raise LighthouseShapeError(f"{what}: hidden (N, D) and weight (V, D) must agree")
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise ValueError(f"{what}: hidden and weight must be bf16, got {hidden.dtype} and {weight.dtype}")
+    N, D = hidden.shape
+    V = weight.shape[0]
+    if D % 8 or not 8 <= D <= 65536 or not 1 <= V <= 1 << 22 or N > 1 << 24:
+        raise LighthouseShapeError(f"{what}: D must be a multiple of 8 and at most 65536, V in [1, 2^22], N at most "
+                                   f"2^24; got D {D}, V {V}, N {N}")
+    if reduction is not None and reduction not in REDUCTIONS:
+        raise ValueError(f"{what}: reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
+    return N, V, D
+
+
+def _loss_outputs(N, reduction, dev):
+    f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)
+    if reduction == "none":
+        return f(N), f(N), f(N), f(0)
+    if N == 0:                                       # nothing counts: the loss is 0
+        return f().zero_(), f(0), f(0), f(1).zero_()
+    return f(), f(N), f(N), f(1)
+
+
+def _loss_ws(N, V, D, backward, dev):
+    n = int(load().lh_linear_loss_workspace_size(N, V, D, backward))
+    return torch.empty(n, dtype=torch.uint8, device=dev), n
+
+
+def linear_xent_fwd(hidden, weight, target, ignore_index: int, reduction: str):
+    """Softmax cross entropy of hidden (N, D) @ weight (V, D)^T against target (N) int64 ->
+    (loss, lse2, tlogit, row_scale, inv_count); the last four are the backward's."""
+    N, V, D = _loss_check("linear_xent", hidden, weight, reduction)
+    if target.shape != (N,) or target.dtype != torch.int64:
+        raise LighthouseShapeError("linear_xent: target must be (N) int64")
+    dev = _on_one_device("linear_xent", hidden, weight, target)
+    loss, lse2, row_scale, inv_count = _loss_outputs(N, reduction, dev)
+    tlogit = torch.empty(N, dtype=torch.float32, device=dev)
+    if N:
+        with torch.cuda.device(dev):
+            hidden, weight, target = _dense16(hidden), _dense16(weight), target.contiguous()
+            ws, n = _loss_ws(N, V, D, 0, dev)
+            _check(load().lh_linear_xent_fwd(_ptr(hidden), _ptr(weight), _ptr(target), ignore_index, N, V, D,
+                                             REDUCTIONS[reduction], _ptr(loss), _ptr(lse2), _ptr(tlogit),
+                                             _ptr(row_scale), _ptr(inv_count), _ptr(ws), n, _stream()))
+    return loss, lse2, tlogit, row_scale, inv_count
+
+
+def _gout_check(what, gout, N, reduced, dev_tensors):
+    if gout.dtype != torch.float32 or gout.numel() != (1 if reduced else N):
+        raise LighthouseShapeError(f"{what}: the loss's gradient must be fp32, one value (reduced) or N")
+    return _on_one_device(what, gout, *dev_tensors)
+
+
+def linear_xent_bwd(hidden, weight, target, lse2, tlogit, row_scale, inv_count, gout, reduction: str):
+    """Gradients (dhidden, dweight) of linear_xent_fwd."""
+    N, V, D = _loss_check("linear_xent_bwd", hidden, weight, reduction)
+    dev = _gout_check("linear_xent_bwd", gout, N, reduction != "none",
+                      (hidden, weight, target, lse2, tlogit, row_scale, inv_count))
+    dh = torch.empty(N, D, dtype=torch.bfloat16, device=dev)
+    if not N:
+        return dh, torch.zeros(V, D, dtype=torch.bfloat16, device=dev)
+    dw = torch.empty(V, D, dtype=torch.bfloat16, device=dev)
+    reduced = reduction != "none"
+    with torch.cuda.device(dev):
+        hidden, weight, target, gout = _dense16(hidden), _dense16(weight), target.contiguous(), gout.contiguous()
+        ws, n = _loss_ws(N, V, D, 1, dev)
+        _check(load().lh_linear_xent_bwd(_ptr(hidden), _ptr(weight), _ptr(target), N, V, D, _ptr(lse2), _ptr(tlogit),
+                                         _ptr(row_scale), _ptr(inv_count) if reduced else None, _ptr(gout),
+                                         0 if reduced else 1, _ptr(dh), _ptr(dw), _ptr(ws), n, _stream()))
+    return dh, dw
+
+
+def linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperature: float, reduction: str):
+    """Distillation of hidden (N, D) @ weight (V, D)^T from a teacher's K logits (N, K) bf16 / fp32 at
+    indices (N, K) int64 -> (loss, lse2, idx, prob, tlogit, row_scale, inv_count)."""
+    N, V, D = _loss_check("linear_distill", hidden, weight, reduction)
+    if teacher_logits.dim() != 2 or teacher_logits.shape[0] != N or teacher_indices.shape != teacher_logits.shape:
+        raise LighthouseShapeError("linear_distill: teacher logits and indices must be (N, K)")
+    K = teacher_logits.shape[1]
+    if not 1 <= K <= 256:
+        raise LighthouseShapeError(f"linear_distill: K must be in [1, 256], got {K}")
+    if teacher_logits.dtype not in LH_DTYPE or teacher_indices.dtype != torch.int64:
+        raise ValueError("linear_distill: teacher logits must be bf16 or fp32, indices int64")
+    if not 0 < temperature < 1e30:
+        raise ValueError(f"linear_distill: temperature must be positive and finite, got {temperature}")
+    dev = _on_one_device("linear_distill", hidden, weight, teacher_logits, teacher_indices)
+    loss, lse2, row_scale, inv_count = _loss_outputs(N, reduction, dev)
+    idx = torch.empty(N, K, dtype=torch.int32, device=dev)
+    prob, tlogit = (torch.empty(N, K, dtype=torch.float32, device=dev) for _ in range(2))
+    if N:
+        with torch.cuda.device(dev):
+            hidden, weight = _dense16(hidden), _dense16(weight)
+            teacher_logits, teacher_indices = teacher_logits.contiguous(), teacher_indices.contiguous()
+            ws, n = _loss_ws(N, V, D, 0, dev)
+            _check(load().lh_linear_distill_fwd(_ptr(hidden), _ptr(weight), _ptr(teacher_logits),
+                                                LH_DTYPE[teacher_logits.dtype], _ptr(teacher_indices), N, V, D, K,
+                                                temperature, REDUCTIONS[reduction], _ptr(loss), _ptr(lse2), _ptr(idx),
+                                                _ptr(prob), _ptr(tlogit), _ptr(row_scale), _ptr(inv_count), _ptr(ws), n,
+                                                _stream()))
+    return loss, lse2, idx, prob, tlogit, row_scale, inv_count
+
+
+def linear_distill_bwd(hidden, weight, lse2, idx, prob, tlogit, row_scale, inv_count, gout, temperature: float,
+                       reduction: str):
+    """Gradients (dhidden, dweight) of linear_distill_fwd."""
+    N, V, D = _loss_check("linear_distill_bwd", hidden, weight, reduction)
+    dev = _gout_check("linear_distill_bwd", gout, N, reduction != "none",
+                      (hidden, weight, lse2, idx, prob, tlogit, row_scale, inv_count))
+    dh = torch.empty(N, D, dtype=torch.bfloat16, device=dev)
+    if not N:
+        return dh, torch.zeros(V, D, dtype=torch.bfloat16, device=dev)
+    dw = torch.empty(V, D, dtype=torch.bfloat16, device=dev)
+    reduced = reduction != "none"
+    with torch.cuda.device(dev):
+        hidden, weight, gout = _dense16(hidden), _dense16(weight), gout.contiguous()
+        ws, n = _loss_ws(N, V, D, 1, dev)
+        _check(load().lh_linear_distill_bwd(_ptr(hidden), _ptr(weight), N, V, D, idx.shape[1], temperature, _ptr(lse2),
+                                            _ptr(idx), _ptr(prob), _ptr(tlogit), _ptr(row_scale),
+                                            _ptr(inv_count) if reduced else None, _ptr(gout), 0 if reduced else 1,
+                                            _ptr(dh), _ptr(dw), _ptr(ws), n, _stream()))
+    return dh, dw

@@ -1,0 +1,846 @@
+// Losses of an output projection whose logits are never stored: softmax cross
+// entropy, and distillation from a teacher's top logits, forward and backward.
+//
+// With hidden rows h_i (N, D), weights w_v (V, D), s_iv = h_i . w_v, and a few
+// targets (v_k, p_k) per row (cross entropy: one, p = 1; distillation: p =
+// softmax(t_k / T) over the row's K teacher logits, s divided by T):
+//   lse_i  = log sum_v exp(s_iv)
+//   loss_i = T^2 (sum_k p_k log p_k - sum_k p_k s_ik + lse_i)
+//   G_iv   = c_i (exp(s_iv - lse_i) - sum_{k: v_k = v} p_k),  c_i = T dloss_i
+//   dH = G W,   dW = G^T H
+// Forward: one GEMM whose epilogue keeps a row's maximum and sum of exponentials
+// per 256 columns, (V / 256) pairs per row, which finish_kernel joins.
+// Backward, in pieces of the vocabulary of C columns: the logits again, their
+// epilogue writing G (N, C) in bf16; then dH += G W_piece and dW_piece = G^T H.
+// G is rounded to bf16 once, as an operand of bf16 MMAs has to be; its relative
+// error of 2^-9 is that of the bf16 gradients it ends in.  All sums are fp32.
+//
+// One persistent GEMM kernel does all four products: a pair of SMs
+// (tcgen05.mma.cta_group::2) per 256 x 256 tile, so that each SM loads 128 rows
+// of either operand and both accumulators (2 x 256 TMEM columns) alternate
+// between the MMAs of one tile and the epilogue of the one before.  Roles: warp
+// 0 TMA producer, warp 1 MMA issuer (leader's), warps 4-7 epilogue (thread = row
+// = TMEM lane).  Operands are K-major or MN-major as they lie in memory: no
+// transposed copy exists.  Where a product has few tiles, its K range is split
+// and the parts meet in fp32 planes which planes_kernel sums in a fixed order.
+// Every mbarrier wait is bounded; on expiry the CTAs leave and a status flag is set.
+#include <cudaTypedefs.h>
+
+#include "lh_common.cuh"
+#include "sm100.cuh"
+
+namespace lh {
+
+using namespace sm100;
+
+__device__ int g_loss_status;    // set to 1 when a bounded wait gave up
+
+namespace ll {
+
+constexpr int kTM = 256, kTN = 256, kTK = 64;    // tile of a pair of SMs
+constexpr int kBox = 64 * 64 * 2;                // one 64 x 64 bf16 TMA box, 128-byte rows
+constexpr int kOpBytes = 2 * kBox;               // 128 rows of an operand: one CTA's share of a stage
+constexpr int kStages = 6;
+constexpr int kThreads = 256;
+constexpr int kOutBuf = 4096;                    // 32 rows x 128 bytes: one store of an epilogue warp
+constexpr int kSmem = 1024 + kStages * 2 * kOpBytes + 4 * 2 * kOutBuf + 512;
+constexpr int kPairs = 74;
+constexpr int kNone = 0x7fffffff;
+constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
+
+enum Mode { kStats, kGrad, kDH, kDW };
+enum Out { kOutBf16, kOutPlane, kOutPlaneAdd };
+
+struct Smem {
+  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem_base;
+  int abort;
+};
+static_assert(sizeof(Smem) <= 512, "barriers do not fit their space");
+
+struct Args {
+  int M, N;                       // rows and columns of the result
+  int tiles_m, tiles_n, splits, kb, gm;
+  int b_off;                      // first row of B's operand (vocabulary piece)
+  int out;                        // kDH, kDW: Out
+  // targets: int64 (K = 1, SPARSE false) or sorted int32 (N, K) with probabilities
+  const long long* target;
+  const int* idx;
+  const float* prob;
+  int K;
+  float a2;                       // log2(e) / T
+  float2* stats;                  // kStats: (tiles_n, M) maximum and sum of every tile's row
+  float* slog;                    // logits of the targets (N, K): kStats writes, kGrad reads
+  const float* lse2;              // kGrad: log2-sum-exp2 of s a2
+  const float *gout, *row_scale, *inv_count;
+  int gstride;
+  float cscale;
+};
+
+// Position of the first of a row's K sorted targets that is >= v.
+__device__ __forceinline__ int lower_bound(const int* __restrict__ idx, int K, int v) {
+  int lo = 0, hi = K;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(idx + mid) < v) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+template <int MODE, bool SPARSE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const __grid_constant__ CUtensorMap tmO, const Args a) {
+  constexpr bool kAMn = MODE == kDW, kBMn = MODE == kDH || MODE == kDW;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = base;
+  uint8_t* sB = base + kStages * kOpBytes;
+  uint8_t* sO = base + 2 * kStages * kOpBytes;
+  Smem* sm = reinterpret_cast<Smem*>(sO + 8 * kOutBuf);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank();
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  const int total = a.tiles_m * a.tiles_n * a.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { mbar_init(&sm->full[s], 1); mbar_init(&sm->empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&sm->acc_full[b], 1); mbar_init(&sm->acc_empty[b], 8); }
+    mbar_init(&sm->drain, 1);
+    // an earlier launch gave up a wait: do nothing until the host resets
+    sm->abort = *reinterpret_cast<volatile int*>(&g_loss_status) ? 2 : 0;
+    fence_mbar_init();
+  }
+  if (warp == 2) tmem_alloc_pair(&sm->tmem_base, 512);
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tbase = sm->tmem_base;
+  volatile int* abort = &sm->abort;
+
+  // tile t -> split, row block, column block: gm row blocks at a time, rows first
+  auto decode = [&](int t, int& m, int& n, int& k0, int& k1, int& split) {
+    const int mn = a.tiles_m * a.tiles_n;
+    split = t / mn;
+    int r = t - split * mn;
+    const int g = r / (a.gm * a.tiles_n);
+    r -= g * a.gm * a.tiles_n;
+    const int rows = min(a.gm, a.tiles_m - g * a.gm);
+    m = g * a.gm + r % rows;
+    n = r / rows;
+    k0 = (int)((long long)a.kb * split / a.splits);
+    k1 = (int)((long long)a.kb * (split + 1) / a.splits);
+  };
+
+  if (*abort == 0) {
+    if (warp == 0) {
+      // ---------------------------------------------------------- TMA producer
+      if (lane == 0) {
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = pair; t < total && ok; t += n_pairs) {
+          int m, n, k0, k1, split;
+          decode(t, m, n, k0, k1, split);
+          const int ra = m * kTM + rank * 128, rb = n * kTN + rank * 128;
+          for (int k = k0; k < k1; ++k, ++it) {
+            const int s = it % kStages;
+            const uint32_t round = it / kStages;
+            if (round > 0 && !mbar_wait(&sm->empty[s], (round - 1) & 1, abort)) { ok = false; break; }
+            if (rank == 0) mbar_expect_tx(&sm->full[s], 4 * kOpBytes);
+            const uint32_t bar = leader_addr(&sm->full[s]);
+            uint8_t* pa = sA + s * kOpBytes;
+            uint8_t* pb = sB + s * kOpBytes;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (kAMn) tma_load_2d_pair(pa + j * kBox, &tmA, bar, ra + 64 * j, k * kTK);
+              else tma_load_2d_pair(pa + j * kBox, &tmA, bar, k * kTK, ra + 64 * j);
+              if (kBMn) tma_load_2d_pair(pb + j * kBox, &tmB, bar, rb + 64 * j, a.b_off + k * kTK);
+              else tma_load_2d_pair(pb + j * kBox, &tmB, bar, k * kTK, a.b_off + rb + 64 * j);
+            }
+          }
+        }
+        // the copies of the last stages have landed before the CTA may leave (on a
+        // normal end the MMAs have already waited for them)
+        if (!ok && rank == 0)
+          for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
+            for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->full[i % kStages], (i / kStages) & 1); ++p) {}
+      }
+    } else if (warp == 1 && rank == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        constexpr uint32_t idesc = idesc_bf16_f32(kTM, kTN, kAMn, kBMn);
+        uint32_t it = 0;
+        int li = 0;
+        bool ok = true;
+        for (int t = pair; t < total && ok; t += n_pairs, ++li) {
+          int m, n, k0, k1, split;
+          decode(t, m, n, k0, k1, split);
+          const int b = li & 1;
+          if (li >= 2 && !mbar_wait_cluster(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort)) break;
+          tc_fence_after();
+          const uint32_t acc = tbase + b * kTN;
+          for (int k = k0; k < k1; ++k, ++it) {
+            const int s = it % kStages;
+            if (!mbar_wait_cluster(&sm->full[s], (it / kStages) & 1, abort)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t pa = smem_u32(sA + s * kOpBytes), pb = smem_u32(sB + s * kOpBytes);
+#pragma unroll
+            for (int kk = 0; kk < kTK / 16; ++kk)
+              mma_ss_pair(acc,
+                          kAMn ? smem_desc_sw128(pa + kk * 2048, kBox, 1024) : smem_desc_sw128(pa + kk * 32, 16, 1024),
+                          kBMn ? smem_desc_sw128(pb + kk * 2048, kBox, 1024) : smem_desc_sw128(pb + kk * 32, 16, 1024),
+                          idesc, (k > k0 || kk > 0) ? 1u : 0u);
+            mma_commit_pair(&sm->empty[s]);
+          }
+          if (ok) mma_commit_pair(&sm->acc_full[b]);
+        }
+        if (*abort) {                            // the MMAs issued so far end before TMEM is freed
+          mma_commit_pair(&sm->drain);
+          for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->drain, 0); ++p) {}
+        }
+      }
+    } else if (warp >= 4) {
+      // ---------------------------------------------------------- epilogue
+      const int quad = warp & 3;
+      const uint32_t lane_base = tbase + ((uint32_t)(quad * 32) << 16);
+      uint8_t* stage = sO + quad * 2 * kOutBuf;
+      const uint32_t acc_empty[2] = {leader_addr(&sm->acc_empty[0]), leader_addr(&sm->acc_empty[1])};
+      int li = 0, buf = 0;
+      // 16 bytes to chunk c of this thread's row of the staging tile (128-byte swizzle)
+      auto put = [&](uint8_t* p, int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+        *reinterpret_cast<uint4*>(p + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(x, y, z, w);
+      };
+      for (int t = pair; t < total; t += n_pairs, ++li) {
+        int m, n, k0, k1, split;
+        decode(t, m, n, k0, k1, split);
+        const int b = li & 1;
+        const uint32_t acc = lane_base + b * kTN;
+        const int row0 = m * kTM + rank * 128 + quad * 32, row = row0 + lane, n0 = n * kTN;
+        const int cols = min(kTN, a.N - n0);
+        const bool live = row < a.M;
+        // next target of this row at or behind the tile's first column, as a column of the tile
+        int cur = 0, next = kNone;
+        const int g0 = MODE == kGrad ? a.b_off + n0 : n0;
+        const int* idx = nullptr;
+        auto advance = [&]() { next = cur < a.K && __ldg(idx + cur) != kNone ? __ldg(idx + cur) - g0 : kNone; };
+        float c = 0.f, lse2 = 0.f;
+        if constexpr (MODE == kStats || MODE == kGrad) {
+          if (live) {
+            if constexpr (SPARSE) {
+              idx = a.idx + (size_t)row * a.K;
+              cur = lower_bound(idx, a.K, g0);
+              advance();
+            } else {
+              const long long tv = __ldg(a.target + row) - g0;
+              if (tv >= 0 && tv < kTN) next = (int)tv;
+            }
+            if constexpr (MODE == kGrad) {
+              const float up = __ldg(a.gout + (size_t)row * a.gstride);
+              if (up != 0.f) c = a.cscale * up * __ldg(a.row_scale + row) * (a.inv_count ? __ldg(a.inv_count) : 1.f);
+              lse2 = __ldg(a.lse2 + row);
+            }
+          }
+        }
+        const bool ok = mbar_wait(&sm->acc_full[b], (li >> 1) & 1, abort);
+        if (__any_sync(~0u, !ok)) break;
+        tc_fence_after();
+        if constexpr (MODE == kStats) {
+          float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
+          for (int cc = 0; cc < kTN / 32; ++cc) {
+            const int left = cols - cc * 32;
+            if (left <= 0) break;
+            uint32_t x[32];
+            tmem_ld32(acc + cc * 32, x);
+            tmem_ld_wait();
+            if (left < 32) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (e >= left) x[e] = __float_as_uint(-INFINITY);
+            }
+            float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              mp[(e >> 1) & 3] = fmax3(mp[(e >> 1) & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+            const float mn = fmaxf(fmaxf(mx, fmaxf(mp[0], mp[1])), fmaxf(mp[2], mp[3]));
+            const float mb = mn == -INFINITY ? 0.f : mn * a.a2;
+            sum *= mx == -INFINITY ? 0.f : ex2(fmaf(mx, a.a2, -mb));
+            mx = mn;
+            float2 sp[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sp[u] = make_float2(0.f, 0.f);
+            const float2 a22 = make_float2(a.a2, a.a2), nb = make_float2(-mb, -mb);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 arg = ffma2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), a22, nb);
+              sp[(e >> 1) & 3] = fadd2(sp[(e >> 1) & 3], make_float2(ex2(arg.x), ex2(arg.y)));
+            }
+            const float2 r = fadd2(fadd2(sp[0], sp[1]), fadd2(sp[2], sp[3]));
+            sum += r.x + r.y;
+          }
+          // logits of the targets in this tile: one TMEM column at a time, all rows that want it at once
+          while (true) {
+            const int want = next < cols ? next : kNone;
+            const int col = (int)__reduce_min_sync(~0u, (unsigned)want);
+            if (col == kNone) break;
+            const uint32_t v = tmem_ld1(acc + col);
+            tmem_ld_wait();
+            while (next == col) {
+              a.slog[(size_t)row * a.K + cur] = __uint_as_float(v);
+              ++cur;
+              if constexpr (SPARSE) advance();
+              else next = kNone;
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acc_empty[b]);
+          if (live) a.stats[(size_t)n * a.M + row] = make_float2(mx, sum);
+        } else {
+          const int width = MODE == kGrad || a.out == kOutBf16 ? 64 : 32;      // columns of one store
+#pragma unroll 1
+          for (int c0 = 0; c0 < kTN; c0 += width) {
+            uint32_t x[32], y[32];
+            tmem_ld32(acc + c0, x);
+            if (width == 64) tmem_ld32(acc + c0 + 32, y);
+            tmem_ld_wait();
+            if (c0 + width == kTN) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(acc_empty[b]);
+            }
+            if (c0 >= cols || row0 >= a.M) continue;
+            uint8_t* p = stage + buf * kOutBuf;
+            if (lane == 0) bulk_wait_read_1();
+            __syncwarp();
+            if constexpr (MODE == kGrad) {
+              if (c == 0.f) {                    // a row without a gradient, whatever its logits are
+#pragma unroll
+                for (int ch = 0; ch < 8; ++ch) put(p, ch, 0, 0, 0, 0);
+              } else {
+                auto grad = [&](uint32_t u) { return c * ex2(fmaf(__uint_as_float(u), a.a2, -lse2)); };
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch)
+                  put(p, ch, pack_bf16(grad(x[8 * ch]), grad(x[8 * ch + 1])),
+                      pack_bf16(grad(x[8 * ch + 2]), grad(x[8 * ch + 3])),
+                      pack_bf16(grad(x[8 * ch + 4]), grad(x[8 * ch + 5])),
+                      pack_bf16(grad(x[8 * ch + 6]), grad(x[8 * ch + 7])));
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch)
+                  put(p, 4 + ch, pack_bf16(grad(y[8 * ch]), grad(y[8 * ch + 1])),
+                      pack_bf16(grad(y[8 * ch + 2]), grad(y[8 * ch + 3])),
+                      pack_bf16(grad(y[8 * ch + 4]), grad(y[8 * ch + 5])),
+                      pack_bf16(grad(y[8 * ch + 6]), grad(y[8 * ch + 7])));
+                while (next < c0 + 64) {         // the row's targets among these columns, from their fp32 logits
+                  const float q = ex2(fmaf(__ldg(a.slog + (size_t)row * a.K + cur), a.a2, -lse2));
+                  const int at = next - c0;
+                  float pr = 1.f;
+                  if constexpr (SPARSE) {
+                    pr = 0.f;
+                    do {
+                      pr += __ldg(a.prob + (size_t)row * a.K + cur);
+                      ++cur;
+                      advance();
+                    } while (next == c0 + at);
+                  } else {
+                    next = kNone;
+                  }
+                  *reinterpret_cast<__nv_bfloat16*>(p + lane * 128 + (((at >> 3) ^ (lane & 7)) << 4) + (at & 7) * 2) =
+                      __float2bfloat16_rn(c * (q - pr));
+                }
+              }
+            } else if (a.out == kOutBf16) {
+#pragma unroll
+              for (int ch = 0; ch < 4; ++ch) {
+                auto pk = [&](const uint32_t* u) { return pack_bf16(__uint_as_float(u[0]), __uint_as_float(u[1])); };
+                put(p, ch, pk(x + 8 * ch), pk(x + 8 * ch + 2), pk(x + 8 * ch + 4), pk(x + 8 * ch + 6));
+                put(p, 4 + ch, pk(y + 8 * ch), pk(y + 8 * ch + 2), pk(y + 8 * ch + 4), pk(y + 8 * ch + 6));
+              }
+            } else {
+#pragma unroll
+              for (int ch = 0; ch < 8; ++ch) put(p, ch, x[4 * ch], x[4 * ch + 1], x[4 * ch + 2], x[4 * ch + 3]);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              if (MODE != kGrad && a.out == kOutPlaneAdd) tma_reduce_add_3d(&tmO, p, n0 + c0, row0, split);
+              else tma_store_3d(&tmO, p, n0 + c0, row0, split);
+              bulk_commit();
+            }
+            buf ^= 1;
+          }
+        }
+      }
+      if (lane == 0) bulk_wait_all();
+    }
+  }
+
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc_pair(tbase, 512);
+  }
+  if (threadIdx.x == 0 && sm->abort) atomicExch(&g_loss_status, 1);
+}
+
+// ---------------------------------------------------------------- small kernels
+// One warp per row: the K teacher entries sorted by vocabulary index (absent
+// ones behind), their probabilities softmax(t / T) and sum p log p.  The rank of
+// an entry is the number of entries before it, ties in their given order.
+//   row_scale: 1, 0 for a row without entries, NaN for one with an index >= V or
+//   a teacher logit that is NaN or +infinity
+template <class T>
+__global__ void __launch_bounds__(128)
+teacher_kernel(const T* __restrict__ tv, const long long* __restrict__ ti, int N, int V, int K, float inv_t,
+               int* __restrict__ idx, float* __restrict__ prob, float* __restrict__ ent, float* __restrict__ row_scale) {
+  extern __shared__ int sh[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* key = sh + warp * K;
+  const int row = blockIdx.x * 4 + warp;
+  if (row >= N) return;
+  const T* tr = tv + (size_t)row * K;
+  const long long* ir = ti + (size_t)row * K;
+  bool bad = false;
+  float mx = -INFINITY;
+  for (int k = lane; k < K; k += 32) {
+    const long long i = ir[k];
+    const bool here = i >= 0 && i < V;
+    const float x = (float)tr[k] * inv_t;
+    bad |= i >= V || (here && x != x);
+    key[k] = here ? (int)i : kNone;
+    if (here) mx = fmaxf(mx, x);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+  bad = __any_sync(~0u, bad);
+  float z = 0.f;
+  for (int k = lane; k < K; k += 32)
+    if (key[k] != kNone && mx != -INFINITY) z += expf((float)tr[k] * inv_t - mx);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(~0u, z, o);
+  const bool some = mx != -INFINITY;
+  const float logz = logf(z);
+  float e = 0.f;
+  bool any_nan = false;
+  for (int k = lane; k < K; k += 32) {
+    const int me = key[k];
+    int r = 0;
+    for (int j = 0; j < K; ++j) r += key[j] < me || (key[j] == me && j < k);
+    float p = 0.f;
+    if (me != kNone && some) {
+      const float x = (float)tr[k] * inv_t - mx - logz;
+      p = expf(x);
+      any_nan |= p != p;
+      if (p > 0.f) e = fmaf(p, x, e);
+    }
+    idx[(size_t)row * K + r] = some ? me : kNone;
+    prob[(size_t)row * K + r] = p;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) e += __shfl_xor_sync(~0u, e, o);
+  any_nan = __any_sync(~0u, any_nan);
+  if (lane == 0) {
+    ent[row] = e;
+    row_scale[row] = bad || any_nan ? __int_as_float(0x7fc00000) : some ? 1.f : 0.f;
+  }
+}
+
+// Joins the tiles' (maximum, sum) of 32 rows per block and forms the rows'
+// losses; partial (sum, count) of the block for the reduced loss.
+template <bool SPARSE>
+__global__ void __launch_bounds__(1024)
+finish_kernel(const float2* __restrict__ stats, int tiles, int N, int V, int K, const long long* __restrict__ target,
+              long long ignore, const int* __restrict__ idx, const float* __restrict__ prob,
+              const float* __restrict__ ent, const float* __restrict__ slog, float a2, float t2,
+              float* __restrict__ row_scale, float* __restrict__ lse2, float* __restrict__ loss_rows,
+              double2* __restrict__ part) {
+  __shared__ float2 sh[32][33];
+  const int lane = threadIdx.x, w = threadIdx.y, nw = blockDim.y;
+  const int row = blockIdx.x * 32 + lane;
+  float mx = -INFINITY, s = 0.f;
+  auto join = [&](float2 v) {
+    const float mn = fmaxf(mx, v.x);
+    const float mb = mn == -INFINITY ? 0.f : mn * a2;
+    s = s * (mx == -INFINITY ? 0.f : exp2f(fmaf(mx, a2, -mb))) + v.y * (v.x == -INFINITY ? 0.f : exp2f(fmaf(v.x, a2, -mb)));
+    if (v.y != v.y) s = v.y;
+    mx = mn;
+  };
+  if (row < N) {
+#pragma unroll 4
+    for (int t = w; t < tiles; t += nw) join(stats[(size_t)t * N + row]);
+  }
+  sh[w][lane] = make_float2(mx, s);
+  __syncthreads();
+  if (w) return;
+  for (int k = 1; k < nw; ++k) join(sh[k][lane]);
+  float loss = 0.f, scale = 0.f;
+  if (row < N) {
+    const float l2 = fmaf(mx, a2, log2f(s));
+    lse2[row] = l2;
+    const float lse = l2 * kLn2, a = a2 * kLn2;         // a = 1 / T
+    if (SPARSE) {
+      scale = row_scale[row];
+      if (scale == 0.f) {
+        loss = 0.f;
+      } else {
+        float x = 0.f;
+        for (int k = 0; k < K; ++k) {
+          if (idx[(size_t)row * K + k] == kNone) break;
+          const float p = prob[(size_t)row * K + k];
+          if (p > 0.f) x = fmaf(p, lse - slog[(size_t)row * K + k] * a, x);
+        }
+        loss = scale * t2 * (ent[row] + x);
+      }
+    } else {
+      const long long t = target[row];
+      if (t != ignore) {
+        const bool in = t >= 0 && t < V;
+        scale = in ? 1.f : __int_as_float(0x7fc00000);
+        loss = in ? lse - slog[row] : scale;
+      }
+      row_scale[row] = scale;
+    }
+    if (loss_rows) loss_rows[row] = loss;
+  }
+  if (part) {
+    double ls = loss, n = scale != 0.f ? 1.0 : 0.0;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      ls += __shfl_xor_sync(~0u, ls, o);
+      n += __shfl_xor_sync(~0u, n, o);
+    }
+    if (lane == 0) part[blockIdx.x] = make_double2(ls, n);
+  }
+}
+
+// The blocks' partial sums -> the loss (sum, or mean over the rows that count,
+// 0 where none does) and 1 / count.
+__global__ void __launch_bounds__(256)
+total_kernel(const double2* __restrict__ part, int n, bool mean, float* loss, float* inv_count) {
+  __shared__ double sh[2][8];
+  double s = 0, c = 0;
+  for (int i = threadIdx.x; i < n; i += 256) { s += part[i].x; c += part[i].y; }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    s += __shfl_xor_sync(~0u, s, o);
+    c += __shfl_xor_sync(~0u, c, o);
+  }
+  if ((threadIdx.x & 31) == 0) { sh[0][threadIdx.x >> 5] = s; sh[1][threadIdx.x >> 5] = c; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) { s += sh[0][w]; c += sh[1][w]; }
+    const double inv = mean ? (c > 0 ? 1.0 / c : 0.0) : 1.0;
+    *loss = (float)(c > 0 ? s * inv : 0.0);
+    *inv_count = (float)inv;
+  }
+}
+
+// out (bf16) = sum of the fp32 planes (rows x cols each), in their order.
+__global__ void __launch_bounds__(256)
+planes_kernel(const float* __restrict__ planes, int n, size_t plane, __nv_bfloat16* __restrict__ out) {
+  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8; i < plane; i += (size_t)gridDim.x * 256 * 8) {
+    float v[8], u[8];
+    load16(planes + i, v);
+    load16(planes + i + 4, v + 4);
+    for (int k = 1; k < n; ++k) {
+      load16(planes + k * plane + i, u);
+      load16(planes + k * plane + i + 4, u + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += u[e];
+    }
+    store16(out + i, v);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (PFN_cuTensorMapEncodeTiled_v12000)p;
+  }();
+  return fn;
+}
+
+// Encoding a tensor map is a driver call and needs a current context, which a
+// thread that has only launched through another thread's calls (autograd's) may
+// not have yet: cudaSetDevice makes the device's primary context current.
+static int make_context_current() {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);
+  if (e != cudaSuccess) { set_error("linear loss: %s", cudaGetErrorString(e)); return LH_ERR_LAUNCH; }
+  return LH_OK;
+}
+
+// bf16 (rows, cols) with a row pitch in elements; 64 x 64 boxes, 128-byte swizzle.
+static int map_load(CUtensorMap* m, const void* p, long long rows, long long cols, long long pitch) {
+  auto enc = encode_fn();
+  if (!enc) { set_error("cuTensorMapEncodeTiled unavailable"); return LH_ERR_LAUNCH; }
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)pitch * 2};
+  cuuint32_t box[2] = {64, 64}, es[2] = {1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, box, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { set_error("linear loss: tensor map of an operand failed (%d)", (int)r); return LH_ERR_LAUNCH; }
+  return LH_OK;
+}
+// Result (planes, rows, cols), bf16 or fp32; boxes of 32 rows x 128 bytes.
+static int map_store(CUtensorMap* m, void* p, bool f32, long long planes, long long rows, long long cols, long long pitch) {
+  auto enc = encode_fn();
+  if (!enc) { set_error("cuTensorMapEncodeTiled unavailable"); return LH_ERR_LAUNCH; }
+  const int es_ = f32 ? 4 : 2;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)pitch * es_, (cuuint64_t)(pitch * rows) * es_};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / es_), 32, 1}, es[3] = {1, 1, 1};
+  CUresult r = enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, p, dims, strides, box,
+                   es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { set_error("linear loss: tensor map of a result failed (%d)", (int)r); return LH_ERR_LAUNCH; }
+  return LH_OK;
+}
+
+template <int MODE, bool SPARSE>
+static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, Args a, long long K, cudaStream_t st) {
+  a.tiles_m = (a.M + kTM - 1) / kTM;
+  a.tiles_n = (a.N + kTN - 1) / kTN;
+  a.kb = (int)((K + kTK - 1) / kTK);
+  // Row blocks walked together: as many as keep their operand rows in about half of L2, at least
+  // eight (eight by nine tiles are one wave of the 74 pairs).
+  long long gm = (48ll << 20) / (kTM * 2ll * a.kb * kTK);
+  if (gm < 8) gm = 8;
+  a.gm = (int)(gm < a.tiles_m ? gm : a.tiles_m);
+  const long long total = (long long)a.tiles_m * a.tiles_n * a.splits;
+  const int pairs = (int)(total < kPairs ? total : kPairs);
+  cudaError_t e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) { set_error("linear loss: %s", cudaGetErrorString(e)); return LH_ERR_LAUNCH; }
+  loss_gemm_kernel<MODE, SPARSE><<<2 * pairs, kThreads, kSmem, st>>>(ma, mb, mo, a);
+  return check_launch("loss_gemm_kernel");
+}
+
+// Parts of the K range of an (M, N) product: the number that makes the shortest
+// rounds of the 74 pairs, counting an epilogue as six 64-deep steps and
+// the planes' traffic.
+static int pick_splits(long long M, long long N, long long K) {
+  const long long tiles = ((M + kTM - 1) / kTM) * ((N + kTN - 1) / kTN), kb = (K + kTK - 1) / kTK;
+  double best = 1e30;
+  int pick = 1;
+  for (int s = 1; s <= kPairs && s <= kb; ++s) {
+    if (s > 1 && tiles * s > 4 * kPairs) break;
+    const double rounds = (double)((tiles * s + kPairs - 1) / kPairs);
+    const double cost = rounds * ((double)((kb + s - 1) / s) + 6.0) + (s > 1 ? 8.0 + 8.0 * s * M * N / 6.5e6 / 0.28 : 0.0);
+    if (cost < best) { best = cost; pick = s; }
+  }
+  return pick;
+}
+
+struct Plan {
+  long long C;                 // columns of a vocabulary piece, a multiple of 256
+  int pieces, dh_splits, dw_splits;
+  bool dh_planes;
+  size_t g, dh, dw, total;     // bytes
+};
+constexpr long long kPieceBytes = 512ll << 20;
+
+static size_t up(size_t n) { return (n + 255) & ~size_t(255); }
+
+static Plan plan(long long N, long long V, long long D) {
+  Plan p;
+  long long C = kPieceBytes / (2 * N) / kTN * kTN;
+  if (C < kTN) C = kTN;
+  const long long Vp = (V + kTN - 1) / kTN * kTN;
+  p.pieces = (int)((Vp + C - 1) / C);
+  p.C = ((Vp + p.pieces - 1) / p.pieces + kTN - 1) / kTN * kTN;      // pieces of about equal size
+  p.pieces = (int)((Vp + p.C - 1) / p.C);
+  p.dh_splits = pick_splits(N, D, p.C < V ? p.C : V);
+  p.dw_splits = pick_splits(p.C < V ? p.C : V, D, N);
+  p.dh_planes = p.pieces > 1 || p.dh_splits > 1;
+  p.g = up((size_t)N * p.C * 2);
+  p.dh = p.dh_planes ? up((size_t)p.dh_splits * N * D * 4) : 0;
+  p.dw = p.dw_splits > 1 ? up((size_t)p.dw_splits * p.C * D * 4) : 0;
+  p.total = p.g + p.dh + p.dw;
+  return p;
+}
+
+static size_t fwd_workspace(long long N, long long V) {
+  return up((size_t)((V + kTN - 1) / kTN) * N * sizeof(float2)) + up((size_t)((N + 31) / 32) * sizeof(double2)) +
+         up((size_t)N * sizeof(float));
+}
+
+static int sum_planes(const float* planes, int n, size_t plane, void* out, cudaStream_t st) {
+  size_t blocks = (plane / 8 + 255) / 256;
+  if (blocks > 148 * 16) blocks = 148 * 16;
+  planes_kernel<<<(unsigned)blocks, 256, 0, st>>>(planes, n, plane, (__nv_bfloat16*)out);
+  return check_launch("planes_kernel");
+}
+
+struct Targets {
+  const long long* target;   // cross entropy
+  long long ignore;
+  const int* idx;            // distillation
+  const float* prob;
+  int K;
+  float T;
+};
+
+template <bool SPARSE>
+static int forward(const void* hidden, const void* weight, int N, int V, int D, const Targets& tg, const float* ent,
+                   int reduction, float* loss, float* lse2, float* slog, float* row_scale, float* inv_count, void* ws,
+                   cudaStream_t st) {
+  int rc = make_context_current();
+  if (rc) return rc;
+  CUtensorMap mh, mw;
+  if ((rc = map_load(&mh, hidden, N, D, D)) || (rc = map_load(&mw, weight, V, D, D))) return rc;
+  const int tiles = (V + kTN - 1) / kTN;
+  float2* stats = (float2*)ws;
+  double2* part = (double2*)((char*)ws + up((size_t)tiles * N * sizeof(float2)));
+  Args a{};
+  a.M = N;
+  a.N = V;
+  a.splits = 1;
+  a.target = tg.target;
+  a.idx = tg.idx;
+  a.prob = tg.prob;
+  a.K = tg.K;
+  a.a2 = kLog2e / tg.T;
+  a.stats = stats;
+  a.slog = slog;
+  if ((rc = launch<kStats, SPARSE>(mh, mw, mw, a, D, st))) return rc;
+  const int blocks = (N + 31) / 32;
+  finish_kernel<SPARSE><<<blocks, dim3(32, tiles < 32 ? tiles : 32), 0, st>>>(
+      stats, tiles, N, V, tg.K, tg.target, tg.ignore, tg.idx, tg.prob, ent, slog, a.a2, tg.T * tg.T, row_scale, lse2,
+      reduction == LH_REDUCE_NONE ? loss : nullptr, reduction == LH_REDUCE_NONE ? nullptr : part);
+  if ((rc = check_launch("finish_kernel"))) return rc;
+  if (reduction == LH_REDUCE_NONE) return LH_OK;
+  total_kernel<<<1, 256, 0, st>>>(part, blocks, reduction == LH_REDUCE_MEAN, loss, inv_count);
+  return check_launch("total_kernel");
+}
+
+template <bool SPARSE>
+static int backward(const void* hidden, const void* weight, int N, int V, int D, const Targets& tg, const float* lse2,
+                    const float* slog, const float* row_scale, const float* inv_count, const float* gout, int gstride,
+                    void* dhidden, void* dweight, void* ws, cudaStream_t st) {
+  int rc = make_context_current();
+  if (rc) return rc;
+  const Plan p = plan(N, V, D);
+  char* g = (char*)ws;
+  float* dh = (float*)(g + p.g);
+  float* dw = (float*)(g + p.g + p.dh);
+  CUtensorMap mh, mw, mdh, mdw, mg, mgo;
+  if ((rc = map_load(&mh, hidden, N, D, D)) || (rc = map_load(&mw, weight, V, D, D))) return rc;
+  if ((rc = p.dh_planes ? map_store(&mdh, dh, true, p.dh_splits, N, D, D) : map_store(&mdh, dhidden, false, 1, N, D, D)))
+    return rc;
+  for (int i = 0; i < p.pieces; ++i) {
+    const long long v0 = i * p.C;
+    const int cols = (int)(V - v0 < p.C ? V - v0 : p.C);
+    if ((rc = map_load(&mg, g, N, cols, p.C)) || (rc = map_store(&mgo, g, false, 1, N, cols, p.C))) return rc;
+    Args a{};
+    a.M = N;
+    a.N = cols;
+    a.splits = 1;
+    a.b_off = (int)v0;
+    a.target = tg.target;
+    a.idx = tg.idx;
+    a.prob = tg.prob;
+    a.K = tg.K;
+    a.a2 = kLog2e / tg.T;
+    a.slog = const_cast<float*>(slog);
+    a.lse2 = lse2;
+    a.row_scale = row_scale;
+    a.inv_count = inv_count;
+    a.gout = gout;
+    a.gstride = gstride;
+    a.cscale = tg.T;
+    if ((rc = launch<kGrad, SPARSE>(mh, mw, mgo, a, D, st))) return rc;
+
+    Args x{};
+    x.M = N;
+    x.N = D;
+    const int kb = (cols + kTK - 1) / kTK;
+    x.splits = p.dh_splits < kb ? p.dh_splits : kb;      // a short last piece may leave planes as they are
+    x.b_off = (int)v0;
+    x.out = !p.dh_planes ? kOutBf16 : i ? kOutPlaneAdd : kOutPlane;
+    if ((rc = launch<kDH, false>(mg, mw, mdh, x, cols, st))) return rc;
+
+    Args y{};
+    y.M = cols;
+    y.N = D;
+    y.splits = p.dw_splits;
+    y.out = p.dw_splits > 1 ? kOutPlane : kOutBf16;
+    char* dw_out = (char*)dweight + (size_t)v0 * D * 2;
+    if ((rc = p.dw_splits > 1 ? map_store(&mdw, dw, true, p.dw_splits, cols, D, D)
+                              : map_store(&mdw, dw_out, false, 1, cols, D, D)))
+      return rc;
+    if ((rc = launch<kDW, false>(mg, mh, mdw, y, N, st))) return rc;
+    if (p.dw_splits > 1 && (rc = sum_planes(dw, p.dw_splits, (size_t)cols * D, dw_out, st))) return rc;
+  }
+  return p.dh_planes ? sum_planes(dh, p.dh_splits, (size_t)N * D, dhidden, st) : LH_OK;
+}
+
+}  // namespace ll
+
+size_t linear_loss_workspace_size(int N, int V, int D, int backward) {
+  return backward ? ll::plan(N, V, D).total : ll::fwd_workspace(N, V);
+}
+
+int linear_xent_fwd(const void* hidden, const void* weight, const long long* target, long long ignore, int N, int V, int D,
+                    int reduction, float* loss, float* lse2, float* tlogit, float* row_scale, float* inv_count, void* ws,
+                    cudaStream_t st) {
+  const ll::Targets tg{target, ignore, nullptr, nullptr, 1, 1.f};
+  return ll::forward<false>(hidden, weight, N, V, D, tg, nullptr, reduction, loss, lse2, tlogit, row_scale, inv_count, ws, st);
+}
+
+int linear_xent_bwd(const void* hidden, const void* weight, const long long* target, int N, int V, int D, const float* lse2,
+                    const float* tlogit, const float* row_scale, const float* inv_count, const float* gout, int gstride,
+                    void* dhidden, void* dweight, void* ws, cudaStream_t st) {
+  const ll::Targets tg{target, 0, nullptr, nullptr, 1, 1.f};
+  return ll::backward<false>(hidden, weight, N, V, D, tg, lse2, tlogit, row_scale, inv_count, gout, gstride, dhidden,
+                             dweight, ws, st);
+}
+
+int linear_distill_fwd(const void* hidden, const void* weight, const void* tv, int tv_dtype, const long long* ti, int N,
+                       int V, int D, int K, float T, int reduction, float* loss, float* lse2, int* idx, float* prob,
+                       float* tlogit, float* row_scale, float* inv_count, void* ws, cudaStream_t st) {
+  float* ent = (float*)((char*)ws + ll::up((size_t)((V + ll::kTN - 1) / ll::kTN) * N * sizeof(float2)) +
+                        ll::up((size_t)((N + 31) / 32) * sizeof(double2)));
+  const unsigned blocks = (unsigned)((N + 3) / 4);
+  if (tv_dtype == LH_DTYPE_BF16)
+    ll::teacher_kernel<<<blocks, 128, 4 * K * sizeof(int), st>>>((const __nv_bfloat16*)tv, ti, N, V, K, 1.f / T, idx, prob,
+                                                                ent, row_scale);
+  else
+    ll::teacher_kernel<<<blocks, 128, 4 * K * sizeof(int), st>>>((const float*)tv, ti, N, V, K, 1.f / T, idx, prob, ent,
+                                                                row_scale);
+  int rc = check_launch("teacher_kernel");
+  if (rc) return rc;
+  const ll::Targets tg{nullptr, 0, idx, prob, K, T};
+  return ll::forward<true>(hidden, weight, N, V, D, tg, ent, reduction, loss, lse2, tlogit, row_scale, inv_count, ws, st);
+}
+
+int linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float T, const float* lse2,
+                       const int* idx, const float* prob, const float* tlogit, const float* row_scale,
+                       const float* inv_count, const float* gout, int gstride, void* dhidden, void* dweight, void* ws,
+                       cudaStream_t st) {
+  const ll::Targets tg{nullptr, 0, idx, prob, K, T};
+  return ll::backward<true>(hidden, weight, N, V, D, tg, lse2, tlogit, row_scale, inv_count, gout, gstride, dhidden,
+                            dweight, ws, st);
+}
+
+int loss_status(int reset) {
+  int h = 0;
+  cudaMemcpyFromSymbol(&h, g_loss_status, sizeof(int));
+  if (reset) { int z = 0; cudaMemcpyToSymbol(g_loss_status, &z, sizeof(int)); }
+  return h;
+}
+
+}  // namespace lh

@@ -279,4 +279,67 @@ def _(x, residual, weight, eps, group):
             x.new_empty(x.shape, dtype=residual.dtype))
 
 
+# --------------------------------------------------------------------------- losses of an output projection
+def _loss_fake(hidden, reduction):
+    f = lambda *s: hidden.new_empty(s, dtype=torch.float32)
+    N = hidden.shape[0]
+    return (f(N) if reduction == "none" else f()), f(N), f(N), f(0 if reduction == "none" else 1)
+
+
+@torch.library.custom_op(f"{NS}::linear_xent", mutates_args=())
+def linear_xent(hidden: Tensor, weight: Tensor, target: Tensor, ignore_index: int,
+                reduction: str) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """Cross entropy of hidden (N,D) weight (V,D)^T: loss, and lse2, tlogit, row_scale (N), inv_count (1) for
+    the backward."""
+    return _native.linear_xent_fwd(hidden, weight, target, ignore_index, reduction)
+
+
+@linear_xent.register_fake
+def _(hidden, weight, target, ignore_index, reduction):
+    loss, lse2, row_scale, inv_count = _loss_fake(hidden, reduction)
+    return loss, lse2, torch.empty_like(lse2), row_scale, inv_count
+
+
+@torch.library.custom_op(f"{NS}::linear_xent_bwd", mutates_args=())
+def linear_xent_bwd(hidden: Tensor, weight: Tensor, target: Tensor, lse2: Tensor, tlogit: Tensor, row_scale: Tensor,
+                    inv_count: Tensor, gout: Tensor, reduction: str) -> tuple[Tensor, Tensor]:
+    """Backward of linear_xent: dhidden (N,D), dweight (V,D)."""
+    return _native.linear_xent_bwd(hidden, weight, target, lse2, tlogit, row_scale, inv_count, gout, reduction)
+
+
+@linear_xent_bwd.register_fake
+def _(hidden, weight, target, lse2, tlogit, row_scale, inv_count, gout, reduction):
+    return hidden.new_empty(hidden.shape), weight.new_empty(weight.shape)
+
+
+@torch.library.custom_op(f"{NS}::linear_distill", mutates_args=())
+def linear_distill(hidden: Tensor, weight: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, temperature: float,
+                   reduction: str) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """Distillation of hidden (N,D) weight (V,D)^T from K teacher logits per row: loss, and lse2, idx, prob,
+    tlogit (N,K), row_scale (N), inv_count (1) for the backward."""
+    return _native.linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
+
+
+@linear_distill.register_fake
+def _(hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
+    loss, lse2, row_scale, inv_count = _loss_fake(hidden, reduction)
+    s = teacher_indices.shape
+    return (loss, lse2, hidden.new_empty(s, dtype=torch.int32), hidden.new_empty(s, dtype=torch.float32),
+            hidden.new_empty(s, dtype=torch.float32), row_scale, inv_count)
+
+
+@torch.library.custom_op(f"{NS}::linear_distill_bwd", mutates_args=())
+def linear_distill_bwd(hidden: Tensor, weight: Tensor, lse2: Tensor, idx: Tensor, prob: Tensor, tlogit: Tensor,
+                       row_scale: Tensor, inv_count: Tensor, gout: Tensor, temperature: float,
+                       reduction: str) -> tuple[Tensor, Tensor]:
+    """Backward of linear_distill: dhidden (N,D), dweight (V,D)."""
+    return _native.linear_distill_bwd(hidden, weight, lse2, idx, prob, tlogit, row_scale, inv_count, gout, temperature,
+                                      reduction)
+
+
+@linear_distill_bwd.register_fake
+def _(hidden, weight, lse2, idx, prob, tlogit, row_scale, inv_count, gout, temperature, reduction):
+    return hidden.new_empty(hidden.shape), weight.new_empty(weight.shape)
+
+
 ops = torch.ops.lighthouse_b200

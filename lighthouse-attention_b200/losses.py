@@ -1,0 +1,89 @@
+"""Losses of an output projection whose logits are never stored (csrc/linear_loss.cu).
+
+``linear_cross_entropy(hidden, weight, target)`` is
+``F.cross_entropy(hidden @ weight.T, target)`` and ``linear_distillation`` the
+divergence from a teacher's top logits, both with gradients for hidden and
+weight.  The logits live in tensor memory, tile by tile; the backward forms them
+again and goes over the vocabulary in pieces, so that memory beyond the inputs
+and gradients stays at about half a gigabyte whatever the vocabulary is.
+
+hidden (..., D) and weight (V, D) are bf16 CUDA tensors, D a multiple of 8.
+Logits, softmax statistics and losses are fp32, gradients bf16.
+"""
+from __future__ import annotations
+
+import torch
+
+from .library import ops as _ops
+
+
+class _LinearXentFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, target, ignore_index, reduction):
+        loss, *kept = _ops.linear_xent(hidden, weight, target, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, target, *kept)
+        ctx.reduction = reduction
+        return loss
+
+    @staticmethod
+    def backward(ctx, gout):
+        dh, dw = _ops.linear_xent_bwd(*ctx.saved_tensors, gout, ctx.reduction)
+        return dh, dw, None, None, None
+
+
+class _LinearDistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
+        loss, *kept = _ops.linear_distill(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
+        ctx.save_for_backward(hidden, weight, *kept)
+        ctx.temperature, ctx.reduction = temperature, reduction
+        return loss
+
+    @staticmethod
+    def backward(ctx, gout):
+        dh, dw = _ops.linear_distill_bwd(*ctx.saved_tensors, gout, ctx.temperature, ctx.reduction)
+        return dh, dw, None, None, None, None
+
+
+def _rows(hidden: torch.Tensor, *per_row: tuple[torch.Tensor, int]):
+    """hidden as (N, D); each (tensor, trailing dimensions) must have its leading dimensions."""
+    lead = hidden.shape[:-1]
+    for t, tail in per_row:
+        if t.shape[:t.dim() - tail] != lead:
+            raise ValueError(f"leading dimensions {tuple(lead)} of hidden and {tuple(t.shape)} differ")
+    return hidden.reshape(-1, hidden.shape[-1])
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of the logits ``hidden @ weight.T``.
+
+    target (...) int64 or int32 has hidden's leading dimensions.  Positions with
+    target ignore_index have loss 0 and no gradient; any other target outside
+    [0, V) makes the position's loss NaN.  reduction "mean" (over the positions
+    that are not ignored; 0 where all are), "sum", or "none" (the loss of every
+    position).  Returns fp32."""
+    h = _rows(hidden, (target, 0))
+    loss = _LinearXentFn.apply(h, weight, target.reshape(-1).to(torch.int64), ignore_index, reduction)
+    return loss.view(target.shape) if reduction == "none" else loss
+
+
+def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor,
+                        teacher_indices: torch.Tensor, temperature: float = 1.0,
+                        reduction: str = "mean") -> torch.Tensor:
+    """Divergence of the student ``softmax(hidden @ weight.T / T)`` from a teacher
+    known by its top logits.
+
+    teacher_logits (..., K) bf16 or fp32 and teacher_indices (..., K) int64 or
+    int32, K at most 256, in any order; a negative index marks an absent entry.
+    With p = softmax(teacher_logits / T) over a position's entries,
+    loss = T^2 sum_k p_k (log p_k - log student_k).  A position without entries
+    has loss 0, no gradient and does not count in the mean.  Entries with the
+    same index add up; an index >= V, or a logit that is NaN or +infinity, makes
+    the position's loss NaN.  The teacher gets no gradient.  Returns fp32."""
+    h = _rows(hidden, (teacher_logits, 1), (teacher_indices, 1))
+    N = h.shape[0]
+    loss = _LinearDistillFn.apply(h, weight, teacher_logits.detach().reshape(N, teacher_logits.shape[-1]),
+                                  teacher_indices.reshape(N, teacher_indices.shape[-1]).to(torch.int64),
+                                  float(temperature), reduction)
+    return loss.view(hidden.shape[:-1]) if reduction == "none" else loss

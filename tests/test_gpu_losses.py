@@ -1,0 +1,368 @@
+"""Cross entropy and distillation of an output projection against the formulas in 64 bits.
+
+Tolerances count roundings.  A logit is a sum of D exact products in fp32, whose
+additions may each cut 2^-23 of the running sum: ds = D 2^-23 sum_d |h_d w_d|
+bounds its error, and a loss is off by at most 2 ds and a few roundings of lse.
+G is rounded to bf16 (2^-8, half a step) and its exponentials carry the logits'
+errors, the products sum in fp32, and the gradients are rounded to bf16."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF = torch.bfloat16
+H8 = 2.0 ** -8
+
+
+def _problem(N, V, D, seed, cuda, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(V, D, generator=g) * scale / D ** 0.5).to(BF).to(cuda)
+    h = (torch.randn(N, D, generator=g) * 2).to(BF).to(cuda)
+    return g, h, w
+
+
+def _ds(h, w):
+    D = h.shape[1]
+    return (h.double().norm(dim=1) * w.double().norm(dim=1).max()) * D * 2.0 ** -23      # >= D 2^-23 sum |h_d w_d|
+
+
+def _formula(h, w, idx, prob, ok, coef, T):
+    """64-bit loss rows and gradients for sparse targets (N, K); coef is dloss of each row."""
+    h, w = h.double(), w.double()
+    s = h @ w.T / T
+    lse = torch.logsumexp(s, -1)
+    st = s.gather(1, idx)
+    ent = torch.where(prob > 0, prob * prob.clamp(min=1e-300).log(), torch.zeros_like(prob))
+    loss = T * T * (ent + torch.where(prob > 0, prob * (lse[:, None] - st), torch.zeros_like(prob))).sum(-1)
+    loss = torch.where(ok, loss, torch.zeros_like(loss))
+    c = (coef.double() * ok * T)[:, None]
+    q = (s - lse[:, None]).exp()
+    p = torch.zeros_like(q).scatter_add_(1, idx, prob)
+    return loss, lse, (c * (q - p)), c.abs() * (q + p)
+
+
+def _check(got_loss, got_dh, got_dw, h, w, idx, prob, ok, coef, T, reduction):
+    ds = _ds(h, w) / T
+    loss, lse, G, A = _formula(h, w, idx, prob, ok, coef, T)
+    n = max(1, int(ok.sum()))
+    ltol = T * T * (2 * ds + 8 * U * (lse.abs() + 16)) * ok
+    if reduction == "none":
+        assert ((got_loss.double() - loss).abs() <= ltol + U * loss.abs()).all()
+    else:
+        k = n if reduction == "mean" else 1
+        assert abs(got_loss.item() - (loss.sum() / k).item()) <= (ltol.sum() / k + 2 * U * loss.sum().abs() / k).item()
+    if got_dh is None:
+        return
+    hd, wd = h.double(), w.double()
+    dsr = (3 * ds + 8 * U * (lse.abs() + 4))[:, None]
+    for got, ref, gabs, aabs, depth in (
+            (got_dh, G @ wd, G.abs() @ wd.abs(), (dsr * A) @ wd.abs(), w.shape[0]),
+            (got_dw, G.T @ hd, G.abs().T @ hd.abs(), (dsr * A).T @ hd.abs(), h.shape[0])):
+        tol = (H8 + depth * 2.0 ** -23) * gabs + aabs
+        tol = tol + H8 * (ref.abs() + tol) + 1e-37
+        bad = (got.double() - ref).abs() > tol
+        assert not bad.any(), f"{int(bad.sum())} outside, worst {((got.double() - ref).abs() / tol).max():.3g} of the bound"
+
+
+def _xent(lh, h, w, target, reduction, dloss=None, ignore_index=-100):
+    h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = lh.linear_cross_entropy(h, w, target, ignore_index=ignore_index, reduction=reduction)
+    dh, dw = torch.autograd.grad(loss, (h, w), dloss)
+    return loss.detach(), dh, dw
+
+
+def _run_xent(lh, cuda, N, V, D, reduction, seed=0, ignore=0.0, scale=1.0):
+    g, h, w = _problem(N, V, D, seed, cuda, scale)
+    target = torch.randint(0, V, (N,), generator=g)
+    if ignore:
+        target[torch.rand(N, generator=g) < ignore] = -100
+    target = target.to(cuda)
+    ok = target != -100
+    dloss = torch.randn(N, generator=g).to(cuda) if reduction == "none" else torch.tensor(1.5, device=cuda)
+    loss, dh, dw = _xent(lh, h, w, target, reduction, dloss)
+    coef = dloss if reduction == "none" else dloss / (max(1, int(ok.sum())) if reduction == "mean" else 1)
+    coef = coef.expand(N)
+    _check(loss, dh, dw, h, w, target.clamp(min=0)[:, None], ok.double()[:, None], ok, coef, 1.0, reduction)
+    assert lh._native.device_status() == 0
+
+
+@pytest.mark.parametrize("N,V,D", [(1, 1, 8), (1, 256, 64), (2, 257, 72), (31, 255, 128), (128, 1000, 64),
+                                   (129, 300, 264), (255, 256, 256), (257, 511, 768), (300, 5003, 96),
+                                   (1000, 769, 136), (64, 2, 4096), (7, 20011, 1024)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_cross_entropy(lh, cuda, N, V, D, reduction):
+    _run_xent(lh, cuda, N, V, D, reduction, seed=N + V)
+
+
+@pytest.mark.parametrize("ignore", [0.3, 0.97])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_cross_entropy_with_ignored_positions(lh, cuda, ignore, reduction):
+    _run_xent(lh, cuda, 333, 1031, 160, reduction, seed=5, ignore=ignore)
+
+
+@pytest.mark.parametrize("N,V,D", [(20000, 256, 256), (3, 131072, 64), (70000, 17, 64)])
+def test_long_sums_are_split(lh, cuda, N, V, D):
+    """Few tiles and a long K: dW over 20000 positions, dH over 131072 columns."""
+    _run_xent(lh, cuda, N, V, D, "mean", seed=9)
+
+
+def test_several_pieces_of_the_vocabulary(lh, cuda):
+    """5000 x 120001: three pieces, the last one ragged; dH sums over all."""
+    _run_xent(lh, cuda, 5000, 120001, 64, "mean", seed=11)
+
+
+def test_peaked_and_large_logits(lh, cuda):
+    _run_xent(lh, cuda, 200, 700, 64, "mean", seed=12, scale=40.0)
+
+
+def test_every_position_ignored(lh, cuda):
+    _, h, w = _problem(70, 300, 64, 1, cuda)
+    target = torch.full((70,), -100, device=cuda)
+    for red in ("mean", "sum"):
+        loss, dh, dw = _xent(lh, h, w, target, red)
+        assert loss.item() == 0 and (dh == 0).all() and (dw == 0).all()
+    loss = lh.linear_cross_entropy(h, w, target, reduction="none")
+    assert (loss == 0).all()
+
+
+def test_ignored_positions_may_hold_anything(lh, cuda):
+    """A finite loss and finite dhidden whatever an ignored position's hidden row holds."""
+    g, h, w = _problem(40, 300, 64, 2, cuda)
+    target = torch.randint(0, 300, (40,), generator=g).to(cuda)
+    target[3] = target[17] = -100
+    h2 = h.clone()
+    h2[3], h2[17, 5] = float("nan"), float("inf")
+    a, b = _xent(lh, h, w, target, "mean"), _xent(lh, h2, w, target, "mean")
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert (b[1][3] == 0).all() and (b[1][17] == 0).all()
+
+
+def test_another_ignore_index_and_bad_targets(lh, cuda):
+    g, h, w = _problem(20, 300, 64, 3, cuda)
+    target = torch.randint(0, 300, (20,), generator=g).to(cuda)
+    target[4] = 7
+    loss = lh.linear_cross_entropy(h, w, target, ignore_index=7, reduction="none")
+    assert loss[4] == 0 and loss.isfinite().all()
+    for bad in (300, -1, -100, 1 << 40, -(1 << 40)):
+        t = target.clone()
+        t[9] = bad
+        loss = lh.linear_cross_entropy(h, w, t, ignore_index=7, reduction="none")
+        assert loss[9].isnan() and loss.isnan().sum() == 1
+        assert lh.linear_cross_entropy(h, w, t, ignore_index=7).isnan()
+    # a bad position without an upstream gradient spoils nothing
+    t[9] = 300
+    dl = torch.ones(20, device=cuda)
+    dl[9] = 0
+    _, dh, dw = _xent(lh, h, w, t, "none", dl, ignore_index=7)
+    assert dh.isfinite().all() and dw.isfinite().all() and (dh[9] == 0).all()
+
+
+def test_infinite_and_nan_logits(lh, cuda):
+    """As torch's cross entropy: -inf logits drop out, +inf and NaN give NaN."""
+    g, h, w = _problem(4, 600, 64, 4, cuda)
+    h = h.abs() + 0.1
+    target = torch.tensor([1, 2, 3, 4], device=cuda)
+    for v, want in ((-float("inf"), False), (float("inf"), True), (float("nan"), True)):
+        w2 = w.clone()
+        w2[500] = v
+        loss = lh.linear_cross_entropy(h, w2, target, reduction="none")
+        ref = torch.nn.functional.cross_entropy(h.double() @ w2.double().T, target, reduction="none")
+        assert bool(loss.isnan().all()) is want and bool(ref.isnan().all()) is want
+        if not want:
+            assert (loss.double() - ref).abs().max() <= 1e-5 * ref.max()
+
+
+# --------------------------------------------------------------------------- distillation
+def _teacher(g, N, V, K, where="spread"):
+    hi = V if where == "spread" else min(V, max(K, 200))
+    ti = torch.stack([torch.randperm(hi, generator=g)[:K] for _ in range(N)])
+    return torch.randn(N, K, generator=g) * 3, ti
+
+
+def _probs(tv, ti, T):
+    here = ti >= 0
+    ok = (here & (tv > -float("inf"))).any(-1)
+    x = (tv.double() / T).masked_fill(~here, -float("inf"))
+    p = torch.zeros_like(x)
+    p[ok] = torch.softmax(x[ok], -1)
+    return p, ok
+
+
+def _run_distill(lh, cuda, N, V, D, K, T, reduction, seed=0, empty=0.0, where="spread", tdt=torch.float32,
+                 idt=torch.int64, edit=None):
+    g, h, w = _problem(N, V, D, seed, cuda)
+    tv, ti = _teacher(g, N, V, K, where)
+    if empty:
+        ti[torch.rand(N, generator=g) < empty] = -1
+    if edit:
+        edit(tv, ti)
+    tv, ti = tv.to(tdt).to(cuda), ti.to(cuda)
+    p, ok = _probs(tv, ti, T)
+    h1, w1 = h.requires_grad_(True), w.requires_grad_(True)
+    loss = lh.linear_distillation(h1, w1, tv, ti.to(idt), temperature=T, reduction=reduction)
+    dloss = torch.randn(N, generator=g).to(cuda) if reduction == "none" else torch.tensor(0.7, device=cuda)
+    dh, dw = torch.autograd.grad(loss, (h1, w1), dloss)
+    coef = dloss if reduction == "none" else dloss / (max(1, int(ok.sum())) if reduction == "mean" else 1)
+    # the probabilities carry fp32 roundings of a softmax over K: inside the logits' bound
+    with torch.no_grad():
+        _check(loss.detach(), dh, dw, h, w, ti.clamp(min=0), p, ok, coef.expand(N), T, reduction)
+    assert lh._native.device_status() == 0
+    return loss.detach(), dh, dw
+
+
+@pytest.mark.parametrize("N,V,D,K,T", [(1, 1, 8, 1, 1.0), (2, 300, 64, 5, 1.0), (33, 256, 128, 16, 2.0),
+                                       (130, 1000, 72, 64, 1.5), (257, 5003, 96, 13, 4.0), (20, 700, 64, 256, 2.0),
+                                       (500, 257, 64, 3, 0.5), (6, 20011, 1024, 128, 1.0)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_distillation(lh, cuda, N, V, D, K, T, reduction):
+    _run_distill(lh, cuda, N, V, D, K, T, reduction, seed=N + K)
+
+
+@pytest.mark.parametrize("where", ["spread", "front"])
+def test_distillation_types_empty_rows_and_crowded_tiles(lh, cuda, where):
+    _run_distill(lh, cuda, 150, 3000, 64, 100, 2.0, "mean", seed=21, empty=0.3, where=where, tdt=BF, idt=torch.int32)
+    _run_distill(lh, cuda, 150, 3000, 64, 100, 2.0, "sum", seed=22, empty=0.9, where=where)
+
+
+def test_distillation_absent_entries_and_minus_infinity(lh, cuda):
+    def edit(tv, ti):
+        ti[0, ::2] = -1
+        ti[1, 1:] = -5
+        tv[2, 3] = -float("inf")
+        tv[3, :] = -float("inf")                     # an empty row, by its logits
+        tv[4, 0] = 1e4                               # one entry takes all
+    loss, dh, _ = _run_distill(lh, cuda, 10, 700, 64, 7, 1.0, "none", seed=23, edit=edit)
+    assert loss[3] == 0 and (dh[3] == 0).all()
+
+
+def test_distillation_same_index_twice(lh, cuda):
+    def edit(tv, ti):
+        ti[0, :] = ti[0, 0]
+        ti[1, 3] = ti[1, 0]
+        ti[2, 5] = ti[2, 6]
+    _run_distill(lh, cuda, 9, 700, 64, 7, 2.0, "mean", seed=24, edit=edit)
+
+
+def test_distillation_bad_teachers(lh, cuda):
+    g, h, w = _problem(6, 300, 64, 25, cuda)
+    tv, ti = (t.to(cuda) for t in _teacher(g, 6, 300, 4))
+    tv[1, 2], tv[3, 0] = float("nan"), float("inf")
+    ti[4, 1] = 300
+    loss = lh.linear_distillation(h, w, tv, ti, reduction="none")
+    assert loss.isnan().tolist() == [False, True, False, True, True, False]
+
+
+def test_distillation_from_one_certain_entry_is_cross_entropy(lh, cuda):
+    g, h, w = _problem(100, 900, 128, 26, cuda)
+    t = torch.randint(0, 900, (100,), generator=g).to(cuda)
+    a = _xent(lh, h, w, t, "mean")
+    h1, w1 = h.requires_grad_(True), w.requires_grad_(True)
+    loss = lh.linear_distillation(h1, w1, torch.zeros(100, 1, device=cuda), t[:, None])
+    b = torch.autograd.grad(loss, (h1, w1))
+    assert abs(loss.item() - a[0].item()) <= 4 * U * (abs(a[0].item()) + 10)
+    assert torch.equal(a[1], b[0]) and torch.equal(a[2], b[1])
+
+
+# --------------------------------------------------------------------------- both
+def test_gradients_against_differences(lh, cuda):
+    """Central differences of the 64-bit formulas at a few coordinates; G's bf16 bounds the gradients."""
+    g, h, w = _problem(5, 40, 64, 30, cuda)
+    tv, ti = (t.to(cuda) for t in _teacher(g, 5, 40, 4))
+    t = torch.randint(0, 40, (5,), generator=g).to(cuda)
+    p, ok = _probs(tv, ti, 2.0)
+
+    def xent(hh, ww):
+        return torch.nn.functional.cross_entropy(hh @ ww.T, t)
+
+    def dist(hh, ww):
+        lq = torch.log_softmax(hh @ ww.T / 2.0, -1).gather(1, ti)
+        return 4 * (p * (p.log() - lq)).sum(-1).mean()
+
+    h1, w1 = h.requires_grad_(True), w.requires_grad_(True)
+    for own, f in ((lambda: lh.linear_cross_entropy(h1, w1, t), xent),
+                   (lambda: lh.linear_distillation(h1, w1, tv, ti, temperature=2.0), dist)):
+        grads = torch.autograd.grad(own(), (h1, w1))
+        vals = [h.detach().double(), w.detach().double()]
+        for k in range(2):
+            scale = grads[k].float().abs().max().item()
+            for pos in (0, 77, 319):
+                d = torch.zeros_like(vals[k])
+                d.view(-1)[pos] = 1e-5
+                up, dn = list(vals), list(vals)
+                up[k], dn[k] = vals[k] + d, vals[k] - d
+                diff = (f(*up) - f(*dn)).item() / 2e-5
+                assert abs(diff - grads[k].view(-1)[pos].item()) <= 2 * H8 * scale + H8 * abs(diff) + 1e-6
+
+
+def test_no_positions(lh, cuda):
+    h = torch.zeros(0, 64, dtype=BF, device=cuda, requires_grad=True)
+    w = torch.randn(50, 64, device=cuda).to(BF).requires_grad_(True)
+    t = torch.zeros(0, dtype=torch.int64, device=cuda)
+    for red in ("mean", "sum"):
+        loss = lh.linear_cross_entropy(h, w, t, reduction=red)
+        dh, dw = torch.autograd.grad(loss, (h, w))
+        assert loss.item() == 0 and dh.shape == (0, 64) and (dw == 0).all()
+    assert lh.linear_cross_entropy(h, w, t, reduction="none").shape == (0,)
+    assert lh.linear_distillation(h, w, torch.zeros(0, 3, device=cuda), torch.zeros(0, 3, dtype=torch.int64,
+                                                                                   device=cuda)).item() == 0
+
+
+def test_strides_alignment_and_leading_dimensions(lh, cuda):
+    g = torch.Generator().manual_seed(31)
+    big = torch.randn(4, 6, 128, generator=g).to(BF).to(cuda)
+    h = big[:, ::2, 64:]
+    flat = torch.randn(300 * 64 + 1, generator=g).to(BF).to(cuda)
+    w = flat[1:].view(300, 64)
+    t = torch.randint(0, 300, (3, 4), generator=g).to(cuda).T           # (4, 3), strided
+    a = lh.linear_cross_entropy(h, w, t, reduction="none")
+    b = lh.linear_cross_entropy(h.reshape(12, 64).clone(), w.clone(), t.reshape(12).to(torch.int32), reduction="none")
+    assert a.shape == (4, 3) and torch.equal(a.reshape(12), b)
+    wt = torch.randn(64, 300, generator=g).to(BF).to(cuda).T             # column-major weights
+    assert torch.equal(lh.linear_cross_entropy(h, wt, t), lh.linear_cross_entropy(h, wt.contiguous(), t))
+
+
+def test_same_results_every_time_on_a_stream_and_in_a_graph(lh, cuda):
+    g, h, w = _problem(600, 3001, 256, 32, cuda)
+    t = torch.randint(0, 3001, (600,), generator=g).to(cuda)
+    tv, ti = (x.to(cuda) for x in _teacher(g, 600, 3001, 20))
+
+    def both():
+        h1, w1 = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        a = lh.linear_cross_entropy(h1, w1, t)
+        out = [a.detach(), *torch.autograd.grad(a, (h1, w1))]
+        b = lh.linear_distillation(h1, w1, tv, ti, temperature=2.0)
+        return out + [b.detach(), *torch.autograd.grad(b, (h1, w1))]
+
+    want = [x.clone() for x in both()]
+    assert all(torch.equal(a, b) for a, b in zip(want, both()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = both()
+    here = both()                                      # the same calls on two streams at once
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and all(torch.equal(a, b) for a, b in zip(want, here))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    h.copy_(torch.randn_like(h))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(both(), out)) and not torch.equal(want[0], out[0])
+    assert lh._native.device_status() == 0
+
+
+def test_opcheck(lh, cuda):
+    ops = torch.ops.lighthouse_b200
+    utils = ("test_schema", "test_faketensor")
+    g, h, w = _problem(40, 300, 64, 33, cuda)
+    t = torch.randint(0, 300, (40,), generator=g).to(cuda)
+    tv, ti = (x.to(cuda) for x in _teacher(g, 40, 300, 5))
+    for red in ("mean", "none"):
+        torch.library.opcheck(ops.linear_xent, (h, w, t, -100, red), test_utils=utils)
+        loss, *kept = ops.linear_xent(h, w, t, -100, red)
+        torch.library.opcheck(ops.linear_xent_bwd, (h, w, t, *kept, torch.ones_like(loss), red), test_utils=utils)
+        torch.library.opcheck(ops.linear_distill, (h, w, tv, ti, 2.0, red), test_utils=utils)
+        loss, *kept = ops.linear_distill(h, w, tv, ti, 2.0, red)
+        torch.library.opcheck(ops.linear_distill_bwd, (h, w, *kept, torch.ones_like(loss), 2.0, red), test_utils=utils)

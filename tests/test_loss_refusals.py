@@ -1,0 +1,101 @@
+"""What the losses of an output projection refuse, on the host: nothing is launched."""
+import ctypes
+
+import pytest
+import torch
+
+BF = torch.bfloat16
+
+
+def _z(*shape, dtype=BF):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def test_shapes_types_and_options_are_refused(lh):
+    E = lh._native.LighthouseShapeError
+    n = lh._native
+    t = _z(4, dtype=torch.int64)
+    with pytest.raises(E, match="agree"):
+        n.linear_xent_fwd(_z(4, 64), _z(10, 72), t, -100, "mean")
+    with pytest.raises(E, match="multiple of 8"):
+        n.linear_xent_fwd(_z(4, 60), _z(10, 60), t, -100, "mean")
+    with pytest.raises(E, match="V in"):
+        n.linear_xent_fwd(_z(4, 64), _z(0, 64), t, -100, "mean")
+    with pytest.raises(ValueError, match="bf16"):
+        n.linear_xent_fwd(_z(4, 64, dtype=torch.float32), _z(10, 64), t, -100, "mean")
+    with pytest.raises(ValueError, match="reduction"):
+        n.linear_xent_fwd(_z(4, 64), _z(10, 64), t, -100, "median")
+    with pytest.raises(E, match="target"):
+        n.linear_xent_fwd(_z(4, 64), _z(10, 64), t[:3], -100, "mean")
+    with pytest.raises(ValueError, match="leading"):
+        lh.linear_cross_entropy(_z(2, 2, 64), _z(10, 64), t)
+    with pytest.raises(ValueError, match="CUDA"):
+        lh.linear_cross_entropy(_z(4, 64), _z(10, 64), t)
+    tv, ti = _z(4, 3, dtype=torch.float32), _z(4, 3, dtype=torch.int64)
+    with pytest.raises(E, match="K must"):
+        n.linear_distill_fwd(_z(4, 64), _z(10, 64), _z(4, 257), _z(4, 257, dtype=torch.int64), 1.0, "mean")
+    with pytest.raises(E, match="K must"):
+        lh.linear_distillation(_z(4, 64), _z(10, 64), _z(4, 0), _z(4, 0, dtype=torch.int64))
+    with pytest.raises(E, match=r"\(N, K\)"):
+        n.linear_distill_fwd(_z(4, 64), _z(10, 64), tv, ti[:, :2], 1.0, "mean")
+    for T in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            n.linear_distill_fwd(_z(4, 64), _z(10, 64), tv, ti, T, "mean")
+    with pytest.raises(ValueError, match="teacher logits"):
+        n.linear_distill_fwd(_z(4, 64), _z(10, 64), tv.half(), ti, 1.0, "mean")
+    with pytest.raises(ValueError, match="CUDA"):
+        lh.linear_distillation(_z(4, 64), _z(10, 64), tv, ti)
+
+
+def test_c_entry_points_check_before_they_touch_a_device(lh):
+    lib = lh._native.load()
+    P = ctypes.c_void_p
+    a = P(4096)                  # aligned and never read: every call below is refused on the host
+    big = 1 << 40
+
+    def xf(h=a, w=a, t=a, N=4, V=10, D=64, red=1, loss=a, inv=a, ws=a, n=big):
+        return lib.lh_linear_xent_fwd(h, w, t, -100, N, V, D, red, loss, a, a, a, inv, ws, n, None)
+
+    assert xf(h=None) == 2 and xf(t=None) == 2 and xf(loss=None) == 2 and xf(inv=None) == 2 and xf(ws=None) == 2
+    assert xf(N=0) == 1 and xf(V=0) == 1 and xf(D=12) == 1 and xf(N=(1 << 24) + 1) == 1 and xf(V=(1 << 22) + 1) == 1
+    assert xf(red=3) == 2 and xf(w=P(4104)) == 2 and xf(ws=P(4096 + 16)) == 2
+    assert xf(n=lib.lh_linear_loss_workspace_size(4, 10, 64, 0) - 1) == 5
+
+    def xb(gout=a, gs=0, dw=a, n=big):
+        return lib.lh_linear_xent_bwd(a, a, a, 4, 10, 64, a, a, a, a, gout, gs, a, dw, a, n, None)
+
+    assert xb(gout=None) == 2 and xb(gs=2) == 2 and xb(dw=P(4100)) == 2
+    assert xb(n=lib.lh_linear_loss_workspace_size(4, 10, 64, 1) - 1) == 5
+
+    def df(K=3, T=1.0, tv=a, dt=1):
+        return lib.lh_linear_distill_fwd(a, a, tv, dt, a, 4, 10, 64, K, T, 1, a, a, a, a, a, a, a, a, big, None)
+
+    assert df(K=0) == 1 and df(K=257) == 1 and df(T=0.0) == 2 and df(tv=None) == 2 and df(dt=2) == 2
+
+    def db(idx=a, gs=0):
+        return lib.lh_linear_distill_bwd(a, a, 4, 10, 64, 3, 1.0, a, idx, a, a, a, a, a, gs, a, a, a, big, None)
+
+    assert db(idx=None) == 2 and db(gs=3) == 2
+
+
+def test_workspace_stays_small(lh):
+    """The backward's workspace does not grow with the vocabulary: at most one 512 MB piece plus
+    fp32 sums of the size of the gradients."""
+    size = lh._native.load().lh_linear_loss_workspace_size
+    for N in (1, 17, 1024, 8192, 65536):
+        for V in (1, 256, 32000, 131072, 1 << 20):
+            for D in (64, 1024, 4096):
+                piece = max(512 << 20, 2 * N * 256)
+                planes = 74 * 4 * 256 * D * 8 + 4 * N * D      # parts only where few tiles are
+                assert 0 < size(N, V, D, 1) <= piece + planes + 4096, (N, V, D)
+                assert size(N, V, D, 0) <= 8 * N * (V // 256 + 1) + 16 * (N // 32 + 1) + 4 * N + 1024
+
+
+def test_fake_kernels(lh):
+    m = lambda *s, d=BF: torch.empty(*s, dtype=d, device="meta", requires_grad=d.is_floating_point)
+    h, w = m(2, 3, 64), m(100, 64)
+    assert lh.linear_cross_entropy(h, w, m(2, 3, d=torch.int64), reduction="none").shape == (2, 3)
+    loss = lh.linear_distillation(h, w, m(2, 3, 5, d=torch.float32), m(2, 3, 5, d=torch.int32), temperature=2.0)
+    assert loss.shape == () and loss.dtype == torch.float32
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    assert dh.shape == h.shape and dw.shape == w.shape and dh.dtype == dw.dtype == BF
