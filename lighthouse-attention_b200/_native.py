@@ -329,31 +329,49 @@ def simple_gla_fwd(q, k, v, g, scale: float, q2=None, k2=None):
 
 
 # --------------------------------------------------------------------------- norm
-def _on_one_device(what: str, *ts) -> torch.device:
+def _on_one_device(what: str, first, *rest) -> torch.device:
     """All tensors are CUDA tensors of one device, which is returned."""
-    _require_cuda(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) != 1:
-        raise ValueError(f"{what}: tensors on different devices: {sorted(map(str, devs))}")
-    return devs.pop()
+    dev = first.device
+    for t in (first, *rest):
+        if t is not None:
+            if not t.is_cuda:
+                raise ValueError("lighthouse_b200 ops take CUDA tensors (no CPU path)")
+            if t.device != dev:
+                raise ValueError(f"{what}: tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
+def _call(dev: torch.device, name: str, *args) -> None:
+    """Entry point `name` with the device's current stream as its last argument,
+    the device being current meanwhile."""
+    fn = getattr(load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        _check(rc)
 
 
 def _dense16(t):
     """t as a contiguous tensor whose first element is 16-byte aligned."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _norm_check(what, x, residual, weight):
-    if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1] or (
-            residual is not None and residual.shape != x.shape):
+    D = x.shape[-1] if x.dim() else 0
+    if weight.shape != (D,) or (residual is not None and residual.shape != x.shape):
         raise LighthouseShapeError(f"{what}: x and residual (..., D) and weight (D) must agree")
     for t in (x, residual, weight):
         if t is not None and t.dtype not in LH_DTYPE:
             raise ValueError(f"{what}: bf16 and fp32 tensors only, got {t.dtype}")
-    D = x.shape[-1]
     if D % 8 or not 8 <= D <= 16384:
         raise LighthouseShapeError(f"{what}: D must be a multiple of 8 and at most 16384, got {D}")
+    return x.numel() // D, D
 
 
 def rms_norm_fwd(x, residual, weight, eps: float, out_dtype, group: int = 0, with_rstd: bool = True):
@@ -362,39 +380,38 @@ def rms_norm_fwd(x, residual, weight, eps: float, out_dtype, group: int = 0, wit
     out_dtype torch.float8_e4m3fn gives y in 8 bits and scale (..., 1), or
     (..., ceil(D / 128)) with group 128; scale is None otherwise.  h is None
     without a residual, rstd (rows) fp32 is None unless asked for."""
-    _norm_check("rms_norm", x, residual, weight)
+    N, D = _norm_check("rms_norm", x, residual, weight)
     fp8 = out_dtype == torch.float8_e4m3fn
     if not fp8 and out_dtype not in LH_DTYPE:
         raise ValueError(f"rms_norm: out_dtype must be bf16, fp32 or float8_e4m3fn, got {out_dtype}")
     if group not in ((0, 128) if fp8 else (0,)):
         raise ValueError("rms_norm: scales per row (group 0) or per 128 columns (group 128)")
     dev = _on_one_device("rms_norm", x, residual, weight)
-    D = x.shape[-1]
-    N = x.numel() // D
     y = torch.empty(x.shape, dtype=out_dtype, device=dev)
-    n_groups = (D + 127) // 128 if group else 1
-    scale = torch.empty(*x.shape[:-1], n_groups, dtype=torch.float32, device=dev) if fp8 else None
-    h = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=dev)
-    rstd = torch.empty(N, dtype=torch.float32, device=dev) if with_rstd else None
+    scale = h = rstd = None
+    if fp8:
+        scale = torch.empty(*x.shape[:-1], (D + 127) // 128 if group else 1, dtype=torch.float32, device=dev)
+    if residual is not None:
+        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+    if with_rstd:
+        rstd = torch.empty(N, dtype=torch.float32, device=dev)
     if N:
-        with torch.cuda.device(dev):
-            x, weight = _dense16(x), _dense16(weight)
-            residual = None if residual is None else _dense16(residual)
-            _check(load().lh_rms_norm_fwd(_ptr(x), LH_DTYPE[x.dtype], _ptr(residual),
-                                          0 if residual is None else LH_DTYPE[residual.dtype], _ptr(weight),
-                                          LH_DTYPE[weight.dtype], N, D, eps, _ptr(y), 2 if fp8 else LH_DTYPE[out_dtype],
-                                          _ptr(scale), group, _ptr(h), _ptr(rstd), _stream()))
+        x, weight = _dense16(x), _dense16(weight)
+        r_dtype = 0
+        if residual is not None:
+            residual, r_dtype = _dense16(residual), LH_DTYPE[residual.dtype]
+        _call(dev, "lh_rms_norm_fwd", x.data_ptr(), LH_DTYPE[x.dtype], _ptr(residual), r_dtype, weight.data_ptr(),
+              LH_DTYPE[weight.dtype], N, D, eps, y.data_ptr(), 2 if fp8 else LH_DTYPE[out_dtype], _ptr(scale), group,
+              _ptr(h), _ptr(rstd))
     return y, scale, h, rstd
 
 
 def rms_norm_bwd(dy, dh, h, weight, rstd, dx_dtype, with_dres: bool):
     """Backward of rms_norm_fwd: (dx, dres, dw); dh may be None, dres is None unless asked for."""
-    _norm_check("rms_norm_bwd", h, dy, weight)
+    N, D = _norm_check("rms_norm_bwd", h, dy, weight)
     if dx_dtype not in LH_DTYPE or (dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype)):
         raise LighthouseShapeError("rms_norm_bwd: dh must have the shape and type of h")
-    dev = _on_one_device("rms_norm_bwd", dy, dh, h, weight, rstd)
-    D = h.shape[-1]
-    N = h.numel() // D
+    dev = _on_one_device("rms_norm_bwd", h, dy, dh, weight, rstd)
     if rstd.dtype != torch.float32 or rstd.numel() != N:
         raise LighthouseShapeError("rms_norm_bwd: rstd must be fp32, one per row")
     dx = torch.empty(h.shape, dtype=dx_dtype, device=dev)
@@ -402,19 +419,18 @@ def rms_norm_bwd(dy, dh, h, weight, rstd, dx_dtype, with_dres: bool):
     if not N:
         return dx, dres, torch.zeros_like(weight)
     dw = torch.empty(D, dtype=weight.dtype, device=dev)
-    with torch.cuda.device(dev):
-        dy, h, weight, rstd = _dense16(dy), _dense16(h), _dense16(weight), rstd.contiguous()
-        dh = None if dh is None else _dense16(dh)
-        ws_bytes = int(load().lh_rms_norm_bwd_workspace_size(N, D))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        _check(load().lh_rms_norm_bwd(_ptr(dy), LH_DTYPE[dy.dtype], _ptr(dh), _ptr(h), LH_DTYPE[h.dtype], _ptr(weight),
-                                      LH_DTYPE[weight.dtype], _ptr(rstd), N, D, _ptr(dx), LH_DTYPE[dx_dtype], _ptr(dres),
-                                      _ptr(dw), _ptr(ws), ws_bytes, _stream()))
+    dy, h, weight, rstd = _dense16(dy), _dense16(h), _dense16(weight), rstd.contiguous()
+    dh = None if dh is None else _dense16(dh)
+    ws_bytes = load().lh_rms_norm_bwd_workspace_size(N, D)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call(dev, "lh_rms_norm_bwd", dy.data_ptr(), LH_DTYPE[dy.dtype], _ptr(dh), h.data_ptr(), LH_DTYPE[h.dtype],
+          weight.data_ptr(), LH_DTYPE[weight.dtype], rstd.data_ptr(), N, D, dx.data_ptr(), LH_DTYPE[dx_dtype], _ptr(dres),
+          dw.data_ptr(), ws.data_ptr(), ws_bytes)
     return dx, dres, dw
 
 
 # --------------------------------------------------------------------------- losses of an output projection
-def _loss_check(what, hidden, weight, reduction=None):
+def _loss_check(what, hidden, weight, reduction):
     if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise LighthouseShapeError(f"{what}: hidden (N, D) and weight (V, D) must agree")
     if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
@@ -424,72 +440,84 @@ def _loss_check(what, hidden, weight, reduction=None):
     if D % 8 or not 8 <= D <= 65536 or not 1 <= V <= 1 << 22 or N > 1 << 24:
         raise LighthouseShapeError(f"{what}: D must be a multiple of 8 and at most 65536, V in [1, 2^22], N at most "
                                    f"2^24; got D {D}, V {V}, N {N}")
-    if reduction is not None and reduction not in REDUCTIONS:
+    if reduction not in REDUCTIONS:
         raise ValueError(f"{what}: reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
     return N, V, D
 
 
-def _loss_outputs(N, reduction, dev):
-    f = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)
-    if reduction == "none":
-        return f(N), f(N), f(N), f(0)
-    if N == 0:                                       # nothing counts: the loss is 0
-        return f().zero_(), f(0), f(0), f(1).zero_()
-    return f(), f(N), f(N), f(1)
+def _loss_out(N, reduction, dev):
+    """The loss's tensor; a reduced loss over no positions is 0."""
+    loss = torch.empty((N,) if reduction == "none" else (), dtype=torch.float32, device=dev)
+    return loss if N else loss.zero_()
 
 
 def _loss_ws(N, V, D, backward, dev):
-    n = int(load().lh_linear_loss_workspace_size(N, V, D, backward))
+    n = load().lh_linear_loss_workspace_size(N, V, D, backward)
     return torch.empty(n, dtype=torch.uint8, device=dev), n
+
+
+def kept_len(N: int, K: int) -> int:
+    """fp32 values that a loss's forward keeps for its backward: lse2 (N), row_scale (N), inv_count (1),
+    the targets' logits (N K) and, for distillation (K > 0), their probabilities (N K)."""
+    return 2 * N + 1 + (2 * N * K if K else N)
+
+
+def _kept_ptrs(kept, N, K):
+    """Addresses of lse2, row_scale, inv_count, tlogit, prob inside kept."""
+    p = kept.data_ptr()
+    t = p + 4 * (2 * N + 1)
+    return p, p + 4 * N, p + 8 * N, t, t + 4 * N * K
 
 
 def linear_xent_fwd(hidden, weight, target, ignore_index: int, reduction: str):
     """Softmax cross entropy of hidden (N, D) @ weight (V, D)^T against target (N) int64 ->
-    (loss, lse2, tlogit, row_scale, inv_count); the last four are the backward's."""
+    (loss, kept); kept is the backward's."""
     N, V, D = _loss_check("linear_xent", hidden, weight, reduction)
     if target.shape != (N,) or target.dtype != torch.int64:
         raise LighthouseShapeError("linear_xent: target must be (N) int64")
     dev = _on_one_device("linear_xent", hidden, weight, target)
-    loss, lse2, row_scale, inv_count = _loss_outputs(N, reduction, dev)
-    tlogit = torch.empty(N, dtype=torch.float32, device=dev)
+    loss = _loss_out(N, reduction, dev)
+    kept = torch.empty(kept_len(N, 0), dtype=torch.float32, device=dev)
     if N:
-        with torch.cuda.device(dev):
-            hidden, weight, target = _dense16(hidden), _dense16(weight), target.contiguous()
-            ws, n = _loss_ws(N, V, D, 0, dev)
-            _check(load().lh_linear_xent_fwd(_ptr(hidden), _ptr(weight), _ptr(target), ignore_index, N, V, D,
-                                             REDUCTIONS[reduction], _ptr(loss), _ptr(lse2), _ptr(tlogit),
-                                             _ptr(row_scale), _ptr(inv_count), _ptr(ws), n, _stream()))
-    return loss, lse2, tlogit, row_scale, inv_count
+        hidden, weight, target = _dense16(hidden), _dense16(weight), target.contiguous()
+        ws, n = _loss_ws(N, V, D, 0, dev)
+        lse2, row_scale, inv_count, tlogit, _ = _kept_ptrs(kept, N, 0)
+        _call(dev, "lh_linear_xent_fwd", hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), ignore_index, N, V, D,
+              REDUCTIONS[reduction], loss.data_ptr(), lse2, tlogit, row_scale, inv_count, ws.data_ptr(), n)
+    return loss, kept
 
 
-def _gout_check(what, gout, N, reduced, dev_tensors):
-    if gout.dtype != torch.float32 or gout.numel() != (1 if reduced else N):
+def _loss_bwd_outputs(what, hidden, weight, kept, gout, reduction, K, *rest):
+    N, V, D = _loss_check(what, hidden, weight, reduction)
+    if gout.dtype != torch.float32 or gout.numel() != (N if reduction == "none" else 1):
         raise LighthouseShapeError(f"{what}: the loss's gradient must be fp32, one value (reduced) or N")
-    return _on_one_device(what, gout, *dev_tensors)
-
-
-def linear_xent_bwd(hidden, weight, target, lse2, tlogit, row_scale, inv_count, gout, reduction: str):
-    """Gradients (dhidden, dweight) of linear_xent_fwd."""
-    N, V, D = _loss_check("linear_xent_bwd", hidden, weight, reduction)
-    dev = _gout_check("linear_xent_bwd", gout, N, reduction != "none",
-                      (hidden, weight, target, lse2, tlogit, row_scale, inv_count))
+    if kept.dtype != torch.float32 or kept.shape != (kept_len(N, K),) or not kept.is_contiguous():
+        raise LighthouseShapeError(f"{what}: kept must be the forward's")
+    dev = _on_one_device(what, hidden, weight, kept, gout, *rest)
     dh = torch.empty(N, D, dtype=torch.bfloat16, device=dev)
-    if not N:
-        return dh, torch.zeros(V, D, dtype=torch.bfloat16, device=dev)
-    dw = torch.empty(V, D, dtype=torch.bfloat16, device=dev)
-    reduced = reduction != "none"
-    with torch.cuda.device(dev):
+    dw = (torch.empty if N else torch.zeros)(V, D, dtype=torch.bfloat16, device=dev)
+    return N, V, D, dev, dh, dw
+
+
+def linear_xent_bwd(hidden, weight, target, kept, gout, reduction: str):
+    """Gradients (dhidden, dweight) of linear_xent_fwd."""
+    N, V, D, dev, dh, dw = _loss_bwd_outputs("linear_xent_bwd", hidden, weight, kept, gout, reduction, 0, target)
+    if target.shape != (N,) or target.dtype != torch.int64:
+        raise LighthouseShapeError("linear_xent_bwd: target must be (N) int64")
+    if N:
+        reduced = reduction != "none"
         hidden, weight, target, gout = _dense16(hidden), _dense16(weight), target.contiguous(), gout.contiguous()
         ws, n = _loss_ws(N, V, D, 1, dev)
-        _check(load().lh_linear_xent_bwd(_ptr(hidden), _ptr(weight), _ptr(target), N, V, D, _ptr(lse2), _ptr(tlogit),
-                                         _ptr(row_scale), _ptr(inv_count) if reduced else None, _ptr(gout),
-                                         0 if reduced else 1, _ptr(dh), _ptr(dw), _ptr(ws), n, _stream()))
+        lse2, row_scale, inv_count, tlogit, _ = _kept_ptrs(kept, N, 0)
+        _call(dev, "lh_linear_xent_bwd", hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), N, V, D, lse2, tlogit,
+              row_scale, inv_count if reduced else None, gout.data_ptr(), 0 if reduced else 1, dh.data_ptr(),
+              dw.data_ptr(), ws.data_ptr(), n)
     return dh, dw
 
 
 def linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperature: float, reduction: str):
     """Distillation of hidden (N, D) @ weight (V, D)^T from a teacher's K logits (N, K) bf16 / fp32 at
-    indices (N, K) int64 -> (loss, lse2, idx, prob, tlogit, row_scale, inv_count)."""
+    indices (N, K) int64 -> (loss, kept, idx); kept and idx (N, K) int32 are the backward's."""
     N, V, D = _loss_check("linear_distill", hidden, weight, reduction)
     if teacher_logits.dim() != 2 or teacher_logits.shape[0] != N or teacher_indices.shape != teacher_logits.shape:
         raise LighthouseShapeError("linear_distill: teacher logits and indices must be (N, K)")
@@ -501,38 +529,32 @@ def linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperat
     if not 0 < temperature < 1e30:
         raise ValueError(f"linear_distill: temperature must be positive and finite, got {temperature}")
     dev = _on_one_device("linear_distill", hidden, weight, teacher_logits, teacher_indices)
-    loss, lse2, row_scale, inv_count = _loss_outputs(N, reduction, dev)
+    loss = _loss_out(N, reduction, dev)
+    kept = torch.empty(kept_len(N, K), dtype=torch.float32, device=dev)
     idx = torch.empty(N, K, dtype=torch.int32, device=dev)
-    prob, tlogit = (torch.empty(N, K, dtype=torch.float32, device=dev) for _ in range(2))
     if N:
-        with torch.cuda.device(dev):
-            hidden, weight = _dense16(hidden), _dense16(weight)
-            teacher_logits, teacher_indices = teacher_logits.contiguous(), teacher_indices.contiguous()
-            ws, n = _loss_ws(N, V, D, 0, dev)
-            _check(load().lh_linear_distill_fwd(_ptr(hidden), _ptr(weight), _ptr(teacher_logits),
-                                                LH_DTYPE[teacher_logits.dtype], _ptr(teacher_indices), N, V, D, K,
-                                                temperature, REDUCTIONS[reduction], _ptr(loss), _ptr(lse2), _ptr(idx),
-                                                _ptr(prob), _ptr(tlogit), _ptr(row_scale), _ptr(inv_count), _ptr(ws), n,
-                                                _stream()))
-    return loss, lse2, idx, prob, tlogit, row_scale, inv_count
+        hidden, weight = _dense16(hidden), _dense16(weight)
+        teacher_logits, teacher_indices = teacher_logits.contiguous(), teacher_indices.contiguous()
+        ws, n = _loss_ws(N, V, D, 0, dev)
+        lse2, row_scale, inv_count, tlogit, prob = _kept_ptrs(kept, N, K)
+        _call(dev, "lh_linear_distill_fwd", hidden.data_ptr(), weight.data_ptr(), teacher_logits.data_ptr(),
+              LH_DTYPE[teacher_logits.dtype], teacher_indices.data_ptr(), N, V, D, K, temperature, REDUCTIONS[reduction],
+              loss.data_ptr(), lse2, idx.data_ptr(), prob, tlogit, row_scale, inv_count, ws.data_ptr(), n)
+    return loss, kept, idx
 
 
-def linear_distill_bwd(hidden, weight, lse2, idx, prob, tlogit, row_scale, inv_count, gout, temperature: float,
-                       reduction: str):
+def linear_distill_bwd(hidden, weight, kept, idx, gout, temperature: float, reduction: str):
     """Gradients (dhidden, dweight) of linear_distill_fwd."""
-    N, V, D = _loss_check("linear_distill_bwd", hidden, weight, reduction)
-    dev = _gout_check("linear_distill_bwd", gout, N, reduction != "none",
-                      (hidden, weight, lse2, idx, prob, tlogit, row_scale, inv_count))
-    dh = torch.empty(N, D, dtype=torch.bfloat16, device=dev)
-    if not N:
-        return dh, torch.zeros(V, D, dtype=torch.bfloat16, device=dev)
-    dw = torch.empty(V, D, dtype=torch.bfloat16, device=dev)
-    reduced = reduction != "none"
-    with torch.cuda.device(dev):
+    K = idx.shape[-1]
+    N, V, D, dev, dh, dw = _loss_bwd_outputs("linear_distill_bwd", hidden, weight, kept, gout, reduction, K, idx)
+    if idx.shape != (N, K) or idx.dtype != torch.int32 or not idx.is_contiguous():
+        raise LighthouseShapeError("linear_distill_bwd: idx must be the forward's")
+    if N:
+        reduced = reduction != "none"
         hidden, weight, gout = _dense16(hidden), _dense16(weight), gout.contiguous()
         ws, n = _loss_ws(N, V, D, 1, dev)
-        _check(load().lh_linear_distill_bwd(_ptr(hidden), _ptr(weight), N, V, D, idx.shape[1], temperature, _ptr(lse2),
-                                            _ptr(idx), _ptr(prob), _ptr(tlogit), _ptr(row_scale),
-                                            _ptr(inv_count) if reduced else None, _ptr(gout), 0 if reduced else 1,
-                                            _ptr(dh), _ptr(dw), _ptr(ws), n, _stream()))
+        lse2, row_scale, inv_count, tlogit, prob = _kept_ptrs(kept, N, K)
+        _call(dev, "lh_linear_distill_bwd", hidden.data_ptr(), weight.data_ptr(), N, V, D, K, temperature, lse2,
+              idx.data_ptr(), prob, tlogit, row_scale, inv_count if reduced else None, gout.data_ptr(),
+              0 if reduced else 1, dh.data_ptr(), dw.data_ptr(), ws.data_ptr(), n)
     return dh, dw

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 from . import _native
 
@@ -280,66 +281,69 @@ def _(x, residual, weight, eps, group):
 
 
 # --------------------------------------------------------------------------- losses of an output projection
-def _loss_fake(hidden, reduction):
+def _loss_fake(hidden, reduction, K):
     f = lambda *s: hidden.new_empty(s, dtype=torch.float32)
     N = hidden.shape[0]
-    return (f(N) if reduction == "none" else f()), f(N), f(N), f(0 if reduction == "none" else 1)
+    return (f(N) if reduction == "none" else f()), f(_native.kept_len(N, K))
 
 
 @torch.library.custom_op(f"{NS}::linear_xent", mutates_args=())
 def linear_xent(hidden: Tensor, weight: Tensor, target: Tensor, ignore_index: int,
-                reduction: str) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """Cross entropy of hidden (N,D) weight (V,D)^T: loss, and lse2, tlogit, row_scale (N), inv_count (1) for
-    the backward."""
+                reduction: str) -> tuple[Tensor, Tensor]:
+    """Cross entropy of hidden (N,D) weight (V,D)^T: loss, and the fp32 values kept for the backward."""
     return _native.linear_xent_fwd(hidden, weight, target, ignore_index, reduction)
 
 
 @linear_xent.register_fake
 def _(hidden, weight, target, ignore_index, reduction):
-    loss, lse2, row_scale, inv_count = _loss_fake(hidden, reduction)
-    return loss, lse2, torch.empty_like(lse2), row_scale, inv_count
+    return _loss_fake(hidden, reduction, 0)
 
 
 @torch.library.custom_op(f"{NS}::linear_xent_bwd", mutates_args=())
-def linear_xent_bwd(hidden: Tensor, weight: Tensor, target: Tensor, lse2: Tensor, tlogit: Tensor, row_scale: Tensor,
-                    inv_count: Tensor, gout: Tensor, reduction: str) -> tuple[Tensor, Tensor]:
+def linear_xent_bwd(hidden: Tensor, weight: Tensor, target: Tensor, kept: Tensor, gout: Tensor,
+                    reduction: str) -> tuple[Tensor, Tensor]:
     """Backward of linear_xent: dhidden (N,D), dweight (V,D)."""
-    return _native.linear_xent_bwd(hidden, weight, target, lse2, tlogit, row_scale, inv_count, gout, reduction)
+    return _native.linear_xent_bwd(hidden, weight, target, kept, gout, reduction)
 
 
 @linear_xent_bwd.register_fake
-def _(hidden, weight, target, lse2, tlogit, row_scale, inv_count, gout, reduction):
+def _(hidden, weight, target, kept, gout, reduction):
     return hidden.new_empty(hidden.shape), weight.new_empty(weight.shape)
 
 
 @torch.library.custom_op(f"{NS}::linear_distill", mutates_args=())
 def linear_distill(hidden: Tensor, weight: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, temperature: float,
-                   reduction: str) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
-    """Distillation of hidden (N,D) weight (V,D)^T from K teacher logits per row: loss, and lse2, idx, prob,
-    tlogit (N,K), row_scale (N), inv_count (1) for the backward."""
+                   reduction: str) -> tuple[Tensor, Tensor, Tensor]:
+    """Distillation of hidden (N,D) weight (V,D)^T from K teacher logits per row: loss, and the fp32 values and
+    sorted indices (N,K) kept for the backward."""
     return _native.linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
 
 
 @linear_distill.register_fake
 def _(hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
-    loss, lse2, row_scale, inv_count = _loss_fake(hidden, reduction)
-    s = teacher_indices.shape
-    return (loss, lse2, hidden.new_empty(s, dtype=torch.int32), hidden.new_empty(s, dtype=torch.float32),
-            hidden.new_empty(s, dtype=torch.float32), row_scale, inv_count)
+    loss, kept = _loss_fake(hidden, reduction, teacher_indices.shape[1])
+    return loss, kept, hidden.new_empty(teacher_indices.shape, dtype=torch.int32)
 
 
 @torch.library.custom_op(f"{NS}::linear_distill_bwd", mutates_args=())
-def linear_distill_bwd(hidden: Tensor, weight: Tensor, lse2: Tensor, idx: Tensor, prob: Tensor, tlogit: Tensor,
-                       row_scale: Tensor, inv_count: Tensor, gout: Tensor, temperature: float,
+def linear_distill_bwd(hidden: Tensor, weight: Tensor, kept: Tensor, idx: Tensor, gout: Tensor, temperature: float,
                        reduction: str) -> tuple[Tensor, Tensor]:
     """Backward of linear_distill: dhidden (N,D), dweight (V,D)."""
-    return _native.linear_distill_bwd(hidden, weight, lse2, idx, prob, tlogit, row_scale, inv_count, gout, temperature,
-                                      reduction)
+    return _native.linear_distill_bwd(hidden, weight, kept, idx, gout, temperature, reduction)
 
 
 @linear_distill_bwd.register_fake
-def _(hidden, weight, lse2, idx, prob, tlogit, row_scale, inv_count, gout, temperature, reduction):
+def _(hidden, weight, kept, idx, gout, temperature, reduction):
     return hidden.new_empty(hidden.shape), weight.new_empty(weight.shape)
+
+
+# --------------------------------------------------------------------------- eager calls
+def direct(t: Tensor) -> bool:
+    """Whether a call on t may go straight to the binding instead of through the
+    custom op: an ordinary CUDA tensor, nothing tracing or intercepting ops.  The
+    op's dispatch costs 20 to 30 us of host time, the small kernels here take less."""
+    return (type(t) in (Tensor, torch.nn.Parameter) and t.is_cuda and not torch.compiler.is_compiling()
+            and not is_in_torch_dispatch_mode())
 
 
 ops = torch.ops.lighthouse_b200

@@ -13,35 +13,45 @@ Logits, softmax statistics and losses are fp32, gradients bf16.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from .library import ops as _ops
+from . import _native
+from .library import direct, ops as _ops
 
 
 class _LinearXentFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
-        loss, *kept = _ops.linear_xent(hidden, weight, target, ignore_index, reduction)
-        ctx.save_for_backward(hidden, weight, target, *kept)
+        f = _native.linear_xent_fwd if direct(hidden) else _ops.linear_xent
+        loss, kept = f(hidden, weight, target, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, target, kept)
         ctx.reduction = reduction
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gout):
-        dh, dw = _ops.linear_xent_bwd(*ctx.saved_tensors, gout, ctx.reduction)
+        hidden, weight, target, kept = ctx.saved_tensors
+        f = _native.linear_xent_bwd if direct(gout) else _ops.linear_xent_bwd
+        dh, dw = f(hidden, weight, target, kept, gout, ctx.reduction)
         return dh, dw, None, None, None
 
 
 class _LinearDistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
-        loss, *kept = _ops.linear_distill(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
-        ctx.save_for_backward(hidden, weight, *kept)
+        f = _native.linear_distill_fwd if direct(hidden) else _ops.linear_distill
+        loss, kept, idx = f(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
+        ctx.save_for_backward(hidden, weight, kept, idx)
         ctx.temperature, ctx.reduction = temperature, reduction
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gout):
-        dh, dw = _ops.linear_distill_bwd(*ctx.saved_tensors, gout, ctx.temperature, ctx.reduction)
+        hidden, weight, kept, idx = ctx.saved_tensors
+        f = _native.linear_distill_bwd if direct(gout) else _ops.linear_distill_bwd
+        dh, dw = f(hidden, weight, kept, idx, gout, ctx.temperature, ctx.reduction)
         return dh, dw, None, None, None, None
 
 

@@ -13,39 +13,55 @@ Outputs are on the inputs' device, computed on its current stream.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from .library import ops as _ops
+from . import _native
+from .library import direct, ops as _ops
 
 
 class _RmsNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps, out_dtype):
-        y, rstd = _ops.rms_norm(x, weight, eps, out_dtype)
+        if direct(x):
+            y, _, _, rstd = _native.rms_norm_fwd(x, None, weight, eps, out_dtype)
+        else:
+            y, rstd = _ops.rms_norm(x, weight, eps, out_dtype)
         ctx.save_for_backward(x, weight, rstd)
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, rstd = ctx.saved_tensors
-        dx, dw = _ops.rms_norm_bwd(dy, x, weight, rstd)
+        if direct(dy):
+            dx, _, dw = _native.rms_norm_bwd(dy, None, x, weight, rstd, x.dtype, False)
+        else:
+            dx, dw = _ops.rms_norm_bwd(dy, x, weight, rstd)
         return dx, dw, None, None
 
 
 class _AddRmsNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps, out_dtype):
-        y, h, rstd = _ops.add_rms_norm(x, residual, weight, eps, out_dtype)
+        if direct(x):
+            y, _, h, rstd = _native.rms_norm_fwd(x, residual, weight, eps, out_dtype)
+        else:
+            y, h, rstd = _ops.add_rms_norm(x, residual, weight, eps, out_dtype)
         ctx.save_for_backward(h, weight, rstd)
-        ctx.x_dtype, ctx.y_dtype = x.dtype, out_dtype
+        ctx.x_dtype = x.dtype
         ctx.set_materialize_grads(False)
         return y, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh):
         h, weight, rstd = ctx.saved_tensors
         if dy is None:                           # only the stream's new value was used
             return (None if dh is None else dh.to(ctx.x_dtype)), dh, None, None, None
-        dx, dres, dw = _ops.add_rms_norm_bwd(dy, dh, h, weight, rstd, ctx.x_dtype)
+        if direct(dy):
+            dx, dres, dw = _native.rms_norm_bwd(dy, dh, h, weight, rstd, ctx.x_dtype, True)
+        else:
+            dx, dres, dw = _ops.add_rms_norm_bwd(dy, dh, h, weight, rstd, ctx.x_dtype)
         return dx, dres, dw, None, None
 
 
@@ -63,11 +79,17 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     return _AddRmsNormFn.apply(x, residual, weight, float(eps), out_dtype or x.dtype)
 
 
+def _needs_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+
+
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, group: int = 0):
     """(q, scale): rms_norm in float8_e4m3fn.  With group 0 one fp32 scale per row,
     (..., 1); with group 128 one per 128 columns, (..., ceil(D / 128)).  q * scale is
     the norm; the largest magnitude of a group has the code 448.  Has no gradient: a
     backward through it raises."""
+    if direct(x) and not _needs_grad(x, weight):
+        return _native.rms_norm_fwd(x, None, weight, float(eps), torch.float8_e4m3fn, group, with_rstd=False)[:2]
     return _ops.rms_norm_fp8(x, weight, float(eps), group)
 
 
@@ -75,4 +97,6 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
                      group: int = 0):
     """(q, scale, h): rms_norm_fp8 of h = x + residual, h in the residual's type.
     Has no gradient: a backward through it raises."""
+    if direct(x) and not _needs_grad(x, residual, weight):
+        return _native.rms_norm_fwd(x, residual, weight, float(eps), torch.float8_e4m3fn, group, with_rstd=False)[:3]
     return _ops.add_rms_norm_fp8(x, residual, weight, float(eps), group)

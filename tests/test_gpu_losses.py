@@ -361,8 +361,8 @@ def test_opcheck(lh, cuda):
     tv, ti = (x.to(cuda) for x in _teacher(g, 40, 300, 5))
     for red in ("mean", "none"):
         torch.library.opcheck(ops.linear_xent, (h, w, t, -100, red), test_utils=utils)
-        loss, *kept = ops.linear_xent(h, w, t, -100, red)
-        torch.library.opcheck(ops.linear_xent_bwd, (h, w, t, *kept, torch.ones_like(loss), red), test_utils=utils)
+        loss, kept = ops.linear_xent(h, w, t, -100, red)
+        torch.library.opcheck(ops.linear_xent_bwd, (h, w, t, kept, torch.ones_like(loss), red), test_utils=utils)
         torch.library.opcheck(ops.linear_distill, (h, w, tv, ti, 2.0, red), test_utils=utils)
         loss, *kept = ops.linear_distill(h, w, tv, ti, 2.0, red)
         torch.library.opcheck(ops.linear_distill_bwd, (h, w, *kept, torch.ones_like(loss), 2.0, red), test_utils=utils)
