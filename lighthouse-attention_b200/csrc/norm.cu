@@ -8,14 +8,19 @@
 //   8 bits: t = h w, a = max(|t|, 2^-100) over a row or 128 columns,
 //           q = e4m3(448 t / a), scale = a rstd / 448       (q scale = y)
 // rstd cancels in t / a, so the codes do not depend on how the mean was summed.
-// The quotient is rounded once (__fdiv_rn): with bf16 factors t and 448 t are
-// exact, and values that lie midway between two codes go to the even one.
+// The quotient is n / a from the rounded reciprocal y of a: q0 = n y, then
+// q0 + (n - q0 a) y with both sums fused.  With q0 = (n / a)(1 + d) the result is
+// (n / a)(1 - d e) before its rounding, e the error of y, d and e about 2^-24: a
+// quotient that fp32 holds comes out exact.  With bf16 factors t and n = 448 t are
+// exact too, so values that lie midway between two codes go to the even one.
+// (One division per element instead takes 300 us where this takes 219, at
+// 32768 x 5120.)
 //   backward, g = dy w:  d = dh + rstd (g - n mean(g n));  dx = dr = d
 //                        dw = sum over rows of dy n
 // Sums and statistics are fp32; each output is rounded once to its type.
 //
-// Bound: HBM.  Each row is read once into registers (8 consecutive elements per
-// thread and chunk, 16-byte accesses) and written once.  Rows of up to 1024
+// Bound: HBM.  Each row is read once into registers (chunks of 8 consecutive
+// elements per thread, 16-byte accesses) and written once.  Rows of up to 256
 // columns take one warp each, longer ones one CTA each.
 #include <cuda_fp8.h>
 
@@ -26,9 +31,6 @@
 namespace lh {
 namespace norm {
 
-constexpr int kChunks = 4;                   // chunks of 8 elements per thread
-constexpr int kWarpRow = 32 * 8 * kChunks;   // longest row that one warp holds
-constexpr int kCtaThreads = 512;             // most threads of a CTA row: D <= 16384
 constexpr float kE4m3Max = 448.f;
 constexpr float kAmaxMin = 7.888609052210118e-31f;   // 2^-100
 
@@ -86,8 +88,8 @@ struct FwdArgs {
   float eps, inv_d;
 };
 
-template <class TX, class TR, class TY, bool CTA>
-__global__ void __launch_bounds__(CTA ? kCtaThreads : 256)
+template <class TX, class TR, class TY, bool CTA, int CH>
+__global__ void __launch_bounds__(CTA ? 1024 : 256)
 rms_norm_fwd_kernel(const FwdArgs a) {
   constexpr bool kRes = !std::is_same<TR, None>::value;
   constexpr bool kFp8 = std::is_same<TY, __nv_fp8_storage_t>::value;
@@ -97,9 +99,9 @@ rms_norm_fwd_kernel(const FwdArgs a) {
   const int t = CTA ? threadIdx.x : (threadIdx.x & 31);
   const int T = CTA ? blockDim.x : 32;
   const size_t base = (size_t)row * a.D;
-  float v[kChunks][8];
+  float v[CH][8];
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
+  for (int c = 0; c < CH; ++c) {
     const int col = (c * T + t) * 8;
     if (col < a.D) {
       load8(reinterpret_cast<const TX*>(a.x) + base + col, v[c]);
@@ -109,14 +111,14 @@ rms_norm_fwd_kernel(const FwdArgs a) {
     }
   }
   if constexpr (kRes) {
-    float r[kChunks][8];
+    float r[CH][8];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       if (col < a.D) load8(reinterpret_cast<const TR*>(a.r) + base + col, r[c]);
     }
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       if (col < a.D) {
 #pragma unroll
@@ -127,13 +129,13 @@ rms_norm_fwd_kernel(const FwdArgs a) {
   }
   float ss = 0.f, mx = 0.f;
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c)
+  for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fmaf(v[c][e], v[c][e], ss);
-  float amax[kChunks];
+  float amax[CH];
   if constexpr (kFp8) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       amax[c] = 0.f;
       if (col < a.D) {
@@ -158,7 +160,7 @@ rms_norm_fwd_kernel(const FwdArgs a) {
     }
     const int n_groups = (a.D + 127) / 128;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       float m = mx;
       if (a.group) {                          // 16 neighbouring lanes hold one group of 128 columns
@@ -170,14 +172,18 @@ rms_norm_fwd_kernel(const FwdArgs a) {
       }
       if (col < a.D) {
         float q[8];
+        const float inv = __frcp_rn(m);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] = __fdiv_rn(v[c][e] * kE4m3Max, m);
+        for (int e = 0; e < 8; ++e) {
+          const float n = v[c][e] * kE4m3Max, q0 = n * inv;
+          q[e] = fmaf(fmaf(-q0, m, n), inv, q0);
+        }
         store8(reinterpret_cast<TY*>(a.y) + base + col, q);
       }
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       if (col < a.D) {
         float w[8], y[8];
@@ -188,6 +194,25 @@ rms_norm_fwd_kernel(const FwdArgs a) {
       }
     }
   }
+}
+
+// Eight elements as they lie in memory, fetched now and opened later.
+template <class T> struct Raw8;
+template <> struct Raw8<__nv_bfloat16> { uint4 a; };
+template <> struct Raw8<float> { uint4 a, b; };
+__device__ __forceinline__ void fetch(const __nv_bfloat16* p, Raw8<__nv_bfloat16>& r) {
+  r.a = __ldg(reinterpret_cast<const uint4*>(p));
+}
+__device__ __forceinline__ void fetch(const float* p, Raw8<float>& r) {
+  r.a = __ldg(reinterpret_cast<const uint4*>(p));
+  r.b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+}
+__device__ __forceinline__ void open8(const Raw8<__nv_bfloat16>& r, float (&f)[8]) {
+  unpack16(r.a, f, (const __nv_bfloat16*)nullptr);
+}
+__device__ __forceinline__ void open8(const Raw8<float>& r, float (&f)[8]) {
+  unpack16(r.a, f, (const float*)nullptr);
+  unpack16(r.b, f + 4, (const float*)nullptr);
 }
 
 struct BwdArgs {
@@ -204,48 +229,61 @@ struct BwdArgs {
 // Persistent: every warp (or CTA) walks rows and keeps its columns' share of dw
 // in registers; the shares meet in dw_part, which dw_reduce_kernel sums in a
 // fixed order (no atomics).
-template <class TY, class TH, class TX, bool CTA>
-__global__ void __launch_bounds__(CTA ? kCtaThreads : 256)
+template <class TY, class TH, class TX, bool CTA, int CH, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB)
 rms_norm_bwd_kernel(const BwdArgs a) {
   __shared__ float2 part[2][32];
   extern __shared__ float dw_sm[];                       // !CTA: 8 x D
   const int t = CTA ? threadIdx.x : (threadIdx.x & 31);
   const int T = CTA ? blockDim.x : 32;
   const long long step = CTA ? gridDim.x : (long long)gridDim.x * 8;
-  float dw[kChunks][8];
+  float dw[CH][8];
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c)
+  for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[c][e] = 0.f;
   int buf = 0;
-  for (long long row = CTA ? blockIdx.x : ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)); row < a.N; row += step) {
-    const size_t base = (size_t)row * a.D;
-    const float rstd = __ldg(a.rstd + row);
-    float n[kChunks][8], g[kChunks][8];
-    float s = 0.f, unused = 0.f;
+  long long row = CTA ? blockIdx.x : ((long long)blockIdx.x * 8 + (threadIdx.x >> 5));
+  Raw8<TH> rh[CH], rd[CH];
+  Raw8<TY> ry[CH];
+  float rs = 0.f;
+  auto get = [&](long long r) {
+    const size_t base = (size_t)r * a.D;
+    rs = __ldg(a.rstd + r);
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       if (col < a.D) {
-        load8(reinterpret_cast<const TH*>(a.h) + base + col, n[c]);
-        load8(reinterpret_cast<const TY*>(a.dy) + base + col, g[c]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) n[c][e] = g[c][e] = 0.f;
+        fetch(reinterpret_cast<const TH*>(a.h) + base + col, rh[c]);
+        fetch(reinterpret_cast<const TY*>(a.dy) + base + col, ry[c]);
+        if (a.dh) fetch(reinterpret_cast<const TH*>(a.dh) + base + col, rd[c]);
       }
     }
+  };
+  if (row < a.N) get(row);
+  for (; row < a.N; row += step) {
+    const size_t base = (size_t)row * a.D;
+    const float rstd = rs;
+    float s = 0.f, unused = 0.f;
+    Raw8<TH> ch[CH], cd[CH];
+    Raw8<TY> cy[CH];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) { ch[c] = rh[c]; cd[c] = rd[c]; cy[c] = ry[c]; }
+    if (row + step < a.N) get(row + step);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       if (col < a.D) {
-        float w[8];
+        float w[8], n[8], g[8];
         load8w(a.w, a.w_f32, col, w);
+        open8(ch[c], n);
+        open8(cy[c], g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          n[c][e] *= rstd;
-          dw[c][e] = fmaf(g[c][e], n[c][e], dw[c][e]);
-          g[c][e] *= w[e];
-          s = fmaf(g[c][e], n[c][e], s);
+          n[e] *= rstd;
+          const float gn = g[e] * n[e];
+          dw[c][e] += gn;
+          s = fmaf(gn, w[e], s);
         }
       }
     }
@@ -253,14 +291,17 @@ rms_norm_bwd_kernel(const BwdArgs a) {
     buf ^= 1;
     const float m = s * a.inv_d;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       if (col < a.D) {
-        float d[8];
-        if (a.dh) load8(reinterpret_cast<const TH*>(a.dh) + base + col, d);
+        float w[8], n[8], g[8], d[8];
+        load8w(a.w, a.w_f32, col, w);
+        open8(ch[c], n);
+        open8(cy[c], g);
+        if (a.dh) open8(cd[c], d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float v = rstd * fmaf(-n[c][e], m, g[c][e]);
+          const float v = rstd * fmaf(-n[e] * rstd, m, g[e] * w[e]);
           d[e] = a.dh ? d[e] + v : v;
         }
         store8(reinterpret_cast<TX*>(a.dx) + base + col, d);
@@ -270,14 +311,14 @@ rms_norm_bwd_kernel(const BwdArgs a) {
   }
   if (CTA) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       if (col < a.D) store8(a.dw_part + (size_t)blockIdx.x * a.D + col, dw[c]);
     }
   } else {
     float* mine = dw_sm + (size_t)(threadIdx.x >> 5) * a.D;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * T + t) * 8;
       if (col < a.D) store8(mine + col, dw[c]);
     }
@@ -312,15 +353,20 @@ dw_reduce_kernel(const float* __restrict__ part, int parts, int D, void* dw, boo
   }
 }
 
-int cta_threads(int D) { return ((D + 8 * kChunks - 1) / (8 * kChunks) + 31) / 32 * 32; }
+// Threads of a CTA whose threads hold ch chunks of a row each.
+int cta_threads(int D, int ch) { return ((D + 8 * ch - 1) / (8 * ch) + 31) / 32 * 32; }
 
+// One chunk per thread wherever a CTA has the threads for it: 8191 x 4096 bf16
+// takes 47 us with one chunk, 55 with two or four, and four single rows with
+// 8-bit output 8.2 against 10.2 (events around the call).
 template <class TX, class TR, class TY>
 int launch_fwd(const FwdArgs& a, cudaStream_t st) {
-  if (a.D <= kWarpRow) {
-    rms_norm_fwd_kernel<TX, TR, TY, false><<<(unsigned)((a.N + 7) / 8), 256, 0, st>>>(a);
-  } else {
-    rms_norm_fwd_kernel<TX, TR, TY, true><<<(unsigned)a.N, cta_threads(a.D), 0, st>>>(a);
-  }
+  if (a.D <= 256)
+    rms_norm_fwd_kernel<TX, TR, TY, false, 1><<<(unsigned)((a.N + 7) / 8), 256, 0, st>>>(a);
+  else if (a.D <= 8192)
+    rms_norm_fwd_kernel<TX, TR, TY, true, 1><<<(unsigned)a.N, cta_threads(a.D, 1), 0, st>>>(a);
+  else
+    rms_norm_fwd_kernel<TX, TR, TY, true, 2><<<(unsigned)a.N, cta_threads(a.D, 2), 0, st>>>(a);
   return check_launch("rms_norm_fwd_kernel");
 }
 
@@ -336,20 +382,36 @@ int fwd_r(const FwdArgs& a, int r_dtype, int y_dtype, cudaStream_t st) {
   return r_dtype == LH_DTYPE_BF16 ? fwd_y<TX, __nv_bfloat16>(a, y_dtype, st) : fwd_y<TX, float>(a, y_dtype, st);
 }
 
-// CTAs of the persistent backward: enough warps to fill the 148 SMs.
+// Shapes of the persistent backward: chunks per thread and CTAs per SM.  The next
+// row's loads are in flight while a row is worked on, in registers, so a thread
+// holds few chunks: 65536 x 1024 (fp32 stream) takes 144 us with one chunk, 161
+// with two; 8191 x 4096 (bf16) 62 us with two chunks and 256 threads.
+enum BwdShape { kWarp, kOne, kTwo, kTwoWide, kFour };
+BwdShape bwd_shape(int D) {
+  return D <= 256 ? kWarp : D <= 2048 ? kOne : D <= 4096 ? kTwo : D <= 8192 ? kTwoWide : kFour;
+}
+int bwd_threads(int D) {
+  const BwdShape s = bwd_shape(D);
+  return s == kWarp ? 256 : cta_threads(D, s == kOne ? 1 : s == kFour ? 4 : 2);
+}
+// CTAs: what the register limits of the launch bounds let live on 148 SMs.
 int bwd_grid(long long N, int D) {
-  const long long want = D <= kWarpRow ? (N + 7) / 8 : N;
-  const long long cap = D <= kWarpRow ? 148 * 2 : 148 * (cta_threads(D) <= 256 ? 4 : cta_threads(D) <= 512 ? 2 : 1);
+  const BwdShape s = bwd_shape(D);
+  const int warps = s == kWarp || s == kOne ? 24 : 16, t = bwd_threads(D) / 32;
+  const long long want = s == kWarp ? (N + 7) / 8 : N, cap = 148ll * (warps / t > 1 ? warps / t : 1);
   return (int)(want < cap ? want : cap);
 }
 
 template <class TY, class TH, class TX>
 int launch_bwd(const BwdArgs& a, void* dw, cudaStream_t st) {
-  const int grid = bwd_grid(a.N, a.D);
-  if (a.D <= kWarpRow)
-    rms_norm_bwd_kernel<TY, TH, TX, false><<<grid, 256, 8 * a.D * sizeof(float), st>>>(a);
-  else
-    rms_norm_bwd_kernel<TY, TH, TX, true><<<grid, cta_threads(a.D), 0, st>>>(a);
+  const int grid = bwd_grid(a.N, a.D), t = bwd_threads(a.D);
+  switch (bwd_shape(a.D)) {
+    case kWarp: rms_norm_bwd_kernel<TY, TH, TX, false, 1, 256, 3><<<grid, t, 8 * a.D * sizeof(float), st>>>(a); break;
+    case kOne: rms_norm_bwd_kernel<TY, TH, TX, true, 1, 256, 3><<<grid, t, 0, st>>>(a); break;
+    case kTwo: rms_norm_bwd_kernel<TY, TH, TX, true, 2, 256, 2><<<grid, t, 0, st>>>(a); break;
+    case kTwoWide: rms_norm_bwd_kernel<TY, TH, TX, true, 2, 512, 1><<<grid, t, 0, st>>>(a); break;
+    case kFour: rms_norm_bwd_kernel<TY, TH, TX, true, 4, 512, 1><<<grid, t, 0, st>>>(a); break;
+  }
   int rc = check_launch("rms_norm_bwd_kernel");
   if (rc) return rc;
   dw_reduce_kernel<<<(a.D + 31) / 32, 1024, 0, st>>>(a.dw_part, grid, a.D, dw, a.w_f32);
