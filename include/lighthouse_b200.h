@@ -252,19 +252,19 @@ int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h,
  * gradients 16-byte aligned.
  *
  * Bytes of workspace that the forward (backward = 0) or the backward (1) of the
- * two losses below needs.  The backward goes over the vocabulary in pieces, so
+ * two losses below needs; K is 0 for the cross entropy.  The backward goes over the vocabulary in pieces, so
  * that its logits' gradients take at most 512 MB (or 256 columns). */
-size_t lh_linear_loss_workspace_size(int N, int V, int D, int backward);
+size_t lh_linear_loss_workspace_size(int N, int V, int D, int K, int backward);
 
 /* Softmax cross entropy: loss_i = log sum_v exp(s_iv) - s_i,target(i).
  *   target     (N) int64; a row with target ignore_index has loss 0 and no
  *              gradient, one with another target outside [0, V) has loss NaN
  *   reduction  LH_REDUCE_NONE: loss (N); MEAN over the rows that are not
  *              ignored (0 where all are) or SUM: loss (1)
- *   lse2, tlogit, row_scale (N) fp32, inv_count (1) fp32 (unused with NONE):
+ *   lse2, tgrad, row_scale (N) fp32, inv_count (1) fp32 (unused with NONE):
  *              kept for the backward */
 int lh_linear_xent_fwd(const void* hidden, const void* weight, const int64_t* target, int64_t ignore_index, int N, int V,
-                       int D, int reduction, float* loss, float* lse2, float* tlogit, float* row_scale,
+                       int D, int reduction, float* loss, float* lse2, float* tgrad, float* row_scale,
                        float* inv_count, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients of lh_linear_xent_fwd.
@@ -273,7 +273,7 @@ int lh_linear_xent_fwd(const void* hidden, const void* weight, const int64_t* ta
  *               (stride 0 for a reduced loss)
  *   dhidden (N, D), dweight (V, D) bf16 out */
 int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* target, int N, int V, int D,
-                       const float* lse2, const float* tlogit, const float* row_scale, const float* inv_count,
+                       const float* lse2, const float* tgrad, const float* row_scale, const float* inv_count,
                        const float* gout, int gout_stride, void* dhidden, void* dweight, void* workspace,
                        size_t workspace_bytes, void* stream);
 
@@ -285,17 +285,17 @@ int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* ta
  *   logits of -infinity only) has loss 0, no gradient and does not count in the
  *   mean; an index >= V or a NaN or +infinite logit gives loss NaN.  Entries
  *   with the same index add up.
- *   idx (N, K) int32, prob, tlogit (N, K) fp32, lse2, row_scale (N), inv_count
- *   (1): kept for the backward */
+ *   idx (K, N) int32, tgrad (K, N) fp32, lse2, row_scale (N), inv_count (1): kept
+ *   for the backward */
 int lh_linear_distill_fwd(const void* hidden, const void* weight, const void* teacher_logits, int t_dtype,
                           const int64_t* teacher_indices, int N, int V, int D, int K, float temperature, int reduction,
-                          float* loss, float* lse2, int32_t* idx, float* prob, float* tlogit, float* row_scale,
-                          float* inv_count, void* workspace, size_t workspace_bytes, void* stream);
+                          float* loss, float* lse2, int32_t* idx, float* tgrad, float* row_scale, float* inv_count,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients of lh_linear_distill_fwd (the teacher has none). */
 int lh_linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float temperature,
-                          const float* lse2, const int32_t* idx, const float* prob, const float* tlogit,
-                          const float* row_scale, const float* inv_count, const float* gout, int gout_stride,
+                          const float* lse2, const int32_t* idx, const float* tgrad, const float* row_scale,
+                          const float* inv_count, const float* gout, int gout_stride,
                           void* dhidden, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

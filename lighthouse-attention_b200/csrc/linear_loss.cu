@@ -9,7 +9,7 @@
 //   G_iv   = c_i (exp(s_iv - lse_i) - sum_{k: v_k = v} p_k),  c_i = T dloss_i
 //   dH = G W,   dW = G^T H
 // Forward: one GEMM whose epilogue keeps a row's maximum and sum of exponentials
-// per 256 columns, (V / 256) pairs per row, which finish_kernel joins.
+// per 128 columns, V / 128 pairs per row, which finish_kernel joins.
 // Backward, in pieces of the vocabulary of C columns: the logits again, their
 // epilogue writing G (N, C) in bf16; then dH += G W_piece and dW_piece = G^T H.
 // G is rounded to bf16 once, as an operand of bf16 MMAs has to be; its relative
@@ -19,8 +19,8 @@
 // (tcgen05.mma.cta_group::2) per 256 x 256 tile, so that each SM loads 128 rows
 // of either operand and both accumulators (2 x 256 TMEM columns) alternate
 // between the MMAs of one tile and the epilogue of the one before.  Roles: warp
-// 0 TMA producer, warp 1 MMA issuer (leader's), warps 4-7 epilogue (thread = row
-// = TMEM lane).  Operands are K-major or MN-major as they lie in memory: no
+// 0 TMA producer, warp 1 MMA issuer (leader's), warps 4-11 epilogue (thread = row
+// = TMEM lane, two warps per row block, half the columns each).  Operands are K-major or MN-major as they lie in memory: no
 // transposed copy exists.  Where a product has few tiles, its K range is split
 // and the parts meet in fp32 planes which planes_kernel sums in a fixed order.
 // Every mbarrier wait is bounded; on expiry the CTAs leave and a status flag is set.
@@ -40,10 +40,8 @@ namespace ll {
 constexpr int kTM = 256, kTN = 256, kTK = 64;    // tile of a pair of SMs
 constexpr int kBox = 64 * 64 * 2;                // one 64 x 64 bf16 TMA box, 128-byte rows
 constexpr int kOpBytes = 2 * kBox;               // 128 rows of an operand: one CTA's share of a stage
-constexpr int kStages = 6;
-constexpr int kThreads = 256;
+constexpr int kThreads = 384;
 constexpr int kOutBuf = 4096;                    // 32 rows x 128 bytes: one store of an epilogue warp
-constexpr int kSmem = 1024 + kStages * 2 * kOpBytes + 4 * 2 * kOutBuf + 512;
 constexpr int kPairs = 74;
 constexpr int kNone = 0x7fffffff;
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
@@ -51,38 +49,46 @@ constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
 enum Mode { kStats, kGrad, kDH, kDW };
 enum Out { kOutBf16, kOutPlane, kOutPlaneAdd };
 
+// Stages of the operand ring and staging buffers per epilogue warp: a warp's half
+// of a bf16 row block is two stores, each with a buffer of its own, so that it
+// waits for a store of the tile before only; kStats stores nothing.
+__host__ __device__ constexpr int stages(int mode) { return mode == kStats ? 6 : 5; }
+__host__ __device__ constexpr int bufs(int mode) { return mode == kStats ? 1 : 2; }
+constexpr int smem_bytes(int mode) { return 1024 + stages(mode) * 2 * kOpBytes + 8 * bufs(mode) * kOutBuf + 512; }
+
 struct Smem {
-  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drain;
   uint32_t tmem_base;
   int abort;
 };
-static_assert(sizeof(Smem) <= 512, "barriers do not fit their space");
+static_assert(sizeof(Smem) <= 512 && smem_bytes(kStats) <= 232448 && smem_bytes(kGrad) <= 232448, "barriers do not fit their space");
 
 struct Args {
   int M, N;                       // rows and columns of the result
   int tiles_m, tiles_n, splits, kb, gm;
+  FastDiv per_split, per_group, per_col, per_col_last;   // tiles of a split, a group, and of its columns
   int b_off;                      // first row of B's operand (vocabulary piece)
   int out;                        // kDH, kDW: Out
-  // targets: int64 (K = 1, SPARSE false) or sorted int32 (N, K) with probabilities
+  // targets: int64 (K = 1, SPARSE false) or sorted int32 (K, M), a row's entries M apart
   const long long* target;
   const int* idx;
-  const float* prob;
   int K;
   float a2;                       // log2(e) / T
-  float2* stats;                  // kStats: (tiles_n, M) maximum and sum of every tile's row
-  float* slog;                    // logits of the targets (N, K): kStats writes, kGrad reads
+  float2* stats;                  // kStats: (2 tiles_n, M) maximum and sum of a row's 128 columns
+  float* slog;                    // kStats: logits of the targets (K, M) out
+  const float* gval;              // kGrad: exp(s - lse) - p at the targets (K, M)
   const float* lse2;              // kGrad: log2-sum-exp2 of s a2
   const float *gout, *row_scale, *inv_count;
   int gstride;
   float cscale;
 };
 
-// Position of the first of a row's K sorted targets that is >= v.
-__device__ __forceinline__ int lower_bound(const int* __restrict__ idx, int K, int v) {
+// Position of the first of a row's K sorted targets, M apart, that is >= v.
+__device__ __forceinline__ int lower_bound(const int* __restrict__ idx, int K, size_t M, int v) {
   int lo = 0, hi = K;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (__ldg(idx + mid) < v) lo = mid + 1;
+    if (__ldg(idx + mid * M) < v) lo = mid + 1;
     else hi = mid;
   }
   return lo;
@@ -93,12 +99,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmO, const Args a) {
   constexpr bool kAMn = MODE == kDW, kBMn = MODE == kDH || MODE == kDW;
+  constexpr int kStages = stages(MODE), kBufs = bufs(MODE);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = base;
   uint8_t* sB = base + kStages * kOpBytes;
   uint8_t* sO = base + 2 * kStages * kOpBytes;
-  Smem* sm = reinterpret_cast<Smem*>(sO + 8 * kOutBuf);
+  Smem* sm = reinterpret_cast<Smem*>(sO + 8 * kBufs * kOutBuf);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
@@ -106,7 +113,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) { mbar_init(&sm->full[s], 1); mbar_init(&sm->empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&sm->acc_full[b], 1); mbar_init(&sm->acc_empty[b], 8); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&sm->acc_full[b], 1); mbar_init(&sm->acc_empty[b], 16); }
     mbar_init(&sm->drain, 1);
     // an earlier launch gave up a wait: do nothing until the host resets
     sm->abort = *reinterpret_cast<volatile int*>(&g_loss_status) ? 2 : 0;
@@ -122,16 +129,17 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   // tile t -> split, row block, column block: gm row blocks at a time, rows first
   auto decode = [&](int t, int& m, int& n, int& k0, int& k1, int& split) {
-    const int mn = a.tiles_m * a.tiles_n;
-    split = t / mn;
-    int r = t - split * mn;
-    const int g = r / (a.gm * a.tiles_n);
-    r -= g * a.gm * a.tiles_n;
-    const int rows = min(a.gm, a.tiles_m - g * a.gm);
-    m = g * a.gm + r % rows;
-    n = r / rows;
-    k0 = (int)((long long)a.kb * split / a.splits);
-    k1 = (int)((long long)a.kb * (split + 1) / a.splits);
+    uint32_t sp, r, g, x, y;
+    a.per_split.divmod(t, sp, r);
+    a.per_group.divmod(r, g, r);
+    if ((int)((g + 1) * a.gm) <= a.tiles_m) a.per_col.divmod(r, x, y);
+    else a.per_col_last.divmod(r, x, y);
+    m = g * a.gm + y;
+    n = x;
+    split = sp;
+    const int q = a.kb / a.splits, rem = a.kb - q * a.splits;
+    k0 = split * q + min(split, rem);
+    k1 = k0 + q + (split < rem ? 1 : 0);
   };
 
   if (*abort == 0) {
@@ -176,16 +184,16 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         uint32_t it = 0;
         int li = 0;
         bool ok = true;
+        const int q = a.kb / a.splits, rem = a.kb - q * a.splits;
         for (int t = pair; t < total && ok; t += n_pairs, ++li) {
-          int m, n, k0, k1, split;
-          decode(t, m, n, k0, k1, split);
+          const int steps = q + ((int)a.per_split.div(t) < rem ? 1 : 0);
           const int b = li & 1;
-          if (li >= 2 && !mbar_wait_cluster(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort)) break;
+          if (li >= 2 && !mbar_wait(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort)) break;
           tc_fence_after();
           const uint32_t acc = tbase + b * kTN;
-          for (int k = k0; k < k1; ++k, ++it) {
+          for (int k = 0; k < steps; ++k, ++it) {
             const int s = it % kStages;
-            if (!mbar_wait_cluster(&sm->full[s], (it / kStages) & 1, abort)) { ok = false; break; }
+            if (!mbar_wait(&sm->full[s], (it / kStages) & 1, abort)) { ok = false; break; }
             tc_fence_after();
             const uint32_t pa = smem_u32(sA + s * kOpBytes), pb = smem_u32(sB + s * kOpBytes);
 #pragma unroll
@@ -193,7 +201,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               mma_ss_pair(acc,
                           kAMn ? smem_desc_sw128(pa + kk * 2048, kBox, 1024) : smem_desc_sw128(pa + kk * 32, 16, 1024),
                           kBMn ? smem_desc_sw128(pb + kk * 2048, kBox, 1024) : smem_desc_sw128(pb + kk * 32, 16, 1024),
-                          idesc, (k > k0 || kk > 0) ? 1u : 0u);
+                          idesc, (k > 0 || kk > 0) ? 1u : 0u);
             mma_commit_pair(&sm->empty[s]);
           }
           if (ok) mma_commit_pair(&sm->acc_full[b]);
@@ -205,12 +213,14 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       }
     } else if (warp >= 4) {
       // ---------------------------------------------------------- epilogue
-      const int quad = warp & 3;
-      const uint32_t lane_base = tbase + ((uint32_t)(quad * 32) << 16);
-      uint8_t* stage = sO + quad * 2 * kOutBuf;
-      const uint32_t acc_empty[2] = {leader_addr(&sm->acc_empty[0]), leader_addr(&sm->acc_empty[1])};
+      // warps 4-7 take columns 0-127 of the tile, warps 8-11 the rest
+      const int quad = warp & 3, half = warp >= 8 ? 1 : 0;
+      constexpr int kCols = kTN / 2;
+      const uint32_t lane_base = tbase + ((uint32_t)(quad * 32) << 16) + half * kCols;
+      uint8_t* stage = sO + (quad + 4 * half) * kBufs * kOutBuf;
+      const uint32_t acc_empty0 = leader_addr(&sm->acc_empty[0]), acc_empty1 = leader_addr(&sm->acc_empty[1]);
       int li = 0, buf = 0;
-      // 16 bytes to chunk c of this thread's row of the staging tile (128-byte swizzle)
+      // 16 bytes to chunk c of this thread's row of a staging tile (128-byte swizzle)
       auto put = [&](uint8_t* p, int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
         *reinterpret_cast<uint4*>(p + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(x, y, z, w);
       };
@@ -219,24 +229,30 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         decode(t, m, n, k0, k1, split);
         const int b = li & 1;
         const uint32_t acc = lane_base + b * kTN;
-        const int row0 = m * kTM + rank * 128 + quad * 32, row = row0 + lane, n0 = n * kTN;
-        const int cols = min(kTN, a.N - n0);
+        const int row0 = m * kTM + rank * 128 + quad * 32, row = row0 + lane, n0 = n * kTN + half * kCols;
+        const int cols = min(kCols, a.N - n0);           // of this warp's half, may be negative
         const bool live = row < a.M;
-        // next target of this row at or behind the tile's first column, as a column of the tile
-        int cur = 0, next = kNone;
+        // next target of this row at or behind the half's first column, as a column of the half,
+        // and the one behind it, fetched ahead
+        int cur = 0, next = kNone, after = kNone;
         const int g0 = MODE == kGrad ? a.b_off + n0 : n0;
         const int* idx = nullptr;
-        auto advance = [&]() { next = cur < a.K && __ldg(idx + cur) != kNone ? __ldg(idx + cur) - g0 : kNone; };
+        auto advance = [&]() {
+          ++cur;
+          next = after == kNone ? kNone : after - g0;
+          after = cur + 1 < a.K ? __ldg(idx + (size_t)(cur + 1) * a.M) : kNone;
+        };
         float c = 0.f, lse2 = 0.f;
         if constexpr (MODE == kStats || MODE == kGrad) {
-          if (live) {
+          if (live && cols > 0) {
             if constexpr (SPARSE) {
-              idx = a.idx + (size_t)row * a.K;
-              cur = lower_bound(idx, a.K, g0);
+              idx = a.idx + row;
+              cur = lower_bound(idx, a.K, a.M, g0) - 1;
+              after = cur + 1 < a.K ? __ldg(idx + (size_t)(cur + 1) * a.M) : kNone;
               advance();
             } else {
               const long long tv = __ldg(a.target + row) - g0;
-              if (tv >= 0 && tv < kTN) next = (int)tv;
+              if (tv >= 0 && tv < kCols) next = (int)tv;
             }
             if constexpr (MODE == kGrad) {
               const float up = __ldg(a.gout + (size_t)row * a.gstride);
@@ -248,15 +264,32 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const bool ok = mbar_wait(&sm->acc_full[b], (li >> 1) & 1, abort);
         if (__any_sync(~0u, !ok)) break;
         tc_fence_after();
+        auto release = [&]() {                           // the tile's TMEM has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_leader(b ? acc_empty1 : acc_empty0);
+        };
         if constexpr (MODE == kStats) {
           float mx = -INFINITY, sum = 0.f;
 #pragma unroll 1
-          for (int cc = 0; cc < kTN / 32; ++cc) {
-            const int left = cols - cc * 32;
+          for (int c0 = 0; c0 < kCols; c0 += 32) {
+            const int left = cols - c0;
             if (left <= 0) break;
             uint32_t x[32];
-            tmem_ld32(acc + cc * 32, x);
+            tmem_ld32(acc + c0, x);
             tmem_ld_wait();
+            // logits of the targets among these columns, by way of this thread's row in shared memory
+            if (__any_sync(~0u, next < c0 + 32)) {
+#pragma unroll
+              for (int ch = 0; ch < 8; ++ch) put(stage, ch, x[4 * ch], x[4 * ch + 1], x[4 * ch + 2], x[4 * ch + 3]);
+              while (next < c0 + 32) {
+                const int at = next - c0;
+                a.slog[(size_t)cur * a.M + row] = *reinterpret_cast<const float*>(
+                    stage + lane * 128 + (((at >> 2) ^ (lane & 7)) << 4) + (at & 3) * 4);
+                if constexpr (SPARSE) advance();
+                else next = kNone;
+              }
+            }
             if (left < 32) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
@@ -282,37 +315,17 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             const float2 r = fadd2(fadd2(sp[0], sp[1]), fadd2(sp[2], sp[3]));
             sum += r.x + r.y;
           }
-          // logits of the targets in this tile: one TMEM column at a time, all rows that want it at once
-          while (true) {
-            const int want = next < cols ? next : kNone;
-            const int col = (int)__reduce_min_sync(~0u, (unsigned)want);
-            if (col == kNone) break;
-            const uint32_t v = tmem_ld1(acc + col);
-            tmem_ld_wait();
-            while (next == col) {
-              a.slog[(size_t)row * a.K + cur] = __uint_as_float(v);
-              ++cur;
-              if constexpr (SPARSE) advance();
-              else next = kNone;
-            }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(acc_empty[b]);
-          if (live) a.stats[(size_t)n * a.M + row] = make_float2(mx, sum);
+          release();
+          if (live) a.stats[(size_t)(2 * n + half) * a.M + row] = make_float2(mx, sum);
         } else {
           const int width = MODE == kGrad || a.out == kOutBf16 ? 64 : 32;      // columns of one store
 #pragma unroll 1
-          for (int c0 = 0; c0 < kTN; c0 += width) {
+          for (int c0 = 0; c0 < kCols; c0 += width) {
             uint32_t x[32], y[32];
             tmem_ld32(acc + c0, x);
             if (width == 64) tmem_ld32(acc + c0 + 32, y);
             tmem_ld_wait();
-            if (c0 + width == kTN) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_cluster(acc_empty[b]);
-            }
+            if (c0 + width == kCols) release();
             if (c0 >= cols || row0 >= a.M) continue;
             uint8_t* p = stage + buf * kOutBuf;
             if (lane == 0) bulk_wait_read_1();
@@ -335,22 +348,12 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                       pack_bf16(grad(y[8 * ch + 2]), grad(y[8 * ch + 3])),
                       pack_bf16(grad(y[8 * ch + 4]), grad(y[8 * ch + 5])),
                       pack_bf16(grad(y[8 * ch + 6]), grad(y[8 * ch + 7])));
-                while (next < c0 + 64) {         // the row's targets among these columns, from their fp32 logits
-                  const float q = ex2(fmaf(__ldg(a.slog + (size_t)row * a.K + cur), a.a2, -lse2));
+                while (next < c0 + 64) {         // the row's targets among these columns (the same one twice: twice alike)
                   const int at = next - c0;
-                  float pr = 1.f;
-                  if constexpr (SPARSE) {
-                    pr = 0.f;
-                    do {
-                      pr += __ldg(a.prob + (size_t)row * a.K + cur);
-                      ++cur;
-                      advance();
-                    } while (next == c0 + at);
-                  } else {
-                    next = kNone;
-                  }
                   *reinterpret_cast<__nv_bfloat16*>(p + lane * 128 + (((at >> 3) ^ (lane & 7)) << 4) + (at & 7) * 2) =
-                      __float2bfloat16_rn(c * (q - pr));
+                      __float2bfloat16_rn(c * __ldg(a.gval + (size_t)cur * a.M + row));
+                  if constexpr (SPARSE) advance();
+                  else next = kNone;
                 }
               }
             } else if (a.out == kOutBf16) {
@@ -391,7 +394,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
 // ---------------------------------------------------------------- small kernels
 // One warp per row: the K teacher entries sorted by vocabulary index (absent
-// ones behind), their probabilities softmax(t / T) and sum p log p.  The rank of
+// ones behind; stored (K, N)), their probabilities softmax(t / T) and sum p log p.  The rank of
 // an entry is the number of entries before it, ties in their given order.
 //   row_scale: 1, 0 for a row without entries, NaN for one with an index >= V or
 //   a teacher logit that is NaN or +infinity
@@ -440,8 +443,8 @@ teacher_kernel(const T* __restrict__ tv, const long long* __restrict__ ti, int N
       any_nan |= p != p;
       if (p > 0.f) e = fmaf(p, x, e);
     }
-    idx[(size_t)row * K + r] = some ? me : kNone;
-    prob[(size_t)row * K + r] = p;
+    idx[(size_t)r * N + row] = some ? me : kNone;
+    prob[(size_t)r * N + row] = p;
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) e += __shfl_xor_sync(~0u, e, o);
@@ -452,13 +455,14 @@ teacher_kernel(const T* __restrict__ tv, const long long* __restrict__ ti, int N
   }
 }
 
-// Joins the tiles' (maximum, sum) of 32 rows per block and forms the rows'
-// losses; partial (sum, count) of the block for the reduced loss.
+// Joins the (maximum, sum) parts of 32 rows per block, forms the rows' losses and
+// turns the targets' logits into exp(s - lse) - p, what the backward takes off the
+// softmax; partial (sum, count) of the block for the reduced loss.
 template <bool SPARSE>
 __global__ void __launch_bounds__(1024)
-finish_kernel(const float2* __restrict__ stats, int tiles, int N, int V, int K, const long long* __restrict__ target,
+finish_kernel(const float2* __restrict__ stats, int parts, int N, int V, int K, const long long* __restrict__ target,
               long long ignore, const int* __restrict__ idx, const float* __restrict__ prob,
-              const float* __restrict__ ent, const float* __restrict__ slog, float a2, float t2,
+              const float* __restrict__ ent, float* __restrict__ slog, float a2, float t2,
               float* __restrict__ row_scale, float* __restrict__ lse2, float* __restrict__ loss_rows,
               double2* __restrict__ part) {
   __shared__ float2 sh[32][33];
@@ -468,45 +472,59 @@ finish_kernel(const float2* __restrict__ stats, int tiles, int N, int V, int K, 
   auto join = [&](float2 v) {
     const float mn = fmaxf(mx, v.x);
     const float mb = mn == -INFINITY ? 0.f : mn * a2;
-    s = s * (mx == -INFINITY ? 0.f : exp2f(fmaf(mx, a2, -mb))) + v.y * (v.x == -INFINITY ? 0.f : exp2f(fmaf(v.x, a2, -mb)));
-    if (v.y != v.y) s = v.y;
+    s = (mx == -INFINITY ? s : s * exp2f(fmaf(mx, a2, -mb))) + (v.x == -INFINITY ? v.y : v.y * exp2f(fmaf(v.x, a2, -mb)));
     mx = mn;
   };
   if (row < N) {
 #pragma unroll 4
-    for (int t = w; t < tiles; t += nw) join(stats[(size_t)t * N + row]);
+    for (int t = w; t < parts; t += nw) join(stats[(size_t)t * N + row]);
   }
   sh[w][lane] = make_float2(mx, s);
   __syncthreads();
-  if (w) return;
-  for (int k = 1; k < nw; ++k) join(sh[k][lane]);
+  mx = -INFINITY;                                 // every warp joins all parts: the same order, the same result
+  s = 0.f;
+  for (int k = 0; k < nw; ++k) join(sh[k][lane]);
+  const float l2 = fmaf(mx, a2, log2f(s));
   float loss = 0.f, scale = 0.f;
-  if (row < N) {
-    const float l2 = fmaf(mx, a2, log2f(s));
-    lse2[row] = l2;
-    const float lse = l2 * kLn2, a = a2 * kLn2;         // a = 1 / T
-    if (SPARSE) {
-      scale = row_scale[row];
-      if (scale == 0.f) {
-        loss = 0.f;
-      } else {
-        float x = 0.f;
-        for (int k = 0; k < K; ++k) {
-          if (idx[(size_t)row * K + k] == kNone) break;
-          const float p = prob[(size_t)row * K + k];
-          if (p > 0.f) x = fmaf(p, lse - slog[(size_t)row * K + k] * a, x);
-        }
-        loss = scale * t2 * (ent[row] + x);
+  if constexpr (SPARSE) {
+    float x = 0.f;
+    if (row < N) {
+      for (int k = w; k < K; k += nw) {
+        const size_t at = (size_t)k * N + row;
+        const int me = idx[at];
+        if (me == kNone) break;
+        const float st = slog[at], p = prob[at];
+        if (p > 0.f) x = fmaf(p, (l2 - st * a2) * kLn2, x);
+        float all = p;                            // entries with the same index add up
+        for (int j = k - 1; j >= 0 && idx[(size_t)j * N + row] == me; --j) all += prob[(size_t)j * N + row];
+        for (int j = k + 1; j < K && idx[(size_t)j * N + row] == me; ++j) all += prob[(size_t)j * N + row];
+        slog[at] = exp2f(fmaf(st, a2, -l2)) - all;
       }
-    } else {
+    }
+    __syncthreads();                              // sh has been read
+    sh[w][lane].x = x;
+    __syncthreads();
+    if (w) return;
+    for (int k = 1; k < nw; ++k) x += sh[k][lane].x;
+    if (row < N) {
+      scale = row_scale[row];
+      if (scale != 0.f) loss = scale * t2 * (ent[row] + x);
+    }
+  } else {
+    if (w) return;
+    if (row < N) {
       const long long t = target[row];
       if (t != ignore) {
         const bool in = t >= 0 && t < V;
         scale = in ? 1.f : __int_as_float(0x7fc00000);
-        loss = in ? lse - slog[row] : scale;
+        loss = in ? l2 * kLn2 - slog[row] : scale;
+        if (in) slog[row] = exp2f(fmaf(slog[row], a2, -l2)) - 1.f;
       }
       row_scale[row] = scale;
     }
+  }
+  if (row < N) {
+    lse2[row] = l2;
     if (loss_rows) loss_rows[row] = loss;
   }
   if (part) {
@@ -621,11 +639,15 @@ static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMa
   long long gm = (48ll << 20) / (kTM * 2ll * a.kb * kTK);
   if (gm < 8) gm = 8;
   a.gm = (int)(gm < a.tiles_m ? gm : a.tiles_m);
+  a.per_split = FastDiv(a.tiles_m * a.tiles_n);
+  a.per_group = FastDiv(a.gm * a.tiles_n);
+  a.per_col = FastDiv(a.gm);
+  a.per_col_last = FastDiv(a.tiles_m % a.gm ? a.tiles_m % a.gm : 1);
   const long long total = (long long)a.tiles_m * a.tiles_n * a.splits;
   const int pairs = (int)(total < kPairs ? total : kPairs);
-  cudaError_t e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  cudaError_t e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MODE));
   if (e != cudaSuccess) { set_error("linear loss: %s", cudaGetErrorString(e)); return LH_ERR_LAUNCH; }
-  loss_gemm_kernel<MODE, SPARSE><<<2 * pairs, kThreads, kSmem, st>>>(ma, mb, mo, a);
+  loss_gemm_kernel<MODE, SPARSE><<<2 * pairs, kThreads, smem_bytes(MODE), st>>>(ma, mb, mo, a);
   return check_launch("loss_gemm_kernel");
 }
 
@@ -673,9 +695,12 @@ static Plan plan(long long N, long long V, long long D) {
   return p;
 }
 
-static size_t fwd_workspace(long long N, long long V) {
-  return up((size_t)((V + kTN - 1) / kTN) * N * sizeof(float2)) + up((size_t)((N + 31) / 32) * sizeof(double2)) +
-         up((size_t)N * sizeof(float));
+// stats, the blocks' sums; distillation (K > 0): sum p log p and p of the rows
+static size_t stats_bytes(long long N, long long V) {
+  return up((size_t)((V + kTN - 1) / kTN) * 2 * N * sizeof(float2)) + up((size_t)((N + 31) / 32) * sizeof(double2));
+}
+static size_t fwd_workspace(long long N, long long V, long long K) {
+  return stats_bytes(N, V) + (K ? up((size_t)N * sizeof(float)) + up((size_t)N * K * sizeof(float)) : 0);
 }
 
 static int sum_planes(const float* planes, int n, size_t plane, void* out, cudaStream_t st) {
@@ -689,37 +714,37 @@ struct Targets {
   const long long* target;   // cross entropy
   long long ignore;
   const int* idx;            // distillation
-  const float* prob;
   int K;
   float T;
 };
 
 template <bool SPARSE>
-static int forward(const void* hidden, const void* weight, int N, int V, int D, const Targets& tg, const float* ent,
-                   int reduction, float* loss, float* lse2, float* slog, float* row_scale, float* inv_count, void* ws,
+static int forward(const void* hidden, const void* weight, int N, int V, int D, const Targets& tg, const float* prob,
+                   const float* ent, int reduction, float* loss, float* lse2, float* slog, float* row_scale, float* inv_count, void* ws,
                    cudaStream_t st) {
   int rc = make_context_current();
   if (rc) return rc;
   CUtensorMap mh, mw;
   if ((rc = map_load(&mh, hidden, N, D, D)) || (rc = map_load(&mw, weight, V, D, D))) return rc;
-  const int tiles = (V + kTN - 1) / kTN;
+  const int parts = (V + kTN - 1) / kTN * 2;
   float2* stats = (float2*)ws;
-  double2* part = (double2*)((char*)ws + up((size_t)tiles * N * sizeof(float2)));
+  double2* part = (double2*)((char*)ws + up((size_t)parts * N * sizeof(float2)));
   Args a{};
   a.M = N;
   a.N = V;
   a.splits = 1;
   a.target = tg.target;
   a.idx = tg.idx;
-  a.prob = tg.prob;
   a.K = tg.K;
   a.a2 = kLog2e / tg.T;
   a.stats = stats;
   a.slog = slog;
   if ((rc = launch<kStats, SPARSE>(mh, mw, mw, a, D, st))) return rc;
   const int blocks = (N + 31) / 32;
-  finish_kernel<SPARSE><<<blocks, dim3(32, tiles < 32 ? tiles : 32), 0, st>>>(
-      stats, tiles, N, V, tg.K, tg.target, tg.ignore, tg.idx, tg.prob, ent, slog, a.a2, tg.T * tg.T, row_scale, lse2,
+  int warps = parts > tg.K ? parts : tg.K;
+  if (warps > 32) warps = 32;
+  finish_kernel<SPARSE><<<blocks, dim3(32, warps), 0, st>>>(
+      stats, parts, N, V, tg.K, tg.target, tg.ignore, tg.idx, prob, ent, slog, a.a2, tg.T * tg.T, row_scale, lse2,
       reduction == LH_REDUCE_NONE ? loss : nullptr, reduction == LH_REDUCE_NONE ? nullptr : part);
   if ((rc = check_launch("finish_kernel"))) return rc;
   if (reduction == LH_REDUCE_NONE) return LH_OK;
@@ -729,7 +754,7 @@ static int forward(const void* hidden, const void* weight, int N, int V, int D, 
 
 template <bool SPARSE>
 static int backward(const void* hidden, const void* weight, int N, int V, int D, const Targets& tg, const float* lse2,
-                    const float* slog, const float* row_scale, const float* inv_count, const float* gout, int gstride,
+                    const float* gval, const float* row_scale, const float* inv_count, const float* gout, int gstride,
                     void* dhidden, void* dweight, void* ws, cudaStream_t st) {
   int rc = make_context_current();
   if (rc) return rc;
@@ -752,10 +777,9 @@ static int backward(const void* hidden, const void* weight, int N, int V, int D,
     a.b_off = (int)v0;
     a.target = tg.target;
     a.idx = tg.idx;
-    a.prob = tg.prob;
     a.K = tg.K;
     a.a2 = kLog2e / tg.T;
-    a.slog = const_cast<float*>(slog);
+    a.gval = gval;
     a.lse2 = lse2;
     a.row_scale = row_scale;
     a.inv_count = inv_count;
@@ -790,30 +814,30 @@ static int backward(const void* hidden, const void* weight, int N, int V, int D,
 
 }  // namespace ll
 
-size_t linear_loss_workspace_size(int N, int V, int D, int backward) {
-  return backward ? ll::plan(N, V, D).total : ll::fwd_workspace(N, V);
+size_t linear_loss_workspace_size(int N, int V, int D, int K, int backward) {
+  return backward ? ll::plan(N, V, D).total : ll::fwd_workspace(N, V, K);
 }
 
 int linear_xent_fwd(const void* hidden, const void* weight, const long long* target, long long ignore, int N, int V, int D,
-                    int reduction, float* loss, float* lse2, float* tlogit, float* row_scale, float* inv_count, void* ws,
+                    int reduction, float* loss, float* lse2, float* tgrad, float* row_scale, float* inv_count, void* ws,
                     cudaStream_t st) {
-  const ll::Targets tg{target, ignore, nullptr, nullptr, 1, 1.f};
-  return ll::forward<false>(hidden, weight, N, V, D, tg, nullptr, reduction, loss, lse2, tlogit, row_scale, inv_count, ws, st);
+  const ll::Targets tg{target, ignore, nullptr, 1, 1.f};
+  return ll::forward<false>(hidden, weight, N, V, D, tg, nullptr, nullptr, reduction, loss, lse2, tgrad, row_scale, inv_count, ws, st);
 }
 
 int linear_xent_bwd(const void* hidden, const void* weight, const long long* target, int N, int V, int D, const float* lse2,
-                    const float* tlogit, const float* row_scale, const float* inv_count, const float* gout, int gstride,
+                    const float* tgrad, const float* row_scale, const float* inv_count, const float* gout, int gstride,
                     void* dhidden, void* dweight, void* ws, cudaStream_t st) {
-  const ll::Targets tg{target, 0, nullptr, nullptr, 1, 1.f};
-  return ll::backward<false>(hidden, weight, N, V, D, tg, lse2, tlogit, row_scale, inv_count, gout, gstride, dhidden,
+  const ll::Targets tg{target, 0, nullptr, 1, 1.f};
+  return ll::backward<false>(hidden, weight, N, V, D, tg, lse2, tgrad, row_scale, inv_count, gout, gstride, dhidden,
                              dweight, ws, st);
 }
 
 int linear_distill_fwd(const void* hidden, const void* weight, const void* tv, int tv_dtype, const long long* ti, int N,
-                       int V, int D, int K, float T, int reduction, float* loss, float* lse2, int* idx, float* prob,
-                       float* tlogit, float* row_scale, float* inv_count, void* ws, cudaStream_t st) {
-  float* ent = (float*)((char*)ws + ll::up((size_t)((V + ll::kTN - 1) / ll::kTN) * N * sizeof(float2)) +
-                        ll::up((size_t)((N + 31) / 32) * sizeof(double2)));
+                       int V, int D, int K, float T, int reduction, float* loss, float* lse2, int* idx, float* tgrad,
+                       float* row_scale, float* inv_count, void* ws, cudaStream_t st) {
+  float* ent = (float*)((char*)ws + ll::stats_bytes(N, V));
+  float* prob = (float*)((char*)ent + ll::up((size_t)N * sizeof(float)));
   const unsigned blocks = (unsigned)((N + 3) / 4);
   if (tv_dtype == LH_DTYPE_BF16)
     ll::teacher_kernel<<<blocks, 128, 4 * K * sizeof(int), st>>>((const __nv_bfloat16*)tv, ti, N, V, K, 1.f / T, idx, prob,
@@ -823,16 +847,16 @@ int linear_distill_fwd(const void* hidden, const void* weight, const void* tv, i
                                                                 row_scale);
   int rc = check_launch("teacher_kernel");
   if (rc) return rc;
-  const ll::Targets tg{nullptr, 0, idx, prob, K, T};
-  return ll::forward<true>(hidden, weight, N, V, D, tg, ent, reduction, loss, lse2, tlogit, row_scale, inv_count, ws, st);
+  const ll::Targets tg{nullptr, 0, idx, K, T};
+  return ll::forward<true>(hidden, weight, N, V, D, tg, prob, ent, reduction, loss, lse2, tgrad, row_scale, inv_count, ws, st);
 }
 
 int linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float T, const float* lse2,
-                       const int* idx, const float* prob, const float* tlogit, const float* row_scale,
+                       const int* idx, const float* tgrad, const float* row_scale,
                        const float* inv_count, const float* gout, int gstride, void* dhidden, void* dweight, void* ws,
                        cudaStream_t st) {
-  const ll::Targets tg{nullptr, 0, idx, prob, K, T};
-  return ll::backward<true>(hidden, weight, N, V, D, tg, lse2, tlogit, row_scale, inv_count, gout, gstride, dhidden,
+  const ll::Targets tg{nullptr, 0, idx, K, T};
+  return ll::backward<true>(hidden, weight, N, V, D, tg, lse2, tgrad, row_scale, inv_count, gout, gstride, dhidden,
                             dweight, ws, st);
 }
 

@@ -315,14 +315,15 @@ def _(hidden, weight, target, kept, gout, reduction):
 def linear_distill(hidden: Tensor, weight: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, temperature: float,
                    reduction: str) -> tuple[Tensor, Tensor, Tensor]:
     """Distillation of hidden (N,D) weight (V,D)^T from K teacher logits per row: loss, and the fp32 values and
-    sorted indices (N,K) kept for the backward."""
+    sorted indices (K,N) kept for the backward."""
     return _native.linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
 
 
 @linear_distill.register_fake
 def _(hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
     loss, kept = _loss_fake(hidden, reduction, teacher_indices.shape[1])
-    return loss, kept, hidden.new_empty(teacher_indices.shape, dtype=torch.int32)
+    N, K = teacher_indices.shape
+    return loss, kept, hidden.new_empty((K, N), dtype=torch.int32)
 
 
 @torch.library.custom_op(f"{NS}::linear_distill_bwd", mutates_args=())
