@@ -331,22 +331,22 @@ def simple_gla_fwd(q, k, v, g, scale: float, q2=None, k2=None):
 # --------------------------------------------------------------------------- norm
 def _on_one_device(what: str, first, *rest) -> torch.device:
     """All tensors are CUDA tensors of one device, which is returned."""
-    dev = first.device
+    index = first.get_device()
     for t in (first, *rest):
-        if t is not None:
+        if t is not None and (t.get_device() != index or not t.is_cuda):
             if not t.is_cuda:
                 raise ValueError("lighthouse_b200 ops take CUDA tensors (no CPU path)")
-            if t.device != dev:
-                raise ValueError(f"{what}: tensors on different devices: {dev} and {t.device}")
-    return dev
+            raise ValueError(f"{what}: tensors on different devices: {first.device} and {t.device}")
+    return first.device
 
 
 def _call(dev: torch.device, name: str, *args) -> None:
     """Entry point `name` with the device's current stream as its last argument,
     the device being current meanwhile."""
-    fn = getattr(load(), name)
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if torch.cuda.current_device() == dev.index:
+    fn = getattr(_lib or load(), name)
+    index = dev.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(dev):

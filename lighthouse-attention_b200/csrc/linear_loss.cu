@@ -76,6 +76,7 @@ struct Args {
   float a2;                       // log2(e) / T
   float2* stats;                  // kStats: (2 tiles_n, M) maximum and sum of a row's 128 columns
   float* slog;                    // kStats: logits of the targets (K, M) out
+  unsigned* ticket;               // kStats: set to 0 for finish_kernel
   const float* gval;              // kGrad: exp(s - lse) - p at the targets (K, M)
   const float* lse2;              // kGrad: log2-sum-exp2 of s a2
   const float *gout, *row_scale, *inv_count;
@@ -112,6 +113,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const int total = a.tiles_m * a.tiles_n * a.splits;
 
   if (threadIdx.x == 0) {
+    if (MODE == kStats && blockIdx.x == 0) *a.ticket = 0;
     for (int s = 0; s < kStages; ++s) { mbar_init(&sm->full[s], 1); mbar_init(&sm->empty[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&sm->acc_full[b], 1); mbar_init(&sm->acc_empty[b], 16); }
     mbar_init(&sm->drain, 1);
@@ -184,13 +186,15 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         uint32_t it = 0;
         int li = 0;
         bool ok = true;
+        // (Looking at the next stage's barrier, or waiting for the next accumulator, before a step's
+        // MMAs are issued makes the kernel 3 to 8 % slower, not faster.)
         const int q = a.kb / a.splits, rem = a.kb - q * a.splits;
         for (int t = pair; t < total && ok; t += n_pairs, ++li) {
           const int steps = q + ((int)a.per_split.div(t) < rem ? 1 : 0);
           const int b = li & 1;
+          const uint32_t acc = tbase + b * kTN;
           if (li >= 2 && !mbar_wait(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort)) break;
           tc_fence_after();
-          const uint32_t acc = tbase + b * kTN;
           for (int k = 0; k < steps; ++k, ++it) {
             const int s = it % kStages;
             if (!mbar_wait(&sm->full[s], (it / kStages) & 1, abort)) { ok = false; break; }
@@ -455,108 +459,129 @@ teacher_kernel(const T* __restrict__ tv, const long long* __restrict__ ti, int N
   }
 }
 
-// Joins the (maximum, sum) parts of 32 rows per block, forms the rows' losses and
-// turns the targets' logits into exp(s - lse) - p, what the backward takes off the
-// softmax; partial (sum, count) of the block for the reduced loss.
-template <bool SPARSE>
+// Joins the (maximum, sum) parts of RB rows per block (thread = row of the block x
+// slot of its parts, slots a power of two), forms the rows' losses and turns the
+// targets' logits into exp(s - lse) - p, what the backward takes off the softmax.
+// The last block to end adds up the blocks' (loss, count) in their order: the
+// reduced loss (sum, or mean over the rows that count; 0 where none does) and
+// 1 / count.
+struct FinishArgs {
+  const float2* stats;
+  int parts, N, V, K, slots, reduction;
+  const long long* target;
+  long long ignore;
+  const int* idx;
+  const float *prob, *ent;
+  float* slog;
+  float a2, t2;
+  float *row_scale, *lse2, *loss, *inv_count;
+  double2* part;
+  unsigned* ticket;
+};
+
+template <bool SPARSE, int RB>
 __global__ void __launch_bounds__(1024)
-finish_kernel(const float2* __restrict__ stats, int parts, int N, int V, int K, const long long* __restrict__ target,
-              long long ignore, const int* __restrict__ idx, const float* __restrict__ prob,
-              const float* __restrict__ ent, float* __restrict__ slog, float a2, float t2,
-              float* __restrict__ row_scale, float* __restrict__ lse2, float* __restrict__ loss_rows,
-              double2* __restrict__ part) {
-  __shared__ float2 sh[32][33];
-  const int lane = threadIdx.x, w = threadIdx.y, nw = blockDim.y;
-  const int row = blockIdx.x * 32 + lane;
-  float mx = -INFINITY, s = 0.f;
-  auto join = [&](float2 v) {
-    const float mn = fmaxf(mx, v.x);
-    const float mb = mn == -INFINITY ? 0.f : mn * a2;
-    s = (mx == -INFINITY ? s : s * exp2f(fmaf(mx, a2, -mb))) + (v.x == -INFINITY ? v.y : v.y * exp2f(fmaf(v.x, a2, -mb)));
-    mx = mn;
+finish_kernel(const FinishArgs a) {
+  __shared__ float2 sh[1024];
+  __shared__ double2 tot[32];
+  __shared__ bool last;
+  const int tid = threadIdx.x, r = tid % RB, slot = tid / RB, N = a.N, K = a.K;
+  const int row = blockIdx.x * RB + r;
+  auto join = [&](float2 u, float2 v) {
+    const float mn = fmaxf(u.x, v.x);
+    const float mb = mn == -INFINITY ? 0.f : mn * a.a2;
+    return make_float2(mn, (u.x == -INFINITY ? u.y : u.y * ex2(fmaf(u.x, a.a2, -mb))) +
+                               (v.x == -INFINITY ? v.y : v.y * ex2(fmaf(v.x, a.a2, -mb))));
   };
+  float2 st = make_float2(-INFINITY, 0.f);
   if (row < N) {
 #pragma unroll 4
-    for (int t = w; t < parts; t += nw) join(stats[(size_t)t * N + row]);
+    for (int t = slot; t < a.parts; t += a.slots) st = join(st, a.stats[(size_t)t * N + row]);
   }
-  sh[w][lane] = make_float2(mx, s);
+  sh[tid] = st;
   __syncthreads();
-  mx = -INFINITY;                                 // every warp joins all parts: the same order, the same result
-  s = 0.f;
-  for (int k = 0; k < nw; ++k) join(sh[k][lane]);
-  const float l2 = fmaf(mx, a2, log2f(s));
+  for (int o = a.slots >> 1; o; o >>= 1) {
+    if (slot < o) sh[tid] = join(sh[tid], sh[tid + o * RB]);
+    __syncthreads();
+  }
+  const float2 all = sh[r];
+  const float l2 = fmaf(all.x, a.a2, log2f(all.y));
   float loss = 0.f, scale = 0.f;
   if constexpr (SPARSE) {
     float x = 0.f;
     if (row < N) {
-      for (int k = w; k < K; k += nw) {
+      for (int k = slot; k < K; k += a.slots) {
         const size_t at = (size_t)k * N + row;
-        const int me = idx[at];
+        const int me = a.idx[at];
         if (me == kNone) break;
-        const float st = slog[at], p = prob[at];
-        if (p > 0.f) x = fmaf(p, (l2 - st * a2) * kLn2, x);
-        float all = p;                            // entries with the same index add up
-        for (int j = k - 1; j >= 0 && idx[(size_t)j * N + row] == me; --j) all += prob[(size_t)j * N + row];
-        for (int j = k + 1; j < K && idx[(size_t)j * N + row] == me; ++j) all += prob[(size_t)j * N + row];
-        slog[at] = exp2f(fmaf(st, a2, -l2)) - all;
+        const float s = a.slog[at], p = a.prob[at];
+        if (p > 0.f) x = fmaf(p, (l2 - s * a.a2) * kLn2, x);
+        float same = p;                            // entries with the same index add up
+        for (int j = k - 1; j >= 0 && a.idx[(size_t)j * N + row] == me; --j) same += a.prob[(size_t)j * N + row];
+        for (int j = k + 1; j < K && a.idx[(size_t)j * N + row] == me; ++j) same += a.prob[(size_t)j * N + row];
+        a.slog[at] = ex2(fmaf(s, a.a2, -l2)) - same;
       }
     }
-    __syncthreads();                              // sh has been read
-    sh[w][lane].x = x;
+    __syncthreads();                               // sh has been read
+    sh[tid].x = x;
     __syncthreads();
-    if (w) return;
-    for (int k = 1; k < nw; ++k) x += sh[k][lane].x;
-    if (row < N) {
-      scale = row_scale[row];
-      if (scale != 0.f) loss = scale * t2 * (ent[row] + x);
+    for (int o = a.slots >> 1; o; o >>= 1) {
+      if (slot < o) sh[tid].x += sh[tid + o * RB].x;
+      __syncthreads();
     }
-  } else {
-    if (w) return;
-    if (row < N) {
-      const long long t = target[row];
-      if (t != ignore) {
-        const bool in = t >= 0 && t < V;
-        scale = in ? 1.f : __int_as_float(0x7fc00000);
-        loss = in ? l2 * kLn2 - slog[row] : scale;
-        if (in) slog[row] = exp2f(fmaf(slog[row], a2, -l2)) - 1.f;
-      }
-      row_scale[row] = scale;
+    if (row < N && slot == 0) {
+      scale = a.row_scale[row];
+      if (scale != 0.f) loss = scale * a.t2 * (a.ent[row] + sh[r].x);
     }
+  } else if (row < N && slot == 0) {
+    const long long t = a.target[row];
+    if (t != a.ignore) {
+      const bool in = t >= 0 && t < a.V;
+      scale = in ? 1.f : __int_as_float(0x7fc00000);
+      loss = in ? l2 * kLn2 - a.slog[row] : scale;
+      if (in) a.slog[row] = ex2(fmaf(a.slog[row], a.a2, -l2)) - 1.f;
+    }
+    a.row_scale[row] = scale;
   }
-  if (row < N) {
-    lse2[row] = l2;
-    if (loss_rows) loss_rows[row] = loss;
+  if (row < N && slot == 0) {
+    a.lse2[row] = l2;
+    if (a.reduction == LH_REDUCE_NONE) a.loss[row] = loss;
   }
-  if (part) {
-    double ls = loss, n = scale != 0.f ? 1.0 : 0.0;
+  if (a.reduction == LH_REDUCE_NONE) return;
+  auto block_sum = [&](double& s, double& c) {     // to thread 0
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-      ls += __shfl_xor_sync(~0u, ls, o);
-      n += __shfl_xor_sync(~0u, n, o);
+      s += __shfl_xor_sync(~0u, s, o);
+      c += __shfl_xor_sync(~0u, c, o);
     }
-    if (lane == 0) part[blockIdx.x] = make_double2(ls, n);
+    if ((tid & 31) == 0) tot[tid >> 5] = make_double2(s, c);
+    __syncthreads();
+    if (tid == 0)
+      for (int w = 1; w < (int)blockDim.x / 32; ++w) { s += tot[w].x; c += tot[w].y; }
+    __syncthreads();
+  };
+  double s = loss, c = scale != 0.f ? 1.0 : 0.0;   // zeros but in slot 0
+  block_sum(s, c);
+  if (tid == 0) {
+    a.part[blockIdx.x] = make_double2(s, c);
+    __threadfence();
+    last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
   }
-}
-
-// The blocks' partial sums -> the loss (sum, or mean over the rows that count,
-// 0 where none does) and 1 / count.
-__global__ void __launch_bounds__(256)
-total_kernel(const double2* __restrict__ part, int n, bool mean, float* loss, float* inv_count) {
-  __shared__ double sh[2][8];
-  double s = 0, c = 0;
-  for (int i = threadIdx.x; i < n; i += 256) { s += part[i].x; c += part[i].y; }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    s += __shfl_xor_sync(~0u, s, o);
-    c += __shfl_xor_sync(~0u, c, o);
-  }
-  if ((threadIdx.x & 31) == 0) { sh[0][threadIdx.x >> 5] = s; sh[1][threadIdx.x >> 5] = c; }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) { s += sh[0][w]; c += sh[1][w]; }
-    const double inv = mean ? (c > 0 ? 1.0 / c : 0.0) : 1.0;
-    *loss = (float)(c > 0 ? s * inv : 0.0);
-    *inv_count = (float)inv;
+  if (!last) return;
+  __threadfence();
+  s = c = 0;
+#pragma unroll 4
+  for (int i = tid; i < (int)gridDim.x; i += blockDim.x) {
+    const double2 v = __ldcg(a.part + i);
+    s += v.x;
+    c += v.y;
+  }
+  block_sum(s, c);
+  if (tid == 0) {
+    const double inv = a.reduction == LH_REDUCE_MEAN ? (c > 0 ? 1.0 / c : 0.0) : 1.0;
+    *a.loss = (float)(c > 0 ? s * inv : 0.0);
+    *a.inv_count = (float)inv;
   }
 }
 
@@ -695,9 +720,9 @@ static Plan plan(long long N, long long V, long long D) {
   return p;
 }
 
-// stats, the blocks' sums; distillation (K > 0): sum p log p and p of the rows
+// stats, the blocks' sums and their ticket; distillation (K > 0): sum p log p and p of the rows
 static size_t stats_bytes(long long N, long long V) {
-  return up((size_t)((V + kTN - 1) / kTN) * 2 * N * sizeof(float2)) + up((size_t)((N + 31) / 32) * sizeof(double2));
+  return up((size_t)((V + kTN - 1) / kTN) * 2 * N * sizeof(float2)) + up((size_t)((N + 7) / 8) * sizeof(double2)) + 256;
 }
 static size_t fwd_workspace(long long N, long long V, long long K) {
   return stats_bytes(N, V) + (K ? up((size_t)N * sizeof(float)) + up((size_t)N * K * sizeof(float)) : 0);
@@ -729,6 +754,7 @@ static int forward(const void* hidden, const void* weight, int N, int V, int D, 
   const int parts = (V + kTN - 1) / kTN * 2;
   float2* stats = (float2*)ws;
   double2* part = (double2*)((char*)ws + up((size_t)parts * N * sizeof(float2)));
+  unsigned* ticket = (unsigned*)((char*)part + up((size_t)((N + 7) / 8) * sizeof(double2)));
   Args a{};
   a.M = N;
   a.N = V;
@@ -739,17 +765,21 @@ static int forward(const void* hidden, const void* weight, int N, int V, int D, 
   a.a2 = kLog2e / tg.T;
   a.stats = stats;
   a.slog = slog;
+  a.ticket = ticket;
   if ((rc = launch<kStats, SPARSE>(mh, mw, mw, a, D, st))) return rc;
-  const int blocks = (N + 31) / 32;
-  int warps = parts > tg.K ? parts : tg.K;
-  if (warps > 32) warps = 32;
-  finish_kernel<SPARSE><<<blocks, dim3(32, warps), 0, st>>>(
-      stats, parts, N, V, tg.K, tg.target, tg.ignore, tg.idx, prob, ent, slog, a.a2, tg.T * tg.T, row_scale, lse2,
-      reduction == LH_REDUCE_NONE ? loss : nullptr, reduction == LH_REDUCE_NONE ? nullptr : part);
-  if ((rc = check_launch("finish_kernel"))) return rc;
-  if (reduction == LH_REDUCE_NONE) return LH_OK;
-  total_kernel<<<1, 256, 0, st>>>(part, blocks, reduction == LH_REDUCE_MEAN, loss, inv_count);
-  return check_launch("total_kernel");
+  // Rows per block: eight with up to 128 slots each where a row has many parts (16 rows of 1000
+  // parts: 7 us, 17 with 32 rows per block), 256 where it has up to four (65536 rows of two parts:
+  // 14 us with 32 rows per block, most of it the 2048 blocks' sum).
+  const int want = parts > tg.K ? parts : tg.K;
+  FinishArgs f{stats, parts, N, V, tg.K, 1, reduction, tg.target, tg.ignore, tg.idx, prob, ent, slog, a.a2, tg.T * tg.T,
+               row_scale, lse2, loss, inv_count, part, ticket};
+  const int rb = want > 32 ? 8 : want > 4 ? 32 : 256;
+  while (f.slots < want && f.slots * rb < 1024) f.slots *= 2;
+  const unsigned blocks = (unsigned)((N + rb - 1) / rb);
+  if (rb == 8) finish_kernel<SPARSE, 8><<<blocks, rb * f.slots, 0, st>>>(f);
+  else if (rb == 256) finish_kernel<SPARSE, 256><<<blocks, rb * f.slots, 0, st>>>(f);
+  else finish_kernel<SPARSE, 32><<<blocks, rb * f.slots, 0, st>>>(f);
+  return check_launch("finish_kernel");
 }
 
 template <bool SPARSE>

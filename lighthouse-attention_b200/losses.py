@@ -61,7 +61,13 @@ def _rows(hidden: torch.Tensor, *per_row: tuple[torch.Tensor, int]):
     for t, tail in per_row:
         if t.shape[:t.dim() - tail] != lead:
             raise ValueError(f"leading dimensions {tuple(lead)} of hidden and {tuple(t.shape)} differ")
-    return hidden.reshape(-1, hidden.shape[-1])
+    return hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
+
+
+def _long(t: torch.Tensor, *shape: int) -> torch.Tensor:
+    """t as int64 of this shape."""
+    t = t if t.dtype == torch.int64 else t.to(torch.int64)
+    return t if t.shape == shape else t.reshape(shape)
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
@@ -74,8 +80,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     that are not ignored; 0 where all are), "sum", or "none" (the loss of every
     position).  Returns fp32."""
     h = _rows(hidden, (target, 0))
-    loss = _LinearXentFn.apply(h, weight, target.reshape(-1).to(torch.int64), ignore_index, reduction)
-    return loss.view(target.shape) if reduction == "none" else loss
+    loss = _LinearXentFn.apply(h, weight, _long(target, h.shape[0]), ignore_index, reduction)
+    return loss.view(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
 
 def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor,
@@ -93,7 +99,7 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logi
     the position's loss NaN.  The teacher gets no gradient.  Returns fp32."""
     h = _rows(hidden, (teacher_logits, 1), (teacher_indices, 1))
     N = h.shape[0]
-    loss = _LinearDistillFn.apply(h, weight, teacher_logits.detach().reshape(N, teacher_logits.shape[-1]),
-                                  teacher_indices.reshape(N, teacher_indices.shape[-1]).to(torch.int64),
+    tl = teacher_logits if teacher_logits.dim() == 2 else teacher_logits.reshape(N, teacher_logits.shape[-1])
+    loss = _LinearDistillFn.apply(h, weight, tl, _long(teacher_indices, N, teacher_indices.shape[-1]),
                                   float(temperature), reduction)
-    return loss.view(hidden.shape[:-1]) if reduction == "none" else loss
+    return loss.view(hidden.shape[:-1]) if reduction == "none" and hidden.dim() != 2 else loss

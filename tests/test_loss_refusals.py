@@ -88,7 +88,7 @@ def test_workspace_stays_small(lh):
                 piece = max(512 << 20, 2 * N * 256)
                 planes = 74 * 4 * 256 * D * 8 + 4 * N * D      # parts only where few tiles are
                 assert 0 < size(N, V, D, 0, 1) <= piece + planes + 4096, (N, V, D)
-                assert size(N, V, D, 0, 0) <= 16 * N * (V // 256 + 1) + 16 * (N // 32 + 1) + 4 * N + 1024
+                assert size(N, V, D, 0, 0) <= 16 * N * (V // 256 + 1) + 2 * N + 4 * N + 2048
 
 
 def test_fake_kernels(lh):
