@@ -248,33 +248,32 @@ int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h,
 
 /* Losses of an output projection without its logits.  hidden (N, D) bf16,
  * weight (V, D) bf16, s = hidden weight^T (fp32, never stored).
- * Limits: D % 8 == 0, N <= 2^24, V <= 2^22, K <= 256; hidden, weight and their
- * gradients 16-byte aligned.
+ * Limits: D % 8 == 0, D <= 65536, N <= 2^24, V <= 2^22, K <= 256; hidden, weight,
+ * kept and the gradients 16-byte aligned, the workspace 256-byte.
  *
  * Bytes of workspace that the forward (backward = 0) or the backward (1) of the
- * two losses below needs; K is 0 for the cross entropy.  The backward goes over the vocabulary in pieces, so
- * that its logits' gradients take at most 512 MB (or 256 columns). */
+ * two losses below needs; K is 0 for the cross entropy.  The backward goes over
+ * the vocabulary in pieces, so that its logits' gradients take at most 512 MB (or
+ * 256 columns). */
 size_t lh_linear_loss_workspace_size(int N, int V, int D, int K, int backward);
+
+/* Bytes of `kept`, which the forward fills for the backward of the same problem. */
+size_t lh_linear_loss_kept_size(int N, int K);
 
 /* Softmax cross entropy: loss_i = log sum_v exp(s_iv) - s_i,target(i).
  *   target     (N) int64; a row with target ignore_index has loss 0 and no
  *              gradient, one with another target outside [0, V) has loss NaN
- *   reduction  LH_REDUCE_NONE: loss (N); MEAN over the rows that are not
- *              ignored (0 where all are) or SUM: loss (1)
- *   lse2, tgrad, row_scale (N) fp32, inv_count (1) fp32 (unused with NONE):
- *              kept for the backward */
+ *   reduction  LH_REDUCE_NONE: loss (N) fp32; MEAN over the rows that are not
+ *              ignored (0 where all are) or SUM: loss (1) */
 int lh_linear_xent_fwd(const void* hidden, const void* weight, const int64_t* target, int64_t ignore_index, int N, int V,
-                       int D, int reduction, float* loss, float* lse2, float* tgrad, float* row_scale,
-                       float* inv_count, void* workspace, size_t workspace_bytes, void* stream);
+                       int D, int reduction, float* loss, void* kept, void* workspace, size_t workspace_bytes,
+                       void* stream);
 
 /* Gradients of lh_linear_xent_fwd.
- *   inv_count   as the forward left it, NULL with LH_REDUCE_NONE
- *   gout        upstream gradient of loss: element i * gout_stride is row i's
- *               (stride 0 for a reduced loss)
+ *   gout    fp32 upstream gradient of loss: (N) with LH_REDUCE_NONE, else (1)
  *   dhidden (N, D), dweight (V, D) bf16 out */
-int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* target, int N, int V, int D,
-                       const float* lse2, const float* tgrad, const float* row_scale, const float* inv_count,
-                       const float* gout, int gout_stride, void* dhidden, void* dweight, void* workspace,
+int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* target, int N, int V, int D, int reduction,
+                       const void* kept, const float* gout, void* dhidden, void* dweight, void* workspace,
                        size_t workspace_bytes, void* stream);
 
 /* Distillation from a teacher's K top logits per row:
@@ -284,19 +283,15 @@ int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* ta
  *   negative one marks an entry that is absent.  A row without entries (or with
  *   logits of -infinity only) has loss 0, no gradient and does not count in the
  *   mean; an index >= V or a NaN or +infinite logit gives loss NaN.  Entries
- *   with the same index add up.
- *   idx (K, N) int32, tgrad (K, N) fp32, lse2, row_scale (N), inv_count (1): kept
- *   for the backward */
+ *   with the same index add up. */
 int lh_linear_distill_fwd(const void* hidden, const void* weight, const void* teacher_logits, int t_dtype,
                           const int64_t* teacher_indices, int N, int V, int D, int K, float temperature, int reduction,
-                          float* loss, float* lse2, int32_t* idx, float* tgrad, float* row_scale, float* inv_count,
-                          void* workspace, size_t workspace_bytes, void* stream);
+                          float* loss, void* kept, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients of lh_linear_distill_fwd (the teacher has none). */
 int lh_linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float temperature,
-                          const float* lse2, const int32_t* idx, const float* tgrad, const float* row_scale,
-                          const float* inv_count, const float* gout, int gout_stride,
-                          void* dhidden, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+                          int reduction, const void* kept, const float* gout, void* dhidden, void* dweight,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

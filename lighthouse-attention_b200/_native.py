@@ -56,14 +56,14 @@ _SIGS = {
                                        ctypes.c_longlong, ctypes.c_int, _VP, ctypes.c_int] + [_VP] * 3
                         + [ctypes.c_size_t, _VP]),
     "lh_linear_loss_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 5),
-    "lh_linear_xent_fwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int64] + [ctypes.c_int] * 4 + [_VP] * 6
+    "lh_linear_loss_kept_size": (ctypes.c_size_t, [ctypes.c_int] * 2),
+    "lh_linear_xent_fwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int64] + [ctypes.c_int] * 4 + [_VP] * 3
                            + [ctypes.c_size_t, _VP]),
-    "lh_linear_xent_bwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int] * 3 + [_VP] * 5 + [ctypes.c_int] + [_VP] * 3
-                           + [ctypes.c_size_t, _VP]),
+    "lh_linear_xent_bwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int] * 4 + [_VP] * 5 + [ctypes.c_size_t, _VP]),
     "lh_linear_distill_fwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int, _VP] + [ctypes.c_int] * 4
-                              + [ctypes.c_float, ctypes.c_int] + [_VP] * 7 + [ctypes.c_size_t, _VP]),
-    "lh_linear_distill_bwd": (ctypes.c_int, [_VP] * 2 + [ctypes.c_int] * 4 + [ctypes.c_float] + [_VP] * 6
-                              + [ctypes.c_int] + [_VP] * 3 + [ctypes.c_size_t, _VP]),
+                              + [ctypes.c_float, ctypes.c_int] + [_VP] * 3 + [ctypes.c_size_t, _VP]),
+    "lh_linear_distill_bwd": (ctypes.c_int, [_VP] * 2 + [ctypes.c_int] * 4 + [ctypes.c_float, ctypes.c_int]
+                              + [_VP] * 5 + [ctypes.c_size_t, _VP]),
 }
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -456,33 +456,25 @@ def _loss_ws(N, V, D, K, backward, dev):
     return torch.empty(n, dtype=torch.uint8, device=dev), n
 
 
-def kept_len(N: int, K: int) -> int:
-    """fp32 values that a loss's forward keeps for its backward: lse2 (N), row_scale (N), inv_count (1)
-    and the softmax less the targets at the targets (N, or K N for distillation)."""
-    return 2 * N + 1 + N * max(K, 1)
-
-
-def _kept_ptrs(kept, N):
-    """Addresses of lse2, row_scale, inv_count, tgrad inside kept."""
-    p = kept.data_ptr()
-    return p, p + 4 * N, p + 8 * N, p + 8 * N + 4
+def kept_size(N: int, K: int) -> int:
+    """Bytes that a loss's forward keeps for its backward."""
+    return load().lh_linear_loss_kept_size(N, K)
 
 
 def linear_xent_fwd(hidden, weight, target, ignore_index: int, reduction: str):
     """Softmax cross entropy of hidden (N, D) @ weight (V, D)^T against target (N) int64 ->
-    (loss, kept); kept is the backward's."""
+    (loss, kept); kept (uint8) is the backward's."""
     N, V, D = _loss_check("linear_xent", hidden, weight, reduction)
     if target.shape != (N,) or target.dtype != torch.int64:
         raise LighthouseShapeError("linear_xent: target must be (N) int64")
     dev = _on_one_device("linear_xent", hidden, weight, target)
     loss = _loss_out(N, reduction, dev)
-    kept = torch.empty(kept_len(N, 0), dtype=torch.float32, device=dev)
+    kept = torch.empty(kept_size(N, 0), dtype=torch.uint8, device=dev)
     if N:
         hidden, weight, target = _dense16(hidden), _dense16(weight), target.contiguous()
         ws, n = _loss_ws(N, V, D, 0, 0, dev)
-        lse2, row_scale, inv_count, tgrad = _kept_ptrs(kept, N)
         _call(dev, "lh_linear_xent_fwd", hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), ignore_index, N, V, D,
-              REDUCTIONS[reduction], loss.data_ptr(), lse2, tgrad, row_scale, inv_count, ws.data_ptr(), n)
+              REDUCTIONS[reduction], loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
     return loss, kept
 
 
@@ -490,7 +482,7 @@ def _loss_bwd_outputs(what, hidden, weight, kept, gout, reduction, K, *rest):
     N, V, D = _loss_check(what, hidden, weight, reduction)
     if gout.dtype != torch.float32 or gout.numel() != (N if reduction == "none" else 1):
         raise LighthouseShapeError(f"{what}: the loss's gradient must be fp32, one value (reduced) or N")
-    if kept.dtype != torch.float32 or kept.shape != (kept_len(N, K),) or not kept.is_contiguous():
+    if kept.dtype != torch.uint8 or kept.shape != (kept_size(N, K),) or not kept.is_contiguous():
         raise LighthouseShapeError(f"{what}: kept must be the forward's")
     dev = _on_one_device(what, hidden, weight, kept, gout, *rest)
     dh = torch.empty(N, D, dtype=torch.bfloat16, device=dev)
@@ -504,19 +496,16 @@ def linear_xent_bwd(hidden, weight, target, kept, gout, reduction: str):
     if target.shape != (N,) or target.dtype != torch.int64:
         raise LighthouseShapeError("linear_xent_bwd: target must be (N) int64")
     if N:
-        reduced = reduction != "none"
         hidden, weight, target, gout = _dense16(hidden), _dense16(weight), target.contiguous(), gout.contiguous()
         ws, n = _loss_ws(N, V, D, 0, 1, dev)
-        lse2, row_scale, inv_count, tgrad = _kept_ptrs(kept, N)
-        _call(dev, "lh_linear_xent_bwd", hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), N, V, D, lse2, tgrad,
-              row_scale, inv_count if reduced else None, gout.data_ptr(), 0 if reduced else 1, dh.data_ptr(),
-              dw.data_ptr(), ws.data_ptr(), n)
+        _call(dev, "lh_linear_xent_bwd", hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), N, V, D,
+              REDUCTIONS[reduction], kept.data_ptr(), gout.data_ptr(), dh.data_ptr(), dw.data_ptr(), ws.data_ptr(), n)
     return dh, dw
 
 
 def linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperature: float, reduction: str):
     """Distillation of hidden (N, D) @ weight (V, D)^T from a teacher's K logits (N, K) bf16 / fp32 at
-    indices (N, K) int64 -> (loss, kept, idx); kept and idx (K, N) int32 are the backward's."""
+    indices (N, K) int64 -> (loss, kept); kept (uint8) is the backward's."""
     N, V, D = _loss_check("linear_distill", hidden, weight, reduction)
     if teacher_logits.dim() != 2 or teacher_logits.shape[0] != N or teacher_indices.shape != teacher_logits.shape:
         raise LighthouseShapeError("linear_distill: teacher logits and indices must be (N, K)")
@@ -529,31 +518,23 @@ def linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperat
         raise ValueError(f"linear_distill: temperature must be positive and finite, got {temperature}")
     dev = _on_one_device("linear_distill", hidden, weight, teacher_logits, teacher_indices)
     loss = _loss_out(N, reduction, dev)
-    kept = torch.empty(kept_len(N, K), dtype=torch.float32, device=dev)
-    idx = torch.empty(K, N, dtype=torch.int32, device=dev)
+    kept = torch.empty(kept_size(N, K), dtype=torch.uint8, device=dev)
     if N:
         hidden, weight = _dense16(hidden), _dense16(weight)
         teacher_logits, teacher_indices = teacher_logits.contiguous(), teacher_indices.contiguous()
         ws, n = _loss_ws(N, V, D, K, 0, dev)
-        lse2, row_scale, inv_count, tgrad = _kept_ptrs(kept, N)
         _call(dev, "lh_linear_distill_fwd", hidden.data_ptr(), weight.data_ptr(), teacher_logits.data_ptr(),
               LH_DTYPE[teacher_logits.dtype], teacher_indices.data_ptr(), N, V, D, K, temperature, REDUCTIONS[reduction],
-              loss.data_ptr(), lse2, idx.data_ptr(), tgrad, row_scale, inv_count, ws.data_ptr(), n)
-    return loss, kept, idx
+              loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
+    return loss, kept
 
 
-def linear_distill_bwd(hidden, weight, kept, idx, gout, temperature: float, reduction: str):
+def linear_distill_bwd(hidden, weight, kept, gout, K: int, temperature: float, reduction: str):
     """Gradients (dhidden, dweight) of linear_distill_fwd."""
-    K = idx.shape[0]
-    N, V, D, dev, dh, dw = _loss_bwd_outputs("linear_distill_bwd", hidden, weight, kept, gout, reduction, K, idx)
-    if idx.shape != (K, N) or idx.dtype != torch.int32 or not idx.is_contiguous():
-        raise LighthouseShapeError("linear_distill_bwd: idx must be the forward's")
+    N, V, D, dev, dh, dw = _loss_bwd_outputs("linear_distill_bwd", hidden, weight, kept, gout, reduction, K)
     if N:
-        reduced = reduction != "none"
         hidden, weight, gout = _dense16(hidden), _dense16(weight), gout.contiguous()
         ws, n = _loss_ws(N, V, D, K, 1, dev)
-        lse2, row_scale, inv_count, tgrad = _kept_ptrs(kept, N)
-        _call(dev, "lh_linear_distill_bwd", hidden.data_ptr(), weight.data_ptr(), N, V, D, K, temperature, lse2,
-              idx.data_ptr(), tgrad, row_scale, inv_count if reduced else None, gout.data_ptr(),
-              0 if reduced else 1, dh.data_ptr(), dw.data_ptr(), ws.data_ptr(), n)
+        _call(dev, "lh_linear_distill_bwd", hidden.data_ptr(), weight.data_ptr(), N, V, D, K, temperature,
+              REDUCTIONS[reduction], kept.data_ptr(), gout.data_ptr(), dh.data_ptr(), dw.data_ptr(), ws.data_ptr(), n)
     return dh, dw

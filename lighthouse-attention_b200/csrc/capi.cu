@@ -79,14 +79,15 @@ int rms_norm_bwd(const void*, int, const void*, const void*, int, const void*, i
                  int, void*, void*, void*, cudaStream_t);
 
 size_t linear_loss_workspace_size(int, int, int, int, int);
-int linear_xent_fwd(const void*, const void*, const long long*, long long, int, int, int, int, float*, float*, float*,
-                    float*, float*, void*, cudaStream_t);
-int linear_xent_bwd(const void*, const void*, const long long*, int, int, int, const float*, const float*, const float*,
-                    const float*, const float*, int, void*, void*, void*, cudaStream_t);
+size_t linear_loss_kept_size(int, int);
+int linear_xent_fwd(const void*, const void*, const long long*, long long, int, int, int, int, float*, void*, void*,
+                    cudaStream_t);
+int linear_xent_bwd(const void*, const void*, const long long*, int, int, int, int, const void*, const float*, void*, void*,
+                    void*, cudaStream_t);
 int linear_distill_fwd(const void*, const void*, const void*, int, const long long*, int, int, int, int, float, int, float*,
-                       float*, int*, float*, float*, float*, void*, cudaStream_t);
-int linear_distill_bwd(const void*, const void*, int, int, int, int, float, const float*, const int*, const float*,
-                       const float*, const float*, const float*, int, void*, void*, void*, cudaStream_t);
+                       void*, void*, cudaStream_t);
+int linear_distill_bwd(const void*, const void*, int, int, int, int, float, int, const void*, const float*, void*, void*,
+                       void*, cudaStream_t);
 int loss_status(int reset);
 
 }  // namespace lh
@@ -328,15 +329,16 @@ int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h,
 }
 
 static int loss_check(const char* what, const void* hidden, const void* weight, int N, int V, int D, int K, float T,
-                      const void* ws, size_t ws_bytes, int backward) {
-  LH_REQUIRE(hidden && weight && ws, LH_ERR_ARG, "%s: null pointer", what);
+                      int reduction, const void* kept, const void* ws, size_t ws_bytes, int backward) {
+  LH_REQUIRE(hidden && weight && kept && ws, LH_ERR_ARG, "%s: null pointer", what);
   LH_REQUIRE(N > 0 && V > 0 && D > 0 && N <= (1 << 24) && V <= (1 << 22), LH_ERR_SHAPE,
              "%s: N must be in [1, 2^24], V in [1, 2^22]", what);
   LH_REQUIRE(D % 8 == 0 && D <= (1 << 16), LH_ERR_SHAPE, "%s: D must be a multiple of 8 and at most 65536, got %d", what, D);
   LH_REQUIRE(K >= 0 && K <= 256, LH_ERR_SHAPE, "%s: K must be in [1, 256], got %d", what, K);
   LH_REQUIRE(T > 0.f && T < 1e30f, LH_ERR_ARG, "%s: temperature must be positive and finite", what);
-  LH_REQUIRE(!(((uintptr_t)hidden | (uintptr_t)weight) & 15) && !((uintptr_t)ws & 255), LH_ERR_ARG,
-             "%s: hidden and weight must be 16-byte aligned, the workspace 256-byte", what);
+  LH_REQUIRE(reduction >= LH_REDUCE_NONE && reduction <= LH_REDUCE_SUM, LH_ERR_ARG, "%s: bad reduction", what);
+  LH_REQUIRE(!(((uintptr_t)hidden | (uintptr_t)weight | (uintptr_t)kept) & 15) && !((uintptr_t)ws & 255), LH_ERR_ARG,
+             "%s: hidden, weight and kept must be 16-byte aligned, the workspace 256-byte", what);
   const size_t need = linear_loss_workspace_size(N, V, D, K, backward);
   LH_REQUIRE(ws_bytes >= need, LH_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu needed", what,
              ws_bytes, need);
@@ -347,70 +349,59 @@ size_t lh_linear_loss_workspace_size(int N, int V, int D, int K, int backward) {
   return N > 0 && V > 0 && D > 0 && K >= 0 ? linear_loss_workspace_size(N, V, D, K, backward) : 0;
 }
 
+size_t lh_linear_loss_kept_size(int N, int K) { return N > 0 && K >= 0 ? linear_loss_kept_size(N, K) : 0; }
+
 int lh_linear_xent_fwd(const void* hidden, const void* weight, const int64_t* target, int64_t ignore_index, int N, int V,
-                       int D, int reduction, float* loss, float* lse2, float* tgrad, float* row_scale,
-                       float* inv_count, void* ws, size_t ws_bytes, void* stream) {
+                       int D, int reduction, float* loss, void* kept, void* ws, size_t ws_bytes, void* stream) {
   g_err[0] = 0;
-  int rc = loss_check("linear_xent", hidden, weight, N, V, D, 0, 1.f, ws, ws_bytes, 0);
+  int rc = loss_check("linear_xent", hidden, weight, N, V, D, 0, 1.f, reduction, kept, ws, ws_bytes, 0);
   if (rc) return rc;
-  LH_REQUIRE(reduction >= LH_REDUCE_NONE && reduction <= LH_REDUCE_SUM, LH_ERR_ARG, "linear_xent: bad reduction");
-  LH_REQUIRE(target && loss && lse2 && tgrad && row_scale && (inv_count || reduction == LH_REDUCE_NONE), LH_ERR_ARG,
-             "linear_xent: null pointer");
+  LH_REQUIRE(target && loss, LH_ERR_ARG, "linear_xent: null pointer");
   LH_ARCH();
-  return linear_xent_fwd(hidden, weight, (const long long*)target, ignore_index, N, V, D, reduction, loss, lse2, tgrad,
-                         row_scale, inv_count, ws, S_(stream));
+  return linear_xent_fwd(hidden, weight, (const long long*)target, ignore_index, N, V, D, reduction, loss, kept, ws,
+                         S_(stream));
 }
 
-int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* target, int N, int V, int D,
-                       const float* lse2, const float* tgrad, const float* row_scale, const float* inv_count,
-                       const float* gout, int gout_stride, void* dhidden, void* dweight, void* ws, size_t ws_bytes,
+int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* target, int N, int V, int D, int reduction,
+                       const void* kept, const float* gout, void* dhidden, void* dweight, void* ws, size_t ws_bytes,
                        void* stream) {
   g_err[0] = 0;
-  int rc = loss_check("linear_xent_bwd", hidden, weight, N, V, D, 0, 1.f, ws, ws_bytes, 1);
+  int rc = loss_check("linear_xent_bwd", hidden, weight, N, V, D, 0, 1.f, reduction, kept, ws, ws_bytes, 1);
   if (rc) return rc;
-  LH_REQUIRE(target && lse2 && tgrad && row_scale && gout && dhidden && dweight, LH_ERR_ARG,
-             "linear_xent_bwd: null pointer");
-  LH_REQUIRE(gout_stride == 0 || gout_stride == 1, LH_ERR_ARG, "linear_xent_bwd: gout_stride must be 0 or 1");
+  LH_REQUIRE(target && gout && dhidden && dweight, LH_ERR_ARG, "linear_xent_bwd: null pointer");
   LH_REQUIRE(!(((uintptr_t)dhidden | (uintptr_t)dweight) & 15), LH_ERR_ARG,
              "linear_xent_bwd: gradients must be 16-byte aligned");
   LH_ARCH();
-  return linear_xent_bwd(hidden, weight, (const long long*)target, N, V, D, lse2, tgrad, row_scale, inv_count, gout,
-                         gout_stride, dhidden, dweight, ws, S_(stream));
+  return linear_xent_bwd(hidden, weight, (const long long*)target, N, V, D, reduction, kept, gout, dhidden, dweight, ws,
+                         S_(stream));
 }
 
 int lh_linear_distill_fwd(const void* hidden, const void* weight, const void* tv, int t_dtype, const int64_t* ti, int N,
-                          int V, int D, int K, float T, int reduction, float* loss, float* lse2, int32_t* idx,
-                          float* tgrad, float* row_scale, float* inv_count, void* ws, size_t ws_bytes,
+                          int V, int D, int K, float T, int reduction, float* loss, void* kept, void* ws, size_t ws_bytes,
                           void* stream) {
   g_err[0] = 0;
-  int rc = loss_check("linear_distill", hidden, weight, N, V, D, K, T, ws, ws_bytes, 0);
+  int rc = loss_check("linear_distill", hidden, weight, N, V, D, K, T, reduction, kept, ws, ws_bytes, 0);
   if (rc) return rc;
   LH_REQUIRE(K >= 1, LH_ERR_SHAPE, "linear_distill: K must be in [1, 256], got %d", K);
   LH_REQUIRE(float_dtype(t_dtype), LH_ERR_ARG, "linear_distill: bad dtype");
-  LH_REQUIRE(reduction >= LH_REDUCE_NONE && reduction <= LH_REDUCE_SUM, LH_ERR_ARG, "linear_distill: bad reduction");
-  LH_REQUIRE(tv && ti && loss && lse2 && idx && tgrad && row_scale && (inv_count || reduction == LH_REDUCE_NONE),
-             LH_ERR_ARG, "linear_distill: null pointer");
+  LH_REQUIRE(tv && ti && loss, LH_ERR_ARG, "linear_distill: null pointer");
   LH_ARCH();
-  return linear_distill_fwd(hidden, weight, tv, t_dtype, (const long long*)ti, N, V, D, K, T, reduction, loss, lse2, idx,
-                            tgrad, row_scale, inv_count, ws, S_(stream));
+  return linear_distill_fwd(hidden, weight, tv, t_dtype, (const long long*)ti, N, V, D, K, T, reduction, loss, kept, ws,
+                            S_(stream));
 }
 
-int lh_linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float T, const float* lse2,
-                          const int32_t* idx, const float* tgrad, const float* row_scale,
-                          const float* inv_count, const float* gout, int gout_stride, void* dhidden, void* dweight,
-                          void* ws, size_t ws_bytes, void* stream) {
+int lh_linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float T, int reduction,
+                          const void* kept, const float* gout, void* dhidden, void* dweight, void* ws, size_t ws_bytes,
+                          void* stream) {
   g_err[0] = 0;
-  int rc = loss_check("linear_distill_bwd", hidden, weight, N, V, D, K, T, ws, ws_bytes, 1);
+  int rc = loss_check("linear_distill_bwd", hidden, weight, N, V, D, K, T, reduction, kept, ws, ws_bytes, 1);
   if (rc) return rc;
   LH_REQUIRE(K >= 1, LH_ERR_SHAPE, "linear_distill_bwd: K must be in [1, 256], got %d", K);
-  LH_REQUIRE(lse2 && idx && tgrad && row_scale && gout && dhidden && dweight, LH_ERR_ARG,
-             "linear_distill_bwd: null pointer");
-  LH_REQUIRE(gout_stride == 0 || gout_stride == 1, LH_ERR_ARG, "linear_distill_bwd: gout_stride must be 0 or 1");
+  LH_REQUIRE(gout && dhidden && dweight, LH_ERR_ARG, "linear_distill_bwd: null pointer");
   LH_REQUIRE(!(((uintptr_t)dhidden | (uintptr_t)dweight) & 15), LH_ERR_ARG,
              "linear_distill_bwd: gradients must be 16-byte aligned");
   LH_ARCH();
-  return linear_distill_bwd(hidden, weight, N, V, D, K, T, lse2, idx, tgrad, row_scale, inv_count, gout,
-                            gout_stride, dhidden, dweight, ws, S_(stream));
+  return linear_distill_bwd(hidden, weight, N, V, D, K, T, reduction, kept, gout, dhidden, dweight, ws, S_(stream));
 }
 
 }  // extern "C"

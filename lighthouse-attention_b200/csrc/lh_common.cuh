@@ -60,7 +60,7 @@ __host__ __device__ inline long long sel_len(long long N, int L, int p, int k) {
 struct FastDiv {
   uint32_t d, m, s;
   __host__ __device__ FastDiv() : d(1), m(0), s(0) {}
-  __host__ explicit FastDiv(uint32_t div) : d(div) {
+  __host__ __device__ explicit FastDiv(uint32_t div) : d(div) {
     s = 0;
     while ((1ull << s) < div) ++s;
     m = (uint32_t)((((1ull << s) - div) << 32) / div + 1);

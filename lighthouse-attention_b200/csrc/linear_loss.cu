@@ -15,6 +15,11 @@
 // G is rounded to bf16 once, as an operand of bf16 MMAs has to be; its relative
 // error of 2^-9 is that of the bf16 gradients it ends in.  All sums are fp32.
 //
+// Rows without a target (ignored positions, rows without a teacher) are left out of
+// all products where those are long enough to pay for it: the rows that count are
+// packed, and the kernels take their number from device memory.  Whatever an
+// ignored row holds, it reaches nothing.
+//
 // One persistent GEMM kernel does all four products: a pair of SMs
 // (tcgen05.mma.cta_group::2) per 256 x 256 tile, so that each SM loads 128 rows
 // of either operand and both accumulators (2 x 256 TMEM columns) alternate
@@ -44,7 +49,7 @@ constexpr int kThreads = 384;
 constexpr int kOutBuf = 4096;                    // 32 rows x 128 bytes: one store of an epilogue warp
 constexpr int kPairs = 74;
 constexpr int kNone = 0x7fffffff;
-constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994531f;
 
 enum Mode { kStats, kGrad, kDH, kDW };
 enum Out { kOutBf16, kOutPlane, kOutPlaneAdd };
@@ -56,28 +61,38 @@ __host__ __device__ constexpr int stages(int mode) { return mode == kStats ? 6 :
 __host__ __device__ constexpr int bufs(int mode) { return mode == kStats ? 1 : 2; }
 constexpr int smem_bytes(int mode) { return 1024 + stages(mode) * 2 * kOpBytes + 8 * bufs(mode) * kOutBuf + 512; }
 
+// Walk of the tiles: split, group of gm row blocks, column block, row block in the group.
+struct Sched {
+  int M, tiles_m, gm, kb, splits, total, packed;
+  FastDiv per_split, per_group, per_col, per_col_last;
+};
+
 struct Smem {
   uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drain;
+  Sched sched;
   uint32_t tmem_base;
   int abort;
 };
 static_assert(sizeof(Smem) <= 512 && smem_bytes(kStats) <= 232448 && smem_bytes(kGrad) <= 232448, "barriers do not fit their space");
 
+constexpr int kSplitTable = 2 * kPairs;
 struct Args {
   int M, N;                       // rows and columns of the result
-  int tiles_m, tiles_n, splits, kb, gm;
-  FastDiv per_split, per_group, per_col, per_col_last;   // tiles of a split, a group, and of its columns
+  int tiles_n, splits, kb, gm;
+  int n_rows;                     // rows of hidden
+  const int* rows;                // NULL, or: number of packed rows, their rows of hidden, (and back)
+  uint8_t split_of[kSplitTable];  // kDH: parts of the K range by the number of row blocks, 1 beyond the table
   int b_off;                      // first row of B's operand (vocabulary piece)
   int out;                        // kDH, kDW: Out
-  // targets: int64 (K = 1, SPARSE false) or sorted int32 (K, M), a row's entries M apart
+  // targets: int64 (K = 1, SPARSE false) or sorted int32 (K, n_rows), a row's entries n_rows apart
   const long long* target;
   const int* idx;
   int K;
-  float a2;                       // log2(e) / T
-  float2* stats;                  // kStats: (2 tiles_n, M) maximum and sum of a row's 128 columns
-  float* slog;                    // kStats: logits of the targets (K, M) out
+  float a2;                       // exponent_scale()
+  float2* stats;                  // kStats: (2 tiles_n, n_rows) maximum and sum of a row's 128 columns
+  float* slog;                    // kStats: logits of the targets (K, n_rows) out
   unsigned* ticket;               // kStats: set to 0 for finish_kernel
-  const float* gval;              // kGrad: exp(s - lse) - p at the targets (K, M)
+  const float* gval;              // kGrad: exp(s - lse) - p at the targets (K, n_rows)
   const float* lse2;              // kGrad: log2-sum-exp2 of s a2
   const float *gout, *row_scale, *inv_count;
   int gstride;
@@ -98,7 +113,9 @@ __device__ __forceinline__ int lower_bound(const int* __restrict__ idx, int K, s
 template <int MODE, bool SPARSE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 const __grid_constant__ CUtensorMap tmO, const Args a) {
+                 const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmP,
+                 const __grid_constant__ Args a) {
+  // tmP: the packed rows, in the place of hidden (A of kStats and kGrad, B of kDW)
   constexpr bool kAMn = MODE == kDW, kBMn = MODE == kDH || MODE == kDW;
   constexpr int kStages = stages(MODE), kBufs = bufs(MODE);
   extern __shared__ uint8_t smem_raw[];
@@ -110,9 +127,27 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
-  const int total = a.tiles_m * a.tiles_n * a.splits;
 
   if (threadIdx.x == 0) {
+    Sched& c = sm->sched;
+    c.M = a.M;
+    c.kb = a.kb;
+    c.packed = 0;
+    if (a.rows) {
+      const int live = *a.rows;
+      if (MODE == kDW) c.kb = (live + kTK - 1) / kTK;
+      else c.M = live;
+      c.packed = live < a.n_rows;
+    }
+    c.tiles_m = (c.M + kTM - 1) / kTM;
+    c.gm = max(1, min(a.gm, c.tiles_m));
+    c.splits = a.splits;
+    if (MODE == kDH) c.splits = min(a.splits, c.tiles_m < kSplitTable ? (int)a.split_of[c.tiles_m] : 1);
+    c.total = c.tiles_m * a.tiles_n * c.splits;
+    c.per_split = FastDiv(max(1, c.tiles_m * a.tiles_n));
+    c.per_group = FastDiv(c.gm * a.tiles_n);
+    c.per_col = FastDiv(c.gm);
+    c.per_col_last = FastDiv(max(1, c.tiles_m % c.gm));
     if (MODE == kStats && blockIdx.x == 0) *a.ticket = 0;
     for (int s = 0; s < kStages; ++s) { mbar_init(&sm->full[s], 1); mbar_init(&sm->empty[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&sm->acc_full[b], 1); mbar_init(&sm->acc_empty[b], 16); }
@@ -128,18 +163,20 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   tc_fence_after();
   const uint32_t tbase = sm->tmem_base;
   volatile int* abort = &sm->abort;
+  const Sched& sched = sm->sched;
+  const int total = sched.total, M = sched.M;
 
-  // tile t -> split, row block, column block: gm row blocks at a time, rows first
+  // tile t -> split, row block, column block
   auto decode = [&](int t, int& m, int& n, int& k0, int& k1, int& split) {
     uint32_t sp, r, g, x, y;
-    a.per_split.divmod(t, sp, r);
-    a.per_group.divmod(r, g, r);
-    if ((int)((g + 1) * a.gm) <= a.tiles_m) a.per_col.divmod(r, x, y);
-    else a.per_col_last.divmod(r, x, y);
-    m = g * a.gm + y;
+    sched.per_split.divmod(t, sp, r);
+    sched.per_group.divmod(r, g, r);
+    if ((int)((g + 1) * sched.gm) <= sched.tiles_m) sched.per_col.divmod(r, x, y);
+    else sched.per_col_last.divmod(r, x, y);
+    m = g * sched.gm + y;
     n = x;
     split = sp;
-    const int q = a.kb / a.splits, rem = a.kb - q * a.splits;
+    const int q = sched.kb / sched.splits, rem = sched.kb - q * sched.splits;
     k0 = split * q + min(split, rem);
     k1 = k0 + q + (split < rem ? 1 : 0);
   };
@@ -148,8 +185,10 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     if (warp == 0) {
       // ---------------------------------------------------------- TMA producer
       if (lane == 0) {
-        tma_prefetch_desc(&tmA);
-        tma_prefetch_desc(&tmB);
+        const CUtensorMap* mapA = kAMn || MODE == kDH || !sched.packed ? &tmA : &tmP;
+        const CUtensorMap* mapB = MODE == kDW && sched.packed ? &tmP : &tmB;
+        tma_prefetch_desc(mapA);
+        tma_prefetch_desc(mapB);
         uint32_t it = 0;
         bool ok = true;
         for (int t = pair; t < total && ok; t += n_pairs) {
@@ -166,10 +205,10 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             uint8_t* pb = sB + s * kOpBytes;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              if (kAMn) tma_load_2d_pair(pa + j * kBox, &tmA, bar, ra + 64 * j, k * kTK);
-              else tma_load_2d_pair(pa + j * kBox, &tmA, bar, k * kTK, ra + 64 * j);
-              if (kBMn) tma_load_2d_pair(pb + j * kBox, &tmB, bar, rb + 64 * j, a.b_off + k * kTK);
-              else tma_load_2d_pair(pb + j * kBox, &tmB, bar, k * kTK, a.b_off + rb + 64 * j);
+              if (kAMn) tma_load_2d_pair(pa + j * kBox, mapA, bar, ra + 64 * j, k * kTK);
+              else tma_load_2d_pair(pa + j * kBox, mapA, bar, k * kTK, ra + 64 * j);
+              if (kBMn) tma_load_2d_pair(pb + j * kBox, mapB, bar, rb + 64 * j, a.b_off + k * kTK);
+              else tma_load_2d_pair(pb + j * kBox, mapB, bar, k * kTK, a.b_off + rb + 64 * j);
             }
           }
         }
@@ -188,9 +227,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         bool ok = true;
         // (Looking at the next stage's barrier, or waiting for the next accumulator, before a step's
         // MMAs are issued makes the kernel 3 to 8 % slower, not faster.)
-        const int q = a.kb / a.splits, rem = a.kb - q * a.splits;
+        const int q = sched.kb / sched.splits, rem = sched.kb - q * sched.splits;
         for (int t = pair; t < total && ok; t += n_pairs, ++li) {
-          const int steps = q + ((int)a.per_split.div(t) < rem ? 1 : 0);
+          const int steps = q + ((int)sched.per_split.div(t) < rem ? 1 : 0);
           const int b = li & 1;
           const uint32_t acc = tbase + b * kTN;
           if (li >= 2 && !mbar_wait(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort)) break;
@@ -235,7 +274,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const uint32_t acc = lane_base + b * kTN;
         const int row0 = m * kTM + rank * 128 + quad * 32, row = row0 + lane, n0 = n * kTN + half * kCols;
         const int cols = min(kCols, a.N - n0);           // of this warp's half, may be negative
-        const bool live = row < a.M;
+        const bool live = row < M;
+        const int orow = live && a.rows ? __ldg(a.rows + 1 + row) : row;      // row of hidden
         // next target of this row at or behind the half's first column, as a column of the half,
         // and the one behind it, fetched ahead
         int cur = 0, next = kNone, after = kNone;
@@ -244,24 +284,24 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         auto advance = [&]() {
           ++cur;
           next = after == kNone ? kNone : after - g0;
-          after = cur + 1 < a.K ? __ldg(idx + (size_t)(cur + 1) * a.M) : kNone;
+          after = cur + 1 < a.K ? __ldg(idx + (size_t)(cur + 1) * a.n_rows) : kNone;
         };
         float c = 0.f, lse2 = 0.f;
         if constexpr (MODE == kStats || MODE == kGrad) {
           if (live && cols > 0) {
             if constexpr (SPARSE) {
-              idx = a.idx + row;
-              cur = lower_bound(idx, a.K, a.M, g0) - 1;
-              after = cur + 1 < a.K ? __ldg(idx + (size_t)(cur + 1) * a.M) : kNone;
+              idx = a.idx + orow;
+              cur = lower_bound(idx, a.K, a.n_rows, g0) - 1;
+              after = cur + 1 < a.K ? __ldg(idx + (size_t)(cur + 1) * a.n_rows) : kNone;
               advance();
             } else {
-              const long long tv = __ldg(a.target + row) - g0;
+              const long long tv = __ldg(a.target + orow) - g0;
               if (tv >= 0 && tv < kCols) next = (int)tv;
             }
             if constexpr (MODE == kGrad) {
-              const float up = __ldg(a.gout + (size_t)row * a.gstride);
-              if (up != 0.f) c = a.cscale * up * __ldg(a.row_scale + row) * (a.inv_count ? __ldg(a.inv_count) : 1.f);
-              lse2 = __ldg(a.lse2 + row);
+              const float up = __ldg(a.gout + (size_t)orow * a.gstride);
+              if (up != 0.f) c = a.cscale * up * __ldg(a.row_scale + orow) * (a.inv_count ? __ldg(a.inv_count) : 1.f);
+              lse2 = __ldg(a.lse2 + orow);
             }
           }
         }
@@ -288,7 +328,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               for (int ch = 0; ch < 8; ++ch) put(stage, ch, x[4 * ch], x[4 * ch + 1], x[4 * ch + 2], x[4 * ch + 3]);
               while (next < c0 + 32) {
                 const int at = next - c0;
-                a.slog[(size_t)cur * a.M + row] = *reinterpret_cast<const float*>(
+                a.slog[(size_t)cur * a.n_rows + orow] = *reinterpret_cast<const float*>(
                     stage + lane * 128 + (((at >> 2) ^ (lane & 7)) << 4) + (at & 3) * 4);
                 if constexpr (SPARSE) advance();
                 else next = kNone;
@@ -320,7 +360,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             sum += r.x + r.y;
           }
           release();
-          if (live) a.stats[(size_t)(2 * n + half) * a.M + row] = make_float2(mx, sum);
+          if (live) a.stats[(size_t)(2 * n + half) * a.n_rows + row] = make_float2(mx, sum);
         } else {
           const int width = MODE == kGrad || a.out == kOutBf16 ? 64 : 32;      // columns of one store
 #pragma unroll 1
@@ -330,7 +370,12 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (width == 64) tmem_ld32(acc + c0 + 32, y);
             tmem_ld_wait();
             if (c0 + width == kCols) release();
-            if (c0 >= cols || row0 >= a.M) continue;
+            // kGrad writes zeros up to the end of the 64 rows that the last step of kDW takes
+            if (c0 >= cols || row0 >= (MODE == kGrad ? (M + 63) / 64 * 64 : M)) continue;
+            if (MODE == kDW && k0 == k1) {       // no rows at all in this part
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = y[e] = 0;
+            }
             uint8_t* p = stage + buf * kOutBuf;
             if (lane == 0) bulk_wait_read_1();
             __syncwarp();
@@ -355,7 +400,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                 while (next < c0 + 64) {         // the row's targets among these columns (the same one twice: twice alike)
                   const int at = next - c0;
                   *reinterpret_cast<__nv_bfloat16*>(p + lane * 128 + (((at >> 3) ^ (lane & 7)) << 4) + (at & 7) * 2) =
-                      __float2bfloat16_rn(c * __ldg(a.gval + (size_t)cur * a.M + row));
+                      __float2bfloat16_rn(c * __ldg(a.gval + (size_t)cur * a.n_rows + orow));
                   if constexpr (SPARSE) advance();
                   else next = kNone;
                 }
@@ -459,6 +504,76 @@ teacher_kernel(const T* __restrict__ tv, const long long* __restrict__ ti, int N
   }
 }
 
+// ---- the rows that count, packed: rows = {their number, row of hidden of each, (n_rows)
+// place of each row of hidden or -1 (n_rows)}.  Blocks of 1024 rows.
+template <bool SPARSE>
+__device__ __forceinline__ bool row_counts(const long long* target, long long ignore, const float* row_scale, int i) {
+  return SPARSE ? row_scale[i] != 0.f : target[i] != ignore;
+}
+// Counts per block; what the losses of the other rows are.
+template <bool SPARSE>
+__global__ void __launch_bounds__(1024)
+mark_kernel(const long long* __restrict__ target, long long ignore, float* row_scale, float* __restrict__ lse2,
+            float* __restrict__ loss_rows, int N, int* __restrict__ counts) {
+  const int i = blockIdx.x * 1024 + threadIdx.x;
+  const bool yes = i < N && row_counts<SPARSE>(target, ignore, row_scale, i);
+  if (i < N && !yes) {
+    row_scale[i] = 0.f;
+    lse2[i] = 0.f;
+    if (loss_rows) loss_rows[i] = 0.f;
+  }
+  const int n = __syncthreads_count(yes);
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+template <bool SPARSE>
+__global__ void __launch_bounds__(1024)
+index_kernel(const long long* __restrict__ target, long long ignore, const float* __restrict__ row_scale, int N,
+             const int* __restrict__ counts, int* __restrict__ rows) {
+  __shared__ int sums[2][32];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  int before = 0, all = 0;
+  for (int b = tid; b < (int)gridDim.x; b += 1024) {
+    const int c = counts[b];
+    all += c;
+    if (b < (int)blockIdx.x) before += c;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    before += __shfl_xor_sync(~0u, before, o);
+    all += __shfl_xor_sync(~0u, all, o);
+  }
+  if (lane == 0) { sums[0][w] = before; sums[1][w] = all; }
+  __syncthreads();
+  before = all = 0;
+  for (int k = 0; k < 32; ++k) { before += sums[0][k]; all += sums[1][k]; }
+  if (blockIdx.x == 0 && tid == 0) rows[0] = all;
+  const int i = blockIdx.x * 1024 + tid;
+  const bool yes = i < N && row_counts<SPARSE>(target, ignore, row_scale, i);
+  const unsigned mask = __ballot_sync(~0u, yes);
+  __syncthreads();
+  if (lane == 0) sums[0][w] = __popc(mask);
+  __syncthreads();
+  int at = before + __popc(mask & ((1u << lane) - 1));
+  for (int k = 0; k < w; ++k) at += sums[0][k];
+  if (yes) rows[1 + at] = i;
+  if (i < N) rows[1 + N + i] = yes ? at : -1;
+}
+// One warp per packed row; zeros behind the last up to a multiple of 64 rows, the
+// depth of kDW's steps.  Nothing to do where every row counts.
+__global__ void __launch_bounds__(256)
+pack_kernel(const uint4* __restrict__ hidden, const int* __restrict__ rows, int N, int chunks, uint4* __restrict__ out) {
+  const int live = rows[0], lane = threadIdx.x & 31;
+  const int j = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (live == N || j >= min(N, (live + 63) / 64 * 64)) return;
+  uint4* o = out + (size_t)j * chunks;
+  if (j < live) {
+    const uint4* h = hidden + (size_t)rows[1 + j] * chunks;
+    for (int c = lane; c < chunks; c += 32) o[c] = __ldg(h + c);
+  } else {
+    for (int c = lane; c < chunks; c += 32) o[c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // Joins the (maximum, sum) parts of RB rows per block (thread = row of the block x
 // slot of its parts, slots a power of two), forms the rows' losses and turns the
 // targets' logits into exp(s - lse) - p, what the backward takes off the softmax.
@@ -467,6 +582,7 @@ teacher_kernel(const T* __restrict__ tv, const long long* __restrict__ ti, int N
 // 1 / count.
 struct FinishArgs {
   const float2* stats;
+  const int* rows;                   // as in Args
   int parts, N, V, K, slots, reduction;
   const long long* target;
   long long ignore;
@@ -477,6 +593,9 @@ struct FinishArgs {
   float *row_scale, *lse2, *loss, *inv_count;
   double2* part;
   unsigned* ticket;
+  float up;                               // what exponent_scale() adds to log2(e) / T, as a factor
+  const __nv_bfloat16 *hidden, *weight;   // the target's logit is summed here in fp32, or NULL
+  int D;
 };
 
 template <bool SPARSE, int RB>
@@ -486,7 +605,9 @@ finish_kernel(const FinishArgs a) {
   __shared__ double2 tot[32];
   __shared__ bool last;
   const int tid = threadIdx.x, r = tid % RB, slot = tid / RB, N = a.N, K = a.K;
-  const int row = blockIdx.x * RB + r;
+  const int j = blockIdx.x * RB + r;
+  const bool live = j < (a.rows ? a.rows[0] : N);
+  const int row = a.rows && live ? a.rows[1 + j] : j;
   auto join = [&](float2 u, float2 v) {
     const float mn = fmaxf(u.x, v.x);
     const float mb = mn == -INFINITY ? 0.f : mn * a.a2;
@@ -494,9 +615,9 @@ finish_kernel(const FinishArgs a) {
                                (v.x == -INFINITY ? v.y : v.y * ex2(fmaf(v.x, a.a2, -mb))));
   };
   float2 st = make_float2(-INFINITY, 0.f);
-  if (row < N) {
+  if (live) {
 #pragma unroll 4
-    for (int t = slot; t < a.parts; t += a.slots) st = join(st, a.stats[(size_t)t * N + row]);
+    for (int t = slot; t < a.parts; t += a.slots) st = join(st, a.stats[(size_t)t * N + j]);
   }
   sh[tid] = st;
   __syncthreads();
@@ -504,12 +625,42 @@ finish_kernel(const FinishArgs a) {
     if (slot < o) sh[tid] = join(sh[tid], sh[tid + o * RB]);
     __syncthreads();
   }
+  if (!SPARSE && RB == 8 && a.hidden) {
+    // 4 warps per row sum the target's logit anew: single logits of the tensor core are off by
+    // 6e-6 at random (D = 4096), too much for the loss of one position
+    __shared__ float dots[8][4];
+    const int w = tid >> 5, lane = tid & 31, jj = blockIdx.x * RB + (w >> 2);
+    float x = 0.f;
+    if (w < 32 && jj < (a.rows ? a.rows[0] : N)) {
+      const int rr = a.rows ? a.rows[1 + jj] : jj;
+      const long long t = a.target[rr];
+      if (t >= 0 && t < a.V) {
+        const __nv_bfloat16 *hp = a.hidden + (size_t)rr * a.D, *wp = a.weight + (size_t)t * a.D;
+        for (int c = ((w & 3) * 32 + lane) * 8; c < a.D; c += 1024) {
+          float u[8], v[8];
+          load16(hp + c, u);
+          load16(wp + c, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x = fmaf(u[e], v[e], x);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+    if (lane == 0) dots[w >> 2][w & 3] = x;
+    __syncthreads();
+    if (live && slot == 0) {
+      const long long t = a.target[row];
+      // in the scale of the tensor core's logits, which the exponents take
+      if (t >= 0 && t < a.V) a.slog[row] = ((dots[r][0] + dots[r][1]) + (dots[r][2] + dots[r][3])) / a.up;
+    }
+  }
   const float2 all = sh[r];
   const float l2 = fmaf(all.x, a.a2, log2f(all.y));
   float loss = 0.f, scale = 0.f;
   if constexpr (SPARSE) {
     float x = 0.f;
-    if (row < N) {
+    if (live) {
       for (int k = slot; k < K; k += a.slots) {
         const size_t at = (size_t)k * N + row;
         const int me = a.idx[at];
@@ -517,8 +668,8 @@ finish_kernel(const FinishArgs a) {
         const float s = a.slog[at], p = a.prob[at];
         if (p > 0.f) x = fmaf(p, (l2 - s * a.a2) * kLn2, x);
         float same = p;                            // entries with the same index add up
-        for (int j = k - 1; j >= 0 && a.idx[(size_t)j * N + row] == me; --j) same += a.prob[(size_t)j * N + row];
-        for (int j = k + 1; j < K && a.idx[(size_t)j * N + row] == me; ++j) same += a.prob[(size_t)j * N + row];
+        for (int i = k - 1; i >= 0 && a.idx[(size_t)i * N + row] == me; --i) same += a.prob[(size_t)i * N + row];
+        for (int i = k + 1; i < K && a.idx[(size_t)i * N + row] == me; ++i) same += a.prob[(size_t)i * N + row];
         a.slog[at] = ex2(fmaf(s, a.a2, -l2)) - same;
       }
     }
@@ -529,21 +680,21 @@ finish_kernel(const FinishArgs a) {
       if (slot < o) sh[tid].x += sh[tid + o * RB].x;
       __syncthreads();
     }
-    if (row < N && slot == 0) {
+    if (live && slot == 0) {
       scale = a.row_scale[row];
       if (scale != 0.f) loss = scale * a.t2 * (a.ent[row] + sh[r].x);
     }
-  } else if (row < N && slot == 0) {
+  } else if (live && slot == 0) {
     const long long t = a.target[row];
     if (t != a.ignore) {
       const bool in = t >= 0 && t < a.V;
       scale = in ? 1.f : __int_as_float(0x7fc00000);
-      loss = in ? l2 * kLn2 - a.slog[row] : scale;
+      loss = in ? (l2 - a.slog[row] * a.a2) * kLn2 : scale;
       if (in) a.slog[row] = ex2(fmaf(a.slog[row], a.a2, -l2)) - 1.f;
     }
     a.row_scale[row] = scale;
   }
-  if (row < N && slot == 0) {
+  if (live && slot == 0) {
     a.lse2[row] = l2;
     if (a.reduction == LH_REDUCE_NONE) a.loss[row] = loss;
   }
@@ -585,20 +736,47 @@ finish_kernel(const FinishArgs a) {
   }
 }
 
-// out (bf16) = sum of the fp32 planes (rows x cols each), in their order.
+// out (bf16) = sum of the fp32 planes (n_rows x cols each), in their order.  With
+// rows: the planes hold packed rows, split_of tells how many planes their number of
+// row blocks had, and a row that does not count is 0.
+struct PlanesArgs {
+  const float* planes;
+  int n, n_rows, cols;
+  const int* rows;
+  uint8_t split_of[kSplitTable];
+  __nv_bfloat16* out;
+};
 __global__ void __launch_bounds__(256)
-planes_kernel(const float* __restrict__ planes, int n, size_t plane, __nv_bfloat16* __restrict__ out) {
-  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8; i < plane; i += (size_t)gridDim.x * 256 * 8) {
-    float v[8], u[8];
-    load16(planes + i, v);
-    load16(planes + i + 4, v + 4);
-    for (int k = 1; k < n; ++k) {
-      load16(planes + k * plane + i, u);
-      load16(planes + k * plane + i + 4, u + 4);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += u[e];
+planes_kernel(const __grid_constant__ PlanesArgs a) {
+  const size_t plane = (size_t)a.n_rows * a.cols;
+  const int chunks = a.cols / 8;
+  int n = a.n;
+  if (a.rows) {
+    const int t = (a.rows[0] + kTM - 1) / kTM;
+    n = min(n, t < kSplitTable ? (int)a.split_of[t] : 1);
+  }
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < plane / 8; i += (size_t)gridDim.x * 256) {
+    size_t from = i;                              // 8-element chunk of a plane
+    bool live = true;
+    if (a.rows) {
+      const size_t row = i / chunks;
+      const int at = a.rows[1 + a.n_rows + row];
+      live = at >= 0;
+      from = (size_t)at * chunks + (i - row * chunks);
     }
-    store16(out + i, v);
+    float v[8] = {};
+    if (live) {
+      const float* p = a.planes + from * 8;
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        float u[8];
+        load16(p + k * plane, u);
+        load16(p + k * plane + 4, u + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += u[e];
+      }
+    }
+    store16(a.out + i * 8, v);
   }
 }
 
@@ -655,24 +833,21 @@ static int map_store(CUtensorMap* m, void* p, bool f32, long long planes, long l
 }
 
 template <int MODE, bool SPARSE>
-static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, Args a, long long K, cudaStream_t st) {
-  a.tiles_m = (a.M + kTM - 1) / kTM;
+static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const CUtensorMap& mp, Args& a,
+                  long long K, cudaStream_t st) {
+  const int tiles_m = (a.M + kTM - 1) / kTM;
   a.tiles_n = (a.N + kTN - 1) / kTN;
   a.kb = (int)((K + kTK - 1) / kTK);
   // Row blocks walked together: as many as keep their operand rows in about half of L2, at least
   // eight (eight by nine tiles are one wave of the 74 pairs).
   long long gm = (48ll << 20) / (kTM * 2ll * a.kb * kTK);
   if (gm < 8) gm = 8;
-  a.gm = (int)(gm < a.tiles_m ? gm : a.tiles_m);
-  a.per_split = FastDiv(a.tiles_m * a.tiles_n);
-  a.per_group = FastDiv(a.gm * a.tiles_n);
-  a.per_col = FastDiv(a.gm);
-  a.per_col_last = FastDiv(a.tiles_m % a.gm ? a.tiles_m % a.gm : 1);
-  const long long total = (long long)a.tiles_m * a.tiles_n * a.splits;
+  a.gm = (int)(gm < tiles_m ? gm : tiles_m);
+  const long long total = (long long)tiles_m * a.tiles_n * a.splits;
   const int pairs = (int)(total < kPairs ? total : kPairs);
   cudaError_t e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MODE));
   if (e != cudaSuccess) { set_error("linear loss: %s", cudaGetErrorString(e)); return LH_ERR_LAUNCH; }
-  loss_gemm_kernel<MODE, SPARSE><<<2 * pairs, kThreads, smem_bytes(MODE), st>>>(ma, mb, mo, a);
+  loss_gemm_kernel<MODE, SPARSE><<<2 * pairs, kThreads, smem_bytes(MODE), st>>>(ma, mb, mo, mp, a);
   return check_launch("loss_gemm_kernel");
 }
 
@@ -692,89 +867,170 @@ static int pick_splits(long long M, long long N, long long K) {
   return pick;
 }
 
+static size_t up(size_t n) { return (n + 255) & ~size_t(255); }
+
+// Whether the rows that count are packed: where the products are long against the
+// three small kernels that do it (about 8 us; a product of 5e10 takes 40 us or more)
+// and more than one row block is there to be saved.
+static bool packs(long long N, long long V, long long D) { return N > kTM && 2.0 * N * V * D >= 5e10; }
+
 struct Plan {
   long long C;                 // columns of a vocabulary piece, a multiple of 256
   int pieces, dh_splits, dw_splits;
+  uint8_t split_of[kSplitTable];
   bool dh_planes;
-  size_t g, dh, dw, total;     // bytes
+  size_t g, dh, dw, packed, total;     // bytes
 };
 constexpr long long kPieceBytes = 512ll << 20;
 
-static size_t up(size_t n) { return (n + 255) & ~size_t(255); }
-
 static Plan plan(long long N, long long V, long long D) {
-  Plan p;
+  Plan p{};
   long long C = kPieceBytes / (2 * N) / kTN * kTN;
   if (C < kTN) C = kTN;
   const long long Vp = (V + kTN - 1) / kTN * kTN;
   p.pieces = (int)((Vp + C - 1) / C);
   p.C = ((Vp + p.pieces - 1) / p.pieces + kTN - 1) / kTN * kTN;      // pieces of about equal size
   p.pieces = (int)((Vp + p.C - 1) / p.C);
-  p.dh_splits = pick_splits(N, D, p.C < V ? p.C : V);
-  p.dw_splits = pick_splits(p.C < V ? p.C : V, D, N);
-  p.dh_planes = p.pieces > 1 || p.dh_splits > 1;
+  const long long cols = p.C < V ? p.C : V, tiles = (N + kTM - 1) / kTM;
+  const bool pack = packs(N, V, D);
+  // dH: the parts by the number of row blocks that are left; at most twice those of all rows
+  p.dh_splits = tiles < kSplitTable ? pick_splits(N, D, cols) : 1;
+  const int most = pack ? 2 * p.dh_splits : p.dh_splits;
+  for (int t = 1; t < kSplitTable; ++t) {
+    int s = t == tiles ? p.dh_splits : t < tiles && pack ? pick_splits((long long)t * kTM, D, cols) : 1;
+    p.split_of[t] = (uint8_t)(s < most ? s : most);
+  }
+  for (int t = 1; t < kSplitTable && t <= tiles; ++t)
+    if (p.split_of[t] > p.dh_splits) p.dh_splits = p.split_of[t];
+  p.dw_splits = pick_splits(cols, D, N);
+  p.dh_planes = pack || p.pieces > 1 || p.dh_splits > 1;
   p.g = up((size_t)N * p.C * 2);
   p.dh = p.dh_planes ? up((size_t)p.dh_splits * N * D * 4) : 0;
   p.dw = p.dw_splits > 1 ? up((size_t)p.dw_splits * p.C * D * 4) : 0;
-  p.total = p.g + p.dh + p.dw;
+  p.packed = pack ? up((size_t)N * D * 2) : 0;
+  p.total = p.g + p.dh + p.dw + p.packed;
   return p;
 }
 
-// stats, the blocks' sums and their ticket; distillation (K > 0): sum p log p and p of the rows
-static size_t stats_bytes(long long N, long long V) {
-  return up((size_t)((V + kTN - 1) / kTN) * 2 * N * sizeof(float2)) + up((size_t)((N + 7) / 8) * sizeof(double2)) + 256;
-}
-static size_t fwd_workspace(long long N, long long V, long long K) {
-  return stats_bytes(N, V) + (K ? up((size_t)N * sizeof(float)) + up((size_t)N * K * sizeof(float)) : 0);
-}
+// What the forward leaves for the backward.
+struct Kept {
+  float *lse2, *row_scale, *inv_count, *tgrad;   // (N), (N), (1), (max(K, 1), N)
+  int *idx, *rows;                               // (K, N) sorted targets, (2 N + 1) packed rows
+  size_t bytes;
+  Kept(void* base, long long N, long long K) {
+    char* p = (char*)base;
+    auto take = [&](size_t n) { char* q = p; p += up(n); return q; };
+    lse2 = (float*)take(4 * N);
+    row_scale = (float*)take(4 * N);
+    inv_count = (float*)take(4);
+    tgrad = (float*)take(4 * N * (K > 1 ? K : 1));
+    idx = (int*)take(4 * N * K);
+    rows = (int*)take(4 * (2 * N + 1));
+    bytes = p - (char*)base;
+  }
+};
 
-static int sum_planes(const float* planes, int n, size_t plane, void* out, cudaStream_t st) {
-  size_t blocks = (plane / 8 + 255) / 256;
-  if (blocks > 148 * 16) blocks = 148 * 16;
-  planes_kernel<<<(unsigned)blocks, 256, 0, st>>>(planes, n, plane, (__nv_bfloat16*)out);
+// Workspace of the forward.
+struct FwdSpace {
+  float2* stats;
+  double2* part;
+  unsigned* ticket;
+  int* counts;
+  float *ent, *prob;           // distillation
+  void* packed;
+  size_t bytes;
+  FwdSpace(void* base, long long N, long long V, long long D, long long K) {
+    char* p = (char*)base;
+    auto take = [&](size_t n) { char* q = p; p += up(n); return q; };
+    stats = (float2*)take((size_t)((V + kTN - 1) / kTN) * 2 * N * sizeof(float2));
+    part = (double2*)take((size_t)((N + 7) / 8) * sizeof(double2));
+    ticket = (unsigned*)take(4);
+    counts = (int*)take(4 * ((N + 1023) / 1024));
+    ent = (float*)take(K ? 4 * N : 0);
+    prob = (float*)take(4 * N * K);
+    packed = take(packs(N, V, D) ? (size_t)N * D * 2 : 0);
+    bytes = p - (char*)base;
+  }
+};
+
+// log2(e) / T, and what the tensor core's sums lose: adding a product it cuts the sum
+// towards zero, so that a logit of D products comes out smaller by 1.02e-9 D of itself on
+// average (measured 1.01 to 1.04e-9 at D from 1024 to 4096; half an ulp of the running
+// sum per 16 products makes it).  The factor takes that out of the exponents and losses:
+// the loss is then off by 1e-7 where it was by 2.5e-6 (D = 4096).
+static float exponent_scale(float T, int D) { return (float)(1.4426950408889634 / T * (1.0 + 1.02e-9 * D)); }
+
+static int sum_planes(const float* planes, const Plan* p, int n, int rows, int cols, const int* packed, void* out,
+                      cudaStream_t st) {
+  PlanesArgs a{planes, n, rows, cols, packed, {}, (__nv_bfloat16*)out};
+  if (p)
+    for (int t = 0; t < kSplitTable; ++t) a.split_of[t] = p->split_of[t];
+  const size_t blocks = ((size_t)rows * (cols / 8) + 255) / 256;
+  planes_kernel<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(a);
   return check_launch("planes_kernel");
 }
 
-struct Targets {
-  const long long* target;   // cross entropy
+static int pack_rows(const void* hidden, const int* rows, int N, int D, void* out, cudaStream_t st) {
+  pack_kernel<<<(N + 7) / 8, 256, 0, st>>>((const uint4*)hidden, rows, N, D / 8, (uint4*)out);
+  return check_launch("pack_kernel");
+}
+
+struct Problem {
+  const void *hidden, *weight;
+  int N, V, D;
+  const long long* target;     // cross entropy
   long long ignore;
-  const int* idx;            // distillation
-  int K;
+  int K;                       // distillation: entries of a row, 0 else
   float T;
 };
 
 template <bool SPARSE>
-static int forward(const void* hidden, const void* weight, int N, int V, int D, const Targets& tg, const float* prob,
-                   const float* ent, int reduction, float* loss, float* lse2, float* slog, float* row_scale, float* inv_count, void* ws,
-                   cudaStream_t st) {
+static int forward(const Problem& q, int reduction, float* loss, const Kept& kp, const FwdSpace& ws, cudaStream_t st) {
   int rc = make_context_current();
   if (rc) return rc;
-  CUtensorMap mh, mw;
-  if ((rc = map_load(&mh, hidden, N, D, D)) || (rc = map_load(&mw, weight, V, D, D))) return rc;
+  const int N = q.N, V = q.V, D = q.D, K = q.K ? q.K : 1;
+  CUtensorMap mh, mw, mp;
+  if ((rc = map_load(&mh, q.hidden, N, D, D)) || (rc = map_load(&mw, q.weight, V, D, D))) return rc;
+  mp = mh;
+  const int* rows = nullptr;
+  if (packs(N, V, D)) {
+    const int blocks = (N + 1023) / 1024;
+    mark_kernel<SPARSE><<<blocks, 1024, 0, st>>>(q.target, q.ignore, kp.row_scale, kp.lse2,
+                                                 reduction == LH_REDUCE_NONE ? loss : nullptr, N, ws.counts);
+    if ((rc = check_launch("mark_kernel"))) return rc;
+    index_kernel<SPARSE><<<blocks, 1024, 0, st>>>(q.target, q.ignore, kp.row_scale, N, ws.counts, kp.rows);
+    if ((rc = check_launch("index_kernel")) || (rc = pack_rows(q.hidden, kp.rows, N, D, ws.packed, st)) ||
+        (rc = map_load(&mp, ws.packed, N, D, D)))
+      return rc;
+    rows = kp.rows;
+  }
   const int parts = (V + kTN - 1) / kTN * 2;
-  float2* stats = (float2*)ws;
-  double2* part = (double2*)((char*)ws + up((size_t)parts * N * sizeof(float2)));
-  unsigned* ticket = (unsigned*)((char*)part + up((size_t)((N + 7) / 8) * sizeof(double2)));
   Args a{};
-  a.M = N;
+  a.M = a.n_rows = N;
   a.N = V;
   a.splits = 1;
-  a.target = tg.target;
-  a.idx = tg.idx;
-  a.K = tg.K;
-  a.a2 = kLog2e / tg.T;
-  a.stats = stats;
-  a.slog = slog;
-  a.ticket = ticket;
-  if ((rc = launch<kStats, SPARSE>(mh, mw, mw, a, D, st))) return rc;
+  a.rows = rows;
+  a.target = q.target;
+  a.idx = kp.idx;
+  a.K = K;
+  a.a2 = exponent_scale(q.T, D);
+  a.stats = ws.stats;
+  a.slog = kp.tgrad;
+  a.ticket = ws.ticket;
+  if ((rc = launch<kStats, SPARSE>(mh, mw, mw, mp, a, D, st))) return rc;
   // Rows per block: eight with up to 128 slots each where a row has many parts (16 rows of 1000
   // parts: 7 us, 17 with 32 rows per block), 256 where it has up to four (65536 rows of two parts:
   // 14 us with 32 rows per block, most of it the 2048 blocks' sum).
-  const int want = parts > tg.K ? parts : tg.K;
-  FinishArgs f{stats, parts, N, V, tg.K, 1, reduction, tg.target, tg.ignore, tg.idx, prob, ent, slog, a.a2, tg.T * tg.T,
-               row_scale, lse2, loss, inv_count, part, ticket};
+  const int want = parts > K ? parts : K;
+  FinishArgs f{ws.stats, rows, parts, N, V, K, 1, reduction, q.target, q.ignore, kp.idx, ws.prob, ws.ent, kp.tgrad, a.a2,
+               q.T * q.T, kp.row_scale, kp.lse2, loss, kp.inv_count, ws.part, ws.ticket, 1.f, nullptr, nullptr, D};
   const int rb = want > 32 ? 8 : want > 4 ? 32 : 256;
   while (f.slots < want && f.slots * rb < 1024) f.slots *= 2;
+  if (!SPARSE && V >= 16384) {       // its reads, 4 N D bytes, take 2.6 % of the product's time there, less above
+    f.up = (float)(1.0 + 1.02e-9 * D);
+    f.hidden = (const __nv_bfloat16*)q.hidden;
+    f.weight = (const __nv_bfloat16*)q.weight;
+  }
   const unsigned blocks = (unsigned)((N + rb - 1) / rb);
   if (rb == 8) finish_kernel<SPARSE, 8><<<blocks, rb * f.slots, 0, st>>>(f);
   else if (rb == 256) finish_kernel<SPARSE, 256><<<blocks, rb * f.slots, 0, st>>>(f);
@@ -783,111 +1039,117 @@ static int forward(const void* hidden, const void* weight, int N, int V, int D, 
 }
 
 template <bool SPARSE>
-static int backward(const void* hidden, const void* weight, int N, int V, int D, const Targets& tg, const float* lse2,
-                    const float* gval, const float* row_scale, const float* inv_count, const float* gout, int gstride,
-                    void* dhidden, void* dweight, void* ws, cudaStream_t st) {
+static int backward(const Problem& q, int reduction, const Kept& kp, const float* gout, void* dhidden, void* dweight,
+                    void* ws, cudaStream_t st) {
   int rc = make_context_current();
   if (rc) return rc;
+  const int N = q.N, V = q.V, D = q.D;
   const Plan p = plan(N, V, D);
   char* g = (char*)ws;
   float* dh = (float*)(g + p.g);
   float* dw = (float*)(g + p.g + p.dh);
-  CUtensorMap mh, mw, mdh, mdw, mg, mgo;
-  if ((rc = map_load(&mh, hidden, N, D, D)) || (rc = map_load(&mw, weight, V, D, D))) return rc;
+  char* packed = g + p.g + p.dh + p.dw;
+  CUtensorMap mh, mw, mp, mdh, mdw, mg, mgo;
+  if ((rc = map_load(&mh, q.hidden, N, D, D)) || (rc = map_load(&mw, q.weight, V, D, D))) return rc;
   if ((rc = p.dh_planes ? map_store(&mdh, dh, true, p.dh_splits, N, D, D) : map_store(&mdh, dhidden, false, 1, N, D, D)))
     return rc;
+  mp = mh;
+  const int* rows = nullptr;
+  if (p.packed) {
+    rows = kp.rows;
+    if ((rc = pack_rows(q.hidden, rows, N, D, packed, st)) || (rc = map_load(&mp, packed, N, D, D))) return rc;
+  }
   for (int i = 0; i < p.pieces; ++i) {
     const long long v0 = i * p.C;
     const int cols = (int)(V - v0 < p.C ? V - v0 : p.C);
     if ((rc = map_load(&mg, g, N, cols, p.C)) || (rc = map_store(&mgo, g, false, 1, N, cols, p.C))) return rc;
     Args a{};
-    a.M = N;
+    a.M = a.n_rows = N;
     a.N = cols;
     a.splits = 1;
+    a.rows = rows;
     a.b_off = (int)v0;
-    a.target = tg.target;
-    a.idx = tg.idx;
-    a.K = tg.K;
-    a.a2 = kLog2e / tg.T;
-    a.gval = gval;
-    a.lse2 = lse2;
-    a.row_scale = row_scale;
-    a.inv_count = inv_count;
+    a.target = q.target;
+    a.idx = kp.idx;
+    a.K = q.K ? q.K : 1;
+    a.a2 = exponent_scale(q.T, D);
+    a.gval = kp.tgrad;
+    a.lse2 = kp.lse2;
+    a.row_scale = kp.row_scale;
+    a.inv_count = reduction == LH_REDUCE_NONE ? nullptr : kp.inv_count;
     a.gout = gout;
-    a.gstride = gstride;
-    a.cscale = tg.T;
-    if ((rc = launch<kGrad, SPARSE>(mh, mw, mgo, a, D, st))) return rc;
+    a.gstride = reduction == LH_REDUCE_NONE ? 1 : 0;
+    a.cscale = q.T;
+    if ((rc = launch<kGrad, SPARSE>(mh, mw, mgo, mp, a, D, st))) return rc;
 
     Args x{};
-    x.M = N;
+    x.M = x.n_rows = N;
     x.N = D;
     const int kb = (cols + kTK - 1) / kTK;
     x.splits = p.dh_splits < kb ? p.dh_splits : kb;      // a short last piece may leave planes as they are
+    for (int t = 0; t < kSplitTable; ++t) x.split_of[t] = p.split_of[t];
+    x.rows = rows;
     x.b_off = (int)v0;
     x.out = !p.dh_planes ? kOutBf16 : i ? kOutPlaneAdd : kOutPlane;
-    if ((rc = launch<kDH, false>(mg, mw, mdh, x, cols, st))) return rc;
+    if ((rc = launch<kDH, false>(mg, mw, mdh, mg, x, cols, st))) return rc;
 
     Args y{};
     y.M = cols;
+    y.n_rows = N;
     y.N = D;
     y.splits = p.dw_splits;
+    y.rows = rows;
     y.out = p.dw_splits > 1 ? kOutPlane : kOutBf16;
     char* dw_out = (char*)dweight + (size_t)v0 * D * 2;
     if ((rc = p.dw_splits > 1 ? map_store(&mdw, dw, true, p.dw_splits, cols, D, D)
                               : map_store(&mdw, dw_out, false, 1, cols, D, D)))
       return rc;
-    if ((rc = launch<kDW, false>(mg, mh, mdw, y, N, st))) return rc;
-    if (p.dw_splits > 1 && (rc = sum_planes(dw, p.dw_splits, (size_t)cols * D, dw_out, st))) return rc;
+    if ((rc = launch<kDW, false>(mg, mh, mdw, mp, y, N, st))) return rc;
+    if (p.dw_splits > 1 && (rc = sum_planes(dw, nullptr, p.dw_splits, cols, D, nullptr, dw_out, st))) return rc;
   }
-  return p.dh_planes ? sum_planes(dh, p.dh_splits, (size_t)N * D, dhidden, st) : LH_OK;
+  return p.dh_planes ? sum_planes(dh, &p, p.dh_splits, N, D, rows, dhidden, st) : LH_OK;
 }
 
 }  // namespace ll
 
 size_t linear_loss_workspace_size(int N, int V, int D, int K, int backward) {
-  return backward ? ll::plan(N, V, D).total : ll::fwd_workspace(N, V, K);
+  return backward ? ll::plan(N, V, D).total : ll::FwdSpace(nullptr, N, V, D, K).bytes;
 }
+
+size_t linear_loss_kept_size(int N, int K) { return ll::Kept(nullptr, N, K).bytes; }
 
 int linear_xent_fwd(const void* hidden, const void* weight, const long long* target, long long ignore, int N, int V, int D,
-                    int reduction, float* loss, float* lse2, float* tgrad, float* row_scale, float* inv_count, void* ws,
-                    cudaStream_t st) {
-  const ll::Targets tg{target, ignore, nullptr, 1, 1.f};
-  return ll::forward<false>(hidden, weight, N, V, D, tg, nullptr, nullptr, reduction, loss, lse2, tgrad, row_scale, inv_count, ws, st);
+                    int reduction, float* loss, void* kept, void* ws, cudaStream_t st) {
+  return ll::forward<false>({hidden, weight, N, V, D, target, ignore, 0, 1.f}, reduction, loss, ll::Kept(kept, N, 0),
+                            ll::FwdSpace(ws, N, V, D, 0), st);
 }
 
-int linear_xent_bwd(const void* hidden, const void* weight, const long long* target, int N, int V, int D, const float* lse2,
-                    const float* tgrad, const float* row_scale, const float* inv_count, const float* gout, int gstride,
-                    void* dhidden, void* dweight, void* ws, cudaStream_t st) {
-  const ll::Targets tg{target, 0, nullptr, 1, 1.f};
-  return ll::backward<false>(hidden, weight, N, V, D, tg, lse2, tgrad, row_scale, inv_count, gout, gstride, dhidden,
-                             dweight, ws, st);
+int linear_xent_bwd(const void* hidden, const void* weight, const long long* target, int N, int V, int D, int reduction,
+                    const void* kept, const float* gout, void* dhidden, void* dweight, void* ws, cudaStream_t st) {
+  return ll::backward<false>({hidden, weight, N, V, D, target, 0, 0, 1.f}, reduction, ll::Kept(const_cast<void*>(kept), N, 0),
+                             gout, dhidden, dweight, ws, st);
 }
 
 int linear_distill_fwd(const void* hidden, const void* weight, const void* tv, int tv_dtype, const long long* ti, int N,
-                       int V, int D, int K, float T, int reduction, float* loss, float* lse2, int* idx, float* tgrad,
-                       float* row_scale, float* inv_count, void* ws, cudaStream_t st) {
-  float* ent = (float*)((char*)ws + ll::stats_bytes(N, V));
-  float* prob = (float*)((char*)ent + ll::up((size_t)N * sizeof(float)));
+                       int V, int D, int K, float T, int reduction, float* loss, void* kept, void* ws, cudaStream_t st) {
+  const ll::Kept kp(kept, N, K);
+  const ll::FwdSpace sp(ws, N, V, D, K);
   const unsigned blocks = (unsigned)((N + 3) / 4);
   if (tv_dtype == LH_DTYPE_BF16)
-    ll::teacher_kernel<<<blocks, 128, 4 * K * sizeof(int), st>>>((const __nv_bfloat16*)tv, ti, N, V, K, 1.f / T, idx, prob,
-                                                                ent, row_scale);
+    ll::teacher_kernel<<<blocks, 128, 4 * K * sizeof(int), st>>>((const __nv_bfloat16*)tv, ti, N, V, K, 1.f / T, kp.idx,
+                                                                sp.prob, sp.ent, kp.row_scale);
   else
-    ll::teacher_kernel<<<blocks, 128, 4 * K * sizeof(int), st>>>((const float*)tv, ti, N, V, K, 1.f / T, idx, prob, ent,
-                                                                row_scale);
+    ll::teacher_kernel<<<blocks, 128, 4 * K * sizeof(int), st>>>((const float*)tv, ti, N, V, K, 1.f / T, kp.idx, sp.prob,
+                                                                sp.ent, kp.row_scale);
   int rc = check_launch("teacher_kernel");
   if (rc) return rc;
-  const ll::Targets tg{nullptr, 0, idx, K, T};
-  return ll::forward<true>(hidden, weight, N, V, D, tg, prob, ent, reduction, loss, lse2, tgrad, row_scale, inv_count, ws, st);
+  return ll::forward<true>({hidden, weight, N, V, D, nullptr, 0, K, T}, reduction, loss, kp, sp, st);
 }
 
-int linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float T, const float* lse2,
-                       const int* idx, const float* tgrad, const float* row_scale,
-                       const float* inv_count, const float* gout, int gstride, void* dhidden, void* dweight, void* ws,
-                       cudaStream_t st) {
-  const ll::Targets tg{nullptr, 0, idx, K, T};
-  return ll::backward<true>(hidden, weight, N, V, D, tg, lse2, tgrad, row_scale, inv_count, gout, gstride, dhidden,
-                            dweight, ws, st);
+int linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float T, int reduction,
+                       const void* kept, const float* gout, void* dhidden, void* dweight, void* ws, cudaStream_t st) {
+  return ll::backward<true>({hidden, weight, N, V, D, nullptr, 0, K, T}, reduction, ll::Kept(const_cast<void*>(kept), N, K),
+                            gout, dhidden, dweight, ws, st);
 }
 
 int loss_status(int reset) {

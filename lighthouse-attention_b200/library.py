@@ -282,15 +282,15 @@ def _(x, residual, weight, eps, group):
 
 # --------------------------------------------------------------------------- losses of an output projection
 def _loss_fake(hidden, reduction, K):
-    f = lambda *s: hidden.new_empty(s, dtype=torch.float32)
     N = hidden.shape[0]
-    return (f(N) if reduction == "none" else f()), f(_native.kept_len(N, K))
+    return (hidden.new_empty((N,) if reduction == "none" else (), dtype=torch.float32),
+            hidden.new_empty(_native.kept_size(N, K), dtype=torch.uint8))
 
 
 @torch.library.custom_op(f"{NS}::linear_xent", mutates_args=())
 def linear_xent(hidden: Tensor, weight: Tensor, target: Tensor, ignore_index: int,
                 reduction: str) -> tuple[Tensor, Tensor]:
-    """Cross entropy of hidden (N,D) weight (V,D)^T: loss, and the fp32 values kept for the backward."""
+    """Cross entropy of hidden (N,D) weight (V,D)^T: loss, and what is kept for the backward (uint8)."""
     return _native.linear_xent_fwd(hidden, weight, target, ignore_index, reduction)
 
 
@@ -313,28 +313,26 @@ def _(hidden, weight, target, kept, gout, reduction):
 
 @torch.library.custom_op(f"{NS}::linear_distill", mutates_args=())
 def linear_distill(hidden: Tensor, weight: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, temperature: float,
-                   reduction: str) -> tuple[Tensor, Tensor, Tensor]:
-    """Distillation of hidden (N,D) weight (V,D)^T from K teacher logits per row: loss, and the fp32 values and
-    sorted indices (K,N) kept for the backward."""
+                   reduction: str) -> tuple[Tensor, Tensor]:
+    """Distillation of hidden (N,D) weight (V,D)^T from K teacher logits per row: loss, and what is kept for the
+    backward (uint8)."""
     return _native.linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
 
 
 @linear_distill.register_fake
 def _(hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
-    loss, kept = _loss_fake(hidden, reduction, teacher_indices.shape[1])
-    N, K = teacher_indices.shape
-    return loss, kept, hidden.new_empty((K, N), dtype=torch.int32)
+    return _loss_fake(hidden, reduction, teacher_indices.shape[1])
 
 
 @torch.library.custom_op(f"{NS}::linear_distill_bwd", mutates_args=())
-def linear_distill_bwd(hidden: Tensor, weight: Tensor, kept: Tensor, idx: Tensor, gout: Tensor, temperature: float,
+def linear_distill_bwd(hidden: Tensor, weight: Tensor, kept: Tensor, gout: Tensor, K: int, temperature: float,
                        reduction: str) -> tuple[Tensor, Tensor]:
     """Backward of linear_distill: dhidden (N,D), dweight (V,D)."""
-    return _native.linear_distill_bwd(hidden, weight, kept, idx, gout, temperature, reduction)
+    return _native.linear_distill_bwd(hidden, weight, kept, gout, K, temperature, reduction)
 
 
 @linear_distill_bwd.register_fake
-def _(hidden, weight, kept, idx, gout, temperature, reduction):
+def _(hidden, weight, kept, gout, K, temperature, reduction):
     return hidden.new_empty(hidden.shape), weight.new_empty(weight.shape)
 
 

@@ -41,17 +41,17 @@ class _LinearDistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
         f = _native.linear_distill_fwd if direct(hidden) else _ops.linear_distill
-        loss, kept, idx = f(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
-        ctx.save_for_backward(hidden, weight, kept, idx)
-        ctx.temperature, ctx.reduction = temperature, reduction
+        loss, kept = f(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
+        ctx.save_for_backward(hidden, weight, kept)
+        ctx.K, ctx.temperature, ctx.reduction = teacher_indices.shape[1], temperature, reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        hidden, weight, kept, idx = ctx.saved_tensors
+        hidden, weight, kept = ctx.saved_tensors
         f = _native.linear_distill_bwd if direct(gout) else _ops.linear_distill_bwd
-        dh, dw = f(hidden, weight, kept, idx, gout, ctx.temperature, ctx.reduction)
+        dh, dw = f(hidden, weight, kept, gout, ctx.K, ctx.temperature, ctx.reduction)
         return dh, dw, None, None, None, None
 
 

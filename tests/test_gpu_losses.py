@@ -112,6 +112,42 @@ def test_several_pieces_of_the_vocabulary(lh, cuda):
     _run_xent(lh, cuda, 5000, 120001, 64, "mean", seed=11)
 
 
+# 2 N V D >= 5e10 and more than 256 positions: the rows that count are packed
+BIG = (1000, 50001, 512)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("ignore", [0.0, 0.4, 0.95])
+def test_packed_positions(lh, cuda, ignore, reduction):
+    _run_xent(lh, cuda, *BIG, reduction, seed=40, ignore=ignore)
+
+
+@pytest.mark.parametrize("live", [0, 1, 64, 256, 257, 999])
+def test_packed_positions_at_the_edges(lh, cuda, live):
+    """A given number of positions with a target, the others' hidden rows holding NaN."""
+    N, V, D = BIG
+    g, h, w = _problem(N, V, D, 41, cuda)
+    target = torch.randint(0, V, (N,), generator=g).to(cuda)
+    keep = torch.zeros(N, dtype=torch.bool)
+    keep[torch.randperm(N, generator=g)[:live]] = True
+    keep = keep.to(cuda)
+    target[~keep] = -100
+    h[~keep] = float("nan")
+    loss, dh, dw = _xent(lh, h, w, target, "mean")
+    clean = torch.where(keep[:, None], h, torch.zeros_like(h))
+    _check(loss, dh, dw, clean, w, target.clamp(min=0)[:, None], keep.double()[:, None], keep,
+           torch.full((N,), 1.0 / max(1, live), device=cuda), 1.0, "mean")
+    assert (dh[~keep] == 0).all()
+    none = lh.linear_cross_entropy(h, w, target, reduction="none")
+    assert (none[~keep] == 0).all() and none.isfinite().all()
+    assert lh._native.device_status() == 0
+
+
+def test_packed_long_product_is_split_by_what_is_left(lh, cuda):
+    """Five row blocks of which two are left, a product over 60000 columns in parts."""
+    _run_xent(lh, cuda, 1200, 60000, 512, "mean", seed=42, ignore=0.65)
+
+
 def test_peaked_and_large_logits(lh, cuda):
     _run_xent(lh, cuda, 200, 700, 64, "mean", seed=12, scale=40.0)
 
@@ -223,6 +259,11 @@ def test_distillation(lh, cuda, N, V, D, K, T, reduction):
 def test_distillation_types_empty_rows_and_crowded_tiles(lh, cuda, where):
     _run_distill(lh, cuda, 150, 3000, 64, 100, 2.0, "mean", seed=21, empty=0.3, where=where, tdt=BF, idt=torch.int32)
     _run_distill(lh, cuda, 150, 3000, 64, 100, 2.0, "sum", seed=22, empty=0.9, where=where)
+
+
+def test_distillation_packed(lh, cuda):
+    _run_distill(lh, cuda, *BIG, 20, 2.0, "mean", seed=43, empty=0.5)
+    _run_distill(lh, cuda, *BIG, 3, 1.0, "none", seed=44, empty=0.2)
 
 
 def test_distillation_absent_entries_and_minus_infinity(lh, cuda):
@@ -364,5 +405,5 @@ def test_opcheck(lh, cuda):
         loss, kept = ops.linear_xent(h, w, t, -100, red)
         torch.library.opcheck(ops.linear_xent_bwd, (h, w, t, kept, torch.ones_like(loss), red), test_utils=utils)
         torch.library.opcheck(ops.linear_distill, (h, w, tv, ti, 2.0, red), test_utils=utils)
-        loss, *kept = ops.linear_distill(h, w, tv, ti, 2.0, red)
-        torch.library.opcheck(ops.linear_distill_bwd, (h, w, *kept, torch.ones_like(loss), 2.0, red), test_utils=utils)
+        loss, kept = ops.linear_distill(h, w, tv, ti, 2.0, red)
+        torch.library.opcheck(ops.linear_distill_bwd, (h, w, kept, torch.ones_like(loss), 5, 2.0, red), test_utils=utils)

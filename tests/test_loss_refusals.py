@@ -53,29 +53,29 @@ def test_c_entry_points_check_before_they_touch_a_device(lh):
     a = P(4096)                  # aligned and never read: every call below is refused on the host
     big = 1 << 40
 
-    def xf(h=a, w=a, t=a, N=4, V=10, D=64, red=1, loss=a, inv=a, ws=a, n=big):
-        return lib.lh_linear_xent_fwd(h, w, t, -100, N, V, D, red, loss, a, a, a, inv, ws, n, None)
+    def xf(h=a, w=a, t=a, N=4, V=10, D=64, red=1, loss=a, kept=a, ws=a, n=big):
+        return lib.lh_linear_xent_fwd(h, w, t, -100, N, V, D, red, loss, kept, ws, n, None)
 
-    assert xf(h=None) == 2 and xf(t=None) == 2 and xf(loss=None) == 2 and xf(inv=None) == 2 and xf(ws=None) == 2
+    assert xf(h=None) == 2 and xf(t=None) == 2 and xf(loss=None) == 2 and xf(kept=None) == 2 and xf(ws=None) == 2
     assert xf(N=0) == 1 and xf(V=0) == 1 and xf(D=12) == 1 and xf(N=(1 << 24) + 1) == 1 and xf(V=(1 << 22) + 1) == 1
-    assert xf(red=3) == 2 and xf(w=P(4104)) == 2 and xf(ws=P(4096 + 16)) == 2
+    assert xf(red=3) == 2 and xf(w=P(4104)) == 2 and xf(kept=P(4104)) == 2 and xf(ws=P(4096 + 16)) == 2
     assert xf(n=lib.lh_linear_loss_workspace_size(4, 10, 64, 0, 0) - 1) == 5
 
-    def xb(gout=a, gs=0, dw=a, n=big):
-        return lib.lh_linear_xent_bwd(a, a, a, 4, 10, 64, a, a, a, a, gout, gs, a, dw, a, n, None)
+    def xb(gout=a, red=1, dw=a, n=big):
+        return lib.lh_linear_xent_bwd(a, a, a, 4, 10, 64, red, a, gout, a, dw, a, n, None)
 
-    assert xb(gout=None) == 2 and xb(gs=2) == 2 and xb(dw=P(4100)) == 2
+    assert xb(gout=None) == 2 and xb(red=-1) == 2 and xb(dw=P(4100)) == 2
     assert xb(n=lib.lh_linear_loss_workspace_size(4, 10, 64, 0, 1) - 1) == 5
 
     def df(K=3, T=1.0, tv=a, dt=1):
-        return lib.lh_linear_distill_fwd(a, a, tv, dt, a, 4, 10, 64, K, T, 1, a, a, a, a, a, a, a, big, None)
+        return lib.lh_linear_distill_fwd(a, a, tv, dt, a, 4, 10, 64, K, T, 1, a, a, a, big, None)
 
     assert df(K=0) == 1 and df(K=257) == 1 and df(T=0.0) == 2 and df(tv=None) == 2 and df(dt=2) == 2
 
-    def db(idx=a, gs=0):
-        return lib.lh_linear_distill_bwd(a, a, 4, 10, 64, 3, 1.0, a, idx, a, a, a, a, gs, a, a, a, big, None)
+    def db(kept=a, K=3):
+        return lib.lh_linear_distill_bwd(a, a, 4, 10, 64, K, 1.0, 1, kept, a, a, a, a, big, None)
 
-    assert db(idx=None) == 2 and db(gs=3) == 2
+    assert db(kept=None) == 2 and db(K=0) == 1
 
 
 def test_workspace_stays_small(lh):
@@ -86,9 +86,9 @@ def test_workspace_stays_small(lh):
         for V in (1, 256, 32000, 131072, 1 << 20):
             for D in (64, 1024, 4096):
                 piece = max(512 << 20, 2 * N * 256)
-                planes = 74 * 4 * 256 * D * 8 + 4 * N * D      # parts only where few tiles are
+                planes = 74 * 4 * 256 * D * 8 + 10 * N * D     # parts only where few tiles are; packed rows
                 assert 0 < size(N, V, D, 0, 1) <= piece + planes + 4096, (N, V, D)
-                assert size(N, V, D, 0, 0) <= 16 * N * (V // 256 + 1) + 2 * N + 4 * N + 2048
+                assert size(N, V, D, 0, 0) <= 16 * N * (V // 256 + 1) + 6 * N + 2 * N * D + 4096
 
 
 def test_fake_kernels(lh):
