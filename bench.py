@@ -354,7 +354,8 @@ def run_model(args, rank, world, local_rank, cp=False):
     # config 5 (CP): seq 262144 with k=1536 is outside the reference's defined
     # domain (its selection writes holes there); its defined twin is seq 196608
     seq = args.seq_len or (196608 if cp else 65536)
-    margs = M.ModelArgs(max_seq_len=seq, lighthouse_topk=args.topk or (1536 if cp else 2048))
+    margs = M.ModelArgs(max_seq_len=seq, lighthouse_topk=args.topk or (1536 if cp else 2048), fused_norm=args.fused,
+                        fused_loss=args.fused)
     torch.manual_seed(0)
     model = M.Transformer(margs).to(dev)
     model.init_weights(0)
@@ -427,9 +428,12 @@ def run_model(args, rank, world, local_rank, cp=False):
                    "l2": "activations far larger than L2"},
         "e2e": {"value": tokens / (e2e_ms * 1e-3), "unit": "tokens/s", "h2d_bytes_per_step": (seq + 1) * 8,
                 "d2h_bytes_per_step": 4, "ms_per_step": e2e_ms, "final_loss": loss},
-        "gpu_launches": 10 * n_layers_lh * args.steps,
+        # fused: a norm is one launch forward and two backward, the loss two and four
+        "gpu_launches": (10 * n_layers_lh + (3 * (2 * margs.n_layers + 1) + 6 if args.fused else 0)) * args.steps,
         "clocks": clocks,
     }
+    if args.fused:
+        line["config"]["fused"] = "residual additions with their norms, loss without logits"
     if per_rank:
         line["per_rank"] = per_rank
     print(json.dumps(line), flush=True)
@@ -706,6 +710,8 @@ def main():
     ap.add_argument("--cp", type=int, default=None,
                     help="model_cp: context-parallel group size (default 2, BASELINE config 5); the rest is data parallel")
     ap.add_argument("--topk", type=int, default=None, help="profiling only: override k")
+    ap.add_argument("--fused", action="store_true",
+                    help="model, model_cp: residual additions fused with their norms, loss without logits")
     args = ap.parse_args()
     if args.seq_len and args.workload in ("layer", "scorer_gla"):
         CFG["S"] = args.seq_len

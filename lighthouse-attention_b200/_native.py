@@ -9,6 +9,7 @@ B200 the call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import pathlib
 
 import torch
@@ -451,11 +452,17 @@ def _loss_out(N, reduction, dev):
     return loss if N else loss.zero_()
 
 
+@functools.lru_cache(maxsize=4096)
+def _loss_ws_size(N, V, D, K, backward) -> int:
+    return load().lh_linear_loss_workspace_size(N, V, D, K, backward)
+
+
 def _loss_ws(N, V, D, K, backward, dev):
-    n = load().lh_linear_loss_workspace_size(N, V, D, K, backward)
+    n = _loss_ws_size(N, V, D, K, backward)
     return torch.empty(n, dtype=torch.uint8, device=dev), n
 
 
+@functools.lru_cache(maxsize=4096)
 def kept_size(N: int, K: int) -> int:
     """Bytes that a loss's forward keeps for its backward."""
     return load().lh_linear_loss_kept_size(N, K)

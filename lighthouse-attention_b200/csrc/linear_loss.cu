@@ -31,6 +31,8 @@
 // Every mbarrier wait is bounded; on expiry the CTAs leave and a status flag is set.
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
 #include "lh_common.cuh"
 #include "sm100.cuh"
 
@@ -845,7 +847,14 @@ static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMa
   a.gm = (int)(gm < tiles_m ? gm : tiles_m);
   const long long total = (long long)tiles_m * a.tiles_n * a.splits;
   const int pairs = (int)(total < kPairs ? total : kPairs);
-  cudaError_t e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MODE));
+  static std::atomic<uint64_t> allowed{0};           // devices on which the kernel may use its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e == cudaSuccess && (dev >= 64 || !(allowed.load() & bit))) {
+    e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MODE));
+    if (e == cudaSuccess && dev < 64) allowed.fetch_or(bit);
+  }
   if (e != cudaSuccess) { set_error("linear loss: %s", cudaGetErrorString(e)); return LH_ERR_LAUNCH; }
   loss_gemm_kernel<MODE, SPARSE><<<2 * pairs, kThreads, smem_bytes(MODE), st>>>(ma, mb, mo, mp, a);
   return check_launch("loss_gemm_kernel");

@@ -17,6 +17,13 @@ every rank holds the load-balanced shard (global chunks r and 2W-1-r) of the
 tokens, labels and RoPE positions (PATCH:822-829); Lighthouse layers run
 LighthouseCP and the full-attention layers run causal attention over the
 all-gathered K/V (cp.py); gradients are averaged over ranks by DDP.
+
+ModelArgs.fused_norm runs each residual addition with the norm behind it in one
+kernel (norm.py), ModelArgs.fused_loss forms train_step's loss without logits
+(losses.py); both are off by default, so that earlier runs repeat bit for bit.
+train_step(teacher=) distils from a teacher's top logits, and
+Transformer.quantize_projections() turns a model into one for inference whose
+projections behind a norm take 8-bit rows and weights.
 """
 from __future__ import annotations
 
@@ -29,6 +36,8 @@ import torch.nn.functional as F
 
 from .library import ops as _ops
 from . import cp as _cp
+from .losses import linear_cross_entropy, linear_distillation
+from .norm import add_rms_norm, add_rms_norm_fp8, rms_norm, rms_norm_fp8
 from .lighthouse_selection import (DilatedLighthouseGLAScorer, DilatedLighthouseScorer, LighthouseLocal,
                                    lighthouse_attention)
 
@@ -53,6 +62,9 @@ class ModelArgs:
     lighthouse_scorer: str = "norm"          # "norm" | "dilated" | "gla"  (context parallelism: "norm" only)
     dilation: int = 4
     lighthouse_full_attn_layers: list = field(default_factory=lambda: [0, 1, 28, 29])
+    fused_norm: bool = False                 # residual addition + norm in one kernel (CUDA)
+    distill_temperature: float = 1.0
+    fused_loss: bool = False                 # train_step's loss without logits (CUDA, bf16 compute)
 
 
 def rope_freqs(head_dim: int, seq_len: int, theta: float, device) -> torch.Tensor:
@@ -92,6 +104,26 @@ def rope_qk(xq: torch.Tensor, xk: torch.Tensor, freqs: torch.Tensor):
     return apply_rope(xq, freqs), apply_rope(xk, freqs)
 
 
+class Fp8Linear(nn.Module):
+    """A bias-free projection in 8 bits for inference: weights in float8_e4m3fn with
+    one fp32 scale per output, inputs the rows and scales of rms_norm_fp8."""
+
+    def __init__(self, linear: nn.Linear):
+        super().__init__()
+        w = linear.weight.detach().float()
+        if w.shape[0] % 16 or w.shape[1] % 16:
+            raise ValueError(f"8-bit projections need dimensions that are multiples of 16, got {tuple(w.shape)}")
+        scale = w.abs().amax(1, keepdim=True).clamp(min=2.0 ** -100) / 448.0
+        self.register_buffer("weight", (w / scale).to(torch.float8_e4m3fn))
+        self.register_buffer("scale", scale.T.contiguous())
+
+    def forward(self, x):
+        q, s = x
+        y = torch._scaled_mm(q.reshape(-1, q.shape[-1]), self.weight.t(), s.reshape(-1, 1), self.scale,
+                             out_dtype=torch.bfloat16)
+        return y.view(*q.shape[:-1], y.shape[-1])
+
+
 class Attention(nn.Module):
     def __init__(self, args: ModelArgs, layer_id: int):
         super().__init__()
@@ -121,7 +153,7 @@ class Attention(nn.Module):
                 self.gate_logit_normalizer = 16
 
     def forward(self, x, freqs, cp_info=None):
-        B, S, _ = x.shape
+        B, S, _ = (x[0] if isinstance(x, tuple) else x).shape       # 8-bit inference: (rows, scales)
         xq = self.wq(x).view(B, S, self.n_heads, self.head_dim)
         xk = self.wk(x).view(B, S, self.n_heads, self.head_dim)
         xv = self.wv(x).view(B, S, self.n_heads, self.head_dim)
@@ -169,6 +201,13 @@ class Block(nn.Module):
         h = x + self.attention(_to_compute_dtype(self.attention_norm(x)), freqs, cp_info)
         return h + self.feed_forward(_to_compute_dtype(self.ffn_norm(h)))
 
+    def forward_stream(self, h, branch, freqs, cp_info=None, fp8=False):
+        """The same with the stream h and the branch that is still to be added to it
+        (None in front of the first block); returns both for the next block."""
+        y, h = _add_norm(branch, h, self.attention_norm, fp8)
+        y, h = _add_norm(self.attention(y, freqs, cp_info), h, self.ffn_norm, fp8)
+        return h, self.feed_forward(y)
+
 
 def _to_compute_dtype(t):
     """Under autocast, cast a normalised fp32 activation to the autocast dtype
@@ -178,6 +217,23 @@ def _to_compute_dtype(t):
     if t.is_cuda and torch.is_autocast_enabled("cuda"):
         return t.to(torch.get_autocast_dtype("cuda"))
     return t
+
+
+def _add_norm(branch, h, norm: nn.RMSNorm, fp8: bool = False):
+    """(norm(h + branch) in the compute dtype, h + branch): one kernel on the GPU, the
+    separate operations on the CPU.  fp8: the normed rows as (codes, scales)."""
+    if not h.is_cuda:
+        h = h if branch is None else h + branch
+        return norm(h), h
+    if fp8:
+        if branch is None:
+            return rms_norm_fp8(h, norm.weight, norm.eps), h
+        q, s, h = add_rms_norm_fp8(branch, h, norm.weight, norm.eps)
+        return (q, s), h
+    dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else h.dtype
+    if branch is None:
+        return rms_norm(h, norm.weight, norm.eps, dtype), h
+    return add_rms_norm(branch, h, norm.weight, norm.eps, dtype)
 
 
 class Transformer(nn.Module):
@@ -190,6 +246,7 @@ class Transformer(nn.Module):
         self.output = nn.Linear(args.dim, args.vocab_size, bias=False)
         self._freqs = None
         self.cp_info = None          # (rank, world_size, group) once set_cp_info is called
+        self.fp8 = False             # quantize_projections() has been called
 
     def set_cp_info(self, rank: int, world_size: int, group) -> None:
         """Context-parallel mode (PATCH:801-816): forward then takes this rank's
@@ -205,7 +262,22 @@ class Transformer(nn.Module):
                 elif name.endswith("wg.bias"):                # gate projection bias (PATCH:687-689)
                     p.zero_()
 
-    def forward(self, tokens):
+    def quantize_projections(self) -> "Transformer":
+        """For inference: wq, wk, wv, w1 and w3 of every block become 8-bit projections
+        (Fp8Linear) that read the norms' 8-bit rows.  In place and final: the projections'
+        fp32 weights are dropped, so the model no longer trains.  CUDA only."""
+        if any(layer.attention.scorer_name == "gla" for layer in self.layers):
+            raise ValueError("the gla scorer's gate reads the norm in full precision: no 8-bit projections")
+        for layer in self.layers:
+            for m, names in ((layer.attention, ("wq", "wk", "wv")), (layer.feed_forward, ("w1", "w3"))):
+                for name in names:
+                    if isinstance(getattr(m, name), nn.Linear):
+                        setattr(m, name, Fp8Linear(getattr(m, name)))
+        self.fp8 = True
+        return self
+
+    def _normed(self, tokens):
+        """The final norm's output (B, S, dim)."""
         B, S = tokens.shape
         W = self.cp_info[1] if self.cp_info else 1
         S_glob = S * W
@@ -216,31 +288,76 @@ class Transformer(nn.Module):
         if self.cp_info:
             freqs = _cp.shard_sequence(freqs, self.cp_info[0], W, dim=0)   # global positions of the shard
         h = self.tok_embeddings(tokens)
+        if self.args.fused_norm or self.fp8:
+            if self.fp8 and not h.is_cuda:
+                raise ValueError("8-bit projections run on CUDA tensors only")
+            branch = None
+            for layer in self.layers:
+                h, branch = layer.forward_stream(h, branch, freqs, self.cp_info, self.fp8)
+            return _add_norm(branch, h, self.norm)[0]
         for layer in self.layers:
             h = layer(h, freqs, self.cp_info)
-        return self.output(self.norm(h))
+        return self.norm(h)
+
+    def forward(self, tokens, labels=None, teacher=None):
+        """Logits (B, S, V); with labels (B, S) the mean cross entropy instead, with teacher
+        (logits, indices), both (B, S, K), the mean distillation loss.  On the GPU and in
+        bf16 the losses form no logits."""
+        y = self._normed(tokens)
+        if labels is None and teacher is None:
+            return self.output(y)
+        if labels is not None and teacher is not None:
+            raise ValueError("either labels or a teacher")
+        y = _to_compute_dtype(y)
+        w = self.output.weight.to(y.dtype)
+        if y.is_cuda and y.dtype == torch.bfloat16:
+            if teacher is not None:
+                return linear_distillation(y, w, *teacher, temperature=self.args.distill_temperature)
+            return linear_cross_entropy(y, w, labels)
+        if teacher is not None:
+            raise ValueError("distillation runs on CUDA tensors in bf16 (autocast)")
+        return F.cross_entropy(F.linear(y, w).float().reshape(-1, w.shape[0]), labels.reshape(-1))
+
+
+@torch.no_grad()
+def teacher_top_logits(model: Transformer, tokens: torch.Tensor, k: int):
+    """(logits, indices) of a teacher's k most likely next tokens at every position of
+    tokens (B, S), each (B, S, k): what Transformer.forward(teacher=) takes."""
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        logits = model(tokens)
+    return torch.topk(logits.float(), k, dim=-1)
 
 
 def num_params(model: nn.Module) -> int:
     return sum(p.numel() for p in model.parameters())
 
 
-def train_step(model, optimizer, tokens: torch.Tensor) -> torch.Tensor:
+def train_step(model, optimizer, tokens: torch.Tensor, teacher=None) -> torch.Tensor:
     """One next-byte-prediction step on tokens (B, S+1): inputs are the first S
     bytes, labels the last S.  bf16 autocast over fp32 master weights (the
     reference trains with bf16 mixed precision).  In context-parallel mode
     (model.set_cp_info) every rank passes the same global tokens and trains on
     its load-balanced shard of inputs and labels; the returned loss is this
-    rank's shard mean.  Returns the loss tensor."""
+    rank's shard mean.  With teacher, (logits, indices) of the first S positions
+    (teacher_top_logits), the step distils from it instead.  Returns the loss
+    tensor."""
     inputs, labels = tokens[:, :-1], tokens[:, 1:]
     core = model.module if hasattr(model, "module") else model
     if core.cp_info:
         rank, W, _ = core.cp_info
         inputs = _cp.shard_sequence(inputs, rank, W, dim=1)
         labels = _cp.shard_sequence(labels, rank, W, dim=1)
+        if teacher is not None:
+            teacher = tuple(_cp.shard_sequence(t, rank, W, dim=1) for t in teacher)
     with torch.autocast("cuda", dtype=torch.bfloat16):
-        logits = model(inputs)
-    loss = F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), labels.reshape(-1))
+        if teacher is not None:
+            loss = model(inputs, teacher=teacher)
+        elif core.args.fused_loss:
+            loss = model(inputs, labels)
+        else:
+            logits = model(inputs)
+    if teacher is None and not core.args.fused_loss:
+        loss = F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), labels.reshape(-1))
     loss.backward()
     optimizer.step()
     optimizer.zero_grad(set_to_none=True)
