@@ -59,9 +59,16 @@ enum Out { kOutBf16, kOutPlane, kOutPlaneAdd };
 // Stages of the operand ring and staging buffers per epilogue warp: a warp's half
 // of a bf16 row block is two stores, each with a buffer of its own, so that it
 // waits for a store of the tile before only; kStats stores nothing.
-__host__ __device__ constexpr int stages(int mode) { return mode == kStats ? 6 : 5; }
-__host__ __device__ constexpr int bufs(int mode) { return mode == kStats ? 1 : 2; }
-constexpr int smem_bytes(int mode) { return 1024 + stages(mode) * 2 * kOpBytes + 8 * bufs(mode) * kOutBuf + 512; }
+// With few rows (kFew at most) the roles turn: the 256 rows of a tile are weights (or
+// columns of dH) and its kFew columns are rows of hidden, so that the MMAs do an eighth
+// of the work and the stages hold weights, which are what has to be read.
+constexpr int kFew = 64;
+__host__ __device__ constexpr int stages(int mode, bool few) { return few ? 10 : mode == kStats ? 6 : 5; }
+__host__ __device__ constexpr int bufs(int mode, bool few) { return few ? 0 : mode == kStats ? 1 : 2; }
+__host__ __device__ constexpr int b_bytes(bool few) { return few ? kFew / 2 * 128 : kOpBytes; }
+constexpr int smem_bytes(int mode, bool few) {
+  return 1024 + stages(mode, few) * (kOpBytes + b_bytes(few)) + 8 * bufs(mode, few) * kOutBuf + 512;
+}
 
 // Walk of the tiles: split, group of gm row blocks, column block, row block in the group.
 struct Sched {
@@ -70,12 +77,14 @@ struct Sched {
 };
 
 struct Smem {
-  uint64_t full[6], empty[6], acc_full[2], acc_empty[2], drain;
+  uint64_t full[10], empty[10], acc_full[2], acc_empty[2], drain;
   Sched sched;
   uint32_t tmem_base;
   int abort;
 };
-static_assert(sizeof(Smem) <= 512 && smem_bytes(kStats) <= 232448 && smem_bytes(kGrad) <= 232448, "barriers do not fit their space");
+static_assert(sizeof(Smem) <= 512, "barriers do not fit their space");
+static_assert(smem_bytes(kStats, false) <= 232448 && smem_bytes(kGrad, false) <= 232448 && smem_bytes(kStats, true) <= 232448,
+              "stages do not fit shared memory");
 
 constexpr int kSplitTable = 2 * kPairs;
 struct Args {
@@ -84,7 +93,7 @@ struct Args {
   int n_rows;                     // rows of hidden
   const int* rows;                // NULL, or: number of packed rows, their rows of hidden, (and back)
   uint8_t split_of[kSplitTable];  // kDH: parts of the K range by the number of row blocks, 1 beyond the table
-  int b_off;                      // first row of B's operand (vocabulary piece)
+  int b_off;                      // first row of the weights, B's operand (few rows: A's): vocabulary piece
   int out;                        // kDH, kDW: Out
   // targets: int64 (K = 1, SPARSE false) or sorted int32 (K, n_rows), a row's entries n_rows apart
   const long long* target;
@@ -99,6 +108,8 @@ struct Args {
   const float *gout, *row_scale, *inv_count;
   int gstride;
   float cscale;
+  void* few_out;                  // few rows: G (bf16, few_pitch), or the planes (fp32) or dH (bf16) of kDH
+  long long few_pitch;
 };
 
 // Position of the first of a row's K sorted targets, M apart, that is >= v.
@@ -112,19 +123,35 @@ __device__ __forceinline__ int lower_bound(const int* __restrict__ idx, int K, s
   return lo;
 }
 
-template <int MODE, bool SPARSE>
+// 32 values per lane, one per column -> in lane e the result of column e over the warp.
+template <class Op>
+__device__ __forceinline__ float reduce_columns(float (&v)[32], int lane, Op op) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float keep = up ? v[i + o] : v[i], give = up ? v[i] : v[i + o];
+      v[i] = op(keep, __shfl_xor_sync(~0u, give, o));
+    }
+  }
+  return v[0];
+}
+
+template <int MODE, bool SPARSE, bool FEW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmP,
                  const __grid_constant__ Args a) {
   // tmP: the packed rows, in the place of hidden (A of kStats and kGrad, B of kDW)
-  constexpr bool kAMn = MODE == kDW, kBMn = MODE == kDH || MODE == kDW;
-  constexpr int kStages = stages(MODE), kBufs = bufs(MODE);
+  constexpr bool kAMn = MODE == kDW || (FEW && MODE == kDH), kBMn = !FEW && (MODE == kDH || MODE == kDW);
+  constexpr int kStages = stages(MODE, FEW), kBufs = bufs(MODE, FEW), kBBytes = b_bytes(FEW);
+  constexpr int kCols = FEW ? kFew : kTN;          // columns of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = base;
   uint8_t* sB = base + kStages * kOpBytes;
-  uint8_t* sO = base + 2 * kStages * kOpBytes;
+  uint8_t* sO = base + kStages * (kOpBytes + kBBytes);
   Smem* sm = reinterpret_cast<Smem*>(sO + 8 * kBufs * kOutBuf);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
@@ -144,7 +171,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     c.tiles_m = (c.M + kTM - 1) / kTM;
     c.gm = max(1, min(a.gm, c.tiles_m));
     c.splits = a.splits;
-    if (MODE == kDH) c.splits = min(a.splits, c.tiles_m < kSplitTable ? (int)a.split_of[c.tiles_m] : 1);
+    if (MODE == kDH && !FEW) c.splits = min(a.splits, c.tiles_m < kSplitTable ? (int)a.split_of[c.tiles_m] : 1);
     c.total = c.tiles_m * a.tiles_n * c.splits;
     c.per_split = FastDiv(max(1, c.tiles_m * a.tiles_n));
     c.per_group = FastDiv(c.gm * a.tiles_n);
@@ -196,21 +223,29 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         for (int t = pair; t < total && ok; t += n_pairs) {
           int m, n, k0, k1, split;
           decode(t, m, n, k0, k1, split);
-          const int ra = m * kTM + rank * 128, rb = n * kTN + rank * 128;
+          const int ra = m * kTM + rank * 128, rb = n * kCols + rank * (kCols / 2);
           for (int k = k0; k < k1; ++k, ++it) {
             const int s = it % kStages;
             const uint32_t round = it / kStages;
             if (round > 0 && !mbar_wait(&sm->empty[s], (round - 1) & 1, abort)) { ok = false; break; }
-            if (rank == 0) mbar_expect_tx(&sm->full[s], 4 * kOpBytes);
+            if (rank == 0) mbar_expect_tx(&sm->full[s], 2 * (kOpBytes + kBBytes));
             const uint32_t bar = leader_addr(&sm->full[s]);
             uint8_t* pa = sA + s * kOpBytes;
-            uint8_t* pb = sB + s * kOpBytes;
+            uint8_t* pb = sB + s * kBBytes;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              if (kAMn) tma_load_2d_pair(pa + j * kBox, mapA, bar, ra + 64 * j, k * kTK);
-              else tma_load_2d_pair(pa + j * kBox, mapA, bar, k * kTK, ra + 64 * j);
-              if (kBMn) tma_load_2d_pair(pb + j * kBox, mapB, bar, rb + 64 * j, a.b_off + k * kTK);
-              else tma_load_2d_pair(pb + j * kBox, mapB, bar, k * kTK, a.b_off + rb + 64 * j);
+              const int a_row = ra + 64 * j + (FEW && !kAMn ? a.b_off : 0), a_k = k * kTK + (FEW && kAMn ? a.b_off : 0);
+              if (kAMn) tma_load_2d_pair(pa + j * kBox, mapA, bar, a_row, a_k);
+              else tma_load_2d_pair(pa + j * kBox, mapA, bar, a_k, a_row);
+            }
+            if constexpr (FEW) {
+              tma_load_2d_pair(pb, mapB, bar, k * kTK, rb);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                if (kBMn) tma_load_2d_pair(pb + j * kBox, mapB, bar, rb + 64 * j, a.b_off + k * kTK);
+                else tma_load_2d_pair(pb + j * kBox, mapB, bar, k * kTK, a.b_off + rb + 64 * j);
+              }
             }
           }
         }
@@ -223,7 +258,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- MMA issuer
       if (lane == 0) {
-        constexpr uint32_t idesc = idesc_bf16_f32(kTM, kTN, kAMn, kBMn);
+        constexpr uint32_t idesc = idesc_bf16_f32(kTM, kCols, kAMn, kBMn);
         uint32_t it = 0;
         int li = 0;
         bool ok = true;
@@ -233,14 +268,14 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         for (int t = pair; t < total && ok; t += n_pairs, ++li) {
           const int steps = q + ((int)sched.per_split.div(t) < rem ? 1 : 0);
           const int b = li & 1;
-          const uint32_t acc = tbase + b * kTN;
+          const uint32_t acc = tbase + b * kCols;
           if (li >= 2 && !mbar_wait(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort)) break;
           tc_fence_after();
           for (int k = 0; k < steps; ++k, ++it) {
             const int s = it % kStages;
             if (!mbar_wait(&sm->full[s], (it / kStages) & 1, abort)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t pa = smem_u32(sA + s * kOpBytes), pb = smem_u32(sB + s * kOpBytes);
+            const uint32_t pa = smem_u32(sA + s * kOpBytes), pb = smem_u32(sB + s * kBBytes);
 #pragma unroll
             for (int kk = 0; kk < kTK / 16; ++kk)
               mma_ss_pair(acc,
@@ -256,12 +291,122 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->drain, 0); ++p) {}
         }
       }
-    } else if (warp >= 4) {
+    } else if (FEW && warp >= 4) {
+      // ---------------------------------------------------------- epilogue, few rows
+      // TMEM lane = row of the weights (column of dH), 32 columns per warp = rows of hidden; what
+      // belongs to a row of hidden is held by the lane of its number and handed out by shuffles
+      const int quad = warp & 3, half = warp >= 8 ? 1 : 0;
+      const uint32_t acc0 = tbase + ((uint32_t)(quad * 32) << 16) + half * 32;
+      const uint32_t acc_empty0 = leader_addr(&sm->acc_empty[0]), acc_empty1 = leader_addr(&sm->acc_empty[1]);
+      const int row = half * 32 + lane;
+      const bool live = row < a.N;
+      const int rows = min(32, a.N - half * 32);         // of this warp, may be negative
+      float mx = -INFINITY, sum = 0.f, c = 0.f, lse2 = 0.f;
+      long long target = -1;
+      if constexpr (MODE == kStats || MODE == kGrad) {
+        if (live && !SPARSE) target = __ldg(a.target + row);
+        if (MODE == kGrad && live) {
+          const float up = __ldg(a.gout + (size_t)row * a.gstride);
+          if (up != 0.f) c = a.cscale * up * __ldg(a.row_scale + row) * (a.inv_count ? __ldg(a.inv_count) : 1.f);
+          lse2 = __ldg(a.lse2 + row);
+        }
+      }
+      int li = 0;
+      for (int t = pair; t < total; t += n_pairs, ++li) {
+        int m, n, k0, k1, split;
+        decode(t, m, n, k0, k1, split);
+        const int b = li & 1;
+        const int v0 = m * kTM + rank * 128 + quad * 32;
+        const int left = min(32, M - v0);                // rows of the weights, may be negative
+        const bool ok = mbar_wait(&sm->acc_full[b], (li >> 1) & 1, abort);
+        if (__any_sync(~0u, !ok)) break;
+        tc_fence_after();
+        uint32_t x[32];
+        tmem_ld32(acc0 + b * kCols, x);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_leader(b ? acc_empty1 : acc_empty0);
+        if (left <= 0 || rows <= 0) continue;
+        if constexpr (MODE == kDH) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            if (e < rows && lane < left) {
+              const size_t at = (size_t)(half * 32 + e) * a.M + v0 + lane;
+              if (a.out == kOutBf16) reinterpret_cast<__nv_bfloat16*>(a.few_out)[at] = __float2bfloat16_rn(__uint_as_float(x[e]));
+              else reinterpret_cast<uint32_t*>(a.few_out)[(size_t)split * a.N * a.M + at] = x[e];
+            }
+          }
+        } else {
+          // dense part
+          if constexpr (MODE == kGrad) {
+            __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(a.few_out) + (size_t)half * 32 * a.few_pitch + v0 + lane;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float ce = __shfl_sync(~0u, c, e), le = __shfl_sync(~0u, lse2, e);
+              if (e < rows && lane < left)
+                g[e * a.few_pitch] = __float2bfloat16_rn(ce == 0.f ? 0.f : ce * ex2(fmaf(__uint_as_float(x[e]), a.a2, -le)));
+            }
+          }
+          // the rows' targets among these weights
+          const int gv0 = v0 + (MODE == kGrad ? a.b_off : 0);
+          int cur = 0, next = kNone;
+          if (live) {
+            if constexpr (SPARSE) {
+              cur = lower_bound(a.idx + row, a.K, a.n_rows, gv0);
+              if (cur < a.K) next = __ldg(a.idx + (size_t)cur * a.n_rows + row);
+              if (next != kNone) next -= gv0;
+            } else if (target >= gv0 && target < gv0 + 32) {
+              next = (int)(target - gv0);
+            }
+          }
+          for (unsigned hit; (hit = __ballot_sync(~0u, next < left)) != 0;) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              if (hit >> e & 1) {
+                const int at = __shfl_sync(~0u, next, e), k = __shfl_sync(~0u, cur, e);
+                const float ce = MODE == kGrad ? __shfl_sync(~0u, c, e) : 0.f;
+                if (lane == at) {
+                  const size_t kept = (size_t)k * a.n_rows + half * 32 + e;
+                  if constexpr (MODE == kStats) a.slog[kept] = __uint_as_float(x[e]);
+                  else if (ce != 0.f)
+                    reinterpret_cast<__nv_bfloat16*>(a.few_out)[(half * 32 + e) * a.few_pitch + v0 + lane] =
+                        __float2bfloat16_rn(ce * __ldg(a.gval + kept));
+                }
+              }
+            }
+            if (next < left) {
+              next = kNone;
+              if (SPARSE && ++cur < a.K) {
+                next = __ldg(a.idx + (size_t)cur * a.n_rows + row);
+                if (next != kNone) next -= gv0;
+              }
+            }
+          }
+          if constexpr (MODE == kStats) {
+            float v[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = lane < left ? __uint_as_float(x[e]) : -INFINITY;
+            const float mn = fmaxf(mx, reduce_columns(v, lane, [](float p, float q) { return fmaxf(p, q); }));
+            const float mb = mn == -INFINITY ? 0.f : mn * a.a2;
+            sum *= mx == -INFINITY ? 0.f : ex2(fmaf(mx, a.a2, -mb));
+            mx = mn;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float be = __shfl_sync(~0u, mb, e);
+              v[e] = lane < left ? ex2(fmaf(__uint_as_float(x[e]), a.a2, -be)) : 0.f;
+            }
+            sum += reduce_columns(v, lane, [](float p, float q) { return p + q; });
+          }
+        }
+      }
+      if (MODE == kStats && live) a.stats[(size_t)(blockIdx.x * 4 + quad) * a.n_rows + row] = make_float2(mx, sum);
+    } else if (!FEW && warp >= 4) {
       // ---------------------------------------------------------- epilogue
       // warps 4-7 take columns 0-127 of the tile, warps 8-11 the rest
       const int quad = warp & 3, half = warp >= 8 ? 1 : 0;
-      constexpr int kCols = kTN / 2;
-      const uint32_t lane_base = tbase + ((uint32_t)(quad * 32) << 16) + half * kCols;
+      constexpr int kHalf = kTN / 2;
+      const uint32_t lane_base = tbase + ((uint32_t)(quad * 32) << 16) + half * kHalf;
       uint8_t* stage = sO + (quad + 4 * half) * kBufs * kOutBuf;
       const uint32_t acc_empty0 = leader_addr(&sm->acc_empty[0]), acc_empty1 = leader_addr(&sm->acc_empty[1]);
       int li = 0, buf = 0;
@@ -274,8 +419,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         decode(t, m, n, k0, k1, split);
         const int b = li & 1;
         const uint32_t acc = lane_base + b * kTN;
-        const int row0 = m * kTM + rank * 128 + quad * 32, row = row0 + lane, n0 = n * kTN + half * kCols;
-        const int cols = min(kCols, a.N - n0);           // of this warp's half, may be negative
+        const int row0 = m * kTM + rank * 128 + quad * 32, row = row0 + lane, n0 = n * kTN + half * kHalf;
+        const int cols = min(kHalf, a.N - n0);           // of this warp's half, may be negative
         const bool live = row < M;
         const int orow = live && a.rows ? __ldg(a.rows + 1 + row) : row;      // row of hidden
         // next target of this row at or behind the half's first column, as a column of the half,
@@ -298,7 +443,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               advance();
             } else {
               const long long tv = __ldg(a.target + orow) - g0;
-              if (tv >= 0 && tv < kCols) next = (int)tv;
+              if (tv >= 0 && tv < kHalf) next = (int)tv;
             }
             if constexpr (MODE == kGrad) {
               const float up = __ldg(a.gout + (size_t)orow * a.gstride);
@@ -318,7 +463,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if constexpr (MODE == kStats) {
           float mx = -INFINITY, sum = 0.f;
 #pragma unroll 1
-          for (int c0 = 0; c0 < kCols; c0 += 32) {
+          for (int c0 = 0; c0 < kHalf; c0 += 32) {
             const int left = cols - c0;
             if (left <= 0) break;
             uint32_t x[32];
@@ -366,12 +511,12 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         } else {
           const int width = MODE == kGrad || a.out == kOutBf16 ? 64 : 32;      // columns of one store
 #pragma unroll 1
-          for (int c0 = 0; c0 < kCols; c0 += width) {
+          for (int c0 = 0; c0 < kHalf; c0 += width) {
             uint32_t x[32], y[32];
             tmem_ld32(acc + c0, x);
             if (width == 64) tmem_ld32(acc + c0 + 32, y);
             tmem_ld_wait();
-            if (c0 + width == kCols) release();
+            if (c0 + width == kHalf) release();
             // kGrad writes zeros up to the end of the 64 rows that the last step of kDW takes
             if (c0 >= cols || row0 >= (MODE == kGrad ? (M + 63) / 64 * 64 : M)) continue;
             if (MODE == kDW && k0 == k1) {       // no rows at all in this part
@@ -806,13 +951,13 @@ static int make_context_current() {
   return LH_OK;
 }
 
-// bf16 (rows, cols) with a row pitch in elements; 64 x 64 boxes, 128-byte swizzle.
-static int map_load(CUtensorMap* m, const void* p, long long rows, long long cols, long long pitch) {
+// bf16 (rows, cols) with a row pitch in elements; boxes of 64 columns, 128-byte swizzle.
+static int map_load(CUtensorMap* m, const void* p, long long rows, long long cols, long long pitch, unsigned box_rows = 64) {
   auto enc = encode_fn();
   if (!enc) { set_error("cuTensorMapEncodeTiled unavailable"); return LH_ERR_LAUNCH; }
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)pitch * 2};
-  cuuint32_t box[2] = {64, 64}, es[2] = {1, 1};
+  cuuint32_t box[2] = {64, box_rows}, es[2] = {1, 1};
   CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, box, es,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -834,11 +979,11 @@ static int map_store(CUtensorMap* m, void* p, bool f32, long long planes, long l
   return LH_OK;
 }
 
-template <int MODE, bool SPARSE>
+template <int MODE, bool SPARSE, bool FEW = false>
 static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const CUtensorMap& mp, Args& a,
                   long long K, cudaStream_t st) {
   const int tiles_m = (a.M + kTM - 1) / kTM;
-  a.tiles_n = (a.N + kTN - 1) / kTN;
+  a.tiles_n = FEW ? 1 : (a.N + kTN - 1) / kTN;
   a.kb = (int)((K + kTK - 1) / kTK);
   // Row blocks walked together: as many as keep their operand rows in about half of L2, at least
   // eight (eight by nine tiles are one wave of the 74 pairs).
@@ -852,11 +997,11 @@ static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMa
   cudaError_t e = cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (e == cudaSuccess && (dev >= 64 || !(allowed.load() & bit))) {
-    e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MODE));
+    e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MODE, FEW));
     if (e == cudaSuccess && dev < 64) allowed.fetch_or(bit);
   }
   if (e != cudaSuccess) { set_error("linear loss: %s", cudaGetErrorString(e)); return LH_ERR_LAUNCH; }
-  loss_gemm_kernel<MODE, SPARSE><<<2 * pairs, kThreads, smem_bytes(MODE), st>>>(ma, mb, mo, mp, a);
+  loss_gemm_kernel<MODE, SPARSE, FEW><<<2 * pairs, kThreads, smem_bytes(MODE, FEW), st>>>(ma, mb, mo, mp, a);
   return check_launch("loss_gemm_kernel");
 }
 
@@ -939,6 +1084,12 @@ struct Kept {
   }
 };
 
+// With few rows, parts of a row: one per TMEM row block of every CTA that kStats has.
+static int few_parts(long long V) {
+  const long long tiles = (V + kTM - 1) / kTM;
+  return 8 * (int)(tiles < kPairs ? tiles : kPairs);
+}
+
 // Workspace of the forward.
 struct FwdSpace {
   float2* stats;
@@ -951,7 +1102,7 @@ struct FwdSpace {
   FwdSpace(void* base, long long N, long long V, long long D, long long K) {
     char* p = (char*)base;
     auto take = [&](size_t n) { char* q = p; p += up(n); return q; };
-    stats = (float2*)take((size_t)((V + kTN - 1) / kTN) * 2 * N * sizeof(float2));
+    stats = (float2*)take((size_t)(N <= kFew ? few_parts(V) : (V + kTN - 1) / kTN * 2) * N * sizeof(float2));
     part = (double2*)take((size_t)((N + 7) / 8) * sizeof(double2));
     ticket = (unsigned*)take(4);
     counts = (int*)take(4 * ((N + 1023) / 1024));
@@ -1013,10 +1164,12 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
       return rc;
     rows = kp.rows;
   }
-  const int parts = (V + kTN - 1) / kTN * 2;
+  const bool few = N <= kFew;
+  const int parts = few ? few_parts(V) : (V + kTN - 1) / kTN * 2;
   Args a{};
-  a.M = a.n_rows = N;
-  a.N = V;
+  a.n_rows = N;
+  a.M = few ? V : N;
+  a.N = few ? N : V;
   a.splits = 1;
   a.rows = rows;
   a.target = q.target;
@@ -1026,7 +1179,12 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
   a.stats = ws.stats;
   a.slog = kp.tgrad;
   a.ticket = ws.ticket;
-  if ((rc = launch<kStats, SPARSE>(mh, mw, mw, mp, a, D, st))) return rc;
+  if (few) {
+    if ((rc = map_load(&mh, q.hidden, N, D, D, kFew / 2)) || (rc = launch<kStats, SPARSE, true>(mw, mh, mw, mw, a, D, st)))
+      return rc;
+  } else if ((rc = launch<kStats, SPARSE>(mh, mw, mw, mp, a, D, st))) {
+    return rc;
+  }
   // Rows per block: eight with up to 128 slots each where a row has many parts (16 rows of 1000
   // parts: 7 us, 17 with 32 rows per block), 256 where it has up to four (65536 rows of two parts:
   // 14 us with 32 rows per block, most of it the 2048 blocks' sum).
@@ -1063,6 +1221,11 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
   if ((rc = p.dh_planes ? map_store(&mdh, dh, true, p.dh_splits, N, D, D) : map_store(&mdh, dhidden, false, 1, N, D, D)))
     return rc;
   mp = mh;
+  // few rows: always one piece (kFew rows of 2^22 columns take 512 MB)
+  const bool few = N <= kFew;
+  CUtensorMap mh_few, mg_few;
+  if (few && ((rc = map_load(&mh_few, q.hidden, N, D, D, kFew / 2)) || (rc = map_load(&mg_few, g, N, V, p.C, kFew / 2))))
+    return rc;
   const int* rows = nullptr;
   if (p.packed) {
     rows = kp.rows;
@@ -1073,9 +1236,12 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     const int cols = (int)(V - v0 < p.C ? V - v0 : p.C);
     if ((rc = map_load(&mg, g, N, cols, p.C)) || (rc = map_store(&mgo, g, false, 1, N, cols, p.C))) return rc;
     Args a{};
-    a.M = a.n_rows = N;
-    a.N = cols;
+    a.n_rows = N;
+    a.M = few ? cols : N;
+    a.N = few ? N : cols;
     a.splits = 1;
+    a.few_out = g;
+    a.few_pitch = p.C;
     a.rows = rows;
     a.b_off = (int)v0;
     a.target = q.target;
@@ -1089,18 +1255,24 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     a.gout = gout;
     a.gstride = reduction == LH_REDUCE_NONE ? 1 : 0;
     a.cscale = q.T;
-    if ((rc = launch<kGrad, SPARSE>(mh, mw, mgo, mp, a, D, st))) return rc;
+    if ((rc = few ? launch<kGrad, SPARSE, true>(mw, mh_few, mw, mw, a, D, st)
+                  : launch<kGrad, SPARSE>(mh, mw, mgo, mp, a, D, st)))
+      return rc;
 
     Args x{};
-    x.M = x.n_rows = N;
-    x.N = D;
+    x.n_rows = N;
+    x.M = few ? D : N;
+    x.N = few ? N : D;
+    x.few_out = p.dh_planes ? (void*)dh : dhidden;
     const int kb = (cols + kTK - 1) / kTK;
     x.splits = p.dh_splits < kb ? p.dh_splits : kb;      // a short last piece may leave planes as they are
     for (int t = 0; t < kSplitTable; ++t) x.split_of[t] = p.split_of[t];
     x.rows = rows;
     x.b_off = (int)v0;
     x.out = !p.dh_planes ? kOutBf16 : i ? kOutPlaneAdd : kOutPlane;
-    if ((rc = launch<kDH, false>(mg, mw, mdh, mg, x, cols, st))) return rc;
+    if ((rc = few ? launch<kDH, false, true>(mw, mg_few, mw, mw, x, cols, st)
+                  : launch<kDH, false>(mg, mw, mdh, mg, x, cols, st)))
+      return rc;
 
     Args y{};
     y.M = cols;

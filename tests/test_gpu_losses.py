@@ -89,7 +89,8 @@ def _run_xent(lh, cuda, N, V, D, reduction, seed=0, ignore=0.0, scale=1.0):
 
 @pytest.mark.parametrize("N,V,D", [(1, 1, 8), (1, 256, 64), (2, 257, 72), (31, 255, 128), (128, 1000, 64),
                                    (129, 300, 264), (255, 256, 256), (257, 511, 768), (300, 5003, 96),
-                                   (1000, 769, 136), (64, 2, 4096), (7, 20011, 1024)])
+                                   (1000, 769, 136), (64, 2, 4096), (7, 20011, 1024), (64, 777, 200), (65, 777, 200),
+                                   (33, 40001, 520), (50, 256, 1032)])
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 def test_cross_entropy(lh, cuda, N, V, D, reduction):
     _run_xent(lh, cuda, N, V, D, reduction, seed=N + V)
@@ -259,6 +260,7 @@ def test_distillation(lh, cuda, N, V, D, K, T, reduction):
 def test_distillation_types_empty_rows_and_crowded_tiles(lh, cuda, where):
     _run_distill(lh, cuda, 150, 3000, 64, 100, 2.0, "mean", seed=21, empty=0.3, where=where, tdt=BF, idt=torch.int32)
     _run_distill(lh, cuda, 150, 3000, 64, 100, 2.0, "sum", seed=22, empty=0.9, where=where)
+    _run_distill(lh, cuda, 60, 3000, 136, 256, 2.0, "none", seed=45, empty=0.2, where=where)
 
 
 def test_distillation_packed(lh, cuda):
