@@ -68,6 +68,7 @@ _SIGS = {
 }
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+_DENSE = torch.contiguous_format
 
 
 def lib_path() -> pathlib.Path:
@@ -412,17 +413,29 @@ def rms_norm_bwd(dy, dh, h, weight, rstd, dx_dtype, with_dres: bool):
     N, D = _norm_check("rms_norm_bwd", h, dy, weight)
     if dx_dtype not in LH_DTYPE or (dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype)):
         raise LighthouseShapeError("rms_norm_bwd: dh must have the shape and type of h")
-    dev = _on_one_device("rms_norm_bwd", h, dy, dh, weight, rstd)
+    _on_one_device("rms_norm_bwd", h, dy, dh, weight, rstd)
     if rstd.dtype != torch.float32 or rstd.numel() != N:
         raise LighthouseShapeError("rms_norm_bwd: rstd must be fp32, one per row")
-    dx = torch.empty(h.shape, dtype=dx_dtype, device=dev)
-    dres = torch.empty(h.shape, dtype=h.dtype, device=dev) if with_dres else None
+    return rms_norm_bwd_unchecked(dy, dh, h, weight, rstd, dx_dtype, with_dres)
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_ws_size(N, D) -> int:
+    return load().lh_rms_norm_bwd_workspace_size(N, D)
+
+
+def rms_norm_bwd_unchecked(dy, dh, h, weight, rstd, dx_dtype, with_dres: bool):
+    """rms_norm_bwd of a forward's own tensors."""
+    dev = h.device
+    N, D = rstd.numel(), h.shape[-1]
+    dx = torch.empty_like(h, dtype=dx_dtype, memory_format=_DENSE)
+    dres = torch.empty_like(h, memory_format=_DENSE) if with_dres else None
     if not N:
         return dx, dres, torch.zeros_like(weight)
-    dw = torch.empty(D, dtype=weight.dtype, device=dev)
+    dw = torch.empty_like(weight, memory_format=_DENSE)
     dy, h, weight, rstd = _dense16(dy), _dense16(h), _dense16(weight), rstd.contiguous()
     dh = None if dh is None else _dense16(dh)
-    ws_bytes = load().lh_rms_norm_bwd_workspace_size(N, D)
+    ws_bytes = _norm_ws_size(N, D)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     _call(dev, "lh_rms_norm_bwd", dy.data_ptr(), LH_DTYPE[dy.dtype], _ptr(dh), h.data_ptr(), LH_DTYPE[h.dtype],
           weight.data_ptr(), LH_DTYPE[weight.dtype], rstd.data_ptr(), N, D, dx.data_ptr(), LH_DTYPE[dx_dtype], _ptr(dres),
@@ -485,28 +498,36 @@ def linear_xent_fwd(hidden, weight, target, ignore_index: int, reduction: str):
     return loss, kept
 
 
-def _loss_bwd_outputs(what, hidden, weight, kept, gout, reduction, K, *rest):
+def _loss_bwd_check(what, hidden, weight, kept, gout, reduction, K, *rest):
     N, V, D = _loss_check(what, hidden, weight, reduction)
     if gout.dtype != torch.float32 or gout.numel() != (N if reduction == "none" else 1):
         raise LighthouseShapeError(f"{what}: the loss's gradient must be fp32, one value (reduced) or N")
     if kept.dtype != torch.uint8 or kept.shape != (kept_size(N, K),) or not kept.is_contiguous():
         raise LighthouseShapeError(f"{what}: kept must be the forward's")
-    dev = _on_one_device(what, hidden, weight, kept, gout, *rest)
-    dh = torch.empty(N, D, dtype=torch.bfloat16, device=dev)
-    dw = (torch.empty if N else torch.zeros)(V, D, dtype=torch.bfloat16, device=dev)
-    return N, V, D, dev, dh, dw
+    return N, _on_one_device(what, hidden, weight, kept, gout, *rest)
 
 
 def linear_xent_bwd(hidden, weight, target, kept, gout, reduction: str):
     """Gradients (dhidden, dweight) of linear_xent_fwd."""
-    N, V, D, dev, dh, dw = _loss_bwd_outputs("linear_xent_bwd", hidden, weight, kept, gout, reduction, 0, target)
+    N, _ = _loss_bwd_check("linear_xent_bwd", hidden, weight, kept, gout, reduction, 0, target)
     if target.shape != (N,) or target.dtype != torch.int64:
         raise LighthouseShapeError("linear_xent_bwd: target must be (N) int64")
-    if N:
-        hidden, weight, target, gout = _dense16(hidden), _dense16(weight), target.contiguous(), gout.contiguous()
-        ws, n = _loss_ws(N, V, D, 0, 1, dev)
-        _call(dev, "lh_linear_xent_bwd", hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), N, V, D,
-              REDUCTIONS[reduction], kept.data_ptr(), gout.data_ptr(), dh.data_ptr(), dw.data_ptr(), ws.data_ptr(), n)
+    return linear_xent_bwd_unchecked(hidden, weight, target, kept, gout, reduction)
+
+
+def linear_xent_bwd_unchecked(hidden, weight, target, kept, gout, reduction: str):
+    """linear_xent_bwd of a forward's own tensors."""
+    dev = hidden.device
+    dh, dw = torch.empty_like(hidden, memory_format=_DENSE), torch.empty_like(weight, memory_format=_DENSE)
+    N, D = hidden.shape
+    if not N:
+        return dh, dw.zero_()
+    V = weight.shape[0]
+    hidden, weight = _dense16(hidden), _dense16(weight)
+    ws, n = _loss_ws(N, V, D, 0, 1, dev)
+    _call(dev, "lh_linear_xent_bwd", hidden.data_ptr(), weight.data_ptr(), target.contiguous().data_ptr(), N, V, D,
+          REDUCTIONS[reduction], kept.data_ptr(), gout.contiguous().data_ptr(), dh.data_ptr(), dw.data_ptr(), ws.data_ptr(),
+          n)
     return dh, dw
 
 
@@ -538,10 +559,21 @@ def linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperat
 
 def linear_distill_bwd(hidden, weight, kept, gout, K: int, temperature: float, reduction: str):
     """Gradients (dhidden, dweight) of linear_distill_fwd."""
-    N, V, D, dev, dh, dw = _loss_bwd_outputs("linear_distill_bwd", hidden, weight, kept, gout, reduction, K)
-    if N:
-        hidden, weight, gout = _dense16(hidden), _dense16(weight), gout.contiguous()
-        ws, n = _loss_ws(N, V, D, K, 1, dev)
-        _call(dev, "lh_linear_distill_bwd", hidden.data_ptr(), weight.data_ptr(), N, V, D, K, temperature,
-              REDUCTIONS[reduction], kept.data_ptr(), gout.data_ptr(), dh.data_ptr(), dw.data_ptr(), ws.data_ptr(), n)
+    _loss_bwd_check("linear_distill_bwd", hidden, weight, kept, gout, reduction, K)
+    return linear_distill_bwd_unchecked(hidden, weight, kept, gout, K, temperature, reduction)
+
+
+def linear_distill_bwd_unchecked(hidden, weight, kept, gout, K: int, temperature: float, reduction: str):
+    """linear_distill_bwd of a forward's own tensors."""
+    dev = hidden.device
+    dh, dw = torch.empty_like(hidden, memory_format=_DENSE), torch.empty_like(weight, memory_format=_DENSE)
+    N, D = hidden.shape
+    if not N:
+        return dh, dw.zero_()
+    V = weight.shape[0]
+    hidden, weight = _dense16(hidden), _dense16(weight)
+    ws, n = _loss_ws(N, V, D, K, 1, dev)
+    _call(dev, "lh_linear_distill_bwd", hidden.data_ptr(), weight.data_ptr(), N, V, D, K, temperature,
+          REDUCTIONS[reduction], kept.data_ptr(), gout.contiguous().data_ptr(), dh.data_ptr(), dw.data_ptr(), ws.data_ptr(),
+          n)
     return dh, dw

@@ -345,4 +345,8 @@ def direct(t: Tensor) -> bool:
             and not is_in_torch_dispatch_mode())
 
 
+def needs_grad(*ts: Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
+
+
 ops = torch.ops.lighthouse_b200

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .library import direct, ops as _ops
+from .library import direct, needs_grad, ops as _ops
 
 
 class _LinearXentFn(torch.autograd.Function):
@@ -32,7 +32,7 @@ class _LinearXentFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout):
         hidden, weight, target, kept = ctx.saved_tensors
-        f = _native.linear_xent_bwd if direct(gout) else _ops.linear_xent_bwd
+        f = _native.linear_xent_bwd_unchecked if direct(gout) else _ops.linear_xent_bwd
         dh, dw = f(hidden, weight, target, kept, gout, ctx.reduction)
         return dh, dw, None, None, None
 
@@ -50,7 +50,7 @@ class _LinearDistillFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout):
         hidden, weight, kept = ctx.saved_tensors
-        f = _native.linear_distill_bwd if direct(gout) else _ops.linear_distill_bwd
+        f = _native.linear_distill_bwd_unchecked if direct(gout) else _ops.linear_distill_bwd
         dh, dw = f(hidden, weight, kept, gout, ctx.K, ctx.temperature, ctx.reduction)
         return dh, dw, None, None, None, None
 
@@ -80,7 +80,11 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     that are not ignored; 0 where all are), "sum", or "none" (the loss of every
     position).  Returns fp32."""
     h = _rows(hidden, (target, 0))
-    loss = _LinearXentFn.apply(h, weight, _long(target, h.shape[0]), ignore_index, reduction)
+    target_ = _long(target, h.shape[0])
+    if direct(h) and not needs_grad(h, weight):
+        loss = _native.linear_xent_fwd(h, weight, target_, ignore_index, reduction)[0]
+    else:
+        loss = _LinearXentFn.apply(h, weight, target_, ignore_index, reduction)
     return loss.view(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
 
@@ -100,6 +104,9 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logi
     h = _rows(hidden, (teacher_logits, 1), (teacher_indices, 1))
     N = h.shape[0]
     tl = teacher_logits if teacher_logits.dim() == 2 else teacher_logits.reshape(N, teacher_logits.shape[-1])
-    loss = _LinearDistillFn.apply(h, weight, tl, _long(teacher_indices, N, teacher_indices.shape[-1]),
-                                  float(temperature), reduction)
+    args = (h, weight, tl, _long(teacher_indices, N, teacher_indices.shape[-1]), float(temperature), reduction)
+    if direct(h) and not needs_grad(h, weight):
+        loss = _native.linear_distill_fwd(*args)[0]
+    else:
+        loss = _LinearDistillFn.apply(*args)
     return loss.view(hidden.shape[:-1]) if reduction == "none" and hidden.dim() != 2 else loss

@@ -88,7 +88,7 @@ def test_workspace_stays_small(lh):
                 piece = max(512 << 20, 2 * N * 256)
                 planes = 74 * 4 * 256 * D * 8 + 10 * N * D     # parts only where few tiles are; packed rows
                 assert 0 < size(N, V, D, 0, 1) <= piece + planes + 4096, (N, V, D)
-                assert size(N, V, D, 0, 0) <= 16 * N * (V // 256 + 1) + 6 * N + 2 * N * D + 4096
+                assert size(N, V, D, 0, 0) <= 64 * N * (V // 256 + 1) + 6 * N + 2 * N * D + 4096
 
 
 def test_fake_kernels(lh):
