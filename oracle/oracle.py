@@ -18,6 +18,7 @@ Reference citations (paths inside the reference project):
 from __future__ import annotations
 
 import ctypes
+import unittest
 import math
 import pathlib
 
@@ -152,6 +153,9 @@ def ref_gpu_lib(p: int):
     """ctypes handle of the reference kernel built for sm_100a (oracle/_ref)."""
     if p not in _ref_gpu:
         so = _REF / f"libref_gpu_p{p}.so"
+        if not so.exists():
+            # as for the kernel on host threads: a test that needs it skips where the reference tree is not there
+            raise unittest.SkipTest(f"{so} not built (oracle/build.py build_ref needs the reference tree)")
         lib = ctypes.CDLL(str(so))
         lib.ref_gpu_topk.restype = ctypes.c_int
         _ref_gpu[p] = lib
