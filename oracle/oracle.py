@@ -18,9 +18,9 @@ Reference citations (paths inside the reference project):
 from __future__ import annotations
 
 import ctypes
-import unittest
 import math
 import pathlib
+import unittest
 
 import numpy as np
 import torch
