@@ -95,15 +95,15 @@ struct Args {
   uint8_t split_of[kSplitTable];  // kDH: parts of the K range by the number of row blocks, 1 beyond the table
   int b_off;                      // first row of the weights, B's operand (few rows: A's): vocabulary piece
   int out;                        // kDH, kDW: Out
-  // targets: int64 (K = 1, SPARSE false) or sorted int32 (K, n_rows), a row's entries n_rows apart
+  // targets: int64 (K = 1, SPARSE false) or sorted int32 (n_rows, K), K a multiple of four then
   const long long* target;
   const int* idx;
   int K;
   float a2;                       // exponent_scale()
   float2* stats;                  // kStats: (2 tiles_n, n_rows) maximum and sum of a row's 128 columns
-  float* slog;                    // kStats: logits of the targets (K, n_rows) out
+  float* slog;                    // kStats: logits of the targets (n_rows, K) out
   unsigned* ticket;               // kStats: set to 0 for finish_kernel
-  const float* gval;              // kGrad: exp(s - lse) - p at the targets (K, n_rows)
+  const float* gval;              // kGrad: exp(s - lse) - p at the targets (n_rows, K)
   const float* lse2;              // kGrad: log2-sum-exp2 of s a2
   const float *gout, *row_scale, *inv_count;
   int gstride;
@@ -112,16 +112,39 @@ struct Args {
   long long few_pitch;
 };
 
-// Position of the first of a row's K sorted targets, M apart, that is >= v.
-__device__ __forceinline__ int lower_bound(const int* __restrict__ idx, int K, size_t M, int v) {
+// Position of the first of a row's K sorted targets that is >= v.
+__device__ __forceinline__ int lower_bound(const int* __restrict__ idx, int K, int v) {
   int lo = 0, hi = K;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (__ldg(idx + mid * M) < v) lo = mid + 1;
+    if (__ldg(idx + mid) < v) lo = mid + 1;
     else hi = mid;
   }
   return lo;
 }
+// A row's K values (K a multiple of four) read one after the other: four at a time, the
+// next four on their way meanwhile (single loads leave a row waiting for each target).
+template <class V4, class V>
+struct Window {
+  const V4* p;
+  V4 now, behind;
+  __device__ __forceinline__ void open(const V* row, int K, int at, V none) {
+    p = reinterpret_cast<const V4*>(row);
+    const V4 empty{none, none, none, none};
+    const int g = at >> 2;
+    now = at < K ? __ldg(p + g) : empty;
+    behind = (g + 1) * 4 < K ? __ldg(p + g + 1) : empty;
+    for (int k = at & 3; k; --k) shift();
+  }
+  __device__ __forceinline__ void shift() { now.x = now.y; now.y = now.z; now.z = now.w; }
+  // to position `at`, the one behind the last
+  __device__ __forceinline__ void step(int K, int at, V none) {
+    if (at & 3) { shift(); return; }
+    now = behind;
+    if (at + 4 < K) behind = __ldg(p + (at >> 2) + 1);
+    else behind = V4{none, none, none, none};
+  }
+};
 
 // 32 values per lane, one per column -> in lane e the result of column e over the warp.
 template <class Op>
@@ -353,8 +376,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           int cur = 0, next = kNone;
           if (live) {
             if constexpr (SPARSE) {
-              cur = lower_bound(a.idx + row, a.K, a.n_rows, gv0);
-              if (cur < a.K) next = __ldg(a.idx + (size_t)cur * a.n_rows + row);
+              cur = lower_bound(a.idx + row * a.K, a.K, gv0);
+              if (cur < a.K) next = __ldg(a.idx + row * a.K + cur);
               if (next != kNone) next -= gv0;
             } else if (target >= gv0 && target < gv0 + 32) {
               next = (int)(target - gv0);
@@ -367,7 +390,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                 const int at = __shfl_sync(~0u, next, e), k = __shfl_sync(~0u, cur, e);
                 const float ce = MODE == kGrad ? __shfl_sync(~0u, c, e) : 0.f;
                 if (lane == at) {
-                  const size_t kept = (size_t)k * a.n_rows + half * 32 + e;
+                  const size_t kept = (size_t)(half * 32 + e) * a.K + k;
                   if constexpr (MODE == kStats) a.slog[kept] = __uint_as_float(x[e]);
                   else if (ce != 0.f)
                     reinterpret_cast<__nv_bfloat16*>(a.few_out)[(half * 32 + e) * a.few_pitch + v0 + lane] =
@@ -378,7 +401,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (next < left) {
               next = kNone;
               if (SPARSE && ++cur < a.K) {
-                next = __ldg(a.idx + (size_t)cur * a.n_rows + row);
+                next = __ldg(a.idx + row * a.K + cur);
                 if (next != kNone) next -= gv0;
               }
             }
@@ -423,27 +446,32 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int cols = min(kHalf, a.N - n0);           // of this warp's half, may be negative
         const bool live = row < M;
         const int orow = live && a.rows ? __ldg(a.rows + 1 + row) : row;      // row of hidden
-        // next target of this row at or behind the half's first column, as a column of the half,
-        // and the one behind it, fetched ahead
-        int cur = 0, next = kNone, after = kNone;
+        // next target of this row at or behind the half's first column, as a column of the half
+        int cur = 0, next = kNone;
         const int g0 = MODE == kGrad ? a.b_off + n0 : n0;
-        const int* idx = nullptr;
+        const size_t kept0 = (size_t)orow * a.K;         // the row's place among the targets' values
+        Window<int4, int> win;
+        Window<float4, float> val;                       // kGrad: the targets' gval
         auto advance = [&]() {
           ++cur;
-          next = after == kNone ? kNone : after - g0;
-          after = cur + 1 < a.K ? __ldg(idx + (size_t)(cur + 1) * a.n_rows) : kNone;
+          win.step(a.K, cur, kNone);
+          if (MODE == kGrad) val.step(a.K, cur, 0.f);
+          next = win.now.x == kNone ? kNone : win.now.x - g0;
         };
         float c = 0.f, lse2 = 0.f;
         if constexpr (MODE == kStats || MODE == kGrad) {
           if (live && cols > 0) {
             if constexpr (SPARSE) {
-              idx = a.idx + orow;
-              cur = lower_bound(idx, a.K, a.n_rows, g0) - 1;
-              after = cur + 1 < a.K ? __ldg(idx + (size_t)(cur + 1) * a.n_rows) : kNone;
-              advance();
+              cur = lower_bound(a.idx + kept0, a.K, g0);
+              win.open(a.idx + kept0, a.K, cur, kNone);
+              if (MODE == kGrad) val.open(a.gval + kept0, a.K, cur, 0.f);
+              next = win.now.x == kNone ? kNone : win.now.x - g0;
             } else {
               const long long tv = __ldg(a.target + orow) - g0;
-              if (tv >= 0 && tv < kHalf) next = (int)tv;
+              if (tv >= 0 && tv < kHalf) {
+                next = (int)tv;
+                if (MODE == kGrad) val.now.x = __ldg(a.gval + orow);
+              }
             }
             if constexpr (MODE == kGrad) {
               const float up = __ldg(a.gout + (size_t)orow * a.gstride);
@@ -475,7 +503,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               for (int ch = 0; ch < 8; ++ch) put(stage, ch, x[4 * ch], x[4 * ch + 1], x[4 * ch + 2], x[4 * ch + 3]);
               while (next < c0 + 32) {
                 const int at = next - c0;
-                a.slog[(size_t)cur * a.n_rows + orow] = *reinterpret_cast<const float*>(
+                a.slog[kept0 + cur] = *reinterpret_cast<const float*>(
                     stage + lane * 128 + (((at >> 2) ^ (lane & 7)) << 4) + (at & 3) * 4);
                 if constexpr (SPARSE) advance();
                 else next = kNone;
@@ -547,7 +575,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                 while (next < c0 + 64) {         // the row's targets among these columns (the same one twice: twice alike)
                   const int at = next - c0;
                   *reinterpret_cast<__nv_bfloat16*>(p + lane * 128 + (((at >> 3) ^ (lane & 7)) << 4) + (at & 7) * 2) =
-                      __float2bfloat16_rn(c * __ldg(a.gval + (size_t)cur * a.n_rows + orow));
+                      __float2bfloat16_rn(c * val.now.x);
                   if constexpr (SPARSE) advance();
                   else next = kNone;
                 }
@@ -589,31 +617,40 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 }
 
 // ---------------------------------------------------------------- small kernels
-// One warp per row: the K teacher entries sorted by vocabulary index (absent
-// ones behind; stored (K, N)), their probabilities softmax(t / T) and sum p log p.  The rank of
-// an entry is the number of entries before it, ties in their given order.
+// One warp per row: the K teacher entries sorted by vocabulary index (absent ones, and
+// those that fill a row up to Kp, a multiple of four, behind), their probabilities
+// softmax(t / T) and sum p log p.  An entry's place is the number of smaller keys, the
+// key being its index with its position in the low eight bits (V <= 2^22, K <= 256).
 //   row_scale: 1, 0 for a row without entries, NaN for one with an index >= V or
 //   a teacher logit that is NaN or +infinity
 template <class T>
 __global__ void __launch_bounds__(128)
 teacher_kernel(const T* __restrict__ tv, const long long* __restrict__ ti, int N, int V, int K, float inv_t,
                int* __restrict__ idx, float* __restrict__ prob, float* __restrict__ ent, float* __restrict__ row_scale) {
-  extern __shared__ int sh[];
+  extern __shared__ int4 sh[];
+  const int Kp = (K + 3) & ~3;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int* key = sh + warp * K;
+  int* key = reinterpret_cast<int*>(sh) + warp * Kp;
   const int row = blockIdx.x * 4 + warp;
   if (row >= N) return;
   const T* tr = tv + (size_t)row * K;
   const long long* ir = ti + (size_t)row * K;
+  idx += (size_t)row * Kp;
+  prob += (size_t)row * Kp;
+  constexpr int kAbsent = 0x7f000000;              // above every key of an entry
   bool bad = false;
   float mx = -INFINITY;
-  for (int k = lane; k < K; k += 32) {
-    const long long i = ir[k];
-    const bool here = i >= 0 && i < V;
-    const float x = (float)tr[k] * inv_t;
-    bad |= i >= V || (here && x != x);
-    key[k] = here ? (int)i : kNone;
-    if (here) mx = fmaxf(mx, x);
+  for (int k = lane; k < Kp; k += 32) {
+    bool here = false;
+    long long i = -1;
+    if (k < K) {
+      i = ir[k];
+      here = i >= 0 && i < V;
+      const float x = (float)tr[k] * inv_t;
+      bad |= i >= V || (here && x != x);
+      if (here) mx = fmaxf(mx, x);
+    }
+    key[k] = here ? (int)i << 8 | k : kAbsent + k;
   }
   __syncwarp();
 #pragma unroll
@@ -621,26 +658,31 @@ teacher_kernel(const T* __restrict__ tv, const long long* __restrict__ ti, int N
   bad = __any_sync(~0u, bad);
   float z = 0.f;
   for (int k = lane; k < K; k += 32)
-    if (key[k] != kNone && mx != -INFINITY) z += expf((float)tr[k] * inv_t - mx);
+    if (key[k] < kAbsent && mx != -INFINITY) z += expf((float)tr[k] * inv_t - mx);
 #pragma unroll
   for (int o = 16; o; o >>= 1) z += __shfl_xor_sync(~0u, z, o);
   const bool some = mx != -INFINITY;
   const float logz = logf(z);
   float e = 0.f;
   bool any_nan = false;
-  for (int k = lane; k < K; k += 32) {
+  const int4* keys = reinterpret_cast<const int4*>(key);
+  for (int k = lane; k < Kp; k += 32) {
     const int me = key[k];
     int r = 0;
-    for (int j = 0; j < K; ++j) r += key[j] < me || (key[j] == me && j < k);
+    for (int j = 0; j < Kp / 4; ++j) {
+      const int4 o = keys[j];
+      r += (o.x < me) + (o.y < me) + (o.z < me) + (o.w < me);
+    }
     float p = 0.f;
-    if (me != kNone && some) {
+    const bool here = me < kAbsent && some;
+    if (here) {
       const float x = (float)tr[k] * inv_t - mx - logz;
       p = expf(x);
       any_nan |= p != p;
       if (p > 0.f) e = fmaf(p, x, e);
     }
-    idx[(size_t)r * N + row] = some ? me : kNone;
-    prob[(size_t)r * N + row] = p;
+    idx[r] = here ? me >> 8 : kNone;
+    prob[r] = p;
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) e += __shfl_xor_sync(~0u, e, o);
@@ -773,17 +815,17 @@ finish_kernel(const FinishArgs a) {
     __syncthreads();
   }
   if (!SPARSE && RB == 8 && a.hidden) {
-    // 4 warps per row sum the target's logit anew: single logits of the tensor core are off by
-    // 6e-6 at random (D = 4096), too much for the loss of one position
+    // One to four warps per row sum the target's logit anew: single logits of the tensor core are
+    // off by 6e-6 at random (D = 4096), too much for the loss of one position.
     __shared__ float dots[8][4];
-    const int w = tid >> 5, lane = tid & 31, jj = blockIdx.x * RB + (w >> 2);
+    const int w = tid >> 5, lane = tid & 31, per = blockDim.x >> 8, jj = blockIdx.x * RB + w / per;
     float x = 0.f;
-    if (w < 32 && jj < (a.rows ? a.rows[0] : N)) {
+    if (jj < (a.rows ? a.rows[0] : N)) {
       const int rr = a.rows ? a.rows[1 + jj] : jj;
       const long long t = a.target[rr];
       if (t >= 0 && t < a.V) {
         const __nv_bfloat16 *hp = a.hidden + (size_t)rr * a.D, *wp = a.weight + (size_t)t * a.D;
-        for (int c = ((w & 3) * 32 + lane) * 8; c < a.D; c += 1024) {
+        for (int c = (w % per * 32 + lane) * 8; c < a.D; c += per * 256) {
           float u[8], v[8];
           load16(hp + c, u);
           load16(wp + c, v);
@@ -794,42 +836,50 @@ finish_kernel(const FinishArgs a) {
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
-    if (lane == 0) dots[w >> 2][w & 3] = x;
+    if (lane == 0) dots[w / per][w % per] = x;
     __syncthreads();
     if (live && slot == 0) {
       const long long t = a.target[row];
       // in the scale of the tensor core's logits, which the exponents take
-      if (t >= 0 && t < a.V) a.slog[row] = ((dots[r][0] + dots[r][1]) + (dots[r][2] + dots[r][3])) / a.up;
+      float sum = 0.f;
+      for (int k = 0; k < per; ++k) sum += dots[r][k];
+      if (t >= 0 && t < a.V) a.slog[row] = sum / a.up;
     }
   }
   const float2 all = sh[r];
   const float l2 = fmaf(all.x, a.a2, log2f(all.y));
   float loss = 0.f, scale = 0.f;
   if constexpr (SPARSE) {
+    // the entries of a row by the threads of consecutive numbers, which read them together
+    __shared__ float lse_sh[RB];
+    if (slot == 0) lse_sh[r] = l2;
+    __syncthreads();
+    const int r2 = tid / a.slots, k0 = tid % a.slots, j2 = blockIdx.x * RB + r2;
     float x = 0.f;
-    if (live) {
-      for (int k = slot; k < K; k += a.slots) {
-        const size_t at = (size_t)k * N + row;
-        const int me = a.idx[at];
+    if (j2 < (a.rows ? a.rows[0] : N)) {
+      const size_t row0 = (size_t)(a.rows ? a.rows[1 + j2] : j2) * K;
+      const int* idx = a.idx + row0;
+      const float lr = lse_sh[r2];
+      for (int k = k0; k < K; k += a.slots) {
+        const int me = idx[k];
         if (me == kNone) break;
-        const float s = a.slog[at], p = a.prob[at];
-        if (p > 0.f) x = fmaf(p, (l2 - s * a.a2) * kLn2, x);
+        const float s = a.slog[row0 + k], p = a.prob[row0 + k];
+        if (p > 0.f) x = fmaf(p, (lr - s * a.a2) * kLn2, x);
         float same = p;                            // entries with the same index add up
-        for (int i = k - 1; i >= 0 && a.idx[(size_t)i * N + row] == me; --i) same += a.prob[(size_t)i * N + row];
-        for (int i = k + 1; i < K && a.idx[(size_t)i * N + row] == me; ++i) same += a.prob[(size_t)i * N + row];
-        a.slog[at] = ex2(fmaf(s, a.a2, -l2)) - same;
+        for (int i = k - 1; i >= 0 && idx[i] == me; --i) same += a.prob[row0 + i];
+        for (int i = k + 1; i < K && idx[i] == me; ++i) same += a.prob[row0 + i];
+        a.slog[row0 + k] = ex2(fmaf(s, a.a2, -lr)) - same;
       }
     }
-    __syncthreads();                               // sh has been read
-    sh[tid].x = x;
+    sh[tid].x = x;                                 // sh was last read before the last __syncthreads
     __syncthreads();
     for (int o = a.slots >> 1; o; o >>= 1) {
-      if (slot < o) sh[tid].x += sh[tid + o * RB].x;
+      if (k0 < o) sh[tid].x += sh[tid + o].x;
       __syncthreads();
     }
     if (live && slot == 0) {
       scale = a.row_scale[row];
-      if (scale != 0.f) loss = scale * a.t2 * (a.ent[row] + sh[r].x);
+      if (scale != 0.f) loss = scale * a.t2 * (a.ent[row] + sh[r * a.slots].x);
     }
   } else if (live && slot == 0) {
     const long long t = a.target[row];
@@ -1066,10 +1116,13 @@ static Plan plan(long long N, long long V, long long D) {
   return p;
 }
 
+// Places of a row's K entries: a multiple of four, for the loads of four.
+static long long entries(long long K) { return (K + 3) & ~3ll; }
+
 // What the forward leaves for the backward.
 struct Kept {
-  float *lse2, *row_scale, *inv_count, *tgrad;   // (N), (N), (1), (max(K, 1), N)
-  int *idx, *rows;                               // (K, N) sorted targets, (2 N + 1) packed rows
+  float *lse2, *row_scale, *inv_count, *tgrad;   // (N), (N), (1), (N, max(K, 1))
+  int *idx, *rows;                               // (N, K) sorted targets, (2 N + 1) packed rows
   size_t bytes;
   Kept(void* base, long long N, long long K) {
     char* p = (char*)base;
@@ -1077,8 +1130,8 @@ struct Kept {
     lse2 = (float*)take(4 * N);
     row_scale = (float*)take(4 * N);
     inv_count = (float*)take(4);
-    tgrad = (float*)take(4 * N * (K > 1 ? K : 1));
-    idx = (int*)take(4 * N * K);
+    tgrad = (float*)take(4 * N * (K ? entries(K) : 1));
+    idx = (int*)take(4 * N * entries(K));
     rows = (int*)take(4 * (2 * N + 1));
     bytes = p - (char*)base;
   }
@@ -1107,7 +1160,7 @@ struct FwdSpace {
     ticket = (unsigned*)take(4);
     counts = (int*)take(4 * ((N + 1023) / 1024));
     ent = (float*)take(K ? 4 * N : 0);
-    prob = (float*)take(4 * N * K);
+    prob = (float*)take(4 * N * entries(K));
     packed = take(packs(N, V, D) ? (size_t)N * D * 2 : 0);
     bytes = p - (char*)base;
   }
@@ -1148,7 +1201,7 @@ template <bool SPARSE>
 static int forward(const Problem& q, int reduction, float* loss, const Kept& kp, const FwdSpace& ws, cudaStream_t st) {
   int rc = make_context_current();
   if (rc) return rc;
-  const int N = q.N, V = q.V, D = q.D, K = q.K ? q.K : 1;
+  const int N = q.N, V = q.V, D = q.D, K = q.K ? (int)entries(q.K) : 1;
   CUtensorMap mh, mw, mp;
   if ((rc = map_load(&mh, q.hidden, N, D, D)) || (rc = map_load(&mw, q.weight, V, D, D))) return rc;
   mp = mh;
@@ -1185,15 +1238,16 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
   } else if ((rc = launch<kStats, SPARSE>(mh, mw, mw, mp, a, D, st))) {
     return rc;
   }
-  // Rows per block: eight with up to 128 slots each where a row has many parts (16 rows of 1000
-  // parts: 7 us, 17 with 32 rows per block), 256 where it has up to four (65536 rows of two parts:
+  // Rows per block: eight with 32 to 128 slots each where a row has many parts or entries, four
+  // per slot (16 rows of 1000 parts: 7 us, 17 with 32 rows per block), 256 where it has up to four (65536 rows of two parts:
   // 14 us with 32 rows per block, most of it the 2048 blocks' sum).
   const int want = parts > K ? parts : K;
   FinishArgs f{ws.stats, rows, parts, N, V, K, 1, reduction, q.target, q.ignore, kp.idx, ws.prob, ws.ent, kp.tgrad, a.a2,
                q.T * q.T, kp.row_scale, kp.lse2, loss, kp.inv_count, ws.part, ws.ticket, 1.f, nullptr, nullptr, D};
   const int rb = want > 32 ? 8 : want > 4 ? 32 : 256;
-  while (f.slots < want && f.slots * rb < 1024) f.slots *= 2;
-  if (!SPARSE && V >= 16384) {       // its reads, 4 N D bytes, take 2.6 % of the product's time there, less above
+  while (f.slots < (rb == 8 ? (want + 3) / 4 : want) && f.slots * rb < 1024) f.slots *= 2;
+  if (rb == 8 && f.slots < 32) f.slots = 32;
+  if (!SPARSE && V >= 16384) {       // rb is 8; its reads, 4 N D bytes, take 2.6 % of the product's time there, less above
     f.up = (float)(1.0 + 1.02e-9 * D);
     f.hidden = (const __nv_bfloat16*)q.hidden;
     f.weight = (const __nv_bfloat16*)q.weight;
@@ -1246,7 +1300,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     a.b_off = (int)v0;
     a.target = q.target;
     a.idx = kp.idx;
-    a.K = q.K ? q.K : 1;
+    a.K = q.K ? (int)entries(q.K) : 1;
     a.a2 = exponent_scale(q.T, D);
     a.gval = kp.tgrad;
     a.lse2 = kp.lse2;
@@ -1317,10 +1371,10 @@ int linear_distill_fwd(const void* hidden, const void* weight, const void* tv, i
   const ll::FwdSpace sp(ws, N, V, D, K);
   const unsigned blocks = (unsigned)((N + 3) / 4);
   if (tv_dtype == LH_DTYPE_BF16)
-    ll::teacher_kernel<<<blocks, 128, 4 * K * sizeof(int), st>>>((const __nv_bfloat16*)tv, ti, N, V, K, 1.f / T, kp.idx,
+    ll::teacher_kernel<<<blocks, 128, 4 * ll::entries(K) * sizeof(int), st>>>((const __nv_bfloat16*)tv, ti, N, V, K, 1.f / T, kp.idx,
                                                                 sp.prob, sp.ent, kp.row_scale);
   else
-    ll::teacher_kernel<<<blocks, 128, 4 * K * sizeof(int), st>>>((const float*)tv, ti, N, V, K, 1.f / T, kp.idx, sp.prob,
+    ll::teacher_kernel<<<blocks, 128, 4 * ll::entries(K) * sizeof(int), st>>>((const float*)tv, ti, N, V, K, 1.f / T, kp.idx, sp.prob,
                                                                 sp.ent, kp.row_scale);
   int rc = check_launch("teacher_kernel");
   if (rc) return rc;
