@@ -333,9 +333,11 @@ def simple_gla_fwd(q, k, v, g, scale: float, q2=None, k2=None):
 # --------------------------------------------------------------------------- norm
 def _on_one_device(what: str, first, *rest) -> torch.device:
     """All tensors are CUDA tensors of one device, which is returned."""
+    if not first.is_cuda:
+        raise ValueError("lighthouse_b200 ops take CUDA tensors (no CPU path)")
     index = first.get_device()
-    for t in (first, *rest):
-        if t is not None and (t.get_device() != index or not t.is_cuda):
+    for t in rest:
+        if t is not None and t.get_device() != index:
             if not t.is_cuda:
                 raise ValueError("lighthouse_b200 ops take CUDA tensors (no CPU path)")
             raise ValueError(f"{what}: tensors on different devices: {first.device} and {t.device}")
@@ -365,12 +367,13 @@ def _dense16(t):
 
 
 def _norm_check(what, x, residual, weight):
-    D = x.shape[-1] if x.dim() else 0
-    if weight.shape != (D,) or (residual is not None and residual.shape != x.shape):
+    shape = x.shape
+    D = shape[-1] if shape else 0
+    if weight.shape != (D,) or (residual is not None and residual.shape != shape):
         raise LighthouseShapeError(f"{what}: x and residual (..., D) and weight (D) must agree")
-    for t in (x, residual, weight):
-        if t is not None and t.dtype not in LH_DTYPE:
-            raise ValueError(f"{what}: bf16 and fp32 tensors only, got {t.dtype}")
+    if x.dtype not in LH_DTYPE or weight.dtype not in LH_DTYPE or (
+            residual is not None and residual.dtype not in LH_DTYPE):
+        raise ValueError(f"{what}: bf16 and fp32 tensors only")
     if D % 8 or not 8 <= D <= 16384:
         raise LighthouseShapeError(f"{what}: D must be a multiple of 8 and at most 16384, got {D}")
     return x.numel() // D, D
@@ -386,25 +389,27 @@ def rms_norm_fwd(x, residual, weight, eps: float, out_dtype, group: int = 0, wit
     fp8 = out_dtype == torch.float8_e4m3fn
     if not fp8 and out_dtype not in LH_DTYPE:
         raise ValueError(f"rms_norm: out_dtype must be bf16, fp32 or float8_e4m3fn, got {out_dtype}")
-    if group not in ((0, 128) if fp8 else (0,)):
+    if group != 0 and not (fp8 and group == 128):
         raise ValueError("rms_norm: scales per row (group 0) or per 128 columns (group 128)")
     dev = _on_one_device("rms_norm", x, residual, weight)
-    y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    y = torch.empty_like(x, dtype=out_dtype, memory_format=_DENSE)
     scale = h = rstd = None
     if fp8:
         scale = torch.empty(*x.shape[:-1], (D + 127) // 128 if group else 1, dtype=torch.float32, device=dev)
     if residual is not None:
-        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+        h = torch.empty_like(residual, memory_format=_DENSE)
     if with_rstd:
         rstd = torch.empty(N, dtype=torch.float32, device=dev)
     if N:
         x, weight = _dense16(x), _dense16(weight)
+        r_ptr = h_ptr = None
         r_dtype = 0
         if residual is not None:
-            residual, r_dtype = _dense16(residual), LH_DTYPE[residual.dtype]
-        _call(dev, "lh_rms_norm_fwd", x.data_ptr(), LH_DTYPE[x.dtype], _ptr(residual), r_dtype, weight.data_ptr(),
-              LH_DTYPE[weight.dtype], N, D, eps, y.data_ptr(), 2 if fp8 else LH_DTYPE[out_dtype], _ptr(scale), group,
-              _ptr(h), _ptr(rstd))
+            residual = _dense16(residual)
+            r_ptr, r_dtype, h_ptr = residual.data_ptr(), LH_DTYPE[residual.dtype], h.data_ptr()
+        _call(dev, "lh_rms_norm_fwd", x.data_ptr(), LH_DTYPE[x.dtype], r_ptr, r_dtype, weight.data_ptr(),
+              LH_DTYPE[weight.dtype], N, D, eps, y.data_ptr(), 2 if fp8 else LH_DTYPE[out_dtype],
+              scale.data_ptr() if fp8 else None, group, h_ptr, rstd.data_ptr() if with_rstd else None)
     return y, scale, h, rstd
 
 
@@ -451,9 +456,9 @@ def _loss_check(what, hidden, weight, reduction):
         raise ValueError(f"{what}: hidden and weight must be bf16, got {hidden.dtype} and {weight.dtype}")
     N, D = hidden.shape
     V = weight.shape[0]
-    if D % 8 or not 8 <= D <= 65536 or not 1 <= V <= 1 << 22 or N > 1 << 24:
+    if D % 8 or not 8 <= D <= 65536 or not 1 <= V <= 1 << 22 or N > 1 << 22:
         raise LighthouseShapeError(f"{what}: D must be a multiple of 8 and at most 65536, V in [1, 2^22], N at most "
-                                   f"2^24; got D {D}, V {V}, N {N}")
+                                   f"2^22; got D {D}, V {V}, N {N}")
     if reduction not in REDUCTIONS:
         raise ValueError(f"{what}: reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
     return N, V, D

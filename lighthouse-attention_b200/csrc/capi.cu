@@ -331,8 +331,8 @@ int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h,
 static int loss_check(const char* what, const void* hidden, const void* weight, int N, int V, int D, int K, float T,
                       int reduction, const void* kept, const void* ws, size_t ws_bytes, int backward) {
   LH_REQUIRE(hidden && weight && kept && ws, LH_ERR_ARG, "%s: null pointer", what);
-  LH_REQUIRE(N > 0 && V > 0 && D > 0 && N <= (1 << 24) && V <= (1 << 22), LH_ERR_SHAPE,
-             "%s: N must be in [1, 2^24], V in [1, 2^22]", what);
+  LH_REQUIRE(N > 0 && V > 0 && D > 0 && N <= (1 << 22) && V <= (1 << 22), LH_ERR_SHAPE,
+             "%s: N and V must be in [1, 2^22]", what);
   LH_REQUIRE(D % 8 == 0 && D <= (1 << 16), LH_ERR_SHAPE, "%s: D must be a multiple of 8 and at most 65536, got %d", what, D);
   LH_REQUIRE(K >= 0 && K <= 256, LH_ERR_SHAPE, "%s: K must be in [1, 256], got %d", what, K);
   LH_REQUIRE(T > 0.f && T < 1e30f, LH_ERR_ARG, "%s: temperature must be positive and finite", what);

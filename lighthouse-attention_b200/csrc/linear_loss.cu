@@ -25,9 +25,10 @@
 // of either operand and both accumulators (2 x 256 TMEM columns) alternate
 // between the MMAs of one tile and the epilogue of the one before.  Roles: warp
 // 0 TMA producer, warp 1 MMA issuer (leader's), warps 4-11 epilogue (thread = row
-// = TMEM lane, two warps per row block, half the columns each).  Operands are K-major or MN-major as they lie in memory: no
-// transposed copy exists.  Where a product has few tiles, its K range is split
-// and the parts meet in fp32 planes which planes_kernel sums in a fixed order.
+// = TMEM lane, two warps per row block, half the columns each).  Operands are
+// K-major or MN-major as they lie in memory: no transposed copy exists.  Where a
+// product has few tiles, its K range is split and the parts meet in fp32 planes
+// which planes_kernel sums in a fixed order.
 // Every mbarrier wait is bounded; on expiry the CTAs leave and a status flag is set.
 #include <cudaTypedefs.h>
 
@@ -194,7 +195,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     c.tiles_m = (c.M + kTM - 1) / kTM;
     c.gm = max(1, min(a.gm, c.tiles_m));
     c.splits = a.splits;
-    if (MODE == kDH && !FEW) c.splits = min(a.splits, c.tiles_m < kSplitTable ? (int)a.split_of[c.tiles_m] : 1);
+    if (MODE == kDH && !FEW) c.splits = max(1, min(a.splits, c.tiles_m < kSplitTable ? (int)a.split_of[c.tiles_m] : 1));
     c.total = c.tiles_m * a.tiles_n * c.splits;
     c.per_split = FastDiv(max(1, c.tiles_m * a.tiles_n));
     c.per_group = FastDiv(c.gm * a.tiles_n);
@@ -272,9 +273,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           }
         }
-        // the copies of the last stages have landed before the CTA may leave (on a
-        // normal end the MMAs have already waited for them)
-        if (!ok && rank == 0)
+        // no copy is in flight when the CTAs leave, whatever the other roles waited for (the
+        // leader's barriers count the copies of both)
+        if (rank == 0)
           for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
             for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->full[i % kStages], (i / kStages) & 1); ++p) {}
       }
@@ -546,7 +547,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             tmem_ld_wait();
             if (c0 + width == kHalf) release();
             // kGrad writes zeros up to the end of the 64 rows that the last step of kDW takes
-            if (c0 >= cols || row0 >= (MODE == kGrad ? (M + 63) / 64 * 64 : M)) continue;
+            if (c0 >= cols || row0 >= (MODE == kGrad ? min(a.n_rows, (M + 63) / 64 * 64) : M)) continue;
             if (MODE == kDW && k0 == k1) {       // no rows at all in this part
 #pragma unroll
               for (int e = 0; e < 32; ++e) x[e] = y[e] = 0;

@@ -337,12 +337,18 @@ def _(hidden, weight, kept, gout, K, temperature, reduction):
 
 
 # --------------------------------------------------------------------------- eager calls
-def direct(t: Tensor) -> bool:
-    """Whether a call on t may go straight to the binding instead of through the
-    custom op: an ordinary CUDA tensor, nothing tracing or intercepting ops.  The
-    op's dispatch costs 20 to 30 us of host time, the small kernels here take less."""
-    return (type(t) in (Tensor, torch.nn.Parameter) and t.is_cuda and not torch.compiler.is_compiling()
-            and not is_in_torch_dispatch_mode())
+_PLAIN = (Tensor, torch.nn.Parameter)
+
+
+def direct(*ts: Tensor) -> bool:
+    """Whether a call on these tensors may go straight to the binding instead of
+    through the custom op: ordinary CUDA tensors, nothing tracing or intercepting
+    ops.  The op's dispatch costs 20 to 30 us of host time, the small kernels here
+    take less."""
+    for t in ts:
+        if type(t) not in _PLAIN or not t.is_cuda:
+            return False
+    return not torch.compiler.is_compiling() and not is_in_torch_dispatch_mode()
 
 
 def needs_grad(*ts: Tensor) -> bool:

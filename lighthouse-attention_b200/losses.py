@@ -22,7 +22,7 @@ from .library import direct, needs_grad, ops as _ops
 class _LinearXentFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
-        f = _native.linear_xent_fwd if direct(hidden) else _ops.linear_xent
+        f = _native.linear_xent_fwd if direct(hidden, weight, target) else _ops.linear_xent
         loss, kept = f(hidden, weight, target, ignore_index, reduction)
         ctx.save_for_backward(hidden, weight, target, kept)
         ctx.reduction = reduction
@@ -32,7 +32,7 @@ class _LinearXentFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout):
         hidden, weight, target, kept = ctx.saved_tensors
-        f = _native.linear_xent_bwd_unchecked if direct(gout) else _ops.linear_xent_bwd
+        f = _native.linear_xent_bwd_unchecked if direct(gout, hidden, weight) else _ops.linear_xent_bwd
         dh, dw = f(hidden, weight, target, kept, gout, ctx.reduction)
         return dh, dw, None, None, None
 
@@ -40,7 +40,7 @@ class _LinearXentFn(torch.autograd.Function):
 class _LinearDistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
-        f = _native.linear_distill_fwd if direct(hidden) else _ops.linear_distill
+        f = _native.linear_distill_fwd if direct(hidden, weight, teacher_logits, teacher_indices) else _ops.linear_distill
         loss, kept = f(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
         ctx.save_for_backward(hidden, weight, kept)
         ctx.K, ctx.temperature, ctx.reduction = teacher_indices.shape[1], temperature, reduction
@@ -50,7 +50,7 @@ class _LinearDistillFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout):
         hidden, weight, kept = ctx.saved_tensors
-        f = _native.linear_distill_bwd_unchecked if direct(gout) else _ops.linear_distill_bwd
+        f = _native.linear_distill_bwd_unchecked if direct(gout, hidden, weight) else _ops.linear_distill_bwd
         dh, dw = f(hidden, weight, kept, gout, ctx.K, ctx.temperature, ctx.reduction)
         return dh, dw, None, None, None, None
 
@@ -66,7 +66,10 @@ def _rows(hidden: torch.Tensor, *per_row: tuple[torch.Tensor, int]):
 
 def _long(t: torch.Tensor, *shape: int) -> torch.Tensor:
     """t as int64 of this shape."""
-    t = t if t.dtype == torch.int64 else t.to(torch.int64)
+    if t.dtype != torch.int64:
+        if t.dtype != torch.int32:
+            raise ValueError(f"targets and indices must be int64 or int32, got {t.dtype}")
+        t = t.to(torch.int64)
     return t if t.shape == shape else t.reshape(shape)
 
 
@@ -81,7 +84,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     position).  Returns fp32."""
     h = _rows(hidden, (target, 0))
     target_ = _long(target, h.shape[0])
-    if direct(h) and not needs_grad(h, weight):
+    if direct(h, weight, target_) and not needs_grad(h, weight):
         loss = _native.linear_xent_fwd(h, weight, target_, ignore_index, reduction)[0]
     else:
         loss = _LinearXentFn.apply(h, weight, target_, ignore_index, reduction)
@@ -105,7 +108,7 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logi
     N = h.shape[0]
     tl = teacher_logits if teacher_logits.dim() == 2 else teacher_logits.reshape(N, teacher_logits.shape[-1])
     args = (h, weight, tl, _long(teacher_indices, N, teacher_indices.shape[-1]), float(temperature), reduction)
-    if direct(h) and not needs_grad(h, weight):
+    if direct(*args[:4]) and not needs_grad(h, weight):
         loss = _native.linear_distill_fwd(*args)[0]
     else:
         loss = _LinearDistillFn.apply(*args)

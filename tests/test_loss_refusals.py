@@ -31,7 +31,11 @@ def test_shapes_types_and_options_are_refused(lh):
         lh.linear_cross_entropy(_z(2, 2, 64), _z(10, 64), t)
     with pytest.raises(ValueError, match="CUDA"):
         lh.linear_cross_entropy(_z(4, 64), _z(10, 64), t)
+    with pytest.raises(ValueError, match="int64 or int32"):
+        lh.linear_cross_entropy(_z(4, 64), _z(10, 64), _z(4, dtype=torch.float32))
     tv, ti = _z(4, 3, dtype=torch.float32), _z(4, 3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="int64 or int32"):
+        lh.linear_distillation(_z(4, 64), _z(10, 64), tv, tv)
     with pytest.raises(E, match="K must"):
         n.linear_distill_fwd(_z(4, 64), _z(10, 64), _z(4, 257), _z(4, 257, dtype=torch.int64), 1.0, "mean")
     with pytest.raises(E, match="K must"):
@@ -57,7 +61,7 @@ def test_c_entry_points_check_before_they_touch_a_device(lh):
         return lib.lh_linear_xent_fwd(h, w, t, -100, N, V, D, red, loss, kept, ws, n, None)
 
     assert xf(h=None) == 2 and xf(t=None) == 2 and xf(loss=None) == 2 and xf(kept=None) == 2 and xf(ws=None) == 2
-    assert xf(N=0) == 1 and xf(V=0) == 1 and xf(D=12) == 1 and xf(N=(1 << 24) + 1) == 1 and xf(V=(1 << 22) + 1) == 1
+    assert xf(N=0) == 1 and xf(V=0) == 1 and xf(D=12) == 1 and xf(N=(1 << 22) + 1) == 1 and xf(V=(1 << 22) + 1) == 1
     assert xf(red=3) == 2 and xf(w=P(4104)) == 2 and xf(kept=P(4104)) == 2 and xf(ws=P(4096 + 16)) == 2
     assert xf(n=lib.lh_linear_loss_workspace_size(4, 10, 64, 0, 0) - 1) == 5
 
