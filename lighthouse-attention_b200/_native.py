@@ -9,13 +9,15 @@ B200 the call raises.
 from __future__ import annotations
 
 import ctypes
-import functools
+import importlib.util
 import pathlib
 
 import torch
 
 _LIB_PATH = pathlib.Path(__file__).resolve().parent / "liblighthouse_b200.so"
+_EAGER_PATH = _LIB_PATH.with_name("_eager.so")
 _lib = None
+_eager = None
 
 LH_DTYPE = {torch.bfloat16: 0, torch.float32: 1}
 _VP = ctypes.c_void_p
@@ -90,6 +92,22 @@ def load() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+def eager():
+    """The eager calls of the norm and the losses (csrc/eager.cpp) on this library.  Its functions
+    take the plain case, dense aligned CUDA tensors, and return None for any other."""
+    global _eager
+    if _eager is None:
+        lib = load()
+        if not _EAGER_PATH.exists():
+            raise ImportError(f"{_EAGER_PATH} is not built; run `python lighthouse-attention_b200/build.py`")
+        spec = importlib.util.spec_from_file_location(f"{__package__}._eager", _EAGER_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind({name: ctypes.cast(getattr(lib, name), _VP).value for name in _SIGS})
+        _eager = mod
+    return _eager
 
 
 def exported_symbols() -> list[str]:
@@ -418,21 +436,9 @@ def rms_norm_bwd(dy, dh, h, weight, rstd, dx_dtype, with_dres: bool):
     N, D = _norm_check("rms_norm_bwd", h, dy, weight)
     if dx_dtype not in LH_DTYPE or (dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype)):
         raise LighthouseShapeError("rms_norm_bwd: dh must have the shape and type of h")
-    _on_one_device("rms_norm_bwd", h, dy, dh, weight, rstd)
+    dev = _on_one_device("rms_norm_bwd", h, dy, dh, weight, rstd)
     if rstd.dtype != torch.float32 or rstd.numel() != N:
         raise LighthouseShapeError("rms_norm_bwd: rstd must be fp32, one per row")
-    return rms_norm_bwd_unchecked(dy, dh, h, weight, rstd, dx_dtype, with_dres)
-
-
-@functools.lru_cache(maxsize=4096)
-def _norm_ws_size(N, D) -> int:
-    return load().lh_rms_norm_bwd_workspace_size(N, D)
-
-
-def rms_norm_bwd_unchecked(dy, dh, h, weight, rstd, dx_dtype, with_dres: bool):
-    """rms_norm_bwd of a forward's own tensors."""
-    dev = h.device
-    N, D = rstd.numel(), h.shape[-1]
     dx = torch.empty_like(h, dtype=dx_dtype, memory_format=_DENSE)
     dres = torch.empty_like(h, memory_format=_DENSE) if with_dres else None
     if not N:
@@ -440,7 +446,7 @@ def rms_norm_bwd_unchecked(dy, dh, h, weight, rstd, dx_dtype, with_dres: bool):
     dw = torch.empty_like(weight, memory_format=_DENSE)
     dy, h, weight, rstd = _dense16(dy), _dense16(h), _dense16(weight), rstd.contiguous()
     dh = None if dh is None else _dense16(dh)
-    ws_bytes = _norm_ws_size(N, D)
+    ws_bytes = load().lh_rms_norm_bwd_workspace_size(N, D)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     _call(dev, "lh_rms_norm_bwd", dy.data_ptr(), LH_DTYPE[dy.dtype], _ptr(dh), h.data_ptr(), LH_DTYPE[h.dtype],
           weight.data_ptr(), LH_DTYPE[weight.dtype], rstd.data_ptr(), N, D, dx.data_ptr(), LH_DTYPE[dx_dtype], _ptr(dres),
@@ -470,17 +476,11 @@ def _loss_out(N, reduction, dev):
     return loss if N else loss.zero_()
 
 
-@functools.lru_cache(maxsize=4096)
-def _loss_ws_size(N, V, D, K, backward) -> int:
-    return load().lh_linear_loss_workspace_size(N, V, D, K, backward)
-
-
 def _loss_ws(N, V, D, K, backward, dev):
-    n = _loss_ws_size(N, V, D, K, backward)
+    n = load().lh_linear_loss_workspace_size(N, V, D, K, backward)
     return torch.empty(n, dtype=torch.uint8, device=dev), n
 
 
-@functools.lru_cache(maxsize=4096)
 def kept_size(N: int, K: int) -> int:
     """Bytes that a loss's forward keeps for its backward."""
     return load().lh_linear_loss_kept_size(N, K)
@@ -514,20 +514,13 @@ def _loss_bwd_check(what, hidden, weight, kept, gout, reduction, K, *rest):
 
 def linear_xent_bwd(hidden, weight, target, kept, gout, reduction: str):
     """Gradients (dhidden, dweight) of linear_xent_fwd."""
-    N, _ = _loss_bwd_check("linear_xent_bwd", hidden, weight, kept, gout, reduction, 0, target)
+    N, dev = _loss_bwd_check("linear_xent_bwd", hidden, weight, kept, gout, reduction, 0, target)
     if target.shape != (N,) or target.dtype != torch.int64:
         raise LighthouseShapeError("linear_xent_bwd: target must be (N) int64")
-    return linear_xent_bwd_unchecked(hidden, weight, target, kept, gout, reduction)
-
-
-def linear_xent_bwd_unchecked(hidden, weight, target, kept, gout, reduction: str):
-    """linear_xent_bwd of a forward's own tensors."""
-    dev = hidden.device
     dh, dw = torch.empty_like(hidden, memory_format=_DENSE), torch.empty_like(weight, memory_format=_DENSE)
-    N, D = hidden.shape
     if not N:
         return dh, dw.zero_()
-    V = weight.shape[0]
+    V, D = weight.shape
     hidden, weight = _dense16(hidden), _dense16(weight)
     ws, n = _loss_ws(N, V, D, 0, 1, dev)
     _call(dev, "lh_linear_xent_bwd", hidden.data_ptr(), weight.data_ptr(), target.contiguous().data_ptr(), N, V, D,
@@ -564,18 +557,11 @@ def linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperat
 
 def linear_distill_bwd(hidden, weight, kept, gout, K: int, temperature: float, reduction: str):
     """Gradients (dhidden, dweight) of linear_distill_fwd."""
-    _loss_bwd_check("linear_distill_bwd", hidden, weight, kept, gout, reduction, K)
-    return linear_distill_bwd_unchecked(hidden, weight, kept, gout, K, temperature, reduction)
-
-
-def linear_distill_bwd_unchecked(hidden, weight, kept, gout, K: int, temperature: float, reduction: str):
-    """linear_distill_bwd of a forward's own tensors."""
-    dev = hidden.device
+    N, dev = _loss_bwd_check("linear_distill_bwd", hidden, weight, kept, gout, reduction, K)
     dh, dw = torch.empty_like(hidden, memory_format=_DENSE), torch.empty_like(weight, memory_format=_DENSE)
-    N, D = hidden.shape
     if not N:
         return dh, dw.zero_()
-    V = weight.shape[0]
+    V, D = weight.shape
     hidden, weight = _dense16(hidden), _dense16(weight)
     ws, n = _loss_ws(N, V, D, K, 1, dev)
     _call(dev, "lh_linear_distill_bwd", hidden.data_ptr(), weight.data_ptr(), N, V, D, K, temperature,

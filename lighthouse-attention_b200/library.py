@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
-from torch.utils._python_dispatch import is_in_torch_dispatch_mode
 
 from . import _native
 
@@ -334,25 +333,6 @@ def linear_distill_bwd(hidden: Tensor, weight: Tensor, kept: Tensor, gout: Tenso
 @linear_distill_bwd.register_fake
 def _(hidden, weight, kept, gout, K, temperature, reduction):
     return hidden.new_empty(hidden.shape), weight.new_empty(weight.shape)
-
-
-# --------------------------------------------------------------------------- eager calls
-_PLAIN = (Tensor, torch.nn.Parameter)
-
-
-def direct(*ts: Tensor) -> bool:
-    """Whether a call on these tensors may go straight to the binding instead of
-    through the custom op: ordinary CUDA tensors, nothing tracing or intercepting
-    ops.  The op's dispatch costs 20 to 30 us of host time, the small kernels here
-    take less."""
-    for t in ts:
-        if type(t) not in _PLAIN or not t.is_cuda:
-            return False
-    return not torch.compiler.is_compiling() and not is_in_torch_dispatch_mode()
-
-
-def needs_grad(*ts: Tensor) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in ts)
 
 
 ops = torch.ops.lighthouse_b200

@@ -16,14 +16,14 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .library import direct, needs_grad, ops as _ops
+from .library import ops as _ops
+from .norm import _eager
 
 
 class _LinearXentFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, ignore_index, reduction):
-        f = _native.linear_xent_fwd if direct(hidden, weight, target) else _ops.linear_xent
-        loss, kept = f(hidden, weight, target, ignore_index, reduction)
+        loss, kept = _ops.linear_xent(hidden, weight, target, ignore_index, reduction)
         ctx.save_for_backward(hidden, weight, target, kept)
         ctx.reduction = reduction
         return loss
@@ -31,17 +31,14 @@ class _LinearXentFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        hidden, weight, target, kept = ctx.saved_tensors
-        f = _native.linear_xent_bwd_unchecked if direct(gout, hidden, weight) else _ops.linear_xent_bwd
-        dh, dw = f(hidden, weight, target, kept, gout, ctx.reduction)
+        dh, dw = _ops.linear_xent_bwd(*ctx.saved_tensors, gout, ctx.reduction)
         return dh, dw, None, None, None
 
 
 class _LinearDistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
-        f = _native.linear_distill_fwd if direct(hidden, weight, teacher_logits, teacher_indices) else _ops.linear_distill
-        loss, kept = f(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
+        loss, kept = _ops.linear_distill(hidden, weight, teacher_logits, teacher_indices, temperature, reduction)
         ctx.save_for_backward(hidden, weight, kept)
         ctx.K, ctx.temperature, ctx.reduction = teacher_indices.shape[1], temperature, reduction
         return loss
@@ -49,9 +46,7 @@ class _LinearDistillFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        hidden, weight, kept = ctx.saved_tensors
-        f = _native.linear_distill_bwd_unchecked if direct(gout, hidden, weight) else _ops.linear_distill_bwd
-        dh, dw = f(hidden, weight, kept, gout, ctx.K, ctx.temperature, ctx.reduction)
+        dh, dw = _ops.linear_distill_bwd(*ctx.saved_tensors, gout, ctx.K, ctx.temperature, ctx.reduction)
         return dh, dw, None, None, None, None
 
 
@@ -84,9 +79,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     position).  Returns fp32."""
     h = _rows(hidden, (target, 0))
     target_ = _long(target, h.shape[0])
-    if direct(h, weight, target_) and not needs_grad(h, weight):
-        loss = _native.linear_xent_fwd(h, weight, target_, ignore_index, reduction)[0]
-    else:
+    loss = _eager("linear_xent", h, weight, target_, ignore_index, _native.REDUCTIONS.get(reduction, -1))
+    if loss is None:
         loss = _LinearXentFn.apply(h, weight, target_, ignore_index, reduction)
     return loss.view(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
@@ -107,9 +101,8 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logi
     h = _rows(hidden, (teacher_logits, 1), (teacher_indices, 1))
     N = h.shape[0]
     tl = teacher_logits if teacher_logits.dim() == 2 else teacher_logits.reshape(N, teacher_logits.shape[-1])
-    args = (h, weight, tl, _long(teacher_indices, N, teacher_indices.shape[-1]), float(temperature), reduction)
-    if direct(*args[:4]) and not needs_grad(h, weight):
-        loss = _native.linear_distill_fwd(*args)[0]
-    else:
-        loss = _LinearDistillFn.apply(*args)
+    ti, temperature = _long(teacher_indices, N, teacher_indices.shape[-1]), float(temperature)
+    loss = _eager("linear_distill", h, weight, tl, ti, temperature, _native.REDUCTIONS.get(reduction, -1))
+    if loss is None:
+        loss = _LinearDistillFn.apply(h, weight, tl, ti, temperature, reduction)
     return loss.view(hidden.shape[:-1]) if reduction == "none" and hidden.dim() != 2 else loss

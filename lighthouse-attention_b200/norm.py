@@ -16,37 +16,27 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .library import direct, needs_grad, ops as _ops
+from .library import ops as _ops
 
 
 class _RmsNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps, out_dtype):
-        if direct(x, weight):
-            y, _, _, rstd = _native.rms_norm_fwd(x, None, weight, eps, out_dtype)
-        else:
-            y, rstd = _ops.rms_norm(x, weight, eps, out_dtype)
+        y, rstd = _ops.rms_norm(x, weight, eps, out_dtype)
         ctx.save_for_backward(x, weight, rstd)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, rstd = ctx.saved_tensors
-        if direct(dy, x, weight):
-            dx, _, dw = _native.rms_norm_bwd_unchecked(dy, None, x, weight, rstd, x.dtype, False)
-        else:
-            dx, dw = _ops.rms_norm_bwd(dy, x, weight, rstd)
+        dx, dw = _ops.rms_norm_bwd(dy, *ctx.saved_tensors)
         return dx, dw, None, None
 
 
 class _AddRmsNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps, out_dtype):
-        if direct(x, residual, weight):
-            y, _, h, rstd = _native.rms_norm_fwd(x, residual, weight, eps, out_dtype)
-        else:
-            y, h, rstd = _ops.add_rms_norm(x, residual, weight, eps, out_dtype)
+        y, h, rstd = _ops.add_rms_norm(x, residual, weight, eps, out_dtype)
         ctx.save_for_backward(h, weight, rstd)
         ctx.x_dtype = x.dtype
         ctx.set_materialize_grads(False)
@@ -55,21 +45,24 @@ class _AddRmsNormFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh):
-        h, weight, rstd = ctx.saved_tensors
         if dy is None:                           # only the stream's new value was used
             return (None if dh is None else dh.to(ctx.x_dtype)), dh, None, None, None
-        if direct(dy, h, weight) and (dh is None or direct(dh)):
-            dx, dres, dw = _native.rms_norm_bwd_unchecked(dy, dh, h, weight, rstd, ctx.x_dtype, True)
-        else:
-            dx, dres, dw = _ops.add_rms_norm_bwd(dy, dh, h, weight, rstd, ctx.x_dtype)
+        dx, dres, dw = _ops.add_rms_norm_bwd(dy, dh, *ctx.saved_tensors, ctx.x_dtype)
         return dx, dres, dw, None, None
+
+
+def _eager(name: str, *args):
+    """The C++ call of this name, or None where it is not a case for it: while a
+    compiler traces, and for tensors that it does not take."""
+    return None if torch.compiler.is_compiling() else getattr(_native.eager(), name)(*args)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, out_dtype: torch.dtype | None = None):
     """x * (mean(x^2) + eps)^-1/2 * weight over the last dimension, in fp32, rounded
     once to out_dtype (default: x's type).  Differentiable in x and weight."""
-    if direct(x, weight) and not needs_grad(x, weight):
-        return _native.rms_norm_fwd(x, None, weight, float(eps), out_dtype or x.dtype, with_rstd=False)[0]
+    y = _eager("rms_norm", x, weight, eps, out_dtype)
+    if y is not None:
+        return y
     return _RmsNormFn.apply(x, weight, float(eps), out_dtype or x.dtype)
 
 
@@ -78,8 +71,9 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     """(y, h): h = x + residual rounded to the residual's type, y = rms_norm(h) in
     out_dtype (default: x's type).  The norm is that of h as stored.  Differentiable
     in x, residual and weight."""
-    if direct(x, residual, weight) and not needs_grad(x, residual, weight):
-        return _native.rms_norm_fwd(x, residual, weight, float(eps), out_dtype or x.dtype, with_rstd=False)[0:3:2]
+    out = _eager("add_rms_norm", x, residual, weight, eps, out_dtype)
+    if out is not None:
+        return out
     return _AddRmsNormFn.apply(x, residual, weight, float(eps), out_dtype or x.dtype)
 
 
@@ -88,8 +82,9 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, group
     (..., 1); with group 128 one per 128 columns, (..., ceil(D / 128)).  q * scale is
     the norm; the largest magnitude of a group has the code 448.  Has no gradient: a
     backward through it raises."""
-    if direct(x, weight) and not needs_grad(x, weight):
-        return _native.rms_norm_fwd(x, None, weight, float(eps), torch.float8_e4m3fn, group, with_rstd=False)[:2]
+    out = _eager("rms_norm_fp8", x, weight, eps, group)
+    if out is not None:
+        return out
     return _ops.rms_norm_fp8(x, weight, float(eps), group)
 
 
@@ -97,6 +92,7 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
                      group: int = 0):
     """(q, scale, h): rms_norm_fp8 of h = x + residual, h in the residual's type.
     Has no gradient: a backward through it raises."""
-    if direct(x, residual, weight) and not needs_grad(x, residual, weight):
-        return _native.rms_norm_fwd(x, residual, weight, float(eps), torch.float8_e4m3fn, group, with_rstd=False)[:3]
+    out = _eager("add_rms_norm_fp8", x, residual, weight, eps, group)
+    if out is not None:
+        return out
     return _ops.add_rms_norm_fp8(x, residual, weight, float(eps), group)

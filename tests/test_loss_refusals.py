@@ -103,3 +103,14 @@ def test_fake_kernels(lh):
     assert loss.shape == () and loss.dtype == torch.float32
     dh, dw = torch.autograd.grad(loss, (h, w))
     assert dh.shape == h.shape and dw.shape == w.shape and dh.dtype == dw.dtype == BF
+
+
+def test_eager_calls_leave_cpu_and_meta_tensors_to_python(lh):
+    e = lh._native.eager()
+    h, w, t = _z(4, 64), _z(10, 64), _z(4, dtype=torch.int64)
+    for dev in ("cpu", "meta"):
+        a, b, c = h.to(dev), w.to(dev), t.to(dev)
+        assert e.linear_xent(a, b, c, -100, 1) is None
+        assert e.linear_distill(a, b, a[:, :3].float(), c[:, None].expand(4, 3), 1.0, 1) is None
+        assert e.rms_norm(a, b[0], 1e-5, None) is None and e.add_rms_norm(a, a, b[0], 1e-5, None) is None
+        assert e.rms_norm_fp8(a, b[0], 1e-5, 0) is None and e.add_rms_norm_fp8(a, a, b[0], 1e-5, 128) is None
