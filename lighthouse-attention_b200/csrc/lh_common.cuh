@@ -126,4 +126,42 @@ __device__ __forceinline__ float round_to(float x, const __nv_bfloat16*) {
 }
 __device__ __forceinline__ float round_to(float x, const float*) { return x; }
 
+// Programmatic dependent launch, for kernels that follow one another in one call: a
+// kernel launched with launch_behind starts, and sets itself up, while the one before
+// it on the stream ends (from when all of that one's CTAs have called let_next_start),
+// and calls after_previous, which waits for that one's end, before it touches memory
+// that any other kernel writes or reads.  What it then reads
+// it reads with plain loads: the read-only path (__ldg, const __restrict__) is for
+// memory that nobody writes while the kernel lives, and the compiler may move such a
+// load across the wait.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void after_previous() {
+  let_next_start();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// 16 bytes by a plain load as VEC floats.
+template <class T>
+__device__ __forceinline__ void plain16(const T* p, float* f) {
+  unpack16(*reinterpret_cast<const uint4*>(p), f, p);
+}
+template <class... P, class... A>
+int launch_behind(const char* what, void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t st,
+                  A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  if (e == cudaSuccess) return LH_OK;
+  set_error("%s: %s", what, cudaGetErrorString(e));
+  cudaGetLastError();
+  return LH_ERR_LAUNCH;
+}
+
 }  // namespace lh

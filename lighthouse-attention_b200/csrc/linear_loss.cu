@@ -114,11 +114,11 @@ struct Args {
 };
 
 // Position of the first of a row's K sorted targets that is >= v.
-__device__ __forceinline__ int lower_bound(const int* __restrict__ idx, int K, int v) {
+__device__ __forceinline__ int lower_bound(const int* idx, int K, int v) {
   int lo = 0, hi = K;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (__ldg(idx + mid) < v) lo = mid + 1;
+    if (idx[mid] < v) lo = mid + 1;
     else hi = mid;
   }
   return lo;
@@ -133,8 +133,8 @@ struct Window {
     p = reinterpret_cast<const V4*>(row);
     const V4 empty{none, none, none, none};
     const int g = at >> 2;
-    now = at < K ? __ldg(p + g) : empty;
-    behind = (g + 1) * 4 < K ? __ldg(p + g + 1) : empty;
+    now = at < K ? p[g] : empty;
+    behind = (g + 1) * 4 < K ? p[g + 1] : empty;
     for (int k = at & 3; k; --k) shift();
   }
   __device__ __forceinline__ void shift() { now.x = now.y; now.y = now.z; now.z = now.w; }
@@ -142,7 +142,7 @@ struct Window {
   __device__ __forceinline__ void step(int K, int at, V none) {
     if (at & 3) { shift(); return; }
     now = behind;
-    if (at + 4 < K) behind = __ldg(p + (at >> 2) + 1);
+    if (at + 4 < K) behind = p[(at >> 2) + 1];
     else behind = V4{none, none, none, none};
   }
 };
@@ -182,6 +182,15 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) { mbar_init(&sm->full[s], 1); mbar_init(&sm->empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&sm->acc_full[b], 1); mbar_init(&sm->acc_empty[b], 16); }
+    mbar_init(&sm->drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 2) tmem_alloc_pair(&sm->tmem_base, 512);
+  __syncwarp();
+  after_previous();                // nothing above touches global memory
+  if (threadIdx.x == 0) {
     Sched& c = sm->sched;
     c.M = a.M;
     c.kb = a.kb;
@@ -202,14 +211,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     c.per_col = FastDiv(c.gm);
     c.per_col_last = FastDiv(max(1, c.tiles_m % c.gm));
     if (MODE == kStats && blockIdx.x == 0) *a.ticket = 0;
-    for (int s = 0; s < kStages; ++s) { mbar_init(&sm->full[s], 1); mbar_init(&sm->empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&sm->acc_full[b], 1); mbar_init(&sm->acc_empty[b], 16); }
-    mbar_init(&sm->drain, 1);
     // an earlier launch gave up a wait: do nothing until the host resets
     sm->abort = *reinterpret_cast<volatile int*>(&g_loss_status) ? 2 : 0;
-    fence_mbar_init();
   }
-  if (warp == 2) tmem_alloc_pair(&sm->tmem_base, 512);
   tc_fence_before();
   __syncwarp();
   cluster_sync();
@@ -328,11 +332,11 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       float mx = -INFINITY, sum = 0.f, c = 0.f, lse2 = 0.f;
       long long target = -1;
       if constexpr (MODE == kStats || MODE == kGrad) {
-        if (live && !SPARSE) target = __ldg(a.target + row);
+        if (live && !SPARSE) target = a.target[row];
         if (MODE == kGrad && live) {
-          const float up = __ldg(a.gout + (size_t)row * a.gstride);
-          if (up != 0.f) c = a.cscale * up * __ldg(a.row_scale + row) * (a.inv_count ? __ldg(a.inv_count) : 1.f);
-          lse2 = __ldg(a.lse2 + row);
+          const float up = a.gout[(size_t)row * a.gstride];
+          if (up != 0.f) c = a.cscale * up * a.row_scale[row] * (a.inv_count ? *a.inv_count : 1.f);
+          lse2 = a.lse2[row];
         }
       }
       int li = 0;
@@ -378,7 +382,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if (live) {
             if constexpr (SPARSE) {
               cur = lower_bound(a.idx + row * a.K, a.K, gv0);
-              if (cur < a.K) next = __ldg(a.idx + row * a.K + cur);
+              if (cur < a.K) next = a.idx[row * a.K + cur];
               if (next != kNone) next -= gv0;
             } else if (target >= gv0 && target < gv0 + 32) {
               next = (int)(target - gv0);
@@ -395,14 +399,14 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                   if constexpr (MODE == kStats) a.slog[kept] = __uint_as_float(x[e]);
                   else if (ce != 0.f)
                     reinterpret_cast<__nv_bfloat16*>(a.few_out)[(half * 32 + e) * a.few_pitch + v0 + lane] =
-                        __float2bfloat16_rn(ce * __ldg(a.gval + kept));
+                        __float2bfloat16_rn(ce * a.gval[kept]);
                 }
               }
             }
             if (next < left) {
               next = kNone;
               if (SPARSE && ++cur < a.K) {
-                next = __ldg(a.idx + row * a.K + cur);
+                next = a.idx[row * a.K + cur];
                 if (next != kNone) next -= gv0;
               }
             }
@@ -446,7 +450,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int row0 = m * kTM + rank * 128 + quad * 32, row = row0 + lane, n0 = n * kTN + half * kHalf;
         const int cols = min(kHalf, a.N - n0);           // of this warp's half, may be negative
         const bool live = row < M;
-        const int orow = live && a.rows ? __ldg(a.rows + 1 + row) : row;      // row of hidden
+        const int orow = live && a.rows ? a.rows[1 + row] : row;      // row of hidden
         // next target of this row at or behind the half's first column, as a column of the half
         int cur = 0, next = kNone;
         const int g0 = MODE == kGrad ? a.b_off + n0 : n0;
@@ -468,16 +472,16 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               if (MODE == kGrad) val.open(a.gval + kept0, a.K, cur, 0.f);
               next = win.now.x == kNone ? kNone : win.now.x - g0;
             } else {
-              const long long tv = __ldg(a.target + orow) - g0;
+              const long long tv = a.target[orow] - g0;
               if (tv >= 0 && tv < kHalf) {
                 next = (int)tv;
-                if (MODE == kGrad) val.now.x = __ldg(a.gval + orow);
+                if (MODE == kGrad) val.now.x = a.gval[orow];
               }
             }
             if constexpr (MODE == kGrad) {
-              const float up = __ldg(a.gout + (size_t)orow * a.gstride);
-              if (up != 0.f) c = a.cscale * up * __ldg(a.row_scale + orow) * (a.inv_count ? __ldg(a.inv_count) : 1.f);
-              lse2 = __ldg(a.lse2 + orow);
+              const float up = a.gout[(size_t)orow * a.gstride];
+              if (up != 0.f) c = a.cscale * up * a.row_scale[orow] * (a.inv_count ? *a.inv_count : 1.f);
+              lse2 = a.lse2[orow];
             }
           }
         }
@@ -626,8 +630,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 //   a teacher logit that is NaN or +infinity
 template <class T>
 __global__ void __launch_bounds__(128)
-teacher_kernel(const T* __restrict__ tv, const long long* __restrict__ ti, int N, int V, int K, float inv_t,
-               int* __restrict__ idx, float* __restrict__ prob, float* __restrict__ ent, float* __restrict__ row_scale) {
+teacher_kernel(const T* tv, const long long* ti, int N, int V, int K, float inv_t,
+               int* idx, float* prob, float* ent, float* row_scale) {
+  after_previous();
   extern __shared__ int4 sh[];
   const int Kp = (K + 3) & ~3;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -703,8 +708,9 @@ __device__ __forceinline__ bool row_counts(const long long* target, long long ig
 // Counts per block; what the losses of the other rows are.
 template <bool SPARSE>
 __global__ void __launch_bounds__(1024)
-mark_kernel(const long long* __restrict__ target, long long ignore, float* row_scale, float* __restrict__ lse2,
-            float* __restrict__ loss_rows, int N, int* __restrict__ counts) {
+mark_kernel(const long long* target, long long ignore, float* row_scale, float* lse2,
+            float* loss_rows, int N, int* counts) {
+  after_previous();
   const int i = blockIdx.x * 1024 + threadIdx.x;
   const bool yes = i < N && row_counts<SPARSE>(target, ignore, row_scale, i);
   if (i < N && !yes) {
@@ -717,8 +723,9 @@ mark_kernel(const long long* __restrict__ target, long long ignore, float* row_s
 }
 template <bool SPARSE>
 __global__ void __launch_bounds__(1024)
-index_kernel(const long long* __restrict__ target, long long ignore, const float* __restrict__ row_scale, int N,
-             const int* __restrict__ counts, int* __restrict__ rows) {
+index_kernel(const long long* target, long long ignore, const float* row_scale, int N,
+             const int* counts, int* rows) {
+  after_previous();
   __shared__ int sums[2][32];
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   int before = 0, all = 0;
@@ -751,14 +758,15 @@ index_kernel(const long long* __restrict__ target, long long ignore, const float
 // One warp per packed row; zeros behind the last up to a multiple of 64 rows, the
 // depth of kDW's steps.  Nothing to do where every row counts.
 __global__ void __launch_bounds__(256)
-pack_kernel(const uint4* __restrict__ hidden, const int* __restrict__ rows, int N, int chunks, uint4* __restrict__ out) {
+pack_kernel(const uint4* hidden, const int* rows, int N, int chunks, uint4* out) {
+  after_previous();
   const int live = rows[0], lane = threadIdx.x & 31;
   const int j = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (live == N || j >= min(N, (live + 63) / 64 * 64)) return;
   uint4* o = out + (size_t)j * chunks;
   if (j < live) {
     const uint4* h = hidden + (size_t)rows[1 + j] * chunks;
-    for (int c = lane; c < chunks; c += 32) o[c] = __ldg(h + c);
+    for (int c = lane; c < chunks; c += 32) o[c] = h[c];
   } else {
     for (int c = lane; c < chunks; c += 32) o[c] = make_uint4(0, 0, 0, 0);
   }
@@ -791,6 +799,7 @@ struct FinishArgs {
 template <bool SPARSE, int RB>
 __global__ void __launch_bounds__(1024)
 finish_kernel(const FinishArgs a) {
+  after_previous();
   __shared__ float2 sh[1024];
   __shared__ double2 tot[32];
   __shared__ bool last;
@@ -828,8 +837,8 @@ finish_kernel(const FinishArgs a) {
         const __nv_bfloat16 *hp = a.hidden + (size_t)rr * a.D, *wp = a.weight + (size_t)t * a.D;
         for (int c = (w % per * 32 + lane) * 8; c < a.D; c += per * 256) {
           float u[8], v[8];
-          load16(hp + c, u);
-          load16(wp + c, v);
+          plain16(hp + c, u);
+          plain16(wp + c, v);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x = fmaf(u[e], v[e], x);
         }
@@ -922,9 +931,9 @@ finish_kernel(const FinishArgs a) {
   s = c = 0;
 #pragma unroll 4
   for (int i = tid; i < (int)gridDim.x; i += blockDim.x) {
-    const double2 v = __ldcg(a.part + i);
-    s += v.x;
-    c += v.y;
+    const volatile double2* v = a.part + i;
+    s += v->x;
+    c += v->y;
   }
   block_sum(s, c);
   if (tid == 0) {
@@ -946,6 +955,7 @@ struct PlanesArgs {
 };
 __global__ void __launch_bounds__(256)
 planes_kernel(const __grid_constant__ PlanesArgs a) {
+  after_previous();
   const size_t plane = (size_t)a.n_rows * a.cols;
   const int chunks = a.cols / 8;
   int n = a.n;
@@ -968,8 +978,8 @@ planes_kernel(const __grid_constant__ PlanesArgs a) {
 #pragma unroll 4
       for (int k = 0; k < n; ++k) {
         float u[8];
-        load16(p + k * plane, u);
-        load16(p + k * plane + 4, u + 4);
+        plain16(p + k * plane, u);
+        plain16(p + k * plane + 4, u + 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += u[e];
       }
@@ -1052,8 +1062,8 @@ static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMa
     if (e == cudaSuccess && dev < 64) allowed.fetch_or(bit);
   }
   if (e != cudaSuccess) { set_error("linear loss: %s", cudaGetErrorString(e)); return LH_ERR_LAUNCH; }
-  loss_gemm_kernel<MODE, SPARSE, FEW><<<2 * pairs, kThreads, smem_bytes(MODE, FEW), st>>>(ma, mb, mo, mp, a);
-  return check_launch("loss_gemm_kernel");
+  return launch_behind("loss_gemm_kernel", loss_gemm_kernel<MODE, SPARSE, FEW>, 2 * pairs, kThreads, smem_bytes(MODE, FEW), st,
+                       ma, mb, mo, mp, a);
 }
 
 // Parts of the K range of an (M, N) product: the number that makes the shortest
@@ -1180,13 +1190,11 @@ static int sum_planes(const float* planes, const Plan* p, int n, int rows, int c
   if (p)
     for (int t = 0; t < kSplitTable; ++t) a.split_of[t] = p->split_of[t];
   const size_t blocks = ((size_t)rows * (cols / 8) + 255) / 256;
-  planes_kernel<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st>>>(a);
-  return check_launch("planes_kernel");
+  return launch_behind("planes_kernel", planes_kernel, (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, st, a);
 }
 
 static int pack_rows(const void* hidden, const int* rows, int N, int D, void* out, cudaStream_t st) {
-  pack_kernel<<<(N + 7) / 8, 256, 0, st>>>((const uint4*)hidden, rows, N, D / 8, (uint4*)out);
-  return check_launch("pack_kernel");
+  return launch_behind("pack_kernel", pack_kernel, (N + 7) / 8, 256, 0, st, (const uint4*)hidden, rows, N, D / 8, (uint4*)out);
 }
 
 struct Problem {
@@ -1209,11 +1217,11 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
   const int* rows = nullptr;
   if (packs(N, V, D)) {
     const int blocks = (N + 1023) / 1024;
-    mark_kernel<SPARSE><<<blocks, 1024, 0, st>>>(q.target, q.ignore, kp.row_scale, kp.lse2,
-                                                 reduction == LH_REDUCE_NONE ? loss : nullptr, N, ws.counts);
-    if ((rc = check_launch("mark_kernel"))) return rc;
-    index_kernel<SPARSE><<<blocks, 1024, 0, st>>>(q.target, q.ignore, kp.row_scale, N, ws.counts, kp.rows);
-    if ((rc = check_launch("index_kernel")) || (rc = pack_rows(q.hidden, kp.rows, N, D, ws.packed, st)) ||
+    if ((rc = launch_behind("mark_kernel", mark_kernel<SPARSE>, blocks, 1024, 0, st, q.target, q.ignore, kp.row_scale, kp.lse2,
+                            reduction == LH_REDUCE_NONE ? loss : nullptr, N, ws.counts)) ||
+        (rc = launch_behind("index_kernel", index_kernel<SPARSE>, blocks, 1024, 0, st, q.target, q.ignore, kp.row_scale, N,
+                            ws.counts, kp.rows)) ||
+        (rc = pack_rows(q.hidden, kp.rows, N, D, ws.packed, st)) ||
         (rc = map_load(&mp, ws.packed, N, D, D)))
       return rc;
     rows = kp.rows;
@@ -1254,10 +1262,9 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
     f.weight = (const __nv_bfloat16*)q.weight;
   }
   const unsigned blocks = (unsigned)((N + rb - 1) / rb);
-  if (rb == 8) finish_kernel<SPARSE, 8><<<blocks, rb * f.slots, 0, st>>>(f);
-  else if (rb == 256) finish_kernel<SPARSE, 256><<<blocks, rb * f.slots, 0, st>>>(f);
-  else finish_kernel<SPARSE, 32><<<blocks, rb * f.slots, 0, st>>>(f);
-  return check_launch("finish_kernel");
+  return launch_behind("finish_kernel", rb == 8 ? finish_kernel<SPARSE, 8> : rb == 256 ? finish_kernel<SPARSE, 256>
+                                                                                   : finish_kernel<SPARSE, 32>,
+                       blocks, rb * f.slots, 0, st, f);
 }
 
 template <bool SPARSE>
@@ -1371,13 +1378,12 @@ int linear_distill_fwd(const void* hidden, const void* weight, const void* tv, i
   const ll::Kept kp(kept, N, K);
   const ll::FwdSpace sp(ws, N, V, D, K);
   const unsigned blocks = (unsigned)((N + 3) / 4);
-  if (tv_dtype == LH_DTYPE_BF16)
-    ll::teacher_kernel<<<blocks, 128, 4 * ll::entries(K) * sizeof(int), st>>>((const __nv_bfloat16*)tv, ti, N, V, K, 1.f / T, kp.idx,
-                                                                sp.prob, sp.ent, kp.row_scale);
-  else
-    ll::teacher_kernel<<<blocks, 128, 4 * ll::entries(K) * sizeof(int), st>>>((const float*)tv, ti, N, V, K, 1.f / T, kp.idx, sp.prob,
-                                                                sp.ent, kp.row_scale);
-  int rc = check_launch("teacher_kernel");
+  const size_t smem = 4 * ll::entries(K) * sizeof(int);
+  int rc = tv_dtype == LH_DTYPE_BF16
+               ? launch_behind("teacher_kernel", ll::teacher_kernel<__nv_bfloat16>, blocks, 128, smem, st,
+                                   (const __nv_bfloat16*)tv, ti, N, V, K, 1.f / T, kp.idx, sp.prob, sp.ent, kp.row_scale)
+               : launch_behind("teacher_kernel", ll::teacher_kernel<float>, blocks, 128, smem, st, (const float*)tv, ti, N, V,
+                                   K, 1.f / T, kp.idx, sp.prob, sp.ent, kp.row_scale);
   if (rc) return rc;
   return ll::forward<true>({hidden, weight, N, V, D, nullptr, 0, K, T}, reduction, loss, kp, sp, st);
 }

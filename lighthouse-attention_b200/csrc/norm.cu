@@ -232,6 +232,7 @@ struct BwdArgs {
 template <class TY, class TH, class TX, bool CTA, int CH, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB)
 rms_norm_bwd_kernel(const BwdArgs a) {
+  let_next_start();                                      // dw_reduce_kernel
   __shared__ float2 part[2][32];
   extern __shared__ float dw_sm[];                       // !CTA: 8 x D
   const int t = CTA ? threadIdx.x : (threadIdx.x & 31);
@@ -335,7 +336,8 @@ rms_norm_bwd_kernel(const BwdArgs a) {
 // dw = column sums of dw_part (parts, D): 32 columns per block, 32 strided
 // slices of the rows, then a tree over the slices.
 __global__ void __launch_bounds__(1024)
-dw_reduce_kernel(const float* __restrict__ part, int parts, int D, void* dw, bool w_f32) {
+dw_reduce_kernel(const float* part, int parts, int D, void* dw, bool w_f32) {
+  after_previous();
   __shared__ float sm[32][33];
   const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + c;
@@ -414,8 +416,7 @@ int launch_bwd(const BwdArgs& a, void* dw, cudaStream_t st) {
   }
   int rc = check_launch("rms_norm_bwd_kernel");
   if (rc) return rc;
-  dw_reduce_kernel<<<(a.D + 31) / 32, 1024, 0, st>>>(a.dw_part, grid, a.D, dw, a.w_f32);
-  return check_launch("dw_reduce_kernel");
+  return launch_behind("dw_reduce_kernel", dw_reduce_kernel, (a.D + 31) / 32, 1024, 0, st, a.dw_part, grid, a.D, dw, a.w_f32);
 }
 
 template <class TY, class TH>
