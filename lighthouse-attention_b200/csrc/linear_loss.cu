@@ -74,7 +74,11 @@ constexpr int smem_bytes(int mode, bool few) {
 // Walk of the tiles: split, group of gm row blocks, column block, row block in the group.
 struct Sched {
   int M, tiles_m, gm, kb, splits, total, packed;
-  FastDiv per_split, per_group, per_col, per_col_last;
+  FastDiv div[4];                 // by the tiles of a split, of a group, of its columns, of the last group's
+  __host__ __device__ uint32_t divisor(int i, int tiles_n) const {
+    const uint32_t d = i == 0 ? tiles_m * tiles_n : i == 1 ? gm * tiles_n : i == 2 ? gm : gm ? tiles_m % gm : 0;
+    return d ? d : 1;
+  }
 };
 
 struct Smem {
@@ -91,6 +95,7 @@ constexpr int kSplitTable = 2 * kPairs;
 struct Args {
   int M, N;                       // rows and columns of the result
   int tiles_n, splits, kb, gm;
+  Sched sched;                    // of all rows
   int n_rows;                     // rows of hidden
   const int* rows;                // NULL, or: number of packed rows, their rows of hidden, (and back)
   uint8_t split_of[kSplitTable];  // kDH: parts of the K range by the number of row blocks, 1 beyond the table
@@ -182,6 +187,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
     for (int s = 0; s < kStages; ++s) { mbar_init(&sm->full[s], 1); mbar_init(&sm->empty[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&sm->acc_full[b], 1); mbar_init(&sm->acc_empty[b], 16); }
     mbar_init(&sm->drain, 1);
@@ -190,29 +197,33 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   if (warp == 2) tmem_alloc_pair(&sm->tmem_base, 512);
   __syncwarp();
   after_previous();                // nothing above touches global memory
-  if (threadIdx.x == 0) {
-    Sched& c = sm->sched;
-    c.M = a.M;
-    c.kb = a.kb;
-    c.packed = 0;
-    if (a.rows) {
-      const int live = *a.rows;
-      if (MODE == kDW) c.kb = (live + kTK - 1) / kTK;
-      else c.M = live;
-      c.packed = live < a.n_rows;
+  if (warp == 3) {
+    // The walk of the host's numbers, or of the packed rows' (each divisor by a lane of its own).
+    const int live = a.rows ? *a.rows : a.n_rows;
+    if (live == a.n_rows) {
+      if (lane == 0) sm->sched = a.sched;
+    } else {
+      Sched c;
+      c.M = MODE == kDW ? a.M : live;
+      c.kb = MODE == kDW ? (live + kTK - 1) / kTK : a.kb;
+      c.packed = 1;
+      c.tiles_m = (c.M + kTM - 1) / kTM;
+      c.gm = max(1, min(a.gm, c.tiles_m));
+      c.splits = a.splits;
+      if (MODE == kDH) c.splits = max(1, min(a.splits, c.tiles_m < kSplitTable ? (int)a.split_of[c.tiles_m] : 1));
+      c.total = c.tiles_m * a.tiles_n * c.splits;
+      const FastDiv mine(c.divisor(lane & 3, a.tiles_n));
+      if (lane < 4) sm->sched.div[lane] = mine;
+      if (lane == 0) {
+        sm->sched.M = c.M; sm->sched.tiles_m = c.tiles_m; sm->sched.gm = c.gm; sm->sched.kb = c.kb;
+        sm->sched.splits = c.splits; sm->sched.total = c.total; sm->sched.packed = 1;
+      }
     }
-    c.tiles_m = (c.M + kTM - 1) / kTM;
-    c.gm = max(1, min(a.gm, c.tiles_m));
-    c.splits = a.splits;
-    if (MODE == kDH && !FEW) c.splits = max(1, min(a.splits, c.tiles_m < kSplitTable ? (int)a.split_of[c.tiles_m] : 1));
-    c.total = c.tiles_m * a.tiles_n * c.splits;
-    c.per_split = FastDiv(max(1, c.tiles_m * a.tiles_n));
-    c.per_group = FastDiv(c.gm * a.tiles_n);
-    c.per_col = FastDiv(c.gm);
-    c.per_col_last = FastDiv(max(1, c.tiles_m % c.gm));
-    if (MODE == kStats && blockIdx.x == 0) *a.ticket = 0;
-    // an earlier launch gave up a wait: do nothing until the host resets
-    sm->abort = *reinterpret_cast<volatile int*>(&g_loss_status) ? 2 : 0;
+    if (lane == 0) {
+      if (MODE == kStats && blockIdx.x == 0) *a.ticket = 0;
+      // an earlier launch gave up a wait: do nothing until the host resets
+      sm->abort = *reinterpret_cast<volatile int*>(&g_loss_status) ? 2 : 0;
+    }
   }
   tc_fence_before();
   __syncwarp();
@@ -226,10 +237,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   // tile t -> split, row block, column block
   auto decode = [&](int t, int& m, int& n, int& k0, int& k1, int& split) {
     uint32_t sp, r, g, x, y;
-    sched.per_split.divmod(t, sp, r);
-    sched.per_group.divmod(r, g, r);
-    if ((int)((g + 1) * sched.gm) <= sched.tiles_m) sched.per_col.divmod(r, x, y);
-    else sched.per_col_last.divmod(r, x, y);
+    sched.div[0].divmod(t, sp, r);
+    sched.div[1].divmod(r, g, r);
+    sched.div[(int)((g + 1) * sched.gm) <= sched.tiles_m ? 2 : 3].divmod(r, x, y);
     m = g * sched.gm + y;
     n = x;
     split = sp;
@@ -244,8 +254,6 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       if (lane == 0) {
         const CUtensorMap* mapA = kAMn || MODE == kDH || !sched.packed ? &tmA : &tmP;
         const CUtensorMap* mapB = MODE == kDW && sched.packed ? &tmP : &tmB;
-        tma_prefetch_desc(mapA);
-        tma_prefetch_desc(mapB);
         uint32_t it = 0;
         bool ok = true;
         for (int t = pair; t < total && ok; t += n_pairs) {
@@ -294,7 +302,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         // MMAs are issued makes the kernel 3 to 8 % slower, not faster.)
         const int q = sched.kb / sched.splits, rem = sched.kb - q * sched.splits;
         for (int t = pair; t < total && ok; t += n_pairs, ++li) {
-          const int steps = q + ((int)sched.per_split.div(t) < rem ? 1 : 0);
+          const int steps = q + ((int)sched.div[0].div(t) < rem ? 1 : 0);
           const int b = li & 1;
           const uint32_t acc = tbase + b * kCols;
           if (li >= 2 && !mbar_wait(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort)) break;
@@ -1051,7 +1059,20 @@ static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMa
   long long gm = (48ll << 20) / (kTM * 2ll * a.kb * kTK);
   if (gm < 8) gm = 8;
   a.gm = (int)(gm < tiles_m ? gm : tiles_m);
-  const long long total = (long long)tiles_m * a.tiles_n * a.splits;
+  Sched& c = a.sched;
+  c.M = a.M;
+  c.kb = a.kb;
+  c.packed = 0;
+  c.tiles_m = tiles_m;
+  c.gm = a.gm;
+  c.splits = a.splits;
+  if (MODE == kDH && !FEW) {         // as the kernel has it for packed rows
+    const int s = tiles_m < kSplitTable ? a.split_of[tiles_m] : 1;
+    if (s < c.splits) c.splits = s > 1 ? s : 1;
+  }
+  c.total = (int)((long long)tiles_m * a.tiles_n * c.splits);
+  const long long total = (long long)tiles_m * a.tiles_n * a.splits;      // at most: packed rows may have more parts
+  for (int i = 0; i < 4; ++i) c.div[i] = FastDiv(c.divisor(i, a.tiles_n));
   const int pairs = (int)(total < kPairs ? total : kPairs);
   static std::atomic<uint64_t> allowed{0};           // devices on which the kernel may use its shared memory
   int dev = 0;
