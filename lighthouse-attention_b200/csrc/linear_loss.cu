@@ -57,18 +57,16 @@ constexpr float kLn2 = 0.69314718055994531f;
 enum Mode { kStats, kGrad, kDH, kDW };
 enum Out { kOutBf16, kOutPlane, kOutPlaneAdd };
 
-// Stages of the operand ring and staging buffers per epilogue warp: a warp's half
-// of a bf16 row block is two stores, each with a buffer of its own, so that it
-// waits for a store of the tile before only; kStats stores nothing.
 // With few rows (kFew at most) the roles turn: the 256 rows of a tile are weights (or
 // columns of dH) and its kFew columns are rows of hidden, so that the MMAs do an eighth
 // of the work and the stages hold weights, which are what has to be read.
 constexpr int kFew = 64;
-__host__ __device__ constexpr int stages(int mode, bool few) { return few ? 10 : mode == kStats ? 6 : 5; }
-__host__ __device__ constexpr int bufs(int mode, bool few) { return few ? 0 : mode == kStats ? 1 : 2; }
+// Six stages of the operands and one store's staging buffer per epilogue warp (five and
+// two: 1 to 2 % slower over the four products).
+__host__ __device__ constexpr int stages(bool few) { return few ? 10 : 6; }
 __host__ __device__ constexpr int b_bytes(bool few) { return few ? kFew / 2 * 128 : kOpBytes; }
-constexpr int smem_bytes(int mode, bool few) {
-  return 1024 + stages(mode, few) * (kOpBytes + b_bytes(few)) + 8 * bufs(mode, few) * kOutBuf + 512;
+constexpr int smem_bytes(bool few) {
+  return 1024 + stages(few) * (kOpBytes + b_bytes(few)) + (few ? 0 : 8 * kOutBuf) + 512;
 }
 
 // Walk of the tiles: split, group of gm row blocks, column block, row block in the group.
@@ -88,8 +86,7 @@ struct Smem {
   int abort;
 };
 static_assert(sizeof(Smem) <= 512, "barriers do not fit their space");
-static_assert(smem_bytes(kStats, false) <= 232448 && smem_bytes(kGrad, false) <= 232448 && smem_bytes(kStats, true) <= 232448,
-              "stages do not fit shared memory");
+static_assert(smem_bytes(false) <= 232448 && smem_bytes(true) <= 232448, "stages do not fit shared memory");
 
 constexpr int kSplitTable = 2 * kPairs;
 struct Args {
@@ -174,14 +171,14 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                  const __grid_constant__ Args a) {
   // tmP: the packed rows, in the place of hidden (A of kStats and kGrad, B of kDW)
   constexpr bool kAMn = MODE == kDW || (FEW && MODE == kDH), kBMn = !FEW && (MODE == kDH || MODE == kDW);
-  constexpr int kStages = stages(MODE, FEW), kBufs = bufs(MODE, FEW), kBBytes = b_bytes(FEW);
+  constexpr int kStages = stages(FEW), kBBytes = b_bytes(FEW);
   constexpr int kCols = FEW ? kFew : kTN;          // columns of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = base;
   uint8_t* sB = base + kStages * kOpBytes;
   uint8_t* sO = base + kStages * (kOpBytes + kBBytes);
-  Smem* sm = reinterpret_cast<Smem*>(sO + 8 * kBufs * kOutBuf);
+  Smem* sm = reinterpret_cast<Smem*>(sO + (FEW ? 0 : 8 * kOutBuf));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
@@ -443,9 +440,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const int quad = warp & 3, half = warp >= 8 ? 1 : 0;
       constexpr int kHalf = kTN / 2;
       const uint32_t lane_base = tbase + ((uint32_t)(quad * 32) << 16) + half * kHalf;
-      uint8_t* stage = sO + (quad + 4 * half) * kBufs * kOutBuf;
+      uint8_t* stage = sO + (quad + 4 * half) * kOutBuf;
       const uint32_t acc_empty0 = leader_addr(&sm->acc_empty[0]), acc_empty1 = leader_addr(&sm->acc_empty[1]);
-      int li = 0, buf = 0;
+      int li = 0;
       // 16 bytes to chunk c of this thread's row of a staging tile (128-byte swizzle)
       auto put = [&](uint8_t* p, int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
         *reinterpret_cast<uint4*>(p + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(x, y, z, w);
@@ -564,8 +561,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
               for (int e = 0; e < 32; ++e) x[e] = y[e] = 0;
             }
-            uint8_t* p = stage + buf * kOutBuf;
-            if (lane == 0) bulk_wait_read_1();
+            uint8_t* p = stage;
+            if (lane == 0) bulk_wait_read_all();
             __syncwarp();
             if constexpr (MODE == kGrad) {
               if (c == 0.f) {                    // a row without a gradient, whatever its logits are
@@ -611,7 +608,6 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               else tma_store_3d(&tmO, p, n0 + c0, row0, split);
               bulk_commit();
             }
-            buf ^= 1;
           }
         }
       }
@@ -1079,11 +1075,11 @@ static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMa
   cudaError_t e = cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (e == cudaSuccess && (dev >= 64 || !(allowed.load() & bit))) {
-    e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MODE, FEW));
+    e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(FEW));
     if (e == cudaSuccess && dev < 64) allowed.fetch_or(bit);
   }
   if (e != cudaSuccess) { set_error("linear loss: %s", cudaGetErrorString(e)); return LH_ERR_LAUNCH; }
-  return launch_behind("loss_gemm_kernel", loss_gemm_kernel<MODE, SPARSE, FEW>, 2 * pairs, kThreads, smem_bytes(MODE, FEW), st,
+  return launch_behind("loss_gemm_kernel", loss_gemm_kernel<MODE, SPARSE, FEW>, 2 * pairs, kThreads, smem_bytes(FEW), st,
                        ma, mb, mo, mp, a);
 }
 
