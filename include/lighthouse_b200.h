@@ -271,7 +271,8 @@ int lh_linear_xent_fwd(const void* hidden, const void* weight, const int64_t* ta
 
 /* Gradients of lh_linear_xent_fwd.
  *   gout    fp32 upstream gradient of loss: (N) with LH_REDUCE_NONE, else (1)
- *   dhidden (N, D), dweight (V, D) bf16 out */
+ *   dhidden (N, D), dweight (V, D) bf16 out; one of them may be NULL, and its
+ *             product is left out then */
 int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* target, int N, int V, int D, int reduction,
                        const void* kept, const float* gout, void* dhidden, void* dweight, void* workspace,
                        size_t workspace_bytes, void* stream);
@@ -288,7 +289,7 @@ int lh_linear_distill_fwd(const void* hidden, const void* weight, const void* te
                           const int64_t* teacher_indices, int N, int V, int D, int K, float temperature, int reduction,
                           float* loss, void* kept, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Gradients of lh_linear_distill_fwd (the teacher has none). */
+/* Gradients of lh_linear_distill_fwd (the teacher has none); NULL as above. */
 int lh_linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float temperature,
                           int reduction, const void* kept, const float* gout, void* dhidden, void* dweight,
                           void* workspace, size_t workspace_bytes, void* stream);

@@ -368,7 +368,7 @@ int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* ta
   g_err[0] = 0;
   int rc = loss_check("linear_xent_bwd", hidden, weight, N, V, D, 0, 1.f, reduction, kept, ws, ws_bytes, 1);
   if (rc) return rc;
-  LH_REQUIRE(target && gout && dhidden && dweight, LH_ERR_ARG, "linear_xent_bwd: null pointer");
+  LH_REQUIRE(target && gout && (dhidden || dweight), LH_ERR_ARG, "linear_xent_bwd: null pointer");
   LH_REQUIRE(!(((uintptr_t)dhidden | (uintptr_t)dweight) & 15), LH_ERR_ARG,
              "linear_xent_bwd: gradients must be 16-byte aligned");
   LH_ARCH();
@@ -397,7 +397,7 @@ int lh_linear_distill_bwd(const void* hidden, const void* weight, int N, int V, 
   int rc = loss_check("linear_distill_bwd", hidden, weight, N, V, D, K, T, reduction, kept, ws, ws_bytes, 1);
   if (rc) return rc;
   LH_REQUIRE(K >= 1, LH_ERR_SHAPE, "linear_distill_bwd: K must be in [1, 256], got %d", K);
-  LH_REQUIRE(gout && dhidden && dweight, LH_ERR_ARG, "linear_distill_bwd: null pointer");
+  LH_REQUIRE(gout && (dhidden || dweight), LH_ERR_ARG, "linear_distill_bwd: null pointer");
   LH_REQUIRE(!(((uintptr_t)dhidden | (uintptr_t)dweight) & 15), LH_ERR_ARG,
              "linear_distill_bwd: gradients must be 16-byte aligned");
   LH_ARCH();

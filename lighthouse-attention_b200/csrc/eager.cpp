@@ -246,19 +246,23 @@ struct LossFn : torch::autograd::Function<LossFn> {
     const int64_t N = h.size(0), D = h.size(1), V = w.size(0), K = ctx->saved_data["K"].toInt();
     const int reduction = (int)ctx->saved_data["reduction"].toInt();
     const Tensor g = grads[0].contiguous();
-    const Tensor dh = empty(h.sizes(), at::kBFloat16, h.device()), dw = empty(w.sizes(), at::kBFloat16, h.device());
+    // a frozen projection, or hidden states that nothing learns from: half of the gradients' products
+    Tensor dh, dw;
+    if (ctx->needs_input_grad(0)) dh = empty(h.sizes(), at::kBFloat16, h.device());
+    if (ctx->needs_input_grad(1)) dw = empty(w.sizes(), at::kBFloat16, h.device());
+    if (!dh.defined() && !dw.defined()) return variable_list(7);
+    void *dhp = dh.defined() ? dh.mutable_data_ptr() : nullptr, *dwp = dw.defined() ? dw.mutable_data_ptr() : nullptr;
     const size_t n = loss_workspace(N, V, D, K, 1);
     const Tensor ws = empty({(int64_t)n}, at::kByte, h.device());
     if (K)
       check(api.distill_bwd(h.const_data_ptr(), w.const_data_ptr(), (int)N, (int)V, (int)D, (int)K,
                             (float)ctx->saved_data["T"].toDouble(), reduction, kept.const_data_ptr(),
-                            (const float*)g.const_data_ptr(), dh.mutable_data_ptr(), dw.mutable_data_ptr(),
-                            ws.mutable_data_ptr(), n, stream(h.device())),
+                            (const float*)g.const_data_ptr(), dhp, dwp, ws.mutable_data_ptr(), n, stream(h.device())),
             "linear_distill_bwd");
     else
       check(api.xent_bwd(h.const_data_ptr(), w.const_data_ptr(), (const int64_t*)target.const_data_ptr(), (int)N, (int)V,
-                         (int)D, reduction, kept.const_data_ptr(), (const float*)g.const_data_ptr(), dh.mutable_data_ptr(),
-                         dw.mutable_data_ptr(), ws.mutable_data_ptr(), n, stream(h.device())),
+                         (int)D, reduction, kept.const_data_ptr(), (const float*)g.const_data_ptr(), dhp, dwp, ws.mutable_data_ptr(),
+                         n, stream(h.device())),
             "linear_xent_bwd");
     return once({dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }

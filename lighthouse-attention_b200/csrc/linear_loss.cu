@@ -17,8 +17,10 @@
 //
 // Rows without a target (ignored positions, rows without a teacher) are left out of
 // all products where those are long enough to pay for it: the rows that count are
-// packed, and the kernels take their number from device memory.  Whatever an
-// ignored row holds, it reaches nothing.
+// packed, and the kernels take their number from device memory.  Elsewhere their rows
+// of G are zeros, and should one of them hold an infinity or a NaN, which a zero does
+// not take out of a product, dW is formed with a copy of hidden that has zeros there.
+// Whatever such a row holds, it reaches nothing.
 //
 // One persistent GEMM kernel does all four products: a pair of SMs
 // (tcgen05.mma.cta_group::2) per 256 x 256 tile, so that each SM loads 128 rows
@@ -106,6 +108,7 @@ struct Args {
   float2* stats;                  // kStats: (2 tiles_n, n_rows) maximum and sum of a row's 128 columns
   float* slog;                    // kStats: logits of the targets (n_rows, K) out
   unsigned* ticket;               // kStats: set to 0 for finish_kernel
+  int* dirty;                     // kStats: set to 0 for finish_kernel; kDW: B is tmP where it is not 0
   const float* gval;              // kGrad: exp(s - lse) - p at the targets (n_rows, K)
   const float* lse2;              // kGrad: log2-sum-exp2 of s a2
   const float *gout, *row_scale, *inv_count;
@@ -217,7 +220,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       }
     }
     if (lane == 0) {
-      if (MODE == kStats && blockIdx.x == 0) *a.ticket = 0;
+      if (MODE == kStats && blockIdx.x == 0) { *a.ticket = 0; *a.dirty = 0; }
       // an earlier launch gave up a wait: do nothing until the host resets
       sm->abort = *reinterpret_cast<volatile int*>(&g_loss_status) ? 2 : 0;
     }
@@ -250,7 +253,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       // ---------------------------------------------------------- TMA producer
       if (lane == 0) {
         const CUtensorMap* mapA = kAMn || MODE == kDH || !sched.packed ? &tmA : &tmP;
-        const CUtensorMap* mapB = MODE == kDW && sched.packed ? &tmP : &tmB;
+        const CUtensorMap* mapB = MODE == kDW && (sched.packed || (a.dirty && *a.dirty)) ? &tmP : &tmB;
         uint32_t it = 0;
         bool ok = true;
         for (int t = pair; t < total && ok; t += n_pairs) {
@@ -776,6 +779,20 @@ pack_kernel(const uint4* hidden, const int* rows, int N, int chunks, uint4* out)
   }
 }
 
+// hidden with zeros in the rows that do not count, where one of those is not finite.
+__global__ void __launch_bounds__(256)
+clean_kernel(const uint4* hidden, const float* row_scale, const int* dirty, int N, int chunks, uint4* out) {
+  after_previous();
+  if (*dirty == 0) return;
+  const int lane = threadIdx.x & 31;
+  for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < N; j += gridDim.x * 8) {
+    const bool yes = row_scale[j] != 0.f;
+    const uint4* h = hidden + (size_t)j * chunks;
+    uint4* o = out + (size_t)j * chunks;
+    for (int c = lane; c < chunks; c += 32) o[c] = yes ? h[c] : make_uint4(0, 0, 0, 0);
+  }
+}
+
 // Joins the (maximum, sum) parts of RB rows per block (thread = row of the block x
 // slot of its parts, slots a power of two), forms the rows' losses and turns the
 // targets' logits into exp(s - lse) - p, what the backward takes off the softmax.
@@ -798,6 +815,8 @@ struct FinishArgs {
   float up;                               // what exponent_scale() adds to log2(e) / T, as a factor
   const __nv_bfloat16 *hidden, *weight;   // the target's logit is summed here in fp32, or NULL
   int D;
+  const uint4* scan;                      // hidden: *dirty is 1 if a row that does not count is not finite
+  int* dirty;                             // NULL where the rows are packed
 };
 
 template <bool SPARSE, int RB>
@@ -908,6 +927,20 @@ finish_kernel(const FinishArgs a) {
   if (live && slot == 0) {
     a.lse2[row] = l2;
     if (a.reduction == LH_REDUCE_NONE) a.loss[row] = loss;
+  }
+  if (a.dirty) {                                   // a warp per row; the rows that count are not read
+    const int lane = tid & 31, chunks = a.D / 8;
+    bool odd = false;
+    for (int w = tid >> 5; w < RB; w += blockDim.x >> 5) {
+      const int jj = blockIdx.x * RB + w;
+      if (jj >= N || (SPARSE ? a.row_scale[jj] != 0.f : a.target[jj] != a.ignore)) continue;
+      for (int c = lane; c < chunks; c += 32) {
+        const uint4 v = a.scan[(size_t)jj * chunks + c];
+        for (uint32_t u : {v.x, v.y, v.z, v.w})
+          odd |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
+      }
+    }
+    if (odd) *a.dirty = 1;
   }
   if (a.reduction == LH_REDUCE_NONE) return;
   auto block_sum = [&](double& s, double& c) {     // to thread 0
@@ -1110,7 +1143,7 @@ struct Plan {
   long long C;                 // columns of a vocabulary piece, a multiple of 256
   int pieces, dh_splits, dw_splits;
   uint8_t split_of[kSplitTable];
-  bool dh_planes;
+  bool dh_planes, pack;
   size_t g, dh, dw, packed, total;     // bytes
 };
 constexpr long long kPieceBytes = 512ll << 20;
@@ -1124,7 +1157,7 @@ static Plan plan(long long N, long long V, long long D) {
   p.C = ((Vp + p.pieces - 1) / p.pieces + kTN - 1) / kTN * kTN;      // pieces of about equal size
   p.pieces = (int)((Vp + p.C - 1) / p.C);
   const long long cols = p.C < V ? p.C : V, tiles = (N + kTM - 1) / kTM;
-  const bool pack = packs(N, V, D);
+  const bool pack = p.pack = packs(N, V, D);
   // dH: the parts by the number of row blocks that are left; at most twice those of all rows
   p.dh_splits = tiles < kSplitTable ? pick_splits(N, D, cols) : 1;
   const int most = pack ? 2 * p.dh_splits : p.dh_splits;
@@ -1139,7 +1172,7 @@ static Plan plan(long long N, long long V, long long D) {
   p.g = up((size_t)N * p.C * 2);
   p.dh = p.dh_planes ? up((size_t)p.dh_splits * N * D * 4) : 0;
   p.dw = p.dw_splits > 1 ? up((size_t)p.dw_splits * p.C * D * 4) : 0;
-  p.packed = pack ? up((size_t)N * D * 2) : 0;
+  p.packed = up((size_t)N * D * 2);       // the packed rows, or clean_kernel's
   p.total = p.g + p.dh + p.dw + p.packed;
   return p;
 }
@@ -1150,7 +1183,7 @@ static long long entries(long long K) { return (K + 3) & ~3ll; }
 // What the forward leaves for the backward.
 struct Kept {
   float *lse2, *row_scale, *inv_count, *tgrad;   // (N), (N), (1), (N, max(K, 1))
-  int *idx, *rows;                               // (N, K) sorted targets, (2 N + 1) packed rows
+  int *idx, *rows, *dirty;                       // (N, K) sorted targets, (2 N + 1) packed rows, (1)
   size_t bytes;
   Kept(void* base, long long N, long long K) {
     char* p = (char*)base;
@@ -1161,6 +1194,7 @@ struct Kept {
     tgrad = (float*)take(4 * N * (K ? entries(K) : 1));
     idx = (int*)take(4 * N * entries(K));
     rows = (int*)take(4 * (2 * N + 1));
+    dirty = (int*)take(4);
     bytes = p - (char*)base;
   }
 };
@@ -1258,6 +1292,7 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
   a.stats = ws.stats;
   a.slog = kp.tgrad;
   a.ticket = ws.ticket;
+  a.dirty = kp.dirty;
   if (few) {
     if ((rc = map_load(&mh, q.hidden, N, D, D, kFew / 2)) || (rc = launch<kStats, SPARSE, true>(mw, mh, mw, mw, a, D, st)))
       return rc;
@@ -1269,7 +1304,8 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
   // 14 us with 32 rows per block, most of it the 2048 blocks' sum).
   const int want = parts > K ? parts : K;
   FinishArgs f{ws.stats, rows, parts, N, V, K, 1, reduction, q.target, q.ignore, kp.idx, ws.prob, ws.ent, kp.tgrad, a.a2,
-               q.T * q.T, kp.row_scale, kp.lse2, loss, kp.inv_count, ws.part, ws.ticket, 1.f, nullptr, nullptr, D};
+               q.T * q.T, kp.row_scale, kp.lse2, loss, kp.inv_count, ws.part, ws.ticket, 1.f, nullptr, nullptr, D,
+               (const uint4*)q.hidden, rows ? nullptr : kp.dirty};
   const int rb = want > 32 ? 8 : want > 4 ? 32 : 256;
   while (f.slots < (rb == 8 ? (want + 3) / 4 : want) && f.slots * rb < 1024) f.slots *= 2;
   if (rb == 8 && f.slots < 32) f.slots = 32;
@@ -1297,7 +1333,8 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
   char* packed = g + p.g + p.dh + p.dw;
   CUtensorMap mh, mw, mp, mdh, mdw, mg, mgo;
   if ((rc = map_load(&mh, q.hidden, N, D, D)) || (rc = map_load(&mw, q.weight, V, D, D))) return rc;
-  if ((rc = p.dh_planes ? map_store(&mdh, dh, true, p.dh_splits, N, D, D) : map_store(&mdh, dhidden, false, 1, N, D, D)))
+  if ((rc = p.dh_planes ? map_store(&mdh, dh, true, p.dh_splits, N, D, D)
+           : dhidden   ? map_store(&mdh, dhidden, false, 1, N, D, D) : LH_OK))
     return rc;
   mp = mh;
   // few rows: always one piece (kFew rows of 2^22 columns take 512 MB)
@@ -1306,10 +1343,15 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
   if (few && ((rc = map_load(&mh_few, q.hidden, N, D, D, kFew / 2)) || (rc = map_load(&mg_few, g, N, V, p.C, kFew / 2))))
     return rc;
   const int* rows = nullptr;
-  if (p.packed) {
+  if (p.pack) {                      // kGrad's operand too
     rows = kp.rows;
-    if ((rc = pack_rows(q.hidden, rows, N, D, packed, st)) || (rc = map_load(&mp, packed, N, D, D))) return rc;
+    rc = pack_rows(q.hidden, rows, N, D, packed, st);
+  } else if (dweight) {
+    const unsigned blocks = (unsigned)((N + 7) / 8);
+    rc = launch_behind("clean_kernel", clean_kernel, blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st, (const uint4*)q.hidden,
+                       kp.row_scale, kp.dirty, N, D / 8, (uint4*)packed);
   }
+  if (rc || (rc = map_load(&mp, packed, N, D, D))) return rc;
   for (int i = 0; i < p.pieces; ++i) {
     const long long v0 = i * p.C;
     const int cols = (int)(V - v0 < p.C ? V - v0 : p.C);
@@ -1338,20 +1380,23 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
                   : launch<kGrad, SPARSE>(mh, mw, mgo, mp, a, D, st)))
       return rc;
 
-    Args x{};
-    x.n_rows = N;
-    x.M = few ? D : N;
-    x.N = few ? N : D;
-    x.few_out = p.dh_planes ? (void*)dh : dhidden;
-    const int kb = (cols + kTK - 1) / kTK;
-    x.splits = p.dh_splits < kb ? p.dh_splits : kb;      // a short last piece may leave planes as they are
-    for (int t = 0; t < kSplitTable; ++t) x.split_of[t] = p.split_of[t];
-    x.rows = rows;
-    x.b_off = (int)v0;
-    x.out = !p.dh_planes ? kOutBf16 : i ? kOutPlaneAdd : kOutPlane;
-    if ((rc = few ? launch<kDH, false, true>(mw, mg_few, mw, mw, x, cols, st)
-                  : launch<kDH, false>(mg, mw, mdh, mg, x, cols, st)))
-      return rc;
+    if (dhidden) {
+      Args x{};
+      x.n_rows = N;
+      x.M = few ? D : N;
+      x.N = few ? N : D;
+      x.few_out = p.dh_planes ? (void*)dh : dhidden;
+      const int kb = (cols + kTK - 1) / kTK;
+      x.splits = p.dh_splits < kb ? p.dh_splits : kb;      // a short last piece may leave planes as they are
+      for (int t = 0; t < kSplitTable; ++t) x.split_of[t] = p.split_of[t];
+      x.rows = rows;
+      x.b_off = (int)v0;
+      x.out = !p.dh_planes ? kOutBf16 : i ? kOutPlaneAdd : kOutPlane;
+      if ((rc = few ? launch<kDH, false, true>(mw, mg_few, mw, mw, x, cols, st)
+                    : launch<kDH, false>(mg, mw, mdh, mg, x, cols, st)))
+        return rc;
+    }
+    if (!dweight) continue;
 
     Args y{};
     y.M = cols;
@@ -1359,6 +1404,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     y.N = D;
     y.splits = p.dw_splits;
     y.rows = rows;
+    y.dirty = rows ? nullptr : kp.dirty;
     y.out = p.dw_splits > 1 ? kOutPlane : kOutBf16;
     char* dw_out = (char*)dweight + (size_t)v0 * D * 2;
     if ((rc = p.dw_splits > 1 ? map_store(&mdw, dw, true, p.dw_splits, cols, D, D)
@@ -1367,7 +1413,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     if ((rc = launch<kDW, false>(mg, mh, mdw, mp, y, N, st))) return rc;
     if (p.dw_splits > 1 && (rc = sum_planes(dw, nullptr, p.dw_splits, cols, D, nullptr, dw_out, st))) return rc;
   }
-  return p.dh_planes ? sum_planes(dh, &p, p.dh_splits, N, D, rows, dhidden, st) : LH_OK;
+  return dhidden && p.dh_planes ? sum_planes(dh, &p, p.dh_splits, N, D, rows, dhidden, st) : LH_OK;
 }
 
 }  // namespace ll

@@ -175,6 +175,56 @@ def test_ignored_positions_may_hold_anything(lh, cuda):
     assert (b[1][3] == 0).all() and (b[1][17] == 0).all()
 
 
+@pytest.mark.parametrize("N,V,D", [(40, 300, 64), (64, 20000, 128), (300, 1000, 72), (700, 90, 264), (20000, 256, 64)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_what_an_ignored_position_holds_reaches_no_gradient(lh, cuda, N, V, D, reduction):
+    """NaN and infinities in ignored rows against zeros there: the same loss, dhidden and dweight."""
+    g, h, w = _problem(N, V, D, 50, cuda)
+    target = torch.randint(0, V, (N,), generator=g)
+    target[torch.rand(N, generator=g) < 0.3] = -100
+    target[-1] = -100
+    off = (target == -100).to(cuda)
+    target = target.to(cuda)
+    dloss = torch.randn(N, generator=g).to(cuda) if reduction == "none" else None
+    zeros, odd = torch.where(off[:, None], 0, h), h.clone()
+    a = _xent(lh, zeros, w, target, reduction, dloss)
+    for x, at in ((float("nan"), slice(None)), (float("inf"), slice(D - 1, D)), (-float("inf"), slice(0, 1))):
+        odd[:, at] = torch.where(off[:, None], x, h[:, at])
+        b = _xent(lh, odd, w, target, reduction, dloss)
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+        odd = h.clone()
+    # one row alone
+    odd[-1] = float("nan")
+    assert all(torch.equal(p, q) for p, q in zip(a, _xent(lh, odd, w, target, reduction, dloss)))
+    tv = torch.randn(N, 5, generator=g).to(cuda)
+    ti = torch.randint(0, V, (N, 5), generator=g).to(cuda)
+    ti[off] = -1
+    res = []
+    for x in (zeros, torch.where(off[:, None], float("nan"), h)):
+        ls = [t.detach().requires_grad_(True) for t in (x, w)]
+        loss = lh.linear_distillation(*ls, tv, ti, reduction=reduction)
+        res.append((loss.detach(), *torch.autograd.grad(loss, ls, dloss)))
+    assert all(torch.equal(p, q) for p, q in zip(*res)) and res[0][2].isfinite().all()
+
+
+@pytest.mark.parametrize("N,V,D", [(16, 20000, 128), (300, 1000, 72), (2000, 24000, 640)])
+def test_one_gradient_of_two(lh, cuda, N, V, D):
+    """A frozen projection, or hidden states that need no gradient: the other one is the same."""
+    g, h, w = _problem(N, V, D, 51, cuda)
+    target = torch.randint(0, V, (N,), generator=g).to(cuda)
+    tv, ti = torch.randn(N, 3, generator=g).to(cuda), torch.randint(0, V, (N, 3), generator=g).to(cuda)
+    for f in (lambda a, b: lh.linear_cross_entropy(a, b, target), lambda a, b: lh.linear_distillation(a, b, tv, ti)):
+        leaf = lambda t: t.detach().requires_grad_(True)
+        a, b = leaf(h), leaf(w)
+        both = torch.autograd.grad(f(a, b), (a, b))
+        a = leaf(h)
+        assert torch.equal(torch.autograd.grad(f(a, w), a)[0], both[0])
+        b = leaf(w)
+        assert torch.equal(torch.autograd.grad(f(h, b), b)[0], both[1])
+        a, b = leaf(h), leaf(w)
+        assert torch.equal(torch.autograd.grad(f(a, b), b)[0], both[1]), "the graph has both, the call asks for one"
+
+
 def test_another_ignore_index_and_bad_targets(lh, cuda):
     g, h, w = _problem(20, 300, 64, 3, cuda)
     target = torch.randint(0, 300, (20,), generator=g).to(cuda)

@@ -80,6 +80,9 @@ def test_c_entry_points_check_before_they_touch_a_device(lh):
         return lib.lh_linear_distill_bwd(a, a, 4, 10, 64, K, 1.0, 1, kept, a, a, a, a, big, None)
 
     assert db(kept=None) == 2 and db(K=0) == 1
+    # one of the gradients may be left out, not both
+    assert lib.lh_linear_xent_bwd(a, a, a, 4, 10, 64, 1, a, a, None, None, a, big, None) == 2
+    assert lib.lh_linear_distill_bwd(a, a, 4, 10, 64, 3, 1.0, 1, a, a, None, None, a, big, None) == 2
 
 
 def test_workspace_stays_small(lh):
