@@ -257,8 +257,12 @@ int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h,
  * 256 columns). */
 size_t lh_linear_loss_workspace_size(int N, int V, int D, int K, int backward);
 
-/* Bytes of `kept`, which the forward fills for the backward of the same problem. */
-size_t lh_linear_loss_kept_size(int N, int K);
+/* Bytes of `kept`, which the forward fills for the backward of the same problem.
+ * gradients = 1: with the logits' gradients but for the loss's own one, 512 N bytes
+ * that spare the backward one of its products.  Only where V <= 256, N > 64 and the
+ * loss is reduced; elsewhere the two sizes are the same.  The forward and the
+ * backward get the same kept_bytes, one of the two sizes, and use what is there. */
+size_t lh_linear_loss_kept_size(int N, int V, int K, int reduction, int gradients);
 
 /* Softmax cross entropy: loss_i = log sum_v exp(s_iv) - s_i,target(i).
  *   target     (N) int64; a row with target ignore_index has loss 0 and no
@@ -266,16 +270,16 @@ size_t lh_linear_loss_kept_size(int N, int K);
  *   reduction  LH_REDUCE_NONE: loss (N) fp32; MEAN over the rows that are not
  *              ignored (0 where all are) or SUM: loss (1) */
 int lh_linear_xent_fwd(const void* hidden, const void* weight, const int64_t* target, int64_t ignore_index, int N, int V,
-                       int D, int reduction, float* loss, void* kept, void* workspace, size_t workspace_bytes,
-                       void* stream);
+                       int D, int reduction, float* loss, void* kept, size_t kept_bytes, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* Gradients of lh_linear_xent_fwd.
  *   gout    fp32 upstream gradient of loss: (N) with LH_REDUCE_NONE, else (1)
  *   dhidden (N, D), dweight (V, D) bf16 out; one of them may be NULL, and its
  *             product is left out then */
 int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* target, int N, int V, int D, int reduction,
-                       const void* kept, const float* gout, void* dhidden, void* dweight, void* workspace,
-                       size_t workspace_bytes, void* stream);
+                       const void* kept, size_t kept_bytes, const float* gout, void* dhidden, void* dweight,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 /* Distillation from a teacher's K top logits per row:
  *   p = softmax(teacher_logits / T) over the row's entries,
@@ -287,12 +291,13 @@ int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* ta
  *   with the same index add up. */
 int lh_linear_distill_fwd(const void* hidden, const void* weight, const void* teacher_logits, int t_dtype,
                           const int64_t* teacher_indices, int N, int V, int D, int K, float temperature, int reduction,
-                          float* loss, void* kept, void* workspace, size_t workspace_bytes, void* stream);
+                          float* loss, void* kept, size_t kept_bytes, void* workspace, size_t workspace_bytes,
+                          void* stream);
 
 /* Gradients of lh_linear_distill_fwd (the teacher has none); NULL as above. */
 int lh_linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float temperature,
-                          int reduction, const void* kept, const float* gout, void* dhidden, void* dweight,
-                          void* workspace, size_t workspace_bytes, void* stream);
+                          int reduction, const void* kept, size_t kept_bytes, const float* gout, void* dhidden,
+                          void* dweight, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

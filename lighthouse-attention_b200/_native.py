@@ -59,14 +59,16 @@ _SIGS = {
                                        ctypes.c_longlong, ctypes.c_int, _VP, ctypes.c_int] + [_VP] * 3
                         + [ctypes.c_size_t, _VP]),
     "lh_linear_loss_workspace_size": (ctypes.c_size_t, [ctypes.c_int] * 5),
-    "lh_linear_loss_kept_size": (ctypes.c_size_t, [ctypes.c_int] * 2),
-    "lh_linear_xent_fwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int64] + [ctypes.c_int] * 4 + [_VP] * 3
+    "lh_linear_loss_kept_size": (ctypes.c_size_t, [ctypes.c_int] * 5),
+    "lh_linear_xent_fwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int64] + [ctypes.c_int] * 4
+                           + [_VP, _VP, ctypes.c_size_t] + [_VP, ctypes.c_size_t, _VP]),
+    "lh_linear_xent_bwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int] * 4 + [_VP, ctypes.c_size_t] + [_VP] * 4
                            + [ctypes.c_size_t, _VP]),
-    "lh_linear_xent_bwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int] * 4 + [_VP] * 5 + [ctypes.c_size_t, _VP]),
     "lh_linear_distill_fwd": (ctypes.c_int, [_VP] * 3 + [ctypes.c_int, _VP] + [ctypes.c_int] * 4
-                              + [ctypes.c_float, ctypes.c_int] + [_VP] * 3 + [ctypes.c_size_t, _VP]),
+                              + [ctypes.c_float, ctypes.c_int] + [_VP, _VP, ctypes.c_size_t]
+                              + [_VP, ctypes.c_size_t, _VP]),
     "lh_linear_distill_bwd": (ctypes.c_int, [_VP] * 2 + [ctypes.c_int] * 4 + [ctypes.c_float, ctypes.c_int]
-                              + [_VP] * 5 + [ctypes.c_size_t, _VP]),
+                              + [_VP, ctypes.c_size_t] + [_VP] * 4 + [ctypes.c_size_t, _VP]),
 }
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -481,9 +483,9 @@ def _loss_ws(N, V, D, K, backward, dev):
     return torch.empty(n, dtype=torch.uint8, device=dev), n
 
 
-def kept_size(N: int, K: int) -> int:
+def kept_size(N: int, V: int, K: int, reduction: str) -> int:
     """Bytes that a loss's forward keeps for its backward."""
-    return load().lh_linear_loss_kept_size(N, K)
+    return load().lh_linear_loss_kept_size(N, V, K, REDUCTIONS[reduction], 1)
 
 
 def linear_xent_fwd(hidden, weight, target, ignore_index: int, reduction: str):
@@ -494,12 +496,12 @@ def linear_xent_fwd(hidden, weight, target, ignore_index: int, reduction: str):
         raise LighthouseShapeError("linear_xent: target must be (N) int64")
     dev = _on_one_device("linear_xent", hidden, weight, target)
     loss = _loss_out(N, reduction, dev)
-    kept = torch.empty(kept_size(N, 0), dtype=torch.uint8, device=dev)
+    kept = torch.empty(kept_size(N, V, 0, reduction), dtype=torch.uint8, device=dev)
     if N:
         hidden, weight, target = _dense16(hidden), _dense16(weight), target.contiguous()
         ws, n = _loss_ws(N, V, D, 0, 0, dev)
         _call(dev, "lh_linear_xent_fwd", hidden.data_ptr(), weight.data_ptr(), target.data_ptr(), ignore_index, N, V, D,
-              REDUCTIONS[reduction], loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
+              REDUCTIONS[reduction], loss.data_ptr(), kept.data_ptr(), kept.numel(), ws.data_ptr(), n)
     return loss, kept
 
 
@@ -507,7 +509,7 @@ def _loss_bwd_check(what, hidden, weight, kept, gout, reduction, K, *rest):
     N, V, D = _loss_check(what, hidden, weight, reduction)
     if gout.dtype != torch.float32 or gout.numel() != (N if reduction == "none" else 1):
         raise LighthouseShapeError(f"{what}: the loss's gradient must be fp32, one value (reduced) or N")
-    if kept.dtype != torch.uint8 or kept.shape != (kept_size(N, K),) or not kept.is_contiguous():
+    if kept.dtype != torch.uint8 or kept.shape != (kept_size(N, V, K, reduction),) or not kept.is_contiguous():
         raise LighthouseShapeError(f"{what}: kept must be the forward's")
     return N, _on_one_device(what, hidden, weight, kept, gout, *rest)
 
@@ -524,8 +526,8 @@ def linear_xent_bwd(hidden, weight, target, kept, gout, reduction: str):
     hidden, weight = _dense16(hidden), _dense16(weight)
     ws, n = _loss_ws(N, V, D, 0, 1, dev)
     _call(dev, "lh_linear_xent_bwd", hidden.data_ptr(), weight.data_ptr(), target.contiguous().data_ptr(), N, V, D,
-          REDUCTIONS[reduction], kept.data_ptr(), gout.contiguous().data_ptr(), dh.data_ptr(), dw.data_ptr(), ws.data_ptr(),
-          n)
+          REDUCTIONS[reduction], kept.data_ptr(), kept.numel(), gout.contiguous().data_ptr(), dh.data_ptr(), dw.data_ptr(),
+          ws.data_ptr(), n)
     return dh, dw
 
 
@@ -544,14 +546,14 @@ def linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperat
         raise ValueError(f"linear_distill: temperature must be positive and finite, got {temperature}")
     dev = _on_one_device("linear_distill", hidden, weight, teacher_logits, teacher_indices)
     loss = _loss_out(N, reduction, dev)
-    kept = torch.empty(kept_size(N, K), dtype=torch.uint8, device=dev)
+    kept = torch.empty(kept_size(N, V, K, reduction), dtype=torch.uint8, device=dev)
     if N:
         hidden, weight = _dense16(hidden), _dense16(weight)
         teacher_logits, teacher_indices = teacher_logits.contiguous(), teacher_indices.contiguous()
         ws, n = _loss_ws(N, V, D, K, 0, dev)
         _call(dev, "lh_linear_distill_fwd", hidden.data_ptr(), weight.data_ptr(), teacher_logits.data_ptr(),
               LH_DTYPE[teacher_logits.dtype], teacher_indices.data_ptr(), N, V, D, K, temperature, REDUCTIONS[reduction],
-              loss.data_ptr(), kept.data_ptr(), ws.data_ptr(), n)
+              loss.data_ptr(), kept.data_ptr(), kept.numel(), ws.data_ptr(), n)
     return loss, kept
 
 
@@ -565,6 +567,6 @@ def linear_distill_bwd(hidden, weight, kept, gout, K: int, temperature: float, r
     hidden, weight = _dense16(hidden), _dense16(weight)
     ws, n = _loss_ws(N, V, D, K, 1, dev)
     _call(dev, "lh_linear_distill_bwd", hidden.data_ptr(), weight.data_ptr(), N, V, D, K, temperature,
-          REDUCTIONS[reduction], kept.data_ptr(), gout.contiguous().data_ptr(), dh.data_ptr(), dw.data_ptr(), ws.data_ptr(),
-          n)
+          REDUCTIONS[reduction], kept.data_ptr(), kept.numel(), gout.contiguous().data_ptr(), dh.data_ptr(), dw.data_ptr(),
+          ws.data_ptr(), n)
     return dh, dw

@@ -79,15 +79,15 @@ int rms_norm_bwd(const void*, int, const void*, const void*, int, const void*, i
                  int, void*, void*, void*, cudaStream_t);
 
 size_t linear_loss_workspace_size(int, int, int, int, int);
-size_t linear_loss_kept_size(int, int);
-int linear_xent_fwd(const void*, const void*, const long long*, long long, int, int, int, int, float*, void*, void*,
-                    cudaStream_t);
-int linear_xent_bwd(const void*, const void*, const long long*, int, int, int, int, const void*, const float*, void*, void*,
+size_t linear_loss_kept_size(int, int, int, int, int);
+int linear_xent_fwd(const void*, const void*, const long long*, long long, int, int, int, int, float*, void*, bool,
                     void*, cudaStream_t);
+int linear_xent_bwd(const void*, const void*, const long long*, int, int, int, int, const void*, bool, const float*, void*,
+                    void*, void*, cudaStream_t);
 int linear_distill_fwd(const void*, const void*, const void*, int, const long long*, int, int, int, int, float, int, float*,
+                       void*, bool, void*, cudaStream_t);
+int linear_distill_bwd(const void*, const void*, int, int, int, int, float, int, const void*, bool, const float*, void*,
                        void*, void*, cudaStream_t);
-int linear_distill_bwd(const void*, const void*, int, int, int, int, float, int, const void*, const float*, void*, void*,
-                       void*, cudaStream_t);
 int loss_status(int reset);
 
 }  // namespace lh
@@ -329,7 +329,8 @@ int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h,
 }
 
 static int loss_check(const char* what, const void* hidden, const void* weight, int N, int V, int D, int K, float T,
-                      int reduction, const void* kept, const void* ws, size_t ws_bytes, int backward) {
+                      int reduction, const void* kept, size_t kept_bytes, const void* ws, size_t ws_bytes, int backward,
+                      bool* gradients) {
   LH_REQUIRE(hidden && weight && kept && ws, LH_ERR_ARG, "%s: null pointer", what);
   LH_REQUIRE(N > 0 && V > 0 && D > 0 && N <= (1 << 22) && V <= (1 << 22), LH_ERR_SHAPE,
              "%s: N and V must be in [1, 2^22]", what);
@@ -342,6 +343,10 @@ static int loss_check(const char* what, const void* hidden, const void* weight, 
   const size_t need = linear_loss_workspace_size(N, V, D, K, backward);
   LH_REQUIRE(ws_bytes >= need, LH_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the %zu needed", what,
              ws_bytes, need);
+  const size_t least = linear_loss_kept_size(N, V, K, reduction, 0);
+  LH_REQUIRE(kept_bytes >= least, LH_ERR_WORKSPACE, "%s: kept of %zu bytes is smaller than the %zu needed", what, kept_bytes,
+             least);
+  *gradients = kept_bytes >= linear_loss_kept_size(N, V, K, reduction, 1);
   return LH_OK;
 }
 
@@ -349,59 +354,71 @@ size_t lh_linear_loss_workspace_size(int N, int V, int D, int K, int backward) {
   return N > 0 && V > 0 && D > 0 && K >= 0 ? linear_loss_workspace_size(N, V, D, K, backward) : 0;
 }
 
-size_t lh_linear_loss_kept_size(int N, int K) { return N > 0 && K >= 0 ? linear_loss_kept_size(N, K) : 0; }
+size_t lh_linear_loss_kept_size(int N, int V, int K, int reduction, int gradients) {
+  return N > 0 && V > 0 && K >= 0 ? linear_loss_kept_size(N, V, K, reduction, gradients) : 0;
+}
 
 int lh_linear_xent_fwd(const void* hidden, const void* weight, const int64_t* target, int64_t ignore_index, int N, int V,
-                       int D, int reduction, float* loss, void* kept, void* ws, size_t ws_bytes, void* stream) {
+                       int D, int reduction, float* loss, void* kept, size_t kept_bytes, void* ws, size_t ws_bytes,
+                       void* stream) {
   g_err[0] = 0;
-  int rc = loss_check("linear_xent", hidden, weight, N, V, D, 0, 1.f, reduction, kept, ws, ws_bytes, 0);
+  bool gradients;
+  int rc = loss_check("linear_xent", hidden, weight, N, V, D, 0, 1.f, reduction, kept, kept_bytes, ws, ws_bytes, 0,
+                      &gradients);
   if (rc) return rc;
   LH_REQUIRE(target && loss, LH_ERR_ARG, "linear_xent: null pointer");
   LH_ARCH();
-  return linear_xent_fwd(hidden, weight, (const long long*)target, ignore_index, N, V, D, reduction, loss, kept, ws,
-                         S_(stream));
+  return linear_xent_fwd(hidden, weight, (const long long*)target, ignore_index, N, V, D, reduction, loss, kept,
+                         gradients, ws, S_(stream));
 }
 
 int lh_linear_xent_bwd(const void* hidden, const void* weight, const int64_t* target, int N, int V, int D, int reduction,
-                       const void* kept, const float* gout, void* dhidden, void* dweight, void* ws, size_t ws_bytes,
-                       void* stream) {
+                       const void* kept, size_t kept_bytes, const float* gout, void* dhidden, void* dweight, void* ws,
+                       size_t ws_bytes, void* stream) {
   g_err[0] = 0;
-  int rc = loss_check("linear_xent_bwd", hidden, weight, N, V, D, 0, 1.f, reduction, kept, ws, ws_bytes, 1);
+  bool gradients;
+  int rc = loss_check("linear_xent_bwd", hidden, weight, N, V, D, 0, 1.f, reduction, kept, kept_bytes, ws, ws_bytes, 1,
+                      &gradients);
   if (rc) return rc;
   LH_REQUIRE(target && gout && (dhidden || dweight), LH_ERR_ARG, "linear_xent_bwd: null pointer");
   LH_REQUIRE(!(((uintptr_t)dhidden | (uintptr_t)dweight) & 15), LH_ERR_ARG,
              "linear_xent_bwd: gradients must be 16-byte aligned");
   LH_ARCH();
-  return linear_xent_bwd(hidden, weight, (const long long*)target, N, V, D, reduction, kept, gout, dhidden, dweight, ws,
-                         S_(stream));
+  return linear_xent_bwd(hidden, weight, (const long long*)target, N, V, D, reduction, kept, gradients, gout, dhidden,
+                         dweight, ws, S_(stream));
 }
 
 int lh_linear_distill_fwd(const void* hidden, const void* weight, const void* tv, int t_dtype, const int64_t* ti, int N,
-                          int V, int D, int K, float T, int reduction, float* loss, void* kept, void* ws, size_t ws_bytes,
-                          void* stream) {
+                          int V, int D, int K, float T, int reduction, float* loss, void* kept, size_t kept_bytes,
+                          void* ws, size_t ws_bytes, void* stream) {
   g_err[0] = 0;
-  int rc = loss_check("linear_distill", hidden, weight, N, V, D, K, T, reduction, kept, ws, ws_bytes, 0);
+  bool gradients;
+  int rc = loss_check("linear_distill", hidden, weight, N, V, D, K, T, reduction, kept, kept_bytes, ws, ws_bytes, 0,
+                      &gradients);
   if (rc) return rc;
   LH_REQUIRE(K >= 1, LH_ERR_SHAPE, "linear_distill: K must be in [1, 256], got %d", K);
   LH_REQUIRE(float_dtype(t_dtype), LH_ERR_ARG, "linear_distill: bad dtype");
   LH_REQUIRE(tv && ti && loss, LH_ERR_ARG, "linear_distill: null pointer");
   LH_ARCH();
-  return linear_distill_fwd(hidden, weight, tv, t_dtype, (const long long*)ti, N, V, D, K, T, reduction, loss, kept, ws,
-                            S_(stream));
+  return linear_distill_fwd(hidden, weight, tv, t_dtype, (const long long*)ti, N, V, D, K, T, reduction, loss, kept,
+                         gradients, ws, S_(stream));
 }
 
 int lh_linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float T, int reduction,
-                          const void* kept, const float* gout, void* dhidden, void* dweight, void* ws, size_t ws_bytes,
-                          void* stream) {
+                          const void* kept, size_t kept_bytes, const float* gout, void* dhidden, void* dweight, void* ws,
+                          size_t ws_bytes, void* stream) {
   g_err[0] = 0;
-  int rc = loss_check("linear_distill_bwd", hidden, weight, N, V, D, K, T, reduction, kept, ws, ws_bytes, 1);
+  bool gradients;
+  int rc = loss_check("linear_distill_bwd", hidden, weight, N, V, D, K, T, reduction, kept, kept_bytes, ws, ws_bytes, 1,
+                      &gradients);
   if (rc) return rc;
   LH_REQUIRE(K >= 1, LH_ERR_SHAPE, "linear_distill_bwd: K must be in [1, 256], got %d", K);
   LH_REQUIRE(gout && (dhidden || dweight), LH_ERR_ARG, "linear_distill_bwd: null pointer");
   LH_REQUIRE(!(((uintptr_t)dhidden | (uintptr_t)dweight) & 15), LH_ERR_ARG,
              "linear_distill_bwd: gradients must be 16-byte aligned");
   LH_ARCH();
-  return linear_distill_bwd(hidden, weight, N, V, D, K, T, reduction, kept, gout, dhidden, dweight, ws, S_(stream));
+  return linear_distill_bwd(hidden, weight, N, V, D, K, T, reduction, kept, gradients, gout, dhidden, dweight, ws,
+                            S_(stream));
 }
 
 }  // extern "C"

@@ -214,24 +214,25 @@ size_t loss_workspace(int64_t N, int64_t V, int64_t D, int64_t K, int back) {
 struct LossFn : torch::autograd::Function<LossFn> {
   // target (N) and K = 0, or teacher logits and indices (N, K)
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& target,
-                        const std::optional<Tensor>& teacher, double temperature, int64_t ignore, int64_t reduction) {
+                        const std::optional<Tensor>& teacher, double temperature, int64_t ignore, int64_t reduction,
+                        bool gradients) {
     const Tensor tl = teacher.value_or(Tensor());
     const c10::cuda::CUDAGuard guard(h.device());
     const int64_t N = h.size(0), D = h.size(1), V = w.size(0), K = tl.defined() ? tl.size(1) : 0;
     const Tensor loss = reduction == LH_REDUCE_NONE ? empty({N}, at::kFloat, h.device()) : empty({}, at::kFloat, h.device());
-    const Tensor kept = empty({(int64_t)api.loss_kept((int)N, (int)K)}, at::kByte, h.device());
+    const Tensor kept = empty({(int64_t)api.loss_kept((int)N, (int)V, (int)K, (int)reduction, gradients)}, at::kByte, h.device());
     const size_t n = loss_workspace(N, V, D, K, 0);
     const Tensor ws = empty({(int64_t)n}, at::kByte, h.device());
     if (K)
       check(api.distill_fwd(h.const_data_ptr(), w.const_data_ptr(), tl.const_data_ptr(), dtype_code(tl.scalar_type()),
                             (const int64_t*)target.const_data_ptr(), (int)N, (int)V, (int)D, (int)K, (float)temperature,
-                            (int)reduction, (float*)loss.mutable_data_ptr(), kept.mutable_data_ptr(), ws.mutable_data_ptr(),
-                            n, stream(h.device())),
+                            (int)reduction, (float*)loss.mutable_data_ptr(), kept.mutable_data_ptr(),
+                            (size_t)kept.numel(), ws.mutable_data_ptr(), n, stream(h.device())),
             "linear_distill");
     else
       check(api.xent_fwd(h.const_data_ptr(), w.const_data_ptr(), (const int64_t*)target.const_data_ptr(), ignore, (int)N,
                          (int)V, (int)D, (int)reduction, (float*)loss.mutable_data_ptr(), kept.mutable_data_ptr(),
-                         ws.mutable_data_ptr(), n, stream(h.device())),
+                         (size_t)kept.numel(), ws.mutable_data_ptr(), n, stream(h.device())),
             "linear_xent");
     ctx->save_for_backward({h, w, K ? Tensor() : target, kept});
     ctx->saved_data["K"] = K;
@@ -250,27 +251,30 @@ struct LossFn : torch::autograd::Function<LossFn> {
     Tensor dh, dw;
     if (ctx->needs_input_grad(0)) dh = empty(h.sizes(), at::kBFloat16, h.device());
     if (ctx->needs_input_grad(1)) dw = empty(w.sizes(), at::kBFloat16, h.device());
-    if (!dh.defined() && !dw.defined()) return variable_list(7);
+    if (!dh.defined() && !dw.defined()) return variable_list(8);
     void *dhp = dh.defined() ? dh.mutable_data_ptr() : nullptr, *dwp = dw.defined() ? dw.mutable_data_ptr() : nullptr;
     const size_t n = loss_workspace(N, V, D, K, 1);
     const Tensor ws = empty({(int64_t)n}, at::kByte, h.device());
     if (K)
       check(api.distill_bwd(h.const_data_ptr(), w.const_data_ptr(), (int)N, (int)V, (int)D, (int)K,
                             (float)ctx->saved_data["T"].toDouble(), reduction, kept.const_data_ptr(),
-                            (const float*)g.const_data_ptr(), dhp, dwp, ws.mutable_data_ptr(), n, stream(h.device())),
+                            (size_t)kept.numel(), (const float*)g.const_data_ptr(), dhp, dwp, ws.mutable_data_ptr(), n, stream(h.device())),
             "linear_distill_bwd");
     else
       check(api.xent_bwd(h.const_data_ptr(), w.const_data_ptr(), (const int64_t*)target.const_data_ptr(), (int)N, (int)V,
-                         (int)D, reduction, kept.const_data_ptr(), (const float*)g.const_data_ptr(), dhp, dwp, ws.mutable_data_ptr(),
+                         (int)D, reduction, kept.const_data_ptr(), (size_t)kept.numel(), (const float*)g.const_data_ptr(), dhp, dwp, ws.mutable_data_ptr(),
                          n, stream(h.device())),
             "linear_xent_bwd");
-    return once({dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+    return once({dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
+bool wants_grad(const Tensor& h, const Tensor& w) {
+  return at::GradMode::is_enabled() && (wants_grad(h) || wants_grad(w));
+}
 py::object linear_xent(const Tensor& h, const Tensor& w, const Tensor& target, int64_t ignore, int64_t reduction) {
   if (!loss_case(h, w, reduction) || !rows_case(target, h, 1) || target.scalar_type() != at::kLong) return py::none();
-  return py::cast(LossFn::apply(h, w, target, std::optional<Tensor>(), 1.0, ignore, reduction));
+  return py::cast(LossFn::apply(h, w, target, std::optional<Tensor>(), 1.0, ignore, reduction, wants_grad(h, w)));
 }
 py::object linear_distill(const Tensor& h, const Tensor& w, const Tensor& tl, const Tensor& ti, double temperature,
                           int64_t reduction) {
@@ -278,7 +282,7 @@ py::object linear_distill(const Tensor& h, const Tensor& w, const Tensor& tl, co
       dtype_code(tl.scalar_type()) < 0 || tl.size(1) != ti.size(1) || tl.size(1) < 1 || tl.size(1) > 256 ||
       !(temperature > 0 && temperature < 1e30))
     return py::none();
-  return py::cast(LossFn::apply(h, w, ti, std::optional<Tensor>(tl.detach()), temperature, 0, reduction));
+  return py::cast(LossFn::apply(h, w, ti, std::optional<Tensor>(tl.detach()), temperature, 0, reduction, wants_grad(h, w)));
 }
 
 }  // namespace

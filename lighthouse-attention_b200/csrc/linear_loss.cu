@@ -15,6 +15,11 @@
 // G is rounded to bf16 once, as an operand of bf16 MMAs has to be; its relative
 // error of 2^-9 is that of the bf16 gradients it ends in.  All sums are fp32.
 //
+// Where a row's vocabulary is one tile (V <= 256) and the loss is reduced, the forward
+// knows a row's lse when its tile ends, and writes G / c there: the backward has one
+// product and a reading of hidden less, and c, the same for all rows, is multiplied
+// into dH and dW.
+//
 // Rows without a target (ignored positions, rows without a teacher) are left out of
 // all products where those are long enough to pay for it: the rows that count are
 // packed, and the kernels take their number from device memory.  Elsewhere their rows
@@ -56,7 +61,7 @@ constexpr int kPairs = 74;
 constexpr int kNone = 0x7fffffff;
 constexpr float kLn2 = 0.69314718055994531f;
 
-enum Mode { kStats, kGrad, kDH, kDW };
+enum Mode { kStats, kWhole, kGrad, kDH, kDW };      // kWhole: kStats and kGrad of rows of one tile
 enum Out { kOutBf16, kOutPlane, kOutPlaneAdd };
 
 // With few rows (kFew at most) the roles turn: the 256 rows of a tile are weights (or
@@ -107,11 +112,13 @@ struct Args {
   float a2;                       // exponent_scale()
   float2* stats;                  // kStats: (2 tiles_n, n_rows) maximum and sum of a row's 128 columns
   float* slog;                    // kStats: logits of the targets (n_rows, K) out
-  unsigned* ticket;               // kStats: set to 0 for finish_kernel
-  int* dirty;                     // kStats: set to 0 for finish_kernel; kDW: B is tmP where it is not 0
+  unsigned* ticket;               // forward: set to 0 for finish_kernel
+  int* dirty;                     // forward: set to 0 for finish_kernel; kDW: B is tmP where it is not 0
   const float* gval;              // kGrad: exp(s - lse) - p at the targets (n_rows, K)
+  const float* prob;              // kWhole: p at the targets (n_rows, K), not read where SPARSE is false
+  long long ignore;               // kWhole, SPARSE false
   const float* lse2;              // kGrad: log2-sum-exp2 of s a2
-  const float *gout, *row_scale, *inv_count;
+  const float *gout, *row_scale, *inv_count;       // kDH, kDW: gout is NULL, or G wants c
   int gstride;
   float cscale;
   void* few_out;                  // few rows: G (bf16, few_pitch), or the planes (fp32) or dH (bf16) of kDH
@@ -151,6 +158,19 @@ struct Window {
     else behind = V4{none, none, none, none};
   }
 };
+
+// Barriers of the two warps that hold the halves of a row block's columns.
+__device__ __forceinline__ void pair_sync(int id) {
+  __syncwarp();
+  asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
+}
+__device__ __forceinline__ bool pair_all(int id, bool v) {
+  uint32_t r;
+  __syncwarp();
+  asm volatile("{.reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.and.pred q, %2, 64, p; selp.u32 %0, 1, 0, q;}"
+               : "=r"(r) : "r"((uint32_t)v), "r"(id) : "memory");
+  return r;
+}
 
 // 32 values per lane, one per column -> in lane e the result of column e over the warp.
 template <class Op>
@@ -220,7 +240,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       }
     }
     if (lane == 0) {
-      if (MODE == kStats && blockIdx.x == 0) { *a.ticket = 0; *a.dirty = 0; }
+      if ((MODE == kStats || MODE == kWhole) && blockIdx.x == 0) { *a.ticket = 0; *a.dirty = 0; }
       // an earlier launch gave up a wait: do nothing until the host resets
       sm->abort = *reinterpret_cast<volatile int*>(&g_loss_status) ? 2 : 0;
     }
@@ -446,6 +466,10 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       uint8_t* stage = sO + (quad + 4 * half) * kOutBuf;
       const uint32_t acc_empty0 = leader_addr(&sm->acc_empty[0]), acc_empty1 = leader_addr(&sm->acc_empty[1]);
       int li = 0;
+      auto upstream = [&]() {                            // c of a reduced loss
+        const float up = *a.gout;
+        return up == 0.f ? 0.f : a.cscale * up * *a.inv_count;
+      };
       // 16 bytes to chunk c of this thread's row of a staging tile (128-byte swizzle)
       auto put = [&](uint8_t* p, int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
         *reinterpret_cast<uint4*>(p + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(x, y, z, w);
@@ -464,23 +488,28 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int g0 = MODE == kGrad ? a.b_off + n0 : n0;
         const size_t kept0 = (size_t)orow * a.K;         // the row's place among the targets' values
         Window<int4, int> win;
-        Window<float4, float> val;                       // kGrad: the targets' gval
+        Window<float4, float> val;                       // kGrad, kWhole: the targets' gval, prob
         auto advance = [&]() {
           ++cur;
           win.step(a.K, cur, kNone);
-          if (MODE == kGrad) val.step(a.K, cur, 0.f);
+          if (MODE == kGrad || MODE == kWhole) val.step(a.K, cur, 0.f);
           next = win.now.x == kNone ? kNone : win.now.x - g0;
         };
         float c = 0.f, lse2 = 0.f;
-        if constexpr (MODE == kStats || MODE == kGrad) {
+        auto first = [&]() {                             // of the targets in this half
+          cur = lower_bound(a.idx + kept0, a.K, g0);
+          win.open(a.idx + kept0, a.K, cur, kNone);
+          if (MODE == kGrad || MODE == kWhole) val.open((MODE == kGrad ? a.gval : a.prob) + kept0, a.K, cur, 0.f);
+          next = win.now.x == kNone ? kNone : win.now.x - g0;
+        };
+        if constexpr (MODE == kStats || MODE == kWhole || MODE == kGrad) {
           if (live && cols > 0) {
             if constexpr (SPARSE) {
-              cur = lower_bound(a.idx + kept0, a.K, g0);
-              win.open(a.idx + kept0, a.K, cur, kNone);
-              if (MODE == kGrad) val.open(a.gval + kept0, a.K, cur, 0.f);
-              next = win.now.x == kNone ? kNone : win.now.x - g0;
+              first();
+              if (MODE == kWhole) c = a.row_scale[orow];
             } else {
               const long long tv = a.target[orow] - g0;
+              if (MODE == kWhole) c = tv + g0 == a.ignore ? 0.f : tv + g0 >= 0 && tv + g0 < a.N ? 1.f : __int_as_float(0x7fc00000);
               if (tv >= 0 && tv < kHalf) {
                 next = (int)tv;
                 if (MODE == kGrad) val.now.x = a.gval[orow];
@@ -493,7 +522,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           }
         }
-        const bool ok = mbar_wait(&sm->acc_full[b], (li >> 1) & 1, abort);
+        bool ok = mbar_wait(&sm->acc_full[b], (li >> 1) & 1, abort);
+        // the two warps of a row go on together or not at all
+        if (MODE == kWhole) ok = pair_all(1 + quad, ok);
         if (__any_sync(~0u, !ok)) break;
         tc_fence_after();
         auto release = [&]() {                           // the tile's TMEM has been read
@@ -501,8 +532,41 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           __syncwarp();
           if (lane == 0) mbar_arrive_leader(b ? acc_empty1 : acc_empty0);
         };
-        if constexpr (MODE == kStats) {
-          float mx = -INFINITY, sum = 0.f;
+        // c exp(s - lse) of 64 columns to the staging, in bf16; 0 for a row without a gradient, whatever
+        // its logits are
+        auto softmax_rows = [&](const uint32_t (&x)[32], const uint32_t (&y)[32], float c, float lse2) {
+          if (c == 0.f) {
+#pragma unroll
+            for (int ch = 0; ch < 8; ++ch) put(stage, ch, 0, 0, 0, 0);
+            return;
+          }
+          auto grad = [&](uint32_t u) { return c * ex2(fmaf(__uint_as_float(u), a.a2, -lse2)); };
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch) {
+            const uint32_t* u = ch < 4 ? x + 8 * ch : y + 8 * (ch - 4);
+            put(stage, ch, pack_bf16(grad(u[0]), grad(u[1])), pack_bf16(grad(u[2]), grad(u[3])),
+                pack_bf16(grad(u[4]), grad(u[5])), pack_bf16(grad(u[6]), grad(u[7])));
+          }
+        };
+        auto put_at = [&](int at, float v) {             // one of the 64 columns again
+          *reinterpret_cast<__nv_bfloat16*>(stage + lane * 128 + (((at >> 3) ^ (lane & 7)) << 4) + (at & 7) * 2) =
+              __float2bfloat16_rn(v);
+        };
+        auto store = [&](int c0) {                       // the staging to columns n0 + c0 of the result
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            if ((MODE == kDH || MODE == kDW) && a.out == kOutPlaneAdd) tma_reduce_add_3d(&tmO, stage, n0 + c0, row0, split);
+            else tma_store_3d(&tmO, stage, n0 + c0, row0, split);
+            bulk_commit();
+          }
+        };
+        if constexpr (MODE == kStats || MODE == kWhole) {
+          float mx = -INFINITY, sum = 0.f, st = 0.f;     // st: the target's logit
+          if (MODE == kWhole) {                          // the last tile's stores have read the staging
+            if (lane == 0) bulk_wait_read_all();
+            __syncwarp();
+          }
 #pragma unroll 1
           for (int c0 = 0; c0 < kHalf; c0 += 32) {
             const int left = cols - c0;
@@ -516,8 +580,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               for (int ch = 0; ch < 8; ++ch) put(stage, ch, x[4 * ch], x[4 * ch + 1], x[4 * ch + 2], x[4 * ch + 3]);
               while (next < c0 + 32) {
                 const int at = next - c0;
-                a.slog[kept0 + cur] = *reinterpret_cast<const float*>(
-                    stage + lane * 128 + (((at >> 2) ^ (lane & 7)) << 4) + (at & 3) * 4);
+                st = *reinterpret_cast<const float*>(stage + lane * 128 + (((at >> 2) ^ (lane & 7)) << 4) + (at & 3) * 4);
+                a.slog[kept0 + cur] = st;
                 if constexpr (SPARSE) advance();
                 else next = kNone;
               }
@@ -547,9 +611,54 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             const float2 r = fadd2(fadd2(sp[0], sp[1]), fadd2(sp[2], sp[3]));
             sum += r.x + r.y;
           }
-          release();
           if (live) a.stats[(size_t)(2 * n + half) * a.n_rows + row] = make_float2(mx, sum);
+          if constexpr (MODE == kStats) {
+            release();
+          } else {
+            // the row's other half, then G / c = (exp(s - lse) - p) row_scale
+            __syncwarp();
+            reinterpret_cast<float2*>(stage)[lane] = make_float2(mx, sum);
+            pair_sync(1 + quad);
+            const float2 o = reinterpret_cast<const float2*>(sO + (quad + 4 * (1 - half)) * kOutBuf)[lane];
+            pair_sync(1 + quad);
+            const float top = fmaxf(mx, o.x), tb = top == -INFINITY ? 0.f : top * a.a2;
+            const float all = (mx == -INFINITY ? sum : sum * ex2(fmaf(mx, a.a2, -tb))) +
+                              (o.x == -INFINITY ? o.y : o.y * ex2(fmaf(o.x, a.a2, -tb)));
+            lse2 = fmaf(top, a.a2, log2f(all));
+            if constexpr (SPARSE) {
+              if (live && cols > 0) first();
+            } else if (live && cols > 0) {
+              const long long tv = a.target[orow] - g0;
+              next = tv >= 0 && tv < kHalf ? (int)tv : kNone;
+            }
+#pragma unroll 1
+            for (int c0 = 0; c0 < kHalf; c0 += 64) {
+              uint32_t x[32], y[32];
+              tmem_ld32(acc + c0, x);
+              tmem_ld32(acc + c0 + 32, y);
+              tmem_ld_wait();
+              if (c0 + 64 == kHalf) release();
+              if (c0 >= cols || row0 >= min(a.n_rows, (M + 63) / 64 * 64)) continue;
+              if (lane == 0) bulk_wait_read_all();
+              __syncwarp();
+              softmax_rows(x, y, c, lse2);
+              while (c != 0.f && next < c0 + 64) {
+                const int at = next;
+                float p = 1.f;
+                if constexpr (SPARSE) {
+                  st = a.slog[kept0 + cur];              // this thread's own
+                  p = 0.f;
+                  do { p += val.now.x; advance(); } while (next == at);    // the same index adds up
+                } else {
+                  next = kNone;
+                }
+                put_at(at - c0, c * (ex2(fmaf(st, a.a2, -lse2)) - p));
+              }
+              store(c0);
+            }
+          }
         } else {
+          const float alpha = (MODE == kDH || MODE == kDW) && a.gout ? upstream() : 1.f;
           const int width = MODE == kGrad || a.out == kOutBf16 ? 64 : 32;      // columns of one store
 #pragma unroll 1
           for (int c0 = 0; c0 < kHalf; c0 += width) {
@@ -564,34 +673,24 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
               for (int e = 0; e < 32; ++e) x[e] = y[e] = 0;
             }
+            if constexpr (MODE == kDH || MODE == kDW) {
+              if (a.gout) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  x[e] = alpha == 0.f ? 0u : __float_as_uint(alpha * __uint_as_float(x[e]));
+                  if (width == 64) y[e] = alpha == 0.f ? 0u : __float_as_uint(alpha * __uint_as_float(y[e]));
+                }
+              }
+            }
             uint8_t* p = stage;
             if (lane == 0) bulk_wait_read_all();
             __syncwarp();
             if constexpr (MODE == kGrad) {
-              if (c == 0.f) {                    // a row without a gradient, whatever its logits are
-#pragma unroll
-                for (int ch = 0; ch < 8; ++ch) put(p, ch, 0, 0, 0, 0);
-              } else {
-                auto grad = [&](uint32_t u) { return c * ex2(fmaf(__uint_as_float(u), a.a2, -lse2)); };
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch)
-                  put(p, ch, pack_bf16(grad(x[8 * ch]), grad(x[8 * ch + 1])),
-                      pack_bf16(grad(x[8 * ch + 2]), grad(x[8 * ch + 3])),
-                      pack_bf16(grad(x[8 * ch + 4]), grad(x[8 * ch + 5])),
-                      pack_bf16(grad(x[8 * ch + 6]), grad(x[8 * ch + 7])));
-#pragma unroll
-                for (int ch = 0; ch < 4; ++ch)
-                  put(p, 4 + ch, pack_bf16(grad(y[8 * ch]), grad(y[8 * ch + 1])),
-                      pack_bf16(grad(y[8 * ch + 2]), grad(y[8 * ch + 3])),
-                      pack_bf16(grad(y[8 * ch + 4]), grad(y[8 * ch + 5])),
-                      pack_bf16(grad(y[8 * ch + 6]), grad(y[8 * ch + 7])));
-                while (next < c0 + 64) {         // the row's targets among these columns (the same one twice: twice alike)
-                  const int at = next - c0;
-                  *reinterpret_cast<__nv_bfloat16*>(p + lane * 128 + (((at >> 3) ^ (lane & 7)) << 4) + (at & 7) * 2) =
-                      __float2bfloat16_rn(c * val.now.x);
-                  if constexpr (SPARSE) advance();
-                  else next = kNone;
-                }
+              softmax_rows(x, y, c, lse2);
+              while (c != 0.f && next < c0 + 64) {       // the row's targets among these columns (the same one twice: twice alike)
+                put_at(next - c0, c * val.now.x);
+                if constexpr (SPARSE) advance();
+                else next = kNone;
               }
             } else if (a.out == kOutBf16) {
 #pragma unroll
@@ -604,13 +703,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
               for (int ch = 0; ch < 8; ++ch) put(p, ch, x[4 * ch], x[4 * ch + 1], x[4 * ch + 2], x[4 * ch + 3]);
             }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-              if (MODE != kGrad && a.out == kOutPlaneAdd) tma_reduce_add_3d(&tmO, p, n0 + c0, row0, split);
-              else tma_store_3d(&tmO, p, n0 + c0, row0, split);
-              bulk_commit();
-            }
+            store(c0);
           }
         }
       }
@@ -1180,12 +1273,18 @@ static Plan plan(long long N, long long V, long long D) {
 // Places of a row's K entries: a multiple of four, for the loads of four.
 static long long entries(long long K) { return (K + 3) & ~3ll; }
 
+// Whether the forward may leave G / c: the rows are whole in one tile, and c is one number
+// (65536 x 256 x 1024, forward and backward: 161 us, 190 where the backward forms the logits
+// again; 16384 rows with 16 targets each: 90 us against 95).
+static bool whole(long long N, long long V, int reduction) { return N > kFew && V <= kTN && reduction != LH_REDUCE_NONE; }
+
 // What the forward leaves for the backward.
 struct Kept {
   float *lse2, *row_scale, *inv_count, *tgrad;   // (N), (N), (1), (N, max(K, 1))
   int *idx, *rows, *dirty;                       // (N, K) sorted targets, (2 N + 1) packed rows, (1)
+  void* g;                                       // NULL or G / c (N, kTN) bf16
   size_t bytes;
-  Kept(void* base, long long N, long long K) {
+  Kept(void* base, long long N, long long V, long long K, int reduction, bool gradients) {
     char* p = (char*)base;
     auto take = [&](size_t n) { char* q = p; p += up(n); return q; };
     lse2 = (float*)take(4 * N);
@@ -1195,6 +1294,7 @@ struct Kept {
     idx = (int*)take(4 * N * entries(K));
     rows = (int*)take(4 * (2 * N + 1));
     dirty = (int*)take(4);
+    g = gradients && whole(N, V, reduction) ? take(N * kTN * 2) : nullptr;
     bytes = p - (char*)base;
   }
 };
@@ -1262,7 +1362,7 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
   int rc = make_context_current();
   if (rc) return rc;
   const int N = q.N, V = q.V, D = q.D, K = q.K ? (int)entries(q.K) : 1;
-  CUtensorMap mh, mw, mp;
+  CUtensorMap mh, mw, mp, mg;
   if ((rc = map_load(&mh, q.hidden, N, D, D)) || (rc = map_load(&mw, q.weight, V, D, D))) return rc;
   mp = mh;
   const int* rows = nullptr;
@@ -1296,6 +1396,11 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
   if (few) {
     if ((rc = map_load(&mh, q.hidden, N, D, D, kFew / 2)) || (rc = launch<kStats, SPARSE, true>(mw, mh, mw, mw, a, D, st)))
       return rc;
+  } else if (kp.g) {
+    a.prob = ws.prob;
+    a.ignore = q.ignore;
+    a.row_scale = kp.row_scale;
+    if ((rc = map_store(&mg, kp.g, false, 1, N, V, kTN)) || (rc = launch<kWhole, SPARSE>(mh, mw, mg, mp, a, D, st))) return rc;
   } else if ((rc = launch<kStats, SPARSE>(mh, mw, mw, mp, a, D, st))) {
     return rc;
   }
@@ -1327,10 +1432,10 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
   if (rc) return rc;
   const int N = q.N, V = q.V, D = q.D;
   const Plan p = plan(N, V, D);
-  char* g = (char*)ws;
-  float* dh = (float*)(g + p.g);
-  float* dw = (float*)(g + p.g + p.dh);
-  char* packed = g + p.g + p.dh + p.dw;
+  char* g = kp.g ? (char*)kp.g : (char*)ws;
+  float* dh = (float*)((char*)ws + p.g);
+  float* dw = (float*)((char*)ws + p.g + p.dh);
+  char* packed = (char*)ws + p.g + p.dh + p.dw;
   CUtensorMap mh, mw, mp, mdh, mdw, mg, mgo;
   if ((rc = map_load(&mh, q.hidden, N, D, D)) || (rc = map_load(&mw, q.weight, V, D, D))) return rc;
   if ((rc = p.dh_planes ? map_store(&mdh, dh, true, p.dh_splits, N, D, D)
@@ -1376,9 +1481,15 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     a.gout = gout;
     a.gstride = reduction == LH_REDUCE_NONE ? 1 : 0;
     a.cscale = q.T;
-    if ((rc = few ? launch<kGrad, SPARSE, true>(mw, mh_few, mw, mw, a, D, st)
-                  : launch<kGrad, SPARSE>(mh, mw, mgo, mp, a, D, st)))
+    if (!kp.g && (rc = few ? launch<kGrad, SPARSE, true>(mw, mh_few, mw, mw, a, D, st)
+                           : launch<kGrad, SPARSE>(mh, mw, mgo, mp, a, D, st)))
       return rc;
+    auto scaled = [&](Args& z) {     // the forward's G wants c
+      if (!kp.g) return;
+      z.gout = gout;
+      z.inv_count = kp.inv_count;
+      z.cscale = q.T;
+    };
 
     if (dhidden) {
       Args x{};
@@ -1389,6 +1500,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
       const int kb = (cols + kTK - 1) / kTK;
       x.splits = p.dh_splits < kb ? p.dh_splits : kb;      // a short last piece may leave planes as they are
       for (int t = 0; t < kSplitTable; ++t) x.split_of[t] = p.split_of[t];
+      scaled(x);
       x.rows = rows;
       x.b_off = (int)v0;
       x.out = !p.dh_planes ? kOutBf16 : i ? kOutPlaneAdd : kOutPlane;
@@ -1403,6 +1515,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     y.n_rows = N;
     y.N = D;
     y.splits = p.dw_splits;
+    scaled(y);
     y.rows = rows;
     y.dirty = rows ? nullptr : kp.dirty;
     y.out = p.dw_splits > 1 ? kOutPlane : kOutBf16;
@@ -1422,23 +1535,27 @@ size_t linear_loss_workspace_size(int N, int V, int D, int K, int backward) {
   return backward ? ll::plan(N, V, D).total : ll::FwdSpace(nullptr, N, V, D, K).bytes;
 }
 
-size_t linear_loss_kept_size(int N, int K) { return ll::Kept(nullptr, N, K).bytes; }
+size_t linear_loss_kept_size(int N, int V, int K, int reduction, int gradients) {
+  return ll::Kept(nullptr, N, V, K, reduction, gradients).bytes;
+}
 
 int linear_xent_fwd(const void* hidden, const void* weight, const long long* target, long long ignore, int N, int V, int D,
-                    int reduction, float* loss, void* kept, void* ws, cudaStream_t st) {
-  return ll::forward<false>({hidden, weight, N, V, D, target, ignore, 0, 1.f}, reduction, loss, ll::Kept(kept, N, 0),
-                            ll::FwdSpace(ws, N, V, D, 0), st);
+                    int reduction, float* loss, void* kept, bool gradients, void* ws, cudaStream_t st) {
+  return ll::forward<false>({hidden, weight, N, V, D, target, ignore, 0, 1.f}, reduction, loss,
+                            ll::Kept(kept, N, V, 0, reduction, gradients), ll::FwdSpace(ws, N, V, D, 0), st);
 }
 
 int linear_xent_bwd(const void* hidden, const void* weight, const long long* target, int N, int V, int D, int reduction,
-                    const void* kept, const float* gout, void* dhidden, void* dweight, void* ws, cudaStream_t st) {
-  return ll::backward<false>({hidden, weight, N, V, D, target, 0, 0, 1.f}, reduction, ll::Kept(const_cast<void*>(kept), N, 0),
-                             gout, dhidden, dweight, ws, st);
+                    const void* kept, bool gradients, const float* gout, void* dhidden, void* dweight, void* ws,
+                    cudaStream_t st) {
+  return ll::backward<false>({hidden, weight, N, V, D, target, 0, 0, 1.f}, reduction,
+                             ll::Kept(const_cast<void*>(kept), N, V, 0, reduction, gradients), gout, dhidden, dweight, ws, st);
 }
 
 int linear_distill_fwd(const void* hidden, const void* weight, const void* tv, int tv_dtype, const long long* ti, int N,
-                       int V, int D, int K, float T, int reduction, float* loss, void* kept, void* ws, cudaStream_t st) {
-  const ll::Kept kp(kept, N, K);
+                       int V, int D, int K, float T, int reduction, float* loss, void* kept, bool gradients, void* ws,
+                       cudaStream_t st) {
+  const ll::Kept kp(kept, N, V, K, reduction, gradients);
   const ll::FwdSpace sp(ws, N, V, D, K);
   const unsigned blocks = (unsigned)((N + 3) / 4);
   const size_t smem = 4 * ll::entries(K) * sizeof(int);
@@ -1452,9 +1569,10 @@ int linear_distill_fwd(const void* hidden, const void* weight, const void* tv, i
 }
 
 int linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int D, int K, float T, int reduction,
-                       const void* kept, const float* gout, void* dhidden, void* dweight, void* ws, cudaStream_t st) {
-  return ll::backward<true>({hidden, weight, N, V, D, nullptr, 0, K, T}, reduction, ll::Kept(const_cast<void*>(kept), N, K),
-                            gout, dhidden, dweight, ws, st);
+                       const void* kept, bool gradients, const float* gout, void* dhidden, void* dweight, void* ws,
+                    cudaStream_t st) {
+  return ll::backward<true>({hidden, weight, N, V, D, nullptr, 0, K, T}, reduction,
+                            ll::Kept(const_cast<void*>(kept), N, V, K, reduction, gradients), gout, dhidden, dweight, ws, st);
 }
 
 int loss_status(int reset) {

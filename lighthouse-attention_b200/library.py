@@ -280,10 +280,10 @@ def _(x, residual, weight, eps, group):
 
 
 # --------------------------------------------------------------------------- losses of an output projection
-def _loss_fake(hidden, reduction, K):
+def _loss_fake(hidden, weight, reduction, K):
     N = hidden.shape[0]
     return (hidden.new_empty((N,) if reduction == "none" else (), dtype=torch.float32),
-            hidden.new_empty(_native.kept_size(N, K), dtype=torch.uint8))
+            hidden.new_empty(_native.kept_size(N, weight.shape[0], K, reduction), dtype=torch.uint8))
 
 
 @torch.library.custom_op(f"{NS}::linear_xent", mutates_args=())
@@ -295,7 +295,7 @@ def linear_xent(hidden: Tensor, weight: Tensor, target: Tensor, ignore_index: in
 
 @linear_xent.register_fake
 def _(hidden, weight, target, ignore_index, reduction):
-    return _loss_fake(hidden, reduction, 0)
+    return _loss_fake(hidden, weight, reduction, 0)
 
 
 @torch.library.custom_op(f"{NS}::linear_xent_bwd", mutates_args=())
@@ -320,7 +320,7 @@ def linear_distill(hidden: Tensor, weight: Tensor, teacher_logits: Tensor, teach
 
 @linear_distill.register_fake
 def _(hidden, weight, teacher_logits, teacher_indices, temperature, reduction):
-    return _loss_fake(hidden, reduction, teacher_indices.shape[1])
+    return _loss_fake(hidden, weight, reduction, teacher_indices.shape[1])
 
 
 @torch.library.custom_op(f"{NS}::linear_distill_bwd", mutates_args=())

@@ -357,6 +357,56 @@ def test_distillation_from_one_certain_entry_is_cross_entropy(lh, cuda):
     assert torch.equal(a[1], b[0]) and torch.equal(a[2], b[1])
 
 
+# --------------------------------------------------------------------------- rows of one tile
+ONE_TILE = [(65, 1, 8), (66, 17, 64), (300, 128, 72), (513, 129, 128), (1000, 200, 264), (20001, 256, 64), (260, 256, 4096)]
+
+
+@pytest.mark.parametrize("N,V,D", ONE_TILE)
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_rows_of_one_tile(lh, cuda, N, V, D, reduction):
+    """The forward leaves the logits' gradients: more tiles than pairs of SMs, ragged rows and columns."""
+    for ignore in (0.0, 0.4):
+        _run_xent(lh, cuda, N, V, D, reduction, seed=60, ignore=ignore)
+    if V > 1:
+        def edit(tv, ti):
+            ti[::7, 0] = ti[::7, -1]                 # the same index twice
+            ti[3::11] = -1
+        _run_distill(lh, cuda, N, V, D, min(V, 9), 2.0, reduction, seed=61, empty=0.2, edit=edit)
+    _run_distill(lh, cuda, N, V, D, min(V, 100), 0.7, reduction, seed=62)
+
+
+def test_rows_of_one_tile_packed(lh, cuda):
+    _run_xent(lh, cuda, 100000, 256, 1024, "mean", seed=63, ignore=0.3)
+    _run_distill(lh, cuda, 100000, 250, 1024, 5, 2.0, "sum", seed=64, empty=0.99)
+    h, w = torch.randn(100000, 1024, device=cuda).to(BF), torch.randn(256, 1024, device=cuda).to(BF)
+    loss, dh, dw = _xent(lh, h, w, torch.full((100000,), -100, device=cuda), "mean")
+    assert loss == 0 and (dh == 0).all() and (dw == 0).all()
+
+
+def test_rows_of_one_tile_upstream_gradients(lh, cuda):
+    """Zero, negative and large upstream gradients, one after the other from the same graph, and a bad target."""
+    g, h, w = _problem(300, 200, 64, 65, cuda)
+    t = torch.randint(0, 200, (300,), generator=g).to(cuda)
+    h1, w1 = h.requires_grad_(True), w.requires_grad_(True)
+    loss = lh.linear_cross_entropy(h1, w1, t)
+    one = torch.autograd.grad(loss, (h1, w1), retain_graph=True)
+    for f in (-4.0, 2.0 ** 40, 2.0 ** -20):          # powers of two: bit for bit
+        got = torch.autograd.grad(loss, (h1, w1), torch.tensor(f, device=cuda), retain_graph=True)
+        assert all(torch.equal(a, b * f) for a, b in zip(got, one))
+    t2 = t.clone()
+    t2[5] = 200
+    loss = lh.linear_cross_entropy(h1, w1, t2)
+    assert loss.isnan()
+    got = torch.autograd.grad(loss, (h1, w1), torch.zeros((), device=cuda), retain_graph=True)
+    assert all((x == 0).all() for x in got)
+    dh, dw = torch.autograd.grad(loss, (h1, w1))
+    assert dh[5].isnan().all() and dw.isnan().all()
+    # without the forward's gradients (reduction "none"): the same up to one rounding more or less
+    none = torch.autograd.grad(lh.linear_cross_entropy(h1, w1, t, reduction="none").mean(), (h1, w1))
+    for a, b in zip(one, none):
+        assert (a.double() - b.double()).norm() <= 2 * H8 * b.double().norm()
+
+
 # --------------------------------------------------------------------------- both
 def test_gradients_against_differences(lh, cuda):
     """Central differences of the 64-bit formulas at a few coordinates; G's bf16 bounds the gradients."""

@@ -57,32 +57,33 @@ def test_c_entry_points_check_before_they_touch_a_device(lh):
     a = P(4096)                  # aligned and never read: every call below is refused on the host
     big = 1 << 40
 
-    def xf(h=a, w=a, t=a, N=4, V=10, D=64, red=1, loss=a, kept=a, ws=a, n=big):
-        return lib.lh_linear_xent_fwd(h, w, t, -100, N, V, D, red, loss, kept, ws, n, None)
+    def xf(h=a, w=a, t=a, N=4, V=10, D=64, red=1, loss=a, kept=a, ws=a, n=big, nk=big):
+        return lib.lh_linear_xent_fwd(h, w, t, -100, N, V, D, red, loss, kept, nk, ws, n, None)
 
     assert xf(h=None) == 2 and xf(t=None) == 2 and xf(loss=None) == 2 and xf(kept=None) == 2 and xf(ws=None) == 2
     assert xf(N=0) == 1 and xf(V=0) == 1 and xf(D=12) == 1 and xf(N=(1 << 22) + 1) == 1 and xf(V=(1 << 22) + 1) == 1
     assert xf(red=3) == 2 and xf(w=P(4104)) == 2 and xf(kept=P(4104)) == 2 and xf(ws=P(4096 + 16)) == 2
     assert xf(n=lib.lh_linear_loss_workspace_size(4, 10, 64, 0, 0) - 1) == 5
+    assert xf(nk=lib.lh_linear_loss_kept_size(4, 10, 0, 1, 0) - 1) == 5
 
     def xb(gout=a, red=1, dw=a, n=big):
-        return lib.lh_linear_xent_bwd(a, a, a, 4, 10, 64, red, a, gout, a, dw, a, n, None)
+        return lib.lh_linear_xent_bwd(a, a, a, 4, 10, 64, red, a, big, gout, a, dw, a, n, None)
 
     assert xb(gout=None) == 2 and xb(red=-1) == 2 and xb(dw=P(4100)) == 2
     assert xb(n=lib.lh_linear_loss_workspace_size(4, 10, 64, 0, 1) - 1) == 5
 
     def df(K=3, T=1.0, tv=a, dt=1):
-        return lib.lh_linear_distill_fwd(a, a, tv, dt, a, 4, 10, 64, K, T, 1, a, a, a, big, None)
+        return lib.lh_linear_distill_fwd(a, a, tv, dt, a, 4, 10, 64, K, T, 1, a, a, big, a, big, None)
 
     assert df(K=0) == 1 and df(K=257) == 1 and df(T=0.0) == 2 and df(tv=None) == 2 and df(dt=2) == 2
 
     def db(kept=a, K=3):
-        return lib.lh_linear_distill_bwd(a, a, 4, 10, 64, K, 1.0, 1, kept, a, a, a, a, big, None)
+        return lib.lh_linear_distill_bwd(a, a, 4, 10, 64, K, 1.0, 1, kept, big, a, a, a, a, big, None)
 
     assert db(kept=None) == 2 and db(K=0) == 1
     # one of the gradients may be left out, not both
-    assert lib.lh_linear_xent_bwd(a, a, a, 4, 10, 64, 1, a, a, None, None, a, big, None) == 2
-    assert lib.lh_linear_distill_bwd(a, a, 4, 10, 64, 3, 1.0, 1, a, a, None, None, a, big, None) == 2
+    assert lib.lh_linear_xent_bwd(a, a, a, 4, 10, 64, 1, a, big, a, None, None, a, big, None) == 2
+    assert lib.lh_linear_distill_bwd(a, a, 4, 10, 64, 3, 1.0, 1, a, big, a, None, None, a, big, None) == 2
 
 
 def test_workspace_stays_small(lh):
@@ -117,3 +118,11 @@ def test_eager_calls_leave_cpu_and_meta_tensors_to_python(lh):
         assert e.linear_distill(a, b, a[:, :3].float(), c[:, None].expand(4, 3), 1.0, 1) is None
         assert e.rms_norm(a, b[0], 1e-5, None) is None and e.add_rms_norm(a, a, b[0], 1e-5, None) is None
         assert e.rms_norm_fp8(a, b[0], 1e-5, 0) is None and e.add_rms_norm_fp8(a, a, b[0], 1e-5, 128) is None
+
+
+def test_kept_size_holds_gradients_of_one_tile_only(lh):
+    size = lh._native.load().lh_linear_loss_kept_size
+    for N, V, red, more in ((65, 256, 1, True), (1000, 1, 2, True), (64, 256, 1, False), (65, 257, 1, False), (65, 256, 0, False)):
+        for K in (0, 16):
+            assert size(N, V, K, red, 1) - size(N, V, K, red, 0) == (512 * N + 255) // 256 * 256 * more
+    assert size(0, 10, 0, 1, 1) == 0
