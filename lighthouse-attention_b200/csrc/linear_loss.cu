@@ -68,12 +68,17 @@ enum Out { kOutBf16, kOutPlane, kOutPlaneAdd };
 // columns of dH) and its kFew columns are rows of hidden, so that the MMAs do an eighth
 // of the work and the stages hold weights, which are what has to be read.
 constexpr int kFew = 64;
-// Six stages of the operands and one store's staging buffer per epilogue warp (five and
-// two: 1 to 2 % slower over the four products).
-__host__ __device__ constexpr int stages(bool few) { return few ? 10 : 6; }
+// A stage holds two steps of 64: its eight MMAs are issued without a stop, as each wait for a
+// stage and each commit of one leaves the tensor pipe empty for about 100 cycles, whatever waits
+// (4096 x 32000 x 4096, forward: 790 us with six stages of one step, 830 with a wait or a commit
+// per step and the other per two; 760 with three stages of two; 855 with two of three, which
+// leaves the loads too little room).  One store's staging buffer per epilogue warp: two, and a
+// step less of operands, are 1 to 2 % slower.
+constexpr int kSubs = 2;
+__host__ __device__ constexpr int stages(bool few) { return few ? 5 : 3; }
 __host__ __device__ constexpr int b_bytes(bool few) { return few ? kFew / 2 * 128 : kOpBytes; }
 constexpr int smem_bytes(bool few) {
-  return 1024 + stages(few) * (kOpBytes + b_bytes(few)) + (few ? 0 : 8 * kOutBuf) + 512;
+  return 1024 + stages(few) * kSubs * (kOpBytes + b_bytes(few)) + (few ? 0 : 8 * kOutBuf) + 512;
 }
 
 // Walk of the tiles: split, group of gm row blocks, column block, row block in the group.
@@ -87,7 +92,7 @@ struct Sched {
 };
 
 struct Smem {
-  uint64_t full[10], empty[10], acc_full[2], acc_empty[2], drain;
+  uint64_t full[5], empty[5], acc_full[2], acc_empty[2], drain;
   Sched sched;
   uint32_t tmem_base;
   int abort;
@@ -199,8 +204,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = base;
-  uint8_t* sB = base + kStages * kOpBytes;
-  uint8_t* sO = base + kStages * (kOpBytes + kBBytes);
+  uint8_t* sB = base + kStages * kSubs * kOpBytes;
+  uint8_t* sO = base + kStages * kSubs * (kOpBytes + kBBytes);
   Smem* sm = reinterpret_cast<Smem*>(sO + (FEW ? 0 : 8 * kOutBuf));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
@@ -271,81 +276,103 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   if (*abort == 0) {
     if (warp == 0) {
       // ---------------------------------------------------------- TMA producer
-      if (lane == 0) {
-        const CUtensorMap* mapA = kAMn || MODE == kDH || !sched.packed ? &tmA : &tmP;
-        const CUtensorMap* mapB = MODE == kDW && (sched.packed || (a.dirty && *a.dirty)) ? &tmP : &tmB;
-        uint32_t it = 0;
-        bool ok = true;
-        for (int t = pair; t < total && ok; t += n_pairs) {
-          int m, n, k0, k1, split;
-          decode(t, m, n, k0, k1, split);
-          const int ra = m * kTM + rank * 128, rb = n * kCols + rank * (kCols / 2);
-          for (int k = k0; k < k1; ++k, ++it) {
-            const int s = it % kStages;
-            const uint32_t round = it / kStages;
-            if (round > 0 && !mbar_wait(&sm->empty[s], (round - 1) & 1, abort)) { ok = false; break; }
-            if (rank == 0) mbar_expect_tx(&sm->full[s], 2 * (kOpBytes + kBBytes));
+      // (The whole warp runs this role and the next one, one lane of it issues: with a single lane in a
+      // branch the operands of each copy and MMA pass through vector registers; 1 to 3 % of the time.)
+      const CUtensorMap* mapA = kAMn || MODE == kDH || !sched.packed ? &tmA : &tmP;
+      const CUtensorMap* mapB = MODE == kDW && (sched.packed || (a.dirty && *a.dirty)) ? &tmP : &tmB;
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += n_pairs) {
+        int m, n, k0, k1, split;
+        decode(t, m, n, k0, k1, split);
+        const int ra = m * kTM + rank * 128, rb = n * kCols + rank * (kCols / 2);
+        for (int kg = k0; kg < k1; kg += kSubs, ++it) {
+          const int s = it % kStages;
+          const uint32_t round = it / kStages;
+          if (round > 0) ok = mbar_wait(&sm->empty[s], (round - 1) & 1, abort);
+          if (__any_sync(~0u, !ok)) { ok = false; break; }
+          if (elect_one()) {
+            const int n_sub = min(kSubs, k1 - kg);
+            if (rank == 0) mbar_expect_tx(&sm->full[s], n_sub * 2 * (kOpBytes + kBBytes));
             const uint32_t bar = leader_addr(&sm->full[s]);
-            uint8_t* pa = sA + s * kOpBytes;
-            uint8_t* pb = sB + s * kBBytes;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int a_row = ra + 64 * j + (FEW && !kAMn ? a.b_off : 0), a_k = k * kTK + (FEW && kAMn ? a.b_off : 0);
-              if (kAMn) tma_load_2d_pair(pa + j * kBox, mapA, bar, a_row, a_k);
-              else tma_load_2d_pair(pa + j * kBox, mapA, bar, a_k, a_row);
-            }
-            if constexpr (FEW) {
-              tma_load_2d_pair(pb, mapB, bar, k * kTK, rb);
-            } else {
+            for (int u = 0; u < kSubs; ++u) {
+              if (u < n_sub) {
+                const int k = kg + u;
+                uint8_t* pa = sA + (s * kSubs + u) * kOpBytes;
+                uint8_t* pb = sB + (s * kSubs + u) * kBBytes;
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                if (kBMn) tma_load_2d_pair(pb + j * kBox, mapB, bar, rb + 64 * j, a.b_off + k * kTK);
-                else tma_load_2d_pair(pb + j * kBox, mapB, bar, k * kTK, a.b_off + rb + 64 * j);
+                for (int j = 0; j < 2; ++j) {
+                  const int a_row = ra + 64 * j + (FEW && !kAMn ? a.b_off : 0), a_k = k * kTK + (FEW && kAMn ? a.b_off : 0);
+                  if (kAMn) tma_load_2d_pair(pa + j * kBox, mapA, bar, a_row, a_k);
+                  else tma_load_2d_pair(pa + j * kBox, mapA, bar, a_k, a_row);
+                }
+                if constexpr (FEW) {
+                  tma_load_2d_pair(pb, mapB, bar, k * kTK, rb);
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 2; ++j) {
+                    if (kBMn) tma_load_2d_pair(pb + j * kBox, mapB, bar, rb + 64 * j, a.b_off + k * kTK);
+                    else tma_load_2d_pair(pb + j * kBox, mapB, bar, k * kTK, a.b_off + rb + 64 * j);
+                  }
+                }
               }
             }
           }
+          __syncwarp();
         }
-        // no copy is in flight when the CTAs leave, whatever the other roles waited for (the
-        // leader's barriers count the copies of both)
-        if (rank == 0)
-          for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
-            for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->full[i % kStages], (i / kStages) & 1); ++p) {}
       }
+      // no copy is in flight when the CTAs leave, whatever the other roles waited for (the
+      // leader's barriers count the copies of both)
+      if (rank == 0 && lane == 0)
+        for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
+          for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->full[i % kStages], (i / kStages) & 1); ++p) {}
     } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- MMA issuer
-      if (lane == 0) {
-        constexpr uint32_t idesc = idesc_bf16_f32(kTM, kCols, kAMn, kBMn);
-        uint32_t it = 0;
-        int li = 0;
-        bool ok = true;
-        // (Looking at the next stage's barrier, or waiting for the next accumulator, before a step's
-        // MMAs are issued makes the kernel 3 to 8 % slower, not faster.)
-        const int q = sched.kb / sched.splits, rem = sched.kb - q * sched.splits;
-        for (int t = pair; t < total && ok; t += n_pairs, ++li) {
-          const int steps = q + ((int)sched.div[0].div(t) < rem ? 1 : 0);
-          const int b = li & 1;
-          const uint32_t acc = tbase + b * kCols;
-          if (li >= 2 && !mbar_wait(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort)) break;
+      constexpr uint32_t idesc = idesc_bf16_f32(kTM, kCols, kAMn, kBMn);
+      uint32_t it = 0;
+      int li = 0;
+      bool ok = true;
+      // (Looking at the next stage's barrier, or waiting for the next accumulator, before a stage's
+      // MMAs are issued makes the kernel 3 to 8 % slower, not faster.)
+      const int q = sched.kb / sched.splits, rem = sched.kb - q * sched.splits;
+      for (int t = pair; t < total && ok; t += n_pairs, ++li) {
+        const int steps = q + ((int)sched.div[0].div(t) < rem ? 1 : 0);
+        const int b = li & 1;
+        const uint32_t acc = tbase + b * kCols;
+        if (li >= 2) ok = mbar_wait(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort);
+        if (__any_sync(~0u, !ok)) break;
+        tc_fence_after();
+        for (int kg = 0; kg < steps; kg += kSubs, ++it) {
+          const int s = it % kStages;
+          ok = mbar_wait(&sm->full[s], (it / kStages) & 1, abort);
+          if (__any_sync(~0u, !ok)) { ok = false; break; }
           tc_fence_after();
-          for (int k = 0; k < steps; ++k, ++it) {
-            const int s = it % kStages;
-            if (!mbar_wait(&sm->full[s], (it / kStages) & 1, abort)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t pa = smem_u32(sA + s * kOpBytes), pb = smem_u32(sB + s * kBBytes);
+          const int n_sub = min(kSubs, steps - kg);
+          if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kTK / 16; ++kk)
-              mma_ss_pair(acc,
-                          kAMn ? smem_desc_sw128(pa + kk * 2048, kBox, 1024) : smem_desc_sw128(pa + kk * 32, 16, 1024),
-                          kBMn ? smem_desc_sw128(pb + kk * 2048, kBox, 1024) : smem_desc_sw128(pb + kk * 32, 16, 1024),
-                          idesc, (k > 0 || kk > 0) ? 1u : 0u);
+            for (int u = 0; u < kSubs; ++u) {
+              if (u < n_sub) {
+                const uint32_t pa = smem_u32(sA + (s * kSubs + u) * kOpBytes), pb = smem_u32(sB + (s * kSubs + u) * kBBytes);
+#pragma unroll
+                for (int kk = 0; kk < kTK / 16; ++kk)
+                  mma_ss_pair(acc,
+                              kAMn ? smem_desc_sw128(pa + kk * 2048, kBox, 1024) : smem_desc_sw128(pa + kk * 32, 16, 1024),
+                              kBMn ? smem_desc_sw128(pb + kk * 2048, kBox, 1024) : smem_desc_sw128(pb + kk * 32, 16, 1024),
+                              idesc, (kg + u > 0 || kk > 0) ? 1u : 0u);
+              }
+            }
             mma_commit_pair(&sm->empty[s]);
+            if (kg + kSubs >= steps) mma_commit_pair(&sm->acc_full[b]);
           }
-          if (ok) mma_commit_pair(&sm->acc_full[b]);
+          __syncwarp();
         }
-        if (*abort) {                            // the MMAs issued so far end before TMEM is freed
-          mma_commit_pair(&sm->drain);
-          for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->drain, 0); ++p) {}
-        }
+        if (steps == 0 && elect_one()) mma_commit_pair(&sm->acc_full[b]);
+        __syncwarp();
+      }
+      if (__any_sync(~0u, *abort) && elect_one()) {      // the MMAs issued so far end before TMEM is freed
+        mma_commit_pair(&sm->drain);
+        for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->drain, 0); ++p) {}
       }
     } else if (FEW && warp >= 4) {
       // ---------------------------------------------------------- epilogue, few rows
