@@ -978,6 +978,7 @@ finish_kernel(const FinishArgs a) {
       const long long t = a.target[rr];
       if (t >= 0 && t < a.V) {
         const __nv_bfloat16 *hp = a.hidden + (size_t)rr * a.D, *wp = a.weight + (size_t)t * a.D;
+#pragma unroll 4
         for (int c = (w % per * 32 + lane) * 8; c < a.D; c += per * 256) {
           float u[8], v[8];
           plain16(hp + c, u);
