@@ -496,6 +496,37 @@ def test_same_results_every_time_on_a_stream_and_in_a_graph(lh, cuda):
     assert lh._native.device_status() == 0
 
 
+@pytest.mark.parametrize("N,V,D", [(600, 200, 64), (40, 3001, 64), (300, 3001, 64), BIG])
+def test_a_replayed_graph_follows_its_inputs(lh, cuda, N, V, D):
+    """Other hidden states, targets and numbers of ignored positions, whose rows hold NaN, in every replay."""
+    g, h, w = _problem(N, V, D, 70, cuda)
+    t = torch.randint(0, V, (N,), generator=g).to(cuda)
+    tv, ti = torch.randn(N, 6, generator=g).to(cuda), torch.randint(0, V, (N, 6), generator=g).to(cuda)
+
+    def both():
+        h1, w1 = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        a = lh.linear_cross_entropy(h1, w1, t)
+        out = [a.detach(), *torch.autograd.grad(a, (h1, w1))]
+        b = lh.linear_distillation(h1, w1, tv, ti, reduction="sum")
+        return out + [b.detach(), *torch.autograd.grad(b, (h1, w1))]
+
+    both()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    for share in (0.0, 0.5, 0.98, 0.2, 1.0, 0.0):
+        off = (torch.rand(N, generator=g) < share).to(cuda)
+        t.copy_(torch.randint(0, V, (N,), generator=g))
+        ti.copy_(torch.randint(0, V, (N, 6), generator=g))
+        t[off], ti[off] = -100, -1
+        h.copy_((torch.randn(N, D, generator=g) * 2).to(BF))
+        h[off] = float("nan")
+        graph.replay()
+        want = both()
+        assert all(torch.equal(a, b) for a, b in zip(want, out)) and all(x.isfinite().all() for x in out)
+    assert lh._native.device_status() == 0
+
+
 def test_opcheck(lh, cuda):
     ops = torch.ops.lighthouse_b200
     utils = ("test_schema", "test_faketensor")
