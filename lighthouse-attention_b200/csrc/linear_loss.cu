@@ -14,11 +14,14 @@
 // epilogue writing G (N, C) in bf16; then dH += G W_piece and dW_piece = G^T H.
 // G is rounded to bf16 once, as an operand of bf16 MMAs has to be; its relative
 // error of 2^-9 is that of the bf16 gradients it ends in.  All sums are fp32.
+// Where the loss is reduced, c is the same for all rows: G / c is what is rounded, and
+// dH and dW are multiplied by c in fp32.  The targets' entries, the largest ones, are
+// then near -1, which bf16 holds, where G's would all be off by c's own rounding (434 x
+// 967 x 296, mean: dH off by 0.0025 of itself, 0.0021 so; 0.0017 is dH's rounding).
 //
 // Where a row's vocabulary is one tile (V <= 256) and the loss is reduced, the forward
 // knows a row's lse when its tile ends, and writes G / c there: the backward has one
-// product and a reading of hidden less, and c, the same for all rows, is multiplied
-// into dH and dW.
+// product and a reading of hidden less.
 //
 // Rows without a target (ignored positions, rows without a teacher) are left out of
 // all products where those are long enough to pay for it: the rows that count are
@@ -123,8 +126,7 @@ struct Args {
   const float* prob;              // kWhole: p at the targets (n_rows, K), not read where SPARSE is false
   long long ignore;               // kWhole, SPARSE false
   const float* lse2;              // kGrad: log2-sum-exp2 of s a2
-  const float *gout, *row_scale, *inv_count;       // kDH, kDW: gout is NULL, or G wants c
-  int gstride;
+  const float *gout, *row_scale, *inv_count;       // gout NULL: c is row_scale (kGrad), or 1 (kDH, kDW)
   float cscale;
   void* few_out;                  // few rows: G (bf16, few_pitch), or the planes (fp32) or dH (bf16) of kDH
   long long few_pitch;
@@ -258,6 +260,10 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   volatile int* abort = &sm->abort;
   const Sched& sched = sm->sched;
   const int total = sched.total, M = sched.M;
+  auto upstream = [&]() {                                // c of a reduced loss
+    const float up = *a.gout;
+    return up == 0.f ? 0.f : a.cscale * up * *a.inv_count;
+  };
 
   // tile t -> split, row block, column block
   auto decode = [&](int t, int& m, int& n, int& k0, int& k1, int& split) {
@@ -385,12 +391,13 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const bool live = row < a.N;
       const int rows = min(32, a.N - half * 32);         // of this warp, may be negative
       float mx = -INFINITY, sum = 0.f, c = 0.f, lse2 = 0.f;
+      const float alpha = MODE == kDH && a.gout ? upstream() : 1.f;
       long long target = -1;
       if constexpr (MODE == kStats || MODE == kGrad) {
         if (live && !SPARSE) target = a.target[row];
         if (MODE == kGrad && live) {
-          const float up = a.gout[(size_t)row * a.gstride];
-          if (up != 0.f) c = a.cscale * up * a.row_scale[row] * (a.inv_count ? *a.inv_count : 1.f);
+          const float up = a.gout ? a.cscale * a.gout[row] : 1.f;
+          if (up != 0.f) c = up * a.row_scale[row];
           lse2 = a.lse2[row];
         }
       }
@@ -416,8 +423,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           for (int e = 0; e < 32; ++e) {
             if (e < rows && lane < left) {
               const size_t at = (size_t)(half * 32 + e) * a.M + v0 + lane;
-              if (a.out == kOutBf16) reinterpret_cast<__nv_bfloat16*>(a.few_out)[at] = __float2bfloat16_rn(__uint_as_float(x[e]));
-              else reinterpret_cast<uint32_t*>(a.few_out)[(size_t)split * a.N * a.M + at] = x[e];
+              const float d = alpha == 0.f ? 0.f : alpha * __uint_as_float(x[e]);
+              if (a.out == kOutBf16) reinterpret_cast<__nv_bfloat16*>(a.few_out)[at] = __float2bfloat16_rn(d);
+              else reinterpret_cast<float*>(a.few_out)[(size_t)split * a.N * a.M + at] = d;
             }
           }
         } else {
@@ -492,11 +500,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const uint32_t lane_base = tbase + ((uint32_t)(quad * 32) << 16) + half * kHalf;
       uint8_t* stage = sO + (quad + 4 * half) * kOutBuf;
       const uint32_t acc_empty0 = leader_addr(&sm->acc_empty[0]), acc_empty1 = leader_addr(&sm->acc_empty[1]);
+      const float alpha = (MODE == kDH || MODE == kDW) && a.gout ? upstream() : 1.f;
       int li = 0;
-      auto upstream = [&]() {                            // c of a reduced loss
-        const float up = *a.gout;
-        return up == 0.f ? 0.f : a.cscale * up * *a.inv_count;
-      };
       // 16 bytes to chunk c of this thread's row of a staging tile (128-byte swizzle)
       auto put = [&](uint8_t* p, int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
         *reinterpret_cast<uint4*>(p + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(x, y, z, w);
@@ -543,8 +548,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               }
             }
             if constexpr (MODE == kGrad) {
-              const float up = a.gout[(size_t)orow * a.gstride];
-              if (up != 0.f) c = a.cscale * up * a.row_scale[orow] * (a.inv_count ? *a.inv_count : 1.f);
+              const float up = a.gout ? a.cscale * a.gout[orow] : 1.f;
+              if (up != 0.f) c = up * a.row_scale[orow];
               lse2 = a.lse2[orow];
             }
           }
@@ -685,7 +690,6 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           }
         } else {
-          const float alpha = (MODE == kDH || MODE == kDW) && a.gout ? upstream() : 1.f;
           const int width = MODE == kGrad || a.out == kOutBf16 ? 64 : 32;      // columns of one store
 #pragma unroll 1
           for (int c0 = 0; c0 < kHalf; c0 += width) {
@@ -1505,15 +1509,13 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     a.gval = kp.tgrad;
     a.lse2 = kp.lse2;
     a.row_scale = kp.row_scale;
-    a.inv_count = reduction == LH_REDUCE_NONE ? nullptr : kp.inv_count;
-    a.gout = gout;
-    a.gstride = reduction == LH_REDUCE_NONE ? 1 : 0;
+    a.gout = reduction == LH_REDUCE_NONE ? gout : nullptr;
     a.cscale = q.T;
     if (!kp.g && (rc = few ? launch<kGrad, SPARSE, true>(mw, mh_few, mw, mw, a, D, st)
                            : launch<kGrad, SPARSE>(mh, mw, mgo, mp, a, D, st)))
       return rc;
-    auto scaled = [&](Args& z) {     // the forward's G wants c
-      if (!kp.g) return;
+    auto scaled = [&](Args& z) {     // what comes of G / c
+      if (reduction == LH_REDUCE_NONE) return;
       z.gout = gout;
       z.inv_count = kp.inv_count;
       z.cscale = q.T;

@@ -383,10 +383,11 @@ def test_rows_of_one_tile_packed(lh, cuda):
     assert loss == 0 and (dh == 0).all() and (dw == 0).all()
 
 
-def test_rows_of_one_tile_upstream_gradients(lh, cuda):
+@pytest.mark.parametrize("N,V", [(300, 200), (300, 967), (40, 967)])
+def test_upstream_gradients_of_a_reduced_loss(lh, cuda, N, V):
     """Zero, negative and large upstream gradients, one after the other from the same graph, and a bad target."""
-    g, h, w = _problem(300, 200, 64, 65, cuda)
-    t = torch.randint(0, 200, (300,), generator=g).to(cuda)
+    g, h, w = _problem(N, V, 64, 65, cuda)
+    t = torch.randint(0, V, (N,), generator=g).to(cuda)
     h1, w1 = h.requires_grad_(True), w.requires_grad_(True)
     loss = lh.linear_cross_entropy(h1, w1, t)
     one = torch.autograd.grad(loss, (h1, w1), retain_graph=True)
@@ -394,7 +395,7 @@ def test_rows_of_one_tile_upstream_gradients(lh, cuda):
         got = torch.autograd.grad(loss, (h1, w1), torch.tensor(f, device=cuda), retain_graph=True)
         assert all(torch.equal(a, b * f) for a, b in zip(got, one))
     t2 = t.clone()
-    t2[5] = 200
+    t2[5] = V
     loss = lh.linear_cross_entropy(h1, w1, t2)
     assert loss.isnan()
     got = torch.autograd.grad(loss, (h1, w1), torch.zeros((), device=cuda), retain_graph=True)
