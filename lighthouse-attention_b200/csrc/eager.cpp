@@ -198,19 +198,6 @@ bool rows_case(const Tensor& t, const Tensor& h, int64_t dim) {
          !t.key_set().has_any(c10::python_ks | c10::functorch_transforms_ks);
 }
 
-// The size of a problem's workspace takes a search over splits: the last few are kept.
-size_t loss_workspace(int64_t N, int64_t V, int64_t D, int64_t K, int back) {
-  struct Entry { int64_t N, V, D, K; int back; size_t n; };
-  static thread_local Entry seen[8] = {};
-  static thread_local int at = 0;
-  for (const Entry& e : seen)
-    if (e.N == N && e.V == V && e.D == D && e.K == K && e.back == back) return e.n;
-  seen[at] = {N, V, D, K, back, api.loss_ws((int)N, (int)V, (int)D, (int)K, back)};
-  const size_t n = seen[at].n;
-  at = (at + 1) % 8;
-  return n;
-}
-
 struct LossFn : torch::autograd::Function<LossFn> {
   // target (N) and K = 0, or teacher logits and indices (N, K)
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& target,
@@ -221,7 +208,7 @@ struct LossFn : torch::autograd::Function<LossFn> {
     const int64_t N = h.size(0), D = h.size(1), V = w.size(0), K = tl.defined() ? tl.size(1) : 0;
     const Tensor loss = reduction == LH_REDUCE_NONE ? empty({N}, at::kFloat, h.device()) : empty({}, at::kFloat, h.device());
     const Tensor kept = empty({(int64_t)api.loss_kept((int)N, (int)V, (int)K, (int)reduction, gradients)}, at::kByte, h.device());
-    const size_t n = loss_workspace(N, V, D, K, 0);
+    const size_t n = api.loss_ws((int)N, (int)V, (int)D, (int)K, 0);
     const Tensor ws = empty({(int64_t)n}, at::kByte, h.device());
     if (K)
       check(api.distill_fwd(h.const_data_ptr(), w.const_data_ptr(), tl.const_data_ptr(), dtype_code(tl.scalar_type()),
@@ -253,7 +240,7 @@ struct LossFn : torch::autograd::Function<LossFn> {
     if (ctx->needs_input_grad(1)) dw = empty(w.sizes(), at::kBFloat16, h.device());
     if (!dh.defined() && !dw.defined()) return variable_list(8);
     void *dhp = dh.defined() ? dh.mutable_data_ptr() : nullptr, *dwp = dw.defined() ? dw.mutable_data_ptr() : nullptr;
-    const size_t n = loss_workspace(N, V, D, K, 1);
+    const size_t n = api.loss_ws((int)N, (int)V, (int)D, (int)K, 1);
     const Tensor ws = empty({(int64_t)n}, at::kByte, h.device());
     if (K)
       check(api.distill_bwd(h.const_data_ptr(), w.const_data_ptr(), (int)N, (int)V, (int)D, (int)K,

@@ -1273,7 +1273,7 @@ struct Plan {
 };
 constexpr long long kPieceBytes = 512ll << 20;
 
-static Plan plan(long long N, long long V, long long D) {
+static Plan make_plan(long long N, long long V, long long D) {
   Plan p{};
   long long C = kPieceBytes / (2 * N) / kTN * kTN;
   if (C < kTN) C = kTN;
@@ -1300,6 +1300,20 @@ static Plan plan(long long N, long long V, long long D) {
   p.packed = up((size_t)N * D * 2);       // the packed rows, or clean_kernel's
   p.total = p.g + p.dh + p.dw + p.packed;
   return p;
+}
+
+// The search over splits takes a few microseconds, a call's check and its launches each want the
+// plan: every thread keeps those of the last sizes.
+static const Plan& plan(long long N, long long V, long long D) {
+  struct Entry { long long N, V, D; Plan p; };
+  static thread_local Entry seen[8] = {};
+  static thread_local int at = 0;
+  for (const Entry& e : seen)
+    if (e.N == N && e.V == V && e.D == D) return e.p;
+  Entry& e = seen[at];
+  at = (at + 1) % 8;
+  e = {N, V, D, make_plan(N, V, D)};
+  return e.p;
 }
 
 // Places of a row's K entries: a multiple of four, for the loads of four.
@@ -1463,7 +1477,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
   int rc = make_context_current();
   if (rc) return rc;
   const int N = q.N, V = q.V, D = q.D;
-  const Plan p = plan(N, V, D);
+  const Plan& p = plan(N, V, D);
   char* g = kp.g ? (char*)kp.g : (char*)ws;
   float* dh = (float*)((char*)ws + p.g);
   float* dw = (float*)((char*)ws + p.g + p.dh);
@@ -1492,7 +1506,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
   for (int i = 0; i < p.pieces; ++i) {
     const long long v0 = i * p.C;
     const int cols = (int)(V - v0 < p.C ? V - v0 : p.C);
-    if ((rc = map_load(&mg, g, N, cols, p.C)) || (rc = map_store(&mgo, g, false, 1, N, cols, p.C))) return rc;
+    if ((rc = map_load(&mg, g, N, cols, p.C)) || (!kp.g && (rc = map_store(&mgo, g, false, 1, N, cols, p.C)))) return rc;
     Args a{};
     a.n_rows = N;
     a.M = few ? cols : N;
