@@ -114,7 +114,7 @@ extern "C" {
 
 const char* lh_last_error(void) { return g_err; }
 
-int lh_abi_version(void) { return 100; }
+int lh_abi_version(void) { return 101; }
 
 int lh_device_status(int reset) { return attn_status(reset) | loss_status(reset); }
 

@@ -4,8 +4,11 @@
 ``F.cross_entropy(hidden @ weight.T, target)`` and ``linear_distillation`` the
 divergence from a teacher's top logits, both with gradients for hidden and
 weight.  The logits live in tensor memory, tile by tile; the backward forms them
-again and goes over the vocabulary in pieces, so that memory beyond the inputs
-and gradients stays at about half a gigabyte whatever the vocabulary is.
+again and goes over the vocabulary in pieces, so that beyond the inputs, the
+gradients and a copy of hidden it takes about half a gigabyte whatever the
+vocabulary is.  Between the two a reduced loss over at most 256 entries keeps 512
+bytes per position (the softmax less the targets); otherwise 20 bytes, and 8 per
+teacher entry.
 
 hidden (..., D) and weight (V, D) are bf16 CUDA tensors, D a multiple of 8.
 Logits, softmax statistics and losses are fp32, gradients bf16.

@@ -497,6 +497,22 @@ def test_same_results_every_time_on_a_stream_and_in_a_graph(lh, cuda):
     assert lh._native.device_status() == 0
 
 
+@pytest.mark.parametrize("V", [8, 64, 300])
+def test_offsets_past_32_bits(lh, cuda, V):
+    """Hidden states of 2.2e9 elements, of which the last rows count (not packed, packed, more than one tile)."""
+    N, D, n = 270000, 8192, 500
+    g, last, w = _problem(n, V, D, 71, cuda)
+    h = torch.full((N, D), float("nan"), dtype=BF, device=cuda)
+    h[-n:] = last
+    target = torch.full((N,), -100, device=cuda)
+    t = target[-n:] = torch.randint(0, V, (n,), generator=g).to(cuda)
+    loss, dh, dw = _xent(lh, h, w, target, "mean")
+    assert all((c == 0).all() for c in dh[:-n].split(50000))
+    one = torch.ones(n, 1, dtype=torch.float64, device=cuda)
+    _check(loss, dh[-n:], dw, last, w, t[:, None], one, one[:, 0] > 0, torch.full((n,), 1.0 / n, device=cuda), 1.0, "mean")
+    assert lh._native.device_status() == 0
+
+
 @pytest.mark.parametrize("N,V,D", [(600, 200, 64), (40, 3001, 64), (300, 3001, 64), BIG])
 def test_a_replayed_graph_follows_its_inputs(lh, cuda, N, V, D):
     """Other hidden states, targets and numbers of ignored positions, whose rows hold NaN, in every replay."""
