@@ -230,3 +230,32 @@ def test_opcheck(lh, cuda):
     torch.library.opcheck(ops.add_rms_norm_bwd, (y, h, h, w, rstd, BF), test_utils=U_)
     torch.library.opcheck(ops.add_rms_norm_bwd, (y, None, h, w, rstd, BF), test_utils=U_)
     torch.library.opcheck(ops.rms_norm_bwd, (y, x, w, rstd), test_utils=U_)
+
+
+@pytest.mark.parametrize("N,D", [(270000, 8192), (11000000, 200)])
+def test_offsets_past_32_bits(lh, cuda, N, D):
+    """The last rows of 2.2e9 elements: what a call with those rows alone gives."""
+    n = 300
+    x, r, w = _inputs(n, D, BF, BF, F32, 5, cuda)
+    dy = torch.randn(n, D, generator=torch.Generator().manual_seed(2)).to(BF).to(cuda)
+
+    def at_the_end(t):
+        big = torch.zeros(N, D, dtype=t.dtype, device=cuda)
+        big[-n:] = t
+        return big
+
+    def run(x, r, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, r, w)]
+        y, h = lh.add_rms_norm(*leaves)
+        return [t.detach()[-n:].clone() for t in (y, h)], torch.autograd.grad((y, h), leaves, (dy, dy))
+
+    small, (dx, dr, dw) = run(x, r, dy)
+    big, (bx, br, bw) = run(at_the_end(x), at_the_end(r), at_the_end(dy))
+    assert all(torch.equal(a, b) for a, b in zip(small, big))
+    assert torch.equal(dx, bx[-n:]) and torch.equal(dr, br[-n:])
+    h, rstd, _ = _ref(x, r, w)
+    _assert_within(bw, dw.double(), 2 * (n + 50) * U * (dy.double() * h * rstd).abs().sum(0), "dw")
+    del bx, br, big
+    q = lh.add_rms_norm_fp8(at_the_end(x), at_the_end(r), w, group=128)
+    assert all(torch.equal(a[-n:].view(torch.uint8), b.view(torch.uint8)) for a, b in
+               zip(q, lh.add_rms_norm_fp8(x, r, w, group=128)))
