@@ -13,7 +13,8 @@
 // Backward, in pieces of the vocabulary of C columns: the logits again, their
 // epilogue writing G (N, C) in bf16; then dH += G W_piece and dW_piece = G^T H.
 // G is rounded to bf16 once, as an operand of bf16 MMAs has to be; its relative
-// error of 2^-9 is that of the bf16 gradients it ends in.  All sums are fp32.
+// error of up to 2^-8 is that of the bf16 gradients it ends in (up to 32 rows: two
+// terms, 2^-16).  All sums are fp32.
 // Where the loss is reduced, c is the same for all rows: G / c is what is rounded, and
 // dH and dW are multiplied by c in fp32.  The targets' entries, the largest ones, are
 // then near -1, which bf16 holds, where G's would all be off by c's own rounding (434 x
@@ -71,6 +72,12 @@ enum Out { kOutBf16, kOutPlane, kOutPlaneAdd };
 // columns of dH) and its kFew columns are rows of hidden, so that the MMAs do an eighth
 // of the work and the stages hold weights, which are what has to be read.
 constexpr int kFew = 64;
+// Up to kTwo rows, G is the sum of two bf16 terms, the second one's rows kTwo behind: a gradient
+// that comes from a handful of entries would be off as a whole by the rounding of one (a row's
+// dH and dW by up to 2^-8), where over many rows the roundings differ and cancel.  The columns
+// of the MMAs and the rows of a K step are there anyway (16 x 32000 x 4096, forward and backward:
+// 243 us, 234 with one term; 32 x 128000 x 2048: 426, 421).
+constexpr int kTwo = kFew / 2;
 // A stage holds two steps of 64: its eight MMAs are issued without a stop, as each wait for a
 // stage and each commit of one leaves the tensor pipe empty for about 100 cycles, whatever waits
 // (4096 x 32000 x 4096, forward: 790 us with six stages of one step, 830 with a wait or a commit
@@ -128,6 +135,7 @@ struct Args {
   const float* lse2;              // kGrad: log2-sum-exp2 of s a2
   const float *gout, *row_scale, *inv_count;       // gout NULL: c is row_scale (kGrad), or 1 (kDH, kDW)
   float cscale;
+  int two;                        // few rows: G has two terms
   void* few_out;                  // few rows: G (bf16, few_pitch), or the planes (fp32) or dH (bf16) of kDH
   long long few_pitch;
 };
@@ -285,7 +293,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       // (The whole warp runs this role and the next one, one lane of it issues: with a single lane in a
       // branch the operands of each copy and MMA pass through vector registers; 1 to 3 % of the time.)
       const CUtensorMap* mapA = kAMn || MODE == kDH || !sched.packed ? &tmA : &tmP;
-      const CUtensorMap* mapB = MODE == kDW && (sched.packed || (a.dirty && *a.dirty)) ? &tmP : &tmB;
+      const CUtensorMap* mapB = MODE == kDW && (sched.packed || a.two || (a.dirty && *a.dirty)) ? &tmP : &tmB;
       uint32_t it = 0;
       bool ok = true;
       for (int t = pair; t < total && ok; t += n_pairs) {
@@ -411,32 +419,43 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const bool ok = mbar_wait(&sm->acc_full[b], (li >> 1) & 1, abort);
         if (__any_sync(~0u, !ok)) break;
         tc_fence_after();
-        uint32_t x[32];
+        uint32_t x[32], y[32];
         tmem_ld32(acc0 + b * kCols, x);
+        const bool two = MODE == kDH && a.two;           // the other half's columns are the same rows' other term
+        if (two) tmem_ld32(acc0 + b * kCols + (half ? -kTwo : kTwo), y);
         tmem_ld_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_leader(b ? acc_empty1 : acc_empty0);
-        if (left <= 0 || rows <= 0) continue;
+        if (left <= 0 || (rows <= 0 && !two)) continue;
         if constexpr (MODE == kDH) {
+          const int row0 = two ? 0 : half * 32;
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            if (e < rows && lane < left) {
-              const size_t at = (size_t)(half * 32 + e) * a.M + v0 + lane;
+            if (two) x[e] = __float_as_uint(__uint_as_float(x[e]) + __uint_as_float(y[e]));
+            if ((two ? e < a.N && e / 16 == half : e < rows) && lane < left) {
+              const size_t at = (size_t)(row0 + e) * a.M + v0 + lane;
               const float d = alpha == 0.f ? 0.f : alpha * __uint_as_float(x[e]);
               if (a.out == kOutBf16) reinterpret_cast<__nv_bfloat16*>(a.few_out)[at] = __float2bfloat16_rn(d);
               else reinterpret_cast<float*>(a.few_out)[(size_t)split * a.N * a.M + at] = d;
             }
           }
         } else {
+          auto put_g = [&](int e, float v) {             // G of row e
+            __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(a.few_out) + (half * 32 + e) * a.few_pitch + v0 + lane;
+            const __nv_bfloat16 first = __float2bfloat16_rn(v);
+            *g = first;
+            const float rest = v - __bfloat162float(first);      // not a number where v is infinite
+            if (a.two) g[kTwo * a.few_pitch] = __float2bfloat16_rn(fabsf(v) < INFINITY && fabsf(rest) < INFINITY ? rest : 0.f);
+          };
           // dense part
           if constexpr (MODE == kGrad) {
-            __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(a.few_out) + (size_t)half * 32 * a.few_pitch + v0 + lane;
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               const float ce = __shfl_sync(~0u, c, e), le = __shfl_sync(~0u, lse2, e);
-              if (e < rows && lane < left)
-                g[e * a.few_pitch] = __float2bfloat16_rn(ce == 0.f ? 0.f : ce * ex2(fmaf(__uint_as_float(x[e]), a.a2, -le)));
+              // (rows up to kTwo that are none are zeros: kDW's step takes them)
+              if ((e < rows || a.two) && lane < left)
+                put_g(e, e >= rows || ce == 0.f ? 0.f : ce * ex2(fmaf(__uint_as_float(x[e]), a.a2, -le)));
             }
           }
           // the rows' targets among these weights
@@ -460,9 +479,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                 if (lane == at) {
                   const size_t kept = (size_t)(half * 32 + e) * a.K + k;
                   if constexpr (MODE == kStats) a.slog[kept] = __uint_as_float(x[e]);
-                  else if (ce != 0.f)
-                    reinterpret_cast<__nv_bfloat16*>(a.few_out)[(half * 32 + e) * a.few_pitch + v0 + lane] =
-                        __float2bfloat16_rn(ce * a.gval[kept]);
+                  else if (ce != 0.f) put_g(e, ce * a.gval[kept]);
                 }
               }
             }
@@ -903,15 +920,17 @@ pack_kernel(const uint4* hidden, const int* rows, int N, int chunks, uint4* out)
   }
 }
 
-// hidden with zeros in the rows that do not count, where one of those is not finite.
+// hidden with zeros in the rows that do not count, where one of those is not finite.  With
+// two: in any case, and up to kTwo rows, twice.
 __global__ void __launch_bounds__(256)
-clean_kernel(const uint4* hidden, const float* row_scale, const int* dirty, int N, int chunks, uint4* out) {
+clean_kernel(const uint4* hidden, const float* row_scale, const int* dirty, int N, int chunks, int two, uint4* out) {
   after_previous();
-  if (*dirty == 0) return;
-  const int lane = threadIdx.x & 31;
-  for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < N; j += gridDim.x * 8) {
-    const bool yes = row_scale[j] != 0.f;
-    const uint4* h = hidden + (size_t)j * chunks;
+  if (!two && *dirty == 0) return;
+  const int lane = threadIdx.x & 31, rows = two ? 2 * kTwo : N;
+  for (int j = blockIdx.x * 8 + (threadIdx.x >> 5); j < rows; j += gridDim.x * 8) {
+    const int row = two ? j % kTwo : j;
+    const bool yes = row < N && row_scale[row] != 0.f;
+    const uint4* h = hidden + (size_t)row * chunks;
     uint4* o = out + (size_t)j * chunks;
     for (int c = lane; c < chunks; c += 32) o[c] = yes ? h[c] : make_uint4(0, 0, 0, 0);
   }
@@ -1268,7 +1287,7 @@ struct Plan {
   long long C;                 // columns of a vocabulary piece, a multiple of 256
   int pieces, dh_splits, dw_splits;
   uint8_t split_of[kSplitTable];
-  bool dh_planes, pack;
+  bool dh_planes, pack, two;
   size_t g, dh, dw, packed, total;     // bytes
 };
 constexpr long long kPieceBytes = 512ll << 20;
@@ -1294,10 +1313,12 @@ static Plan make_plan(long long N, long long V, long long D) {
     if (p.split_of[t] > p.dh_splits) p.dh_splits = p.split_of[t];
   p.dw_splits = pick_splits(cols, D, N);
   p.dh_planes = pack || p.pieces > 1 || p.dh_splits > 1;
-  p.g = up((size_t)N * p.C * 2);
+  p.two = N <= kTwo;
+  const long long rows = p.two ? 2 * kTwo : N;
+  p.g = up((size_t)rows * p.C * 2);
   p.dh = p.dh_planes ? up((size_t)p.dh_splits * N * D * 4) : 0;
   p.dw = p.dw_splits > 1 ? up((size_t)p.dw_splits * p.C * D * 4) : 0;
-  p.packed = up((size_t)N * D * 2);       // the packed rows, or clean_kernel's
+  p.packed = up((size_t)rows * D * 2);    // the packed rows, or clean_kernel's
   p.total = p.g + p.dh + p.dw + p.packed;
   return p;
 }
@@ -1490,23 +1511,24 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
   mp = mh;
   // few rows: always one piece (kFew rows of 2^22 columns take 512 MB)
   const bool few = N <= kFew;
+  const int g_rows = p.two ? 2 * kTwo : N;
   CUtensorMap mh_few, mg_few;
-  if (few && ((rc = map_load(&mh_few, q.hidden, N, D, D, kFew / 2)) || (rc = map_load(&mg_few, g, N, V, p.C, kFew / 2))))
+  if (few && ((rc = map_load(&mh_few, q.hidden, N, D, D, kFew / 2)) || (rc = map_load(&mg_few, g, g_rows, V, p.C, kFew / 2))))
     return rc;
   const int* rows = nullptr;
   if (p.pack) {                      // kGrad's operand too
     rows = kp.rows;
     rc = pack_rows(q.hidden, rows, N, D, packed, st);
   } else if (dweight) {
-    const unsigned blocks = (unsigned)((N + 7) / 8);
+    const unsigned blocks = (unsigned)((g_rows + 7) / 8);
     rc = launch_behind("clean_kernel", clean_kernel, blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st, (const uint4*)q.hidden,
-                       kp.row_scale, kp.dirty, N, D / 8, (uint4*)packed);
+                       kp.row_scale, kp.dirty, N, D / 8, (int)p.two, (uint4*)packed);
   }
-  if (rc || (rc = map_load(&mp, packed, N, D, D))) return rc;
+  if (rc || (rc = map_load(&mp, packed, g_rows, D, D))) return rc;
   for (int i = 0; i < p.pieces; ++i) {
     const long long v0 = i * p.C;
     const int cols = (int)(V - v0 < p.C ? V - v0 : p.C);
-    if ((rc = map_load(&mg, g, N, cols, p.C)) || (!kp.g && (rc = map_store(&mgo, g, false, 1, N, cols, p.C)))) return rc;
+    if ((rc = map_load(&mg, g, g_rows, cols, p.C)) || (!kp.g && (rc = map_store(&mgo, g, false, 1, N, cols, p.C)))) return rc;
     Args a{};
     a.n_rows = N;
     a.M = few ? cols : N;
@@ -1514,6 +1536,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     a.splits = 1;
     a.few_out = g;
     a.few_pitch = p.C;
+    a.two = p.two;
     a.rows = rows;
     a.b_off = (int)v0;
     a.target = q.target;
@@ -1545,6 +1568,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
       x.splits = p.dh_splits < kb ? p.dh_splits : kb;      // a short last piece may leave planes as they are
       for (int t = 0; t < kSplitTable; ++t) x.split_of[t] = p.split_of[t];
       scaled(x);
+      x.two = p.two;
       x.rows = rows;
       x.b_off = (int)v0;
       x.out = !p.dh_planes ? kOutBf16 : i ? kOutPlaneAdd : kOutPlane;
@@ -1560,6 +1584,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     y.N = D;
     y.splits = p.dw_splits;
     scaled(y);
+    y.two = p.two;
     y.rows = rows;
     y.dirty = rows ? nullptr : kp.dirty;
     y.out = p.dw_splits > 1 ? kOutPlane : kOutBf16;
@@ -1567,7 +1592,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     if ((rc = p.dw_splits > 1 ? map_store(&mdw, dw, true, p.dw_splits, cols, D, D)
                               : map_store(&mdw, dw_out, false, 1, cols, D, D)))
       return rc;
-    if ((rc = launch<kDW, false>(mg, mh, mdw, mp, y, N, st))) return rc;
+    if ((rc = launch<kDW, false>(mg, mh, mdw, mp, y, g_rows, st))) return rc;
     if (p.dw_splits > 1 && (rc = sum_planes(dw, nullptr, p.dw_splits, cols, D, nullptr, dw_out, st))) return rc;
   }
   return dhidden && p.dh_planes ? sum_planes(dh, &p, p.dh_splits, N, D, rows, dhidden, st) : LH_OK;
