@@ -187,6 +187,12 @@ __device__ __forceinline__ bool pair_all(int id, bool v) {
   return r;
 }
 
+// A row's sum of exponentials is relative to 2^scaled(m, a2), m its maximum so far: where the
+// maximum moves, the sum is multiplied by 2^(scaled(old) - scaled(new)), which is one where it
+// stays.  (With the unrounded m a2 in the place of one of the two, every join would multiply the
+// sum by the rounding of m a2 once more: 1e-5 of a row whose largest logit is 20, 7e-5 at 90.)
+__device__ __forceinline__ float scaled(float m, float a2) { return m == -INFINITY ? 0.f : __fmul_rn(m, a2); }
+
 // 32 values per lane, one per column -> in lane e the result of column e over the warp.
 template <class Op>
 __device__ __forceinline__ float reduce_columns(float (&v)[32], int lane, Op op) {
@@ -496,8 +502,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = lane < left ? __uint_as_float(x[e]) : -INFINITY;
             const float mn = fmaxf(mx, reduce_columns(v, lane, [](float p, float q) { return fmaxf(p, q); }));
-            const float mb = mn == -INFINITY ? 0.f : mn * a.a2;
-            sum *= mx == -INFINITY ? 0.f : ex2(fmaf(mx, a.a2, -mb));
+            const float mb = scaled(mn, a.a2);
+            sum *= mx == -INFINITY ? 0.f : ex2(scaled(mx, a.a2) - mb);
             mx = mn;
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
@@ -645,8 +651,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             for (int e = 0; e < 32; e += 2)
               mp[(e >> 1) & 3] = fmax3(mp[(e >> 1) & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
             const float mn = fmaxf(fmaxf(mx, fmaxf(mp[0], mp[1])), fmaxf(mp[2], mp[3]));
-            const float mb = mn == -INFINITY ? 0.f : mn * a.a2;
-            sum *= mx == -INFINITY ? 0.f : ex2(fmaf(mx, a.a2, -mb));
+            const float mb = scaled(mn, a.a2);
+            sum *= mx == -INFINITY ? 0.f : ex2(scaled(mx, a.a2) - mb);
             mx = mn;
             float2 sp[4];
 #pragma unroll
@@ -670,10 +676,10 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             pair_sync(1 + quad);
             const float2 o = reinterpret_cast<const float2*>(sO + (quad + 4 * (1 - half)) * kOutBuf)[lane];
             pair_sync(1 + quad);
-            const float top = fmaxf(mx, o.x), tb = top == -INFINITY ? 0.f : top * a.a2;
-            const float all = (mx == -INFINITY ? sum : sum * ex2(fmaf(mx, a.a2, -tb))) +
-                              (o.x == -INFINITY ? o.y : o.y * ex2(fmaf(o.x, a.a2, -tb)));
-            lse2 = fmaf(top, a.a2, log2f(all));
+            const float top = fmaxf(mx, o.x), tb = scaled(top, a.a2);
+            const float all = (mx == -INFINITY ? sum : sum * ex2(scaled(mx, a.a2) - tb)) +
+                              (o.x == -INFINITY ? o.y : o.y * ex2(scaled(o.x, a.a2) - tb));
+            lse2 = tb + log2f(all);
             if constexpr (SPARSE) {
               if (live && cols > 0) first();
             } else if (live && cols > 0) {
@@ -974,10 +980,9 @@ finish_kernel(const FinishArgs a) {
   const bool live = j < (a.rows ? a.rows[0] : N);
   const int row = a.rows && live ? a.rows[1 + j] : j;
   auto join = [&](float2 u, float2 v) {
-    const float mn = fmaxf(u.x, v.x);
-    const float mb = mn == -INFINITY ? 0.f : mn * a.a2;
-    return make_float2(mn, (u.x == -INFINITY ? u.y : u.y * ex2(fmaf(u.x, a.a2, -mb))) +
-                               (v.x == -INFINITY ? v.y : v.y * ex2(fmaf(v.x, a.a2, -mb))));
+    const float mn = fmaxf(u.x, v.x), mb = scaled(mn, a.a2);
+    return make_float2(mn, (u.x == -INFINITY ? u.y : u.y * ex2(scaled(u.x, a.a2) - mb)) +
+                               (v.x == -INFINITY ? v.y : v.y * ex2(scaled(v.x, a.a2) - mb)));
   };
   float2 st = make_float2(-INFINITY, 0.f);
   if (live) {
@@ -1023,29 +1028,30 @@ finish_kernel(const FinishArgs a) {
       if (t >= 0 && t < a.V) a.slog[row] = sum / a.up;
     }
   }
-  const float2 all = sh[r];
-  const float l2 = fmaf(all.x, a.a2, log2f(all.y));
+  // lse2 = top + rest; a loss takes its logit off top first, so that what is left of a row with one
+  // large logit does not carry lse2's rounding
+  const float top = scaled(sh[r].x, a.a2), rest = log2f(sh[r].y), l2 = top + rest;
   float loss = 0.f, scale = 0.f;
   if constexpr (SPARSE) {
     // the entries of a row by the threads of consecutive numbers, which read them together
-    __shared__ float lse_sh[RB];
-    if (slot == 0) lse_sh[r] = l2;
+    __shared__ float2 lse_sh[RB];
+    if (slot == 0) lse_sh[r] = make_float2(top, rest);
     __syncthreads();
     const int r2 = tid / a.slots, k0 = tid % a.slots, j2 = blockIdx.x * RB + r2;
     float x = 0.f;
     if (j2 < (a.rows ? a.rows[0] : N)) {
       const size_t row0 = (size_t)(a.rows ? a.rows[1 + j2] : j2) * K;
       const int* idx = a.idx + row0;
-      const float lr = lse_sh[r2];
+      const float2 lr = lse_sh[r2];
       for (int k = k0; k < K; k += a.slots) {
         const int me = idx[k];
         if (me == kNone) break;
-        const float s = a.slog[row0 + k], p = a.prob[row0 + k];
-        if (p > 0.f) x = fmaf(p, (lr - s * a.a2) * kLn2, x);
+        const float p = a.prob[row0 + k], q = fmaf(-a.slog[row0 + k], a.a2, lr.x) + lr.y;   // -log2 of the student's
+        if (p > 0.f) x = fmaf(p, q * kLn2, x);
         float same = p;                            // entries with the same index add up
         for (int i = k - 1; i >= 0 && idx[i] == me; --i) same += a.prob[row0 + i];
         for (int i = k + 1; i < K && idx[i] == me; ++i) same += a.prob[row0 + i];
-        a.slog[row0 + k] = ex2(fmaf(s, a.a2, -lr)) - same;
+        a.slog[row0 + k] = ex2(-q) - same;
       }
     }
     sh[tid].x = x;                                 // sh was last read before the last __syncthreads
@@ -1063,8 +1069,9 @@ finish_kernel(const FinishArgs a) {
     if (t != a.ignore) {
       const bool in = t >= 0 && t < a.V;
       scale = in ? 1.f : __int_as_float(0x7fc00000);
-      loss = in ? (l2 - a.slog[row] * a.a2) * kLn2 : scale;
-      if (in) a.slog[row] = ex2(fmaf(a.slog[row], a.a2, -l2)) - 1.f;
+      const float q = in ? fmaf(-a.slog[row], a.a2, top) + rest : scale;      // -log2 of the target's probability
+      loss = q < 0.f ? 0.f : q * kLn2;             // a rounding may leave it below zero
+      if (in) a.slog[row] = ex2(-q) - 1.f;
     }
     a.row_scale[row] = scale;
   }

@@ -575,3 +575,48 @@ def test_opcheck(lh, cuda):
         torch.library.opcheck(ops.linear_distill, (h, w, tv, ti, 2.0, red), test_utils=utils)
         loss, kept = ops.linear_distill(h, w, tv, ti, 2.0, red)
         torch.library.opcheck(ops.linear_distill_bwd, (h, w, kept, torch.ones_like(loss), 5, 2.0, red), test_utils=utils)
+
+
+@pytest.mark.parametrize("N,V", [(9, 300), (9, 15001), (80, 200), (80, 5003), (80, 15001)])
+@pytest.mark.parametrize("top", [20.625, 90.5])
+def test_one_large_logit_per_row(lh, cuda, N, V, top):
+    """Logits that fp32 holds, one of them far above the others.
+
+    Of the steps to a loss, the exponent of the largest logit is taken from its exact product with log2(e)
+    less that product's rounding; ex2 is off by 2 ulp, a sum near one passes at most 4 joins in its tile,
+    4 adds of 32 values each, and 24 joins of parts (2^-24 each): under 64 U.  log2(e) and ln 2 are off by
+    U each, so are the two products and a sum of losses at its end: 6 U of the loss."""
+    g = torch.Generator().manual_seed(N + V)
+    big = torch.randint(0, V, (N,), generator=g)
+    h = torch.zeros(N, 88)
+    h[:, :8] = torch.randint(0, 4, (N, 8), generator=g).float()
+    w = torch.zeros(V, 88)
+    w[:, :8] = torch.randint(-2, 3, (V, 8), generator=g).float() / 8
+    # channel 8 + n of row n takes its large logit to `top`, which is one of a row of its own there
+    n = torch.arange(N)
+    h[n, 8 + n] = 1.0
+    w[big] = 0
+    w[big, 8 + n] = top
+    h, w = h.to(BF).to(cuda), w.to(BF).to(cuda)
+    s = h.double() @ w.double().T
+    lse = torch.logsumexp(s, -1)
+    for t in (s.argmax(-1), s.argmin(-1)):
+        for red in ("none", "sum"):                   # "sum" of one-tile rows: the forward's gradients
+            loss, dh, dw = _xent(lh, h, w, t, red, torch.ones(N, device=cuda) if red == "none" else None)
+            want = lse - s.gather(1, t[:, None])[:, 0]
+            tol = 64 * U + 6 * U * want
+            got = loss.double()
+            assert (got >= 0).all()
+            assert ((got - (want if red == "none" else want.sum())).abs() <= (tol if red == "none" else tol.sum())).all()
+            # gradients of the same accuracy: an exponential carries the rounding of lse (U of it, and of log2(e)),
+            # the target's entry those of the loss; what is below 2^-126 may be cut
+            q, one = (s - lse[:, None]).exp(), torch.nn.functional.one_hot(t, V).double()
+            G = q - one
+            E = H8 * G.abs() + (64 * U + 2 * U * lse.abs()[:, None]) * q + 64 * U * one + 2.0 ** -126
+            hd, wd = h.double(), w.double()
+            for got, ref, err, sums in ((dh, G @ wd, E @ wd.abs(), V * 2.0 ** -23 * (G.abs() @ wd.abs())),
+                                        (dw, G.T @ hd, E.T @ hd.abs(), N * 2.0 ** -23 * (G.abs().T @ hd.abs()))):
+                tol = err + sums
+                assert ((got.double() - ref).abs() <= tol + H8 * (ref.abs() + tol)).all()
+    loss = lh.linear_distillation(h, w, torch.ones(N, 1, device=cuda), s.argmax(-1)[:, None], reduction="none")
+    assert ((loss.double() - (lse - s.amax(-1))).abs() <= 64 * U).all()
