@@ -85,6 +85,15 @@ constexpr int kTwo = kFew / 2;
 // leaves the loads too little room).  One store's staging buffer per epilogue warp: two, and a
 // step less of operands, are 1 to 2 % slower.
 constexpr int kSubs = 2;
+// Adding products the tensor core cuts the sum towards zero, which makes a logit of D products smaller by
+// about 1e-9 D of itself, by twice that where its large products come first, by nothing where they come
+// last or the sum is exact: no factor takes that out.  So the forward sums a logit in parts of kPart steps,
+// which the epilogue adds in registers, rounding to nearest; what is lost no longer grows with D.  (65536 x
+// 256 x 1024, the mean's error and the forward: 2.7e-6 and 50 us in one part, 1.3e-6 and 50 in parts of 8
+// steps, 0.9e-6 and 51 of 6, 0.6e-6 and 54 of 4, whose accumulators the epilogue does not keep up with:
+// 1999 x 50261 x 768 takes 100, 100, 100, 113 us.)  The backward's logits are one sum: their exponentials
+// are rounded to 2^-9.
+constexpr int kPart = 6;
 __host__ __device__ constexpr int stages(bool few) { return few ? 5 : 3; }
 __host__ __device__ constexpr int b_bytes(bool few) { return few ? kFew / 2 * 128 : kOpBytes; }
 constexpr int smem_bytes(bool few) {
@@ -214,6 +223,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                  const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmP,
                  const __grid_constant__ Args a) {
   // tmP: the packed rows, in the place of hidden (A of kStats and kGrad, B of kDW)
+  constexpr bool kParts = MODE == kStats || MODE == kWhole;
   constexpr bool kAMn = MODE == kDW || (FEW && MODE == kDH), kBMn = !FEW && (MODE == kDH || MODE == kDW);
   constexpr int kStages = stages(FEW), kBBytes = b_bytes(FEW);
   constexpr int kCols = FEW ? kFew : kTN;          // columns of a tile
@@ -293,8 +303,11 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     k1 = k0 + q + (split < rem ? 1 : 0);
   };
 
-  if (*abort == 0) {
-    if (warp == 0) {
+  // A thread of the epilogue holds its half row of logits: registers of warps 0-3 go there (128 x 56 +
+  // 256 x 224 are the launch's 384 x 168).
+  if (warp < 4) {
+    if constexpr (kParts && !FEW) regs_shrink<56>();
+    if (warp == 0 && *abort == 0) {
       // ---------------------------------------------------------- TMA producer
       // (The whole warp runs this role and the next one, one lane of it issues: with a single lane in a
       // branch the operands of each copy and MMA pass through vector registers; 1 to 3 % of the time.)
@@ -347,54 +360,64 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       if (rank == 0 && lane == 0)
         for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
           for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->full[i % kStages], (i / kStages) & 1); ++p) {}
-    } else if (warp == 1 && rank == 0) {
+    } else if (warp == 1 && rank == 0 && *abort == 0) {
       // ---------------------------------------------------------- MMA issuer
       constexpr uint32_t idesc = idesc_bf16_f32(kTM, kCols, kAMn, kBMn);
       uint32_t it = 0;
-      int li = 0;
+      int li = 0;                                        // accumulators so far
       bool ok = true;
       // (Looking at the next stage's barrier, or waiting for the next accumulator, before a stage's
       // MMAs are issued makes the kernel 3 to 8 % slower, not faster.)
       const int q = sched.kb / sched.splits, rem = sched.kb - q * sched.splits;
-      for (int t = pair; t < total && ok; t += n_pairs, ++li) {
+      for (int t = pair; t < total && ok; t += n_pairs) {
         const int steps = q + ((int)sched.div[0].div(t) < rem ? 1 : 0);
-        const int b = li & 1;
-        const uint32_t acc = tbase + b * kCols;
-        if (li >= 2) ok = mbar_wait(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort);
-        if (__any_sync(~0u, !ok)) break;
-        tc_fence_after();
-        for (int kg = 0; kg < steps; kg += kSubs, ++it) {
-          const int s = it % kStages;
-          ok = mbar_wait(&sm->full[s], (it / kStages) & 1, abort);
+        int from = 0;
+        do {                                             // a part, or all steps
+          const int to = kParts ? min(from + kPart, steps) : steps, b = li & 1;
+          const uint32_t acc = tbase + b * kCols;
+          if (li >= 2) ok = mbar_wait(&sm->acc_empty[b], ((li >> 1) - 1) & 1, abort);
           if (__any_sync(~0u, !ok)) { ok = false; break; }
           tc_fence_after();
-          const int n_sub = min(kSubs, steps - kg);
-          if (elect_one()) {
+          for (int kg = from; kg < to; kg += kSubs, ++it) {
+            const int s = it % kStages;
+            ok = mbar_wait(&sm->full[s], (it / kStages) & 1, abort);
+            if (__any_sync(~0u, !ok)) { ok = false; break; }
+            tc_fence_after();
+            const int n_sub = min(kSubs, to - kg);
+            if (elect_one()) {
 #pragma unroll
-            for (int u = 0; u < kSubs; ++u) {
-              if (u < n_sub) {
-                const uint32_t pa = smem_u32(sA + (s * kSubs + u) * kOpBytes), pb = smem_u32(sB + (s * kSubs + u) * kBBytes);
+              for (int u = 0; u < kSubs; ++u) {
+                if (u < n_sub) {
+                  const uint32_t pa = smem_u32(sA + (s * kSubs + u) * kOpBytes), pb = smem_u32(sB + (s * kSubs + u) * kBBytes);
 #pragma unroll
-                for (int kk = 0; kk < kTK / 16; ++kk)
-                  mma_ss_pair(acc,
-                              kAMn ? smem_desc_sw128(pa + kk * 2048, kBox, 1024) : smem_desc_sw128(pa + kk * 32, 16, 1024),
-                              kBMn ? smem_desc_sw128(pb + kk * 2048, kBox, 1024) : smem_desc_sw128(pb + kk * 32, 16, 1024),
-                              idesc, (kg + u > 0 || kk > 0) ? 1u : 0u);
+                  for (int kk = 0; kk < kTK / 16; ++kk)
+                    mma_ss_pair(acc,
+                                kAMn ? smem_desc_sw128(pa + kk * 2048, kBox, 1024) : smem_desc_sw128(pa + kk * 32, 16, 1024),
+                                kBMn ? smem_desc_sw128(pb + kk * 2048, kBox, 1024) : smem_desc_sw128(pb + kk * 32, 16, 1024),
+                                idesc, (kg + u > from || kk > 0) ? 1u : 0u);
+                }
               }
+              mma_commit_pair(&sm->empty[s]);
+              if (kg + kSubs >= to) mma_commit_pair(&sm->acc_full[b]);
             }
-            mma_commit_pair(&sm->empty[s]);
-            if (kg + kSubs >= steps) mma_commit_pair(&sm->acc_full[b]);
+            __syncwarp();
           }
+          if (steps == 0 && elect_one()) mma_commit_pair(&sm->acc_full[b]);
           __syncwarp();
-        }
-        if (steps == 0 && elect_one()) mma_commit_pair(&sm->acc_full[b]);
-        __syncwarp();
+          ++li;
+          from = to;
+        } while (ok && from < steps);
       }
       if (__any_sync(~0u, *abort) && elect_one()) {      // the MMAs issued so far end before TMEM is freed
         mma_commit_pair(&sm->drain);
         for (uint32_t p = 0; p < kSpinLimit && !mbar_try_wait(&sm->drain, 0); ++p) {}
       }
-    } else if (FEW && warp >= 4) {
+    }
+  } else {
+    if constexpr (kParts && !FEW) regs_grow<224>();
+    if (*abort != 0) {
+      // nothing to do
+    } else if constexpr (FEW) {
       // ---------------------------------------------------------- epilogue, few rows
       // TMEM lane = row of the weights (column of dH), 32 columns per warp = rows of hidden; what
       // belongs to a row of hidden is held by the lane of its number and handed out by shuffles
@@ -415,24 +438,34 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           lse2 = a.lse2[row];
         }
       }
-      int li = 0;
-      for (int t = pair; t < total; t += n_pairs, ++li) {
+      int li = 0;                                        // accumulators so far
+      const int parts = kParts ? (sched.kb + kPart - 1) / kPart : 1;
+      for (int t = pair; t < total; t += n_pairs) {
         int m, n, k0, k1, split;
         decode(t, m, n, k0, k1, split);
-        const int b = li & 1;
         const int v0 = m * kTM + rank * 128 + quad * 32;
         const int left = min(32, M - v0);                // rows of the weights, may be negative
-        const bool ok = mbar_wait(&sm->acc_full[b], (li >> 1) & 1, abort);
-        if (__any_sync(~0u, !ok)) break;
-        tc_fence_after();
-        uint32_t x[32], y[32];
-        tmem_ld32(acc0 + b * kCols, x);
         const bool two = MODE == kDH && a.two;           // the other half's columns are the same rows' other term
-        if (two) tmem_ld32(acc0 + b * kCols + (half ? -kTwo : kTwo), y);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_leader(b ? acc_empty1 : acc_empty0);
+        uint32_t x[32], y[32];
+        bool ok = true;
+        for (int p = 0; p < parts; ++p, ++li) {
+          const int b = li & 1;
+          ok = mbar_wait(&sm->acc_full[b], (li >> 1) & 1, abort);
+          if (__any_sync(~0u, !ok)) { ok = false; break; }
+          tc_fence_after();
+          if (!kParts || p == 0) tmem_ld32(acc0 + b * kCols, x);
+          else tmem_ld32(acc0 + b * kCols, y);
+          if (two) tmem_ld32(acc0 + b * kCols + (half ? -kTwo : kTwo), y);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_leader(b ? acc_empty1 : acc_empty0);
+          if (kParts && p > 0) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) + __uint_as_float(y[e]));
+          }
+        }
+        if (!ok) break;
         if (left <= 0 || (rows <= 0 && !two)) continue;
         if constexpr (MODE == kDH) {
           const int row0 = two ? 0 : half * 32;
@@ -515,7 +548,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
       }
       if (MODE == kStats && live) a.stats[(size_t)(blockIdx.x * 4 + quad) * a.n_rows + row] = make_float2(mx, sum);
-    } else if (!FEW && warp >= 4) {
+    } else {
       // ---------------------------------------------------------- epilogue
       // warps 4-7 take columns 0-127 of the tile, warps 8-11 the rest
       const int quad = warp & 3, half = warp >= 8 ? 1 : 0;
@@ -524,16 +557,14 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       uint8_t* stage = sO + (quad + 4 * half) * kOutBuf;
       const uint32_t acc_empty0 = leader_addr(&sm->acc_empty[0]), acc_empty1 = leader_addr(&sm->acc_empty[1]);
       const float alpha = (MODE == kDH || MODE == kDW) && a.gout ? upstream() : 1.f;
-      int li = 0;
+      int li = 0;                                        // accumulators so far
       // 16 bytes to chunk c of this thread's row of a staging tile (128-byte swizzle)
       auto put = [&](uint8_t* p, int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
         *reinterpret_cast<uint4*>(p + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(x, y, z, w);
       };
-      for (int t = pair; t < total; t += n_pairs, ++li) {
+      for (int t = pair; t < total; t += n_pairs) {
         int m, n, k0, k1, split;
         decode(t, m, n, k0, k1, split);
-        const int b = li & 1;
-        const uint32_t acc = lane_base + b * kTN;
         const int row0 = m * kTM + rank * 128 + quad * 32, row = row0 + lane, n0 = n * kTN + half * kHalf;
         const int cols = min(kHalf, a.N - n0);           // of this warp's half, may be negative
         const bool live = row < M;
@@ -557,7 +588,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if (MODE == kGrad || MODE == kWhole) val.open((MODE == kGrad ? a.gval : a.prob) + kept0, a.K, cur, 0.f);
           next = win.now.x == kNone ? kNone : win.now.x - g0;
         };
-        if constexpr (MODE == kStats || MODE == kWhole || MODE == kGrad) {
+        auto targets = [&]() {
           if (live && cols > 0) {
             if constexpr (SPARSE) {
               first();
@@ -576,31 +607,32 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               lse2 = a.lse2[orow];
             }
           }
-        }
-        bool ok = mbar_wait(&sm->acc_full[b], (li >> 1) & 1, abort);
-        // the two warps of a row go on together or not at all
-        if (MODE == kWhole) ok = pair_all(1 + quad, ok);
-        if (__any_sync(~0u, !ok)) break;
-        tc_fence_after();
-        auto release = [&]() {                           // the tile's TMEM has been read
+        };
+        if (MODE == kGrad) targets();
+        auto filled = [&]() {                            // the next accumulator, unless a wait gave up
+          const bool ok = mbar_wait(&sm->acc_full[li & 1], (li >> 1) & 1, abort);
+          if (__any_sync(~0u, !ok)) return false;
+          tc_fence_after();
+          return true;
+        };
+        auto release = [&]() {                           // its TMEM has been read
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_leader(b ? acc_empty1 : acc_empty0);
+          if (lane == 0) mbar_arrive_leader(li & 1 ? acc_empty1 : acc_empty0);
+          ++li;
         };
-        // c exp(s - lse) of 64 columns to the staging, in bf16; 0 for a row without a gradient, whatever
-        // its logits are
-        auto softmax_rows = [&](const uint32_t (&x)[32], const uint32_t (&y)[32], float c, float lse2) {
-          if (c == 0.f) {
+        // 64 columns of G to the staging, in bf16; zeros for a row without a gradient, whatever its logits are
+        auto g_rows = [&](bool some, auto g) {
+          if (!some) {
 #pragma unroll
             for (int ch = 0; ch < 8; ++ch) put(stage, ch, 0, 0, 0, 0);
             return;
           }
-          auto grad = [&](uint32_t u) { return c * ex2(fmaf(__uint_as_float(u), a.a2, -lse2)); };
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
-            const uint32_t* u = ch < 4 ? x + 8 * ch : y + 8 * (ch - 4);
-            put(stage, ch, pack_bf16(grad(u[0]), grad(u[1])), pack_bf16(grad(u[2]), grad(u[3])),
-                pack_bf16(grad(u[4]), grad(u[5])), pack_bf16(grad(u[6]), grad(u[7])));
+            const int e = 8 * ch;
+            put(stage, ch, pack_bf16(g(e), g(e + 1)), pack_bf16(g(e + 2), g(e + 3)), pack_bf16(g(e + 4), g(e + 5)),
+                pack_bf16(g(e + 6), g(e + 7)));
           }
         };
         auto put_at = [&](int at, float v) {             // one of the 64 columns again
@@ -616,23 +648,40 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             bulk_commit();
           }
         };
-        if constexpr (MODE == kStats || MODE == kWhole) {
-          float mx = -INFINITY, sum = 0.f, st = 0.f;     // st: the target's logit
+        if constexpr (kParts) {
+          float s[kHalf];                                // logits of this row
+#pragma unroll
+          for (int e = 0; e < kHalf; ++e) s[e] = 0.f;
+          bool ok = true;
+          for (int k = 0; k < sched.kb; k += kPart) {
+            if (!(ok = filled())) break;
+#pragma unroll
+            for (int c0 = 0; c0 < kHalf; c0 += 32) {
+              uint32_t x[32];
+              tmem_ld32(lane_base + (li & 1) * kTN + c0, x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) s[c0 + e] += __uint_as_float(x[e]);
+            }
+            release();
+            if (k == 0) targets();                       // their loads meet the wait for the next part
+          }
+          if (MODE == kWhole) ok = pair_all(1 + quad, ok);      // the two warps of a row go on together or not at all
+          if (!ok) break;
           if (MODE == kWhole) {                          // the last tile's stores have read the staging
             if (lane == 0) bulk_wait_read_all();
             __syncwarp();
           }
-#pragma unroll 1
+          float st = 0.f;                                // the target's logit
+#pragma unroll
           for (int c0 = 0; c0 < kHalf; c0 += 32) {
-            const int left = cols - c0;
-            if (left <= 0) break;
-            uint32_t x[32];
-            tmem_ld32(acc + c0, x);
-            tmem_ld_wait();
             // logits of the targets among these columns, by way of this thread's row in shared memory
             if (__any_sync(~0u, next < c0 + 32)) {
 #pragma unroll
-              for (int ch = 0; ch < 8; ++ch) put(stage, ch, x[4 * ch], x[4 * ch + 1], x[4 * ch + 2], x[4 * ch + 3]);
+              for (int ch = 0; ch < 8; ++ch) {
+                auto u = [&](int e) { return __float_as_uint(s[c0 + 4 * ch + e]); };
+                put(stage, ch, u(0), u(1), u(2), u(3));
+              }
               while (next < c0 + 32) {
                 const int at = next - c0;
                 st = *reinterpret_cast<const float*>(stage + lane * 128 + (((at >> 2) ^ (lane & 7)) << 4) + (at & 3) * 4);
@@ -641,35 +690,31 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                 else next = kNone;
               }
             }
-            if (left < 32) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (e >= left) x[e] = __float_as_uint(-INFINITY);
-            }
-            float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int e = 0; e < 32; e += 2)
-              mp[(e >> 1) & 3] = fmax3(mp[(e >> 1) & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-            const float mn = fmaxf(fmaxf(mx, fmaxf(mp[0], mp[1])), fmaxf(mp[2], mp[3]));
-            const float mb = scaled(mn, a.a2);
-            sum *= mx == -INFINITY ? 0.f : ex2(scaled(mx, a.a2) - mb);
-            mx = mn;
-            float2 sp[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) sp[u] = make_float2(0.f, 0.f);
-            const float2 a22 = make_float2(a.a2, a.a2), nb = make_float2(-mb, -mb);
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 arg = ffma2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), a22, nb);
-              sp[(e >> 1) & 3] = fadd2(sp[(e >> 1) & 3], make_float2(ex2(arg.x), ex2(arg.y)));
-            }
-            const float2 r = fadd2(fadd2(sp[0], sp[1]), fadd2(sp[2], sp[3]));
-            sum += r.x + r.y;
           }
+          if (cols < kHalf) {
+#pragma unroll
+            for (int e = 0; e < kHalf; ++e)
+              if (e >= cols) s[e] = -INFINITY;
+          }
+          // maximum of the half row, then its exponentials, which take the logits' place
+          float mp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < kHalf; e += 2) mp[(e >> 1) & 3] = fmax3(mp[(e >> 1) & 3], s[e], s[e + 1]);
+          const float mx = fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])), mb = scaled(mx, a.a2);
+          float2 sp[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) sp[u] = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < kHalf; e += 2) {
+            const float2 arg = ffma2(make_float2(s[e], s[e + 1]), make_float2(a.a2, a.a2), make_float2(-mb, -mb));
+            s[e] = ex2(arg.x);
+            s[e + 1] = ex2(arg.y);
+            sp[(e >> 1) & 3] = fadd2(sp[(e >> 1) & 3], make_float2(s[e], s[e + 1]));
+          }
+          const float2 r = fadd2(fadd2(sp[0], sp[1]), fadd2(sp[2], sp[3]));
+          const float sum = r.x + r.y;
           if (live) a.stats[(size_t)(2 * n + half) * a.n_rows + row] = make_float2(mx, sum);
-          if constexpr (MODE == kStats) {
-            release();
-          } else {
+          if constexpr (MODE == kWhole) {
             // the row's other half, then G / c = (exp(s - lse) - p) row_scale
             __syncwarp();
             reinterpret_cast<float2*>(stage)[lane] = make_float2(mx, sum);
@@ -680,23 +725,20 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             const float all = (mx == -INFINITY ? sum : sum * ex2(scaled(mx, a.a2) - tb)) +
                               (o.x == -INFINITY ? o.y : o.y * ex2(scaled(o.x, a.a2) - tb));
             lse2 = tb + log2f(all);
+            // c / sum of the exponentials; a half of -infinities only has none (NaN where the whole row has none)
+            const float f = c * (mx == -INFINITY ? 0.f * lse2 : ex2(mb - lse2));
             if constexpr (SPARSE) {
               if (live && cols > 0) first();
             } else if (live && cols > 0) {
               const long long tv = a.target[orow] - g0;
               next = tv >= 0 && tv < kHalf ? (int)tv : kNone;
             }
-#pragma unroll 1
+#pragma unroll
             for (int c0 = 0; c0 < kHalf; c0 += 64) {
-              uint32_t x[32], y[32];
-              tmem_ld32(acc + c0, x);
-              tmem_ld32(acc + c0 + 32, y);
-              tmem_ld_wait();
-              if (c0 + 64 == kHalf) release();
               if (c0 >= cols || row0 >= min(a.n_rows, (M + 63) / 64 * 64)) continue;
               if (lane == 0) bulk_wait_read_all();
               __syncwarp();
-              softmax_rows(x, y, c, lse2);
+              g_rows(c != 0.f, [&](int e) { return f * s[c0 + e]; });
               while (c != 0.f && next < c0 + 64) {
                 const int at = next;
                 float p = 1.f;
@@ -713,6 +755,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           }
         } else {
+          if (!filled()) break;
+          const uint32_t acc = lane_base + (li & 1) * kTN;
           const int width = MODE == kGrad || a.out == kOutBf16 ? 64 : 32;      // columns of one store
 #pragma unroll 1
           for (int c0 = 0; c0 < kHalf; c0 += width) {
@@ -740,7 +784,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (lane == 0) bulk_wait_read_all();
             __syncwarp();
             if constexpr (MODE == kGrad) {
-              softmax_rows(x, y, c, lse2);
+              g_rows(c != 0.f, [&](int e) { return c * ex2(fmaf(__uint_as_float(e < 32 ? x[e] : y[e - 32]), a.a2, -lse2)); });
               while (c != 0.f && next < c0 + 64) {       // the row's targets among these columns (the same one twice: twice alike)
                 put_at(next - c0, c * val.now.x);
                 if constexpr (SPARSE) advance();
@@ -961,8 +1005,6 @@ struct FinishArgs {
   float *row_scale, *lse2, *loss, *inv_count;
   double2* part;
   unsigned* ticket;
-  float up;                               // what exponent_scale() adds to log2(e) / T, as a factor
-  const __nv_bfloat16 *hidden, *weight;   // the target's logit is summed here in fp32, or NULL
   int D;
   const uint4* scan;                      // hidden: *dirty is 1 if a row that does not count is not finite
   int* dirty;                             // NULL where the rows are packed
@@ -994,39 +1036,6 @@ finish_kernel(const FinishArgs a) {
   for (int o = a.slots >> 1; o; o >>= 1) {
     if (slot < o) sh[tid] = join(sh[tid], sh[tid + o * RB]);
     __syncthreads();
-  }
-  if (!SPARSE && RB == 8 && a.hidden) {
-    // One to four warps per row sum the target's logit anew: single logits of the tensor core are
-    // off by 6e-6 at random (D = 4096), too much for the loss of one position.
-    __shared__ float dots[8][4];
-    const int w = tid >> 5, lane = tid & 31, per = blockDim.x >> 8, jj = blockIdx.x * RB + w / per;
-    float x = 0.f;
-    if (jj < (a.rows ? a.rows[0] : N)) {
-      const int rr = a.rows ? a.rows[1 + jj] : jj;
-      const long long t = a.target[rr];
-      if (t >= 0 && t < a.V) {
-        const __nv_bfloat16 *hp = a.hidden + (size_t)rr * a.D, *wp = a.weight + (size_t)t * a.D;
-#pragma unroll 4
-        for (int c = (w % per * 32 + lane) * 8; c < a.D; c += per * 256) {
-          float u[8], v[8];
-          plain16(hp + c, u);
-          plain16(wp + c, v);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x = fmaf(u[e], v[e], x);
-        }
-      }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
-    if (lane == 0) dots[w / per][w % per] = x;
-    __syncthreads();
-    if (live && slot == 0) {
-      const long long t = a.target[row];
-      // in the scale of the tensor core's logits, which the exponents take
-      float sum = 0.f;
-      for (int k = 0; k < per; ++k) sum += dots[r][k];
-      if (t >= 0 && t < a.V) a.slog[row] = sum / a.up;
-    }
   }
   // lse2 = top + rest; a loss takes its logit off top first, so that what is left of a row with one
   // large logit does not carry lse2's rounding
@@ -1402,12 +1411,8 @@ struct FwdSpace {
   }
 };
 
-// log2(e) / T, and what the tensor core's sums lose: adding a product it cuts the sum
-// towards zero, so that a logit of D products comes out smaller by 1.02e-9 D of itself on
-// average (measured 1.01 to 1.04e-9 at D from 1024 to 4096; half an ulp of the running
-// sum per 16 products makes it).  The factor takes that out of the exponents and losses:
-// the loss is then off by 1e-7 where it was by 2.5e-6 (D = 4096).
-static float exponent_scale(float T, int D) { return (float)(1.4426950408889634 / T * (1.0 + 1.02e-9 * D)); }
+// log2(e) / T: logits to exponents of 2.
+static float exponent_scale(float T) { return (float)(1.4426950408889634 / T); }
 
 static int sum_planes(const float* planes, const Plan* p, int n, int rows, int cols, const int* packed, void* out,
                       cudaStream_t st) {
@@ -1462,7 +1467,7 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
   a.target = q.target;
   a.idx = kp.idx;
   a.K = K;
-  a.a2 = exponent_scale(q.T, D);
+  a.a2 = exponent_scale(q.T);
   a.stats = ws.stats;
   a.slog = kp.tgrad;
   a.ticket = ws.ticket;
@@ -1483,16 +1488,11 @@ static int forward(const Problem& q, int reduction, float* loss, const Kept& kp,
   // 14 us with 32 rows per block, most of it the 2048 blocks' sum).
   const int want = parts > K ? parts : K;
   FinishArgs f{ws.stats, rows, parts, N, V, K, 1, reduction, q.target, q.ignore, kp.idx, ws.prob, ws.ent, kp.tgrad, a.a2,
-               q.T * q.T, kp.row_scale, kp.lse2, loss, kp.inv_count, ws.part, ws.ticket, 1.f, nullptr, nullptr, D,
+               q.T * q.T, kp.row_scale, kp.lse2, loss, kp.inv_count, ws.part, ws.ticket, D,
                (const uint4*)q.hidden, rows ? nullptr : kp.dirty};
   const int rb = want > 32 ? 8 : want > 4 ? 32 : 256;
   while (f.slots < (rb == 8 ? (want + 3) / 4 : want) && f.slots * rb < 1024) f.slots *= 2;
   if (rb == 8 && f.slots < 32) f.slots = 32;
-  if (!SPARSE && V >= 16384) {       // rb is 8; its reads, 4 N D bytes, take 2.6 % of the product's time there, less above
-    f.up = (float)(1.0 + 1.02e-9 * D);
-    f.hidden = (const __nv_bfloat16*)q.hidden;
-    f.weight = (const __nv_bfloat16*)q.weight;
-  }
   const unsigned blocks = (unsigned)((N + rb - 1) / rb);
   return launch_behind("finish_kernel", rb == 8 ? finish_kernel<SPARSE, 8> : rb == 256 ? finish_kernel<SPARSE, 256>
                                                                                    : finish_kernel<SPARSE, 32>,
@@ -1549,7 +1549,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     a.target = q.target;
     a.idx = kp.idx;
     a.K = q.K ? (int)entries(q.K) : 1;
-    a.a2 = exponent_scale(q.T, D);
+    a.a2 = exponent_scale(q.T);
     a.gval = kp.tgrad;
     a.lse2 = kp.lse2;
     a.row_scale = kp.row_scale;

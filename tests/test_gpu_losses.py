@@ -577,7 +577,7 @@ def test_opcheck(lh, cuda):
         torch.library.opcheck(ops.linear_distill_bwd, (h, w, kept, torch.ones_like(loss), 5, 2.0, red), test_utils=utils)
 
 
-@pytest.mark.parametrize("N,V", [(9, 300), (9, 15001), (80, 200), (80, 5003), (80, 15001)])
+@pytest.mark.parametrize("N,V", [(9, 300), (9, 15001), (9, 20000), (80, 200), (80, 5003), (80, 15001), (80, 20000)])
 @pytest.mark.parametrize("top", [20.625, 90.5])
 def test_one_large_logit_per_row(lh, cuda, N, V, top):
     """Logits that fp32 holds, one of them far above the others.
@@ -620,3 +620,58 @@ def test_one_large_logit_per_row(lh, cuda, N, V, top):
                 assert ((got.double() - ref).abs() <= tol + H8 * (ref.abs() + tol)).all()
     loss = lh.linear_distillation(h, w, torch.ones(N, 1, device=cuda), s.argmax(-1)[:, None], reduction="none")
     assert ((loss.double() - (lse - s.amax(-1))).abs() <= 64 * U).all()
+
+
+@pytest.mark.parametrize("N,V", [(9, 300), (9, 20000), (80, 200), (80, 300), (80, 20000)])
+@pytest.mark.parametrize("D", [520, 4096, 65536])
+def test_exact_logits_of_long_rows(lh, cuda, N, V, D):
+    """A few products per row that fp32 adds exactly, wherever in the row they are: no logit may be off.
+
+    The tolerance is that of one large logit per row: 64 U, and 6 U of the loss."""
+    g = torch.Generator().manual_seed(D + V)
+    at = torch.randperm(D, generator=g)[:24]
+    h, w = torch.zeros(N, D, dtype=BF), torch.zeros(V, D, dtype=BF)
+    h[:, at] = torch.randint(-3, 4, (N, 24), generator=g).to(BF)
+    w[:, at] = (torch.randint(-8, 9, (V, 24), generator=g) / 8).to(BF)
+    h, w = h.to(cuda), w.to(cuda)
+    s = h[:, at.to(cuda)].double() @ w[:, at.to(cuda)].double().T
+    lse = torch.logsumexp(s, -1)
+    t = torch.randint(0, V, (N,), generator=g).to(cuda)
+    for target in (t, s.argmax(-1)):
+        want = lse - s.gather(1, target[:, None])[:, 0]
+        loss = lh.linear_cross_entropy(h, w, target, reduction="none").double()
+        assert ((loss - want).abs() <= 64 * U + 6 * U * want).all()
+        loss = lh.linear_distillation(h, w, torch.zeros(N, 1, device=cuda), target[:, None], reduction="none").double()
+        assert ((loss - want).abs() <= 64 * U + 6 * U * want).all()
+        assert abs(lh.linear_cross_entropy(h, w, target).item() - want.mean().item()) <= 64 * U + 8 * U * want.mean().item()
+    assert lh._native.device_status() == 0
+
+
+@pytest.mark.parametrize("N,V", [(50, 5003), (256, 250), (256, 5003), (256, 20001)])
+@pytest.mark.parametrize("kind", ["even", "first", "last"])
+def test_sums_of_logits_are_not_cut(lh, cuda, N, V, kind):
+    """The mean error of the losses over rows of 16384 products, whose large ones lie anywhere, first or last.
+
+    A part of a sum has 24 steps of 16 products.  A step cuts half an ulp on average, U of what the part has so
+    far, which grows to the part's own sum: 12 U of the parts' sums, 12 U of a logit, in the target's and in the
+    others' mean under the softmax.  Roundings to nearest do not add up; 16 U is for those of lse."""
+    D = 16384
+    g = torch.Generator(device=cuda).manual_seed(N + V)
+    size = torch.full((D,), 0.3, device=cuda)
+    if kind == "even":
+        size[:] = 1
+    else:
+        size[:D // 64] = 8
+    if kind == "last":
+        size = size.flip(0)
+    h = torch.randn(N, D, generator=g, device=cuda) * size
+    w = torch.randn(V, D, generator=g, device=cuda) * 1.5 / D ** 0.5
+    t = torch.randperm(V, generator=g, device=cuda)[:N] if N <= V else torch.randint(0, V, (N,), generator=g, device=cuda)
+    w.index_add_(0, t, h * (4 / h.square().sum(1, keepdim=True)))
+    h, w = h.to(BF), w.to(BF)
+    s = h.double() @ w.double().T
+    lse = torch.logsumexp(s, -1)
+    st = s.gather(1, t[:, None])[:, 0]
+    loss = lh.linear_cross_entropy(h, w, t, reduction="none").double()
+    bound = 12 * U * (st.abs() + ((s - lse[:, None]).exp() * s.abs()).sum(-1)).mean() + 16 * U
+    assert abs((loss - (lse - st)).mean()) <= bound
