@@ -46,9 +46,12 @@ const char* lh_last_error(void);
 /* ABI version (major*100 + minor). */
 int lh_abi_version(void);
 
-/* 1 if an attention kernel on the current device left a bounded wait
- * (mbarrier spin limit) since the last reset, else 0.  Synchronises with the
- * device.  `reset` != 0 clears the flag. */
+/* 1 if an attention kernel or a kernel of a linear loss on the current device
+ * left a bounded wait (mbarrier spin limit) since the last reset, else 0.
+ * Until the reset, attention kernels write nothing; losses, and gradients that
+ * were not all formed, are NaN.  Synchronises with the device.  `reset` > 0
+ * clears the flags; `reset` < 0 sets the losses' one, as an expired wait would,
+ * so that a program can test what it does then. */
 int lh_device_status(int reset);
 
 /* Pyramid + norm scores.

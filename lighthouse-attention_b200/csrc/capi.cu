@@ -116,7 +116,7 @@ const char* lh_last_error(void) { return g_err; }
 
 int lh_abi_version(void) { return 101; }
 
-int lh_device_status(int reset) { return attn_status(reset) | loss_status(reset); }
+int lh_device_status(int reset) { return attn_status(reset > 0) | loss_status(reset); }
 
 int lh_pyramid_score_fwd(const void* xq, const void* xk, const void* xv, int dtype, int B, int S, int H,
                          int D, int L, int p, void* pq, void* pk, void* pv, float* sqk, float* skq,

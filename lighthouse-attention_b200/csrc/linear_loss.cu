@@ -40,7 +40,8 @@
 // K-major or MN-major as they lie in memory: no transposed copy exists.  Where a
 // product has few tiles, its K range is split and the parts meet in fp32 planes
 // which planes_kernel sums in a fixed order.
-// Every mbarrier wait is bounded; on expiry the CTAs leave and a status flag is set.
+// Every mbarrier wait is bounded; on expiry the CTAs leave and a status flag is set.  Launches that find the
+// flag set compute nothing; losses, and gradients that miss a tile, are NaN then.
 #include <cudaTypedefs.h>
 
 #include <atomic>
@@ -53,6 +54,7 @@ namespace lh {
 using namespace sm100;
 
 __device__ int g_loss_status;    // set to 1 when a bounded wait gave up
+__device__ __forceinline__ bool gave_up() { return *reinterpret_cast<volatile int*>(&g_loss_status) != 0; }
 
 namespace ll {
 
@@ -145,7 +147,7 @@ struct Args {
   const float *gout, *row_scale, *inv_count;       // gout NULL: c is row_scale (kGrad), or 1 (kDH, kDW)
   float cscale;
   int two;                        // few rows: G has two terms
-  void* few_out;                  // few rows: G (bf16, few_pitch), or the planes (fp32) or dH (bf16) of kDH
+  void* result;                   // few rows: G (bf16, few_pitch), or the planes (fp32) of kDH; kOutBf16: dH, dW
   long long few_pitch;
 };
 
@@ -273,7 +275,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     if (lane == 0) {
       if ((MODE == kStats || MODE == kWhole) && blockIdx.x == 0) { *a.ticket = 0; *a.dirty = 0; }
       // an earlier launch gave up a wait: do nothing until the host resets
-      sm->abort = *reinterpret_cast<volatile int*>(&g_loss_status) ? 2 : 0;
+      sm->abort = gave_up() ? 2 : 0;
     }
   }
   tc_fence_before();
@@ -475,13 +477,13 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if ((two ? e < a.N && e / 16 == half : e < rows) && lane < left) {
               const size_t at = (size_t)(row0 + e) * a.M + v0 + lane;
               const float d = alpha == 0.f ? 0.f : alpha * __uint_as_float(x[e]);
-              if (a.out == kOutBf16) reinterpret_cast<__nv_bfloat16*>(a.few_out)[at] = __float2bfloat16_rn(d);
-              else reinterpret_cast<float*>(a.few_out)[(size_t)split * a.N * a.M + at] = d;
+              if (a.out == kOutBf16) reinterpret_cast<__nv_bfloat16*>(a.result)[at] = __float2bfloat16_rn(d);
+              else reinterpret_cast<float*>(a.result)[(size_t)split * a.N * a.M + at] = d;
             }
           }
         } else {
           auto put_g = [&](int e, float v) {             // G of row e
-            __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(a.few_out) + (half * 32 + e) * a.few_pitch + v0 + lane;
+            __nv_bfloat16* g = reinterpret_cast<__nv_bfloat16*>(a.result) + (half * 32 + e) * a.few_pitch + v0 + lane;
             const __nv_bfloat16 first = __float2bfloat16_rn(v);
             *g = first;
             const float rest = v - __bfloat162float(first);      // not a number where v is infinite
@@ -817,6 +819,20 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     tmem_dealloc_pair(tbase, 512);
   }
   if (threadIdx.x == 0 && sm->abort) atomicExch(&g_loss_status, 1);
+  if constexpr (MODE == kDH || MODE == kDW) {
+    // this CTA's rows of its tiles (planes: planes_kernel's rows)
+    if (sm->abort && a.out == kOutBf16) {
+      __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.result);
+      for (int t = pair; t < total; t += n_pairs) {
+        int m, n, k0, k1, split;
+        decode(t, m, n, k0, k1, split);
+        for (int i = threadIdx.x; i < 128 * kCols; i += kThreads) {
+          const int r = m * kTM + rank * 128 + i / kCols, v = n * kCols + i % kCols;
+          if (r < M && v < a.N) out[FEW ? (size_t)v * a.M + r : (size_t)r * a.N + v] = __float2bfloat16_rn(__int_as_float(0x7fc00000));
+        }
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------- small kernels
@@ -1017,6 +1033,7 @@ finish_kernel(const FinishArgs a) {
   __shared__ float2 sh[1024];
   __shared__ double2 tot[32];
   __shared__ bool last;
+  const bool lost = gave_up();                     // the statistics are not there: NaN
   const int tid = threadIdx.x, r = tid % RB, slot = tid / RB, N = a.N, K = a.K;
   const int j = blockIdx.x * RB + r;
   const bool live = j < (a.rows ? a.rows[0] : N);
@@ -1071,12 +1088,13 @@ finish_kernel(const FinishArgs a) {
     }
     if (live && slot == 0) {
       scale = a.row_scale[row];
+      if (lost && scale != 0.f) a.row_scale[row] = scale = __int_as_float(0x7fc00000);
       if (scale != 0.f) loss = scale * a.t2 * (a.ent[row] + sh[r * a.slots].x);
     }
   } else if (live && slot == 0) {
     const long long t = a.target[row];
     if (t != a.ignore) {
-      const bool in = t >= 0 && t < a.V;
+      const bool in = t >= 0 && t < a.V && !lost;
       scale = in ? 1.f : __int_as_float(0x7fc00000);
       const float q = in ? fmaf(-a.slog[row], a.a2, top) + rest : scale;      // -log2 of the target's probability
       loss = q < 0.f ? 0.f : q * kLn2;             // a rounding may leave it below zero
@@ -1135,8 +1153,8 @@ finish_kernel(const FinishArgs a) {
   block_sum(s, c);
   if (tid == 0) {
     const double inv = a.reduction == LH_REDUCE_MEAN ? (c > 0 ? 1.0 / c : 0.0) : 1.0;
-    *a.loss = (float)(c > 0 ? s * inv : 0.0);
-    *a.inv_count = (float)inv;
+    *a.loss = lost ? __int_as_float(0x7fc00000) : (float)(c > 0 ? s * inv : 0.0);
+    *a.inv_count = lost ? __int_as_float(0x7fc00000) : (float)inv;
   }
 }
 
@@ -1153,6 +1171,7 @@ struct PlanesArgs {
 __global__ void __launch_bounds__(256)
 planes_kernel(const __grid_constant__ PlanesArgs a) {
   after_previous();
+  const bool lost = gave_up();
   const size_t plane = (size_t)a.n_rows * a.cols;
   const int chunks = a.cols / 8;
   int n = a.n;
@@ -1179,6 +1198,10 @@ planes_kernel(const __grid_constant__ PlanesArgs a) {
         plain16(p + k * plane + 4, u + 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += u[e];
+      }
+      if (lost) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __int_as_float(0x7fc00000);
       }
     }
     store16(a.out + i * 8, v);
@@ -1541,7 +1564,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     a.M = few ? cols : N;
     a.N = few ? N : cols;
     a.splits = 1;
-    a.few_out = g;
+    a.result = g;
     a.few_pitch = p.C;
     a.two = p.two;
     a.rows = rows;
@@ -1570,7 +1593,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
       x.n_rows = N;
       x.M = few ? D : N;
       x.N = few ? N : D;
-      x.few_out = p.dh_planes ? (void*)dh : dhidden;
+      x.result = p.dh_planes ? (void*)dh : dhidden;
       const int kb = (cols + kTK - 1) / kTK;
       x.splits = p.dh_splits < kb ? p.dh_splits : kb;      // a short last piece may leave planes as they are
       for (int t = 0; t < kSplitTable; ++t) x.split_of[t] = p.split_of[t];
@@ -1596,6 +1619,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     y.dirty = rows ? nullptr : kp.dirty;
     y.out = p.dw_splits > 1 ? kOutPlane : kOutBf16;
     char* dw_out = (char*)dweight + (size_t)v0 * D * 2;
+    y.result = dw_out;
     if ((rc = p.dw_splits > 1 ? map_store(&mdw, dw, true, p.dw_splits, cols, D, D)
                               : map_store(&mdw, dw_out, false, 1, cols, D, D)))
       return rc;
@@ -1654,7 +1678,7 @@ int linear_distill_bwd(const void* hidden, const void* weight, int N, int V, int
 int loss_status(int reset) {
   int h = 0;
   cudaMemcpyFromSymbol(&h, g_loss_status, sizeof(int));
-  if (reset) { int z = 0; cudaMemcpyToSymbol(g_loss_status, &z, sizeof(int)); }
+  if (reset) { const int z = reset < 0; cudaMemcpyToSymbol(g_loss_status, &z, sizeof(int)); }
   return h;
 }
 

@@ -675,3 +675,50 @@ def test_sums_of_logits_are_not_cut(lh, cuda, N, V, kind):
     loss = lh.linear_cross_entropy(h, w, t, reduction="none").double()
     bound = 12 * U * (st.abs() + ((s - lse[:, None]).exp() * s.abs()).sum(-1)).mean() + 16 * U
     assert abs((loss - (lse - st)).mean()) <= bound
+
+
+@pytest.fixture
+def gave_up(lh, cuda):
+    """Sets the losses' status flag from the host, as a wait that gives up would; clears it in the end."""
+    assert lh._native.device_status() == 0
+    yield lambda: lh._native.load().lh_device_status(-1)
+    lh._native.device_status()
+    assert lh._native.device_status() == 0
+
+
+@pytest.mark.parametrize("N,V,D", [(16, 300, 64), (16, 20000, 512), (60, 3001, 64), (300, 200, 64), (300, 3001, 72),
+                                   (20000, 17, 64), (5000, 120001, 64), BIG])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("loss_kind", ["xent", "distill"])
+def test_a_wait_that_gave_up_shows_in_losses_and_gradients(lh, cuda, gave_up, N, V, D, reduction, loss_kind):
+    """NaN in the place of what memory held before: few rows, one tile, parts and pieces of dH and dW, packed rows."""
+    g, h, w = _problem(N, V, D, 80, cuda)
+    t = torch.randint(0, V, (N,), generator=g)
+    t[::3] = -100
+    counts = (t != -100).to(cuda)
+    tv, ti = torch.randn(N, 1, generator=g).to(cuda), t.clamp(min=-1)[:, None].to(cuda)
+    t = t.to(cuda)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+
+    def forward():
+        if loss_kind == "xent":
+            return lh.linear_cross_entropy(h, w, t, reduction=reduction)
+        return lh.linear_distillation(h, w, tv, ti, reduction=reduction)
+
+    def backward(loss):
+        return torch.autograd.grad(loss, (h, w), torch.ones_like(loss), retain_graph=True)
+
+    good = forward()
+    want = [x.clone() for x in (good.detach(), *backward(good))]
+    gave_up()
+    dh, dw = backward(good)                              # of a sound forward
+    assert dw.isnan().all() and dh[counts].isnan().all()
+    bad = forward()
+    assert (bad[counts] if reduction == "none" else bad).isnan().all()
+    dh, dw = backward(bad)
+    assert dw.isnan().all() and dh[counts].isnan().all()
+    assert lh._native.device_status() == 1               # cleared; what the forward kept is no less lost
+    dh, dw = backward(bad)
+    assert dw.isnan().all() and dh[counts].isnan().all()
+    again = forward()
+    assert all(torch.equal(a, b) for a, b in zip(want, (again.detach(), *backward(again))))
