@@ -488,6 +488,17 @@ def kept_size(N: int, V: int, K: int, reduction: str) -> int:
     return load().lh_linear_loss_kept_size(N, V, K, REDUCTIONS[reduction], 1)
 
 
+def kept_bytes(N, V, K, reduction: str):
+    """kept_size as an expression, for sizes that are symbols of a traced graph: lse and scale of
+    a row, its targets' values and sorted indices, the packed rows' numbers, and G / c of one-tile
+    rows, each from a multiple of 256 bytes on (linear_loss.cu, Kept)."""
+    up = lambda n: (n + 255) // 256 * 256
+    at_least = lambda n: torch.sym_min(torch.sym_max(N - n + 1, 0), 1)       # 1 or 0, without a branch on N
+    Kp = (K + 3) // 4 * 4
+    whole = at_least(65) * up(512 * N) if V <= 256 and REDUCTIONS[reduction] else 0
+    return at_least(1) * (2 * up(4 * N) + 2 * up(4) + up(4 * N * (Kp if K else 1)) + up(4 * N * Kp) + up(8 * N + 4) + whole)
+
+
 def linear_xent_fwd(hidden, weight, target, ignore_index: int, reduction: str):
     """Softmax cross entropy of hidden (N, D) @ weight (V, D)^T against target (N) int64 ->
     (loss, kept); kept (uint8) is the backward's."""

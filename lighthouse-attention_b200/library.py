@@ -283,7 +283,7 @@ def _(x, residual, weight, eps, group):
 def _loss_fake(hidden, weight, reduction, K):
     N = hidden.shape[0]
     return (hidden.new_empty((N,) if reduction == "none" else (), dtype=torch.float32),
-            hidden.new_empty(_native.kept_size(N, weight.shape[0], K, reduction), dtype=torch.uint8))
+            hidden.new_empty(_native.kept_bytes(N, weight.shape[0], K, reduction), dtype=torch.uint8))
 
 
 @torch.library.custom_op(f"{NS}::linear_xent", mutates_args=())

@@ -722,3 +722,26 @@ def test_a_wait_that_gave_up_shows_in_losses_and_gradients(lh, cuda, gave_up, N,
     assert dw.isnan().all() and dh[counts].isnan().all()
     again = forward()
     assert all(torch.equal(a, b) for a, b in zip(want, (again.detach(), *backward(again))))
+
+
+def test_compiled_with_any_number_of_positions(lh, cuda):
+    """One graph for several numbers of positions, the results of the eager calls."""
+    g, h, w = _problem(400, 300, 64, 81, cuda)
+    t = torch.randint(0, 300, (400,), generator=g).to(cuda)
+    tv, ti = (x.to(cuda) for x in _teacher(g, 400, 300, 5))
+
+    def f(h, w, t, tv, ti):
+        return lh.linear_cross_entropy(h, w, t), lh.linear_distillation(h, w, tv, ti)
+
+    torch._dynamo.reset()
+    fn = torch.compile(f, fullgraph=True, backend="aot_eager")
+    for n in (20, 65, 400):
+        res = []
+        for call in (fn, f):
+            ls = [h[:n].detach().requires_grad_(True), w.detach().requires_grad_(True)]
+            args = (t[:n], tv[:n], ti[:n])
+            for x in (ls[0], *args):
+                torch._dynamo.mark_dynamic(x, 0)
+            loss = call(*ls, *args)
+            res.append([x.detach() for x in loss] + list(torch.autograd.grad(loss[0] + loss[1], ls)))
+        assert all(torch.equal(a, b) for a, b in zip(*res))

@@ -126,3 +126,45 @@ def test_kept_size_holds_gradients_of_one_tile_only(lh):
         for K in (0, 16):
             assert size(N, V, K, red, 1) - size(N, V, K, red, 0) == (512 * N + 255) // 256 * 256 * more
     assert size(0, 10, 0, 1, 1) == 0
+
+
+def test_kept_bytes_are_those_of_the_library(lh):
+    n = lh._native
+    for N in (0, 1, 3, 31, 64, 65, 777, 5000, 1 << 22):
+        for V in (1, 256, 257, 50261):
+            for K in (0, 1, 3, 16, 250, 256):
+                for red in ("none", "mean", "sum"):
+                    assert n.kept_bytes(N, V, K, red) == n.kept_size(N, V, K, red), (N, V, K, red)
+
+
+@pytest.mark.parametrize("V", [100, 300])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_one_graph_for_any_number_of_positions(lh, V, reduction):
+    """Losses and gradients traced with a symbolic number of positions (and of teacher entries): one
+    compilation serves them all, whatever the sizes of what is kept."""
+    compiled = []
+
+    def backend(gm, inputs):
+        compiled.append(gm)
+        return torch._dynamo.backends.debugging.aot_eager(gm, inputs)
+
+    def f(h, w, t, tv, ti):
+        a = lh.linear_cross_entropy(h, w, t, reduction=reduction)
+        b = lh.linear_distillation(h, w, tv, ti, temperature=2.0, reduction=reduction)
+        return a + b
+
+    torch._dynamo.reset()
+    fn = torch.compile(f, fullgraph=True, backend=backend)
+    for N, K in ((40, 5), (70, 6), (300, 9), (5000, 33)):
+        m = lambda *s, d=BF: torch.empty(*s, dtype=d, device="meta", requires_grad=d == BF)
+        h, w, t = m(N, 64), m(V, 64), m(N, d=torch.int64)
+        tv, ti = m(N, K, d=torch.float32), m(N, K, d=torch.int64)
+        for x in (h, t, tv, ti):
+            torch._dynamo.mark_dynamic(x, 0)
+        for x in (tv, ti):
+            torch._dynamo.mark_dynamic(x, 1)
+        loss = fn(h, w, t, tv, ti)
+        assert loss.shape == ((N,) if reduction == "none" else ())
+        dh, dw = torch.autograd.grad(loss.sum(), (h, w))
+        assert dh.shape == h.shape and dw.shape == w.shape
+    assert len(compiled) == 1
