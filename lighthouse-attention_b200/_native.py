@@ -411,6 +411,8 @@ def rms_norm_fwd(x, residual, weight, eps: float, out_dtype, group: int = 0, wit
         raise ValueError(f"rms_norm: out_dtype must be bf16, fp32 or float8_e4m3fn, got {out_dtype}")
     if group != 0 and not (fp8 and group == 128):
         raise ValueError("rms_norm: scales per row (group 0) or per 128 columns (group 128)")
+    if fp8 and with_rstd:                        # the callers that want rstd return no scales
+        raise ValueError("rms_norm: an 8-bit output is nothing without its scales: rms_norm_fp8")
     dev = _on_one_device("rms_norm", x, residual, weight)
     y = torch.empty_like(x, dtype=out_dtype, memory_format=_DENSE)
     scale = h = rstd = None

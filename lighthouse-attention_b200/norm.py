@@ -57,13 +57,19 @@ def _eager(name: str, *args):
     return None if torch.compiler.is_compiling() else getattr(_native.eager(), name)(*args)
 
 
+def _out_dtype(out_dtype: torch.dtype | None, x: torch.Tensor) -> torch.dtype:
+    if out_dtype == torch.float8_e4m3fn:
+        raise ValueError("rms_norm: an 8-bit output is nothing without its scales: rms_norm_fp8, add_rms_norm_fp8")
+    return out_dtype or x.dtype
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, out_dtype: torch.dtype | None = None):
     """x * (mean(x^2) + eps)^-1/2 * weight over the last dimension, in fp32, rounded
     once to out_dtype (default: x's type).  Differentiable in x and weight."""
     y = _eager("rms_norm", x, weight, eps, out_dtype)
     if y is not None:
         return y
-    return _RmsNormFn.apply(x, weight, float(eps), out_dtype or x.dtype)
+    return _RmsNormFn.apply(x, weight, float(eps), _out_dtype(out_dtype, x))
 
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
@@ -74,7 +80,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
     out = _eager("add_rms_norm", x, residual, weight, eps, out_dtype)
     if out is not None:
         return out
-    return _AddRmsNormFn.apply(x, residual, weight, float(eps), out_dtype or x.dtype)
+    return _AddRmsNormFn.apply(x, residual, weight, float(eps), _out_dtype(out_dtype, x))
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, group: int = 0):

@@ -67,3 +67,16 @@ def test_fake_kernels(lh):
     assert q.dtype == torch.float8_e4m3fn and s.shape == (5, 2)
     q, s, h = lh.add_rms_norm_fp8(m(5, 200), m(5, 200, d=torch.float32), m(200))
     assert s.shape == (5, 1) and h.dtype == torch.float32
+
+
+@pytest.mark.parametrize("device", ["cpu", "meta"])
+def test_an_8_bit_output_without_scales_is_refused(lh, device):
+    """rms_norm and add_rms_norm return no scales, and the codes are nothing without them."""
+    x, w = _t(2, 16).to(device), _t(16).to(device)
+    for call in (lambda: lh.rms_norm(x, w, out_dtype=torch.float8_e4m3fn),
+                 lambda: lh.add_rms_norm(x, x, w, out_dtype=torch.float8_e4m3fn)):
+        with pytest.raises(ValueError, match="scales"):
+            call()
+    if device == "cpu":
+        with pytest.raises(ValueError, match="scales"):
+            lh._native.rms_norm_fwd(x, None, w, 1e-5, torch.float8_e4m3fn)
