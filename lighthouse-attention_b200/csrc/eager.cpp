@@ -77,6 +77,14 @@ Tensor dense16(const Tensor& t) {
 }
 void* stream(at::Device dev) { return at::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
+// A saved tensor, dense and aligned again: hooks on saved tensors may give back other strides, and must not
+// give back anything else.
+Tensor unpacked(const Tensor& t, at::IntArrayRef size, at::ScalarType type, at::Device dev) {
+  TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.sizes() == size && t.scalar_type() == type && t.device() == dev,
+              "lighthouse_b200: a saved tensor came back with another shape, type or device");
+  return dense16(t);
+}
+
 // Gradients of these functions have no graph of their own: a second derivative raises.
 variable_list once(variable_list out) {
   if (at::GradMode::is_enabled()) {
@@ -133,21 +141,25 @@ struct NormFn : torch::autograd::Function<NormFn> {
     NormOut o = norm_forward(x, r, w, eps, out, 0, true);
     ctx->save_for_backward({r.defined() ? o.h : x, w, o.rstd});
     ctx->saved_data["x"] = (int64_t)x.scalar_type();
+    ctx->saved_data["h"] = (int64_t)(r.defined() ? r : x).scalar_type();
+    ctx->saved_data["w"] = (int64_t)w.scalar_type();
     ctx->saved_data["res"] = r.defined();
     ctx->set_materialize_grads(false);
     return r.defined() ? variable_list{o.y, o.h} : variable_list{o.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &h = saved[0], &rstd = saved[2];
     const auto x_type = (at::ScalarType)ctx->saved_data["x"].toInt();
     const bool res = ctx->saved_data["res"].toBool();
     const Tensor dh_in = res ? grads[1] : Tensor();
     if (!grads[0].defined())                      // only the stream's new value was used
       return once({dh_in.defined() ? dh_in.to(x_type) : Tensor(), dh_in, Tensor(), Tensor(), Tensor()});
-    const c10::cuda::CUDAGuard guard(h.device());
-    const Tensor dy = dense16(grads[0]), w = saved[1], dh = dh_in.defined() ? dense16(dh_in) : Tensor();
-    const int64_t D = h.size(-1), N = h.numel() / D;
+    const Tensor dy = dense16(grads[0]), dh = dh_in.defined() ? dense16(dh_in) : Tensor();
+    const c10::cuda::CUDAGuard guard(dy.device());
+    const int64_t D = dy.size(-1), N = dy.numel() / D;
+    const Tensor h = unpacked(saved[0], dy.sizes(), (at::ScalarType)ctx->saved_data["h"].toInt(), dy.device());
+    const Tensor w = unpacked(saved[1], {D}, (at::ScalarType)ctx->saved_data["w"].toInt(), dy.device());
+    const Tensor rstd = unpacked(saved[2], {N}, at::kFloat, dy.device());
     const Tensor dx = empty(h.sizes(), x_type, h.device());
     const Tensor dr = res ? empty(h.sizes(), h.scalar_type(), h.device()) : Tensor();
     const Tensor dw = empty({D}, w.scalar_type(), h.device());
@@ -225,15 +237,23 @@ struct LossFn : torch::autograd::Function<LossFn> {
     ctx->saved_data["K"] = K;
     ctx->saved_data["T"] = temperature;
     ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["N"] = N;
+    ctx->saved_data["V"] = V;
+    ctx->saved_data["D"] = D;
+    ctx->saved_data["kept"] = kept.numel();
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &h = saved[0], &w = saved[1], &target = saved[2], &kept = saved[3];
-    const c10::cuda::CUDAGuard guard(h.device());
-    const int64_t N = h.size(0), D = h.size(1), V = w.size(0), K = ctx->saved_data["K"].toInt();
-    const int reduction = (int)ctx->saved_data["reduction"].toInt();
     const Tensor g = grads[0].contiguous();
+    const c10::cuda::CUDAGuard guard(g.device());
+    auto number = [&](const char* name) { return ctx->saved_data[name].toInt(); };
+    const int64_t N = number("N"), V = number("V"), D = number("D"), K = number("K");
+    const int reduction = (int)number("reduction");
+    const Tensor h = unpacked(saved[0], {N, D}, at::kBFloat16, g.device());
+    const Tensor w = unpacked(saved[1], {V, D}, at::kBFloat16, g.device());
+    const Tensor target = K ? Tensor() : unpacked(saved[2], {N}, at::kLong, g.device());
+    const Tensor kept = unpacked(saved[3], {number("kept")}, at::kByte, g.device());
     // a frozen projection, or hidden states that nothing learns from: half of the gradients' products
     Tensor dh, dw;
     if (ctx->needs_input_grad(0)) dh = empty(h.sizes(), at::kBFloat16, h.device());

@@ -149,3 +149,40 @@ def test_calls_from_several_threads(lh, cuda):
         for o in res[i][1:]:
             assert all(torch.equal(a, b) for a, b in zip(o, res[i][0]))
     assert lh._native.device_status() == 0
+
+
+def _strided(t):
+    """The same values with every element at a stride of two."""
+    big = torch.empty(*t.shape, 2, dtype=t.dtype, device=t.device)
+    big[..., 0] = t
+    return big[..., 0]
+
+
+@pytest.mark.parametrize("call", ["norm", "add_norm", "xent", "distill", "xent_one_tile"])
+def test_hooks_on_saved_tensors(lh, cuda, call):
+    """Saved tensors that come back from the host, or with other strides, give the same gradients; one of
+    another type or shape is refused."""
+    x, r, w = _norm_inputs(cuda)
+    h, wt, t, tl, ti = _loss_inputs(cuda)
+    if call == "xent_one_tile":
+        wt, t = wt[:200], t % 200
+    f, ls = {"norm": (lambda a, c: lh.rms_norm(a, c), (x, w)),
+             "add_norm": (lambda a, b, c: sum(o.float() for o in lh.add_rms_norm(a, b, c)), (x, r, w)),
+             "xent": (lambda a, b: lh.linear_cross_entropy(a, b, t), (h, wt)),
+             "xent_one_tile": (lambda a, b: lh.linear_cross_entropy(a, b, t), (h, wt)),
+             "distill": (lambda a, b: lh.linear_distillation(a, b, tl, ti), (h, wt))}[call]
+    ls = _leaves(*ls)
+    y = f(*ls)
+    up = torch.randn(y.shape, generator=torch.Generator().manual_seed(3)).to(y)
+    want = torch.autograd.grad(y, ls, up)
+    with torch.autograd.graph.save_on_cpu():
+        y = f(*ls)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y, ls, up)))
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: s, _strided):
+        y = f(*ls)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(y, ls, up)))
+    for other in (lambda s: s.double(), lambda s: s[:-1]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s, other):
+            y = f(*ls)
+        with pytest.raises(RuntimeError, match="saved tensor"):
+            torch.autograd.grad(y, ls, up)
