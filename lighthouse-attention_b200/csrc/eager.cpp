@@ -72,7 +72,7 @@ Tensor empty(at::IntArrayRef size, at::ScalarType dtype, at::Device dev) {
   return at::detail::empty_cuda(size, dtype, dev, std::nullopt);
 }
 Tensor dense16(const Tensor& t) {
-  Tensor c = t.contiguous();
+  Tensor c = t.resolve_neg().contiguous();          // the bit that says minus is not in the memory
   return aligned(c) ? c : c.clone();
 }
 void* stream(at::Device dev) { return at::cuda::getCurrentCUDAStream(dev.index()).stream(); }
@@ -206,7 +206,7 @@ bool loss_case(const Tensor& h, const Tensor& w, int64_t reduction) {
          D % 8 == 0 && D >= 8 && D <= 65536 && N >= 1 && N <= most && V >= 1 && V <= most;
 }
 bool rows_case(const Tensor& t, const Tensor& h, int64_t dim) {
-  return t.defined() && t.is_cuda() && t.is_contiguous() && t.dim() == dim && t.size(0) == h.size(0) && t.device() == h.device() &&
+  return t.defined() && t.is_cuda() && t.is_contiguous() && !t.is_neg() && t.dim() == dim && t.size(0) == h.size(0) && t.device() == h.device() &&
          !t.key_set().has_any(c10::python_ks | c10::functorch_transforms_ks);
 }
 
@@ -245,7 +245,7 @@ struct LossFn : torch::autograd::Function<LossFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor g = grads[0].contiguous();
+    const Tensor g = dense16(grads[0]);
     const c10::cuda::CUDAGuard guard(g.device());
     auto number = [&](const char* name) { return ctx->saved_data[name].toInt(); };
     const int64_t N = number("N"), V = number("V"), D = number("D"), K = number("K");

@@ -186,3 +186,24 @@ def test_hooks_on_saved_tensors(lh, cuda, call):
             y = f(*ls)
         with pytest.raises(RuntimeError, match="saved tensor"):
             torch.autograd.grad(y, ls, up)
+
+
+def test_tensors_with_a_lazy_minus(lh, cuda):
+    """Inputs and upstream gradients whose minus is a bit beside the memory (what torch.imag makes of a conjugate)."""
+    x, r, w = _norm_inputs(cuda)
+    h, wt, t, tl, ti = _loss_inputs(cuda)
+    minus = torch._neg_view
+    assert torch.equal(lh.linear_distillation(h, wt, minus(tl), ti), lh.linear_distillation(h, wt, -tl, ti))
+    assert torch.equal(lh.linear_cross_entropy(minus(h), wt, t), lh.linear_cross_entropy(-h, wt, t))
+    assert torch.equal(lh.rms_norm(minus(x), w), lh.rms_norm(-x, w))
+    ls = _leaves(x, r, w)
+    up = torch.randn_like(r)
+    for a, b in ((minus(up), -up), (torch.complex(up, up).conj().imag, -up)):
+        y, s = lh.add_rms_norm(*ls, out_dtype=torch.float32)
+        got = torch.autograd.grad((y, s), ls, (a, a), retain_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(got, torch.autograd.grad((y, s), ls, (b, b))))
+    ls = _leaves(h, wt)
+    up = torch.randn(h.shape[0], device=cuda)
+    loss = lh.linear_cross_entropy(*ls, t, reduction="none")
+    got = torch.autograd.grad(loss, ls, minus(up), retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, torch.autograd.grad(loss, ls, -up)))
