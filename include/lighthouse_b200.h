@@ -255,9 +255,12 @@ int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h,
  * kept and the gradients 16-byte aligned, the workspace 256-byte.
  *
  * Bytes of workspace that the forward (backward = 0) or the backward (1) of the
- * two losses below needs; K is 0 for the cross entropy.  The backward goes over
- * the vocabulary in pieces, so that its logits' gradients take at most 512 MB (or
- * 256 columns). */
+ * two losses below needs; K is 0 for the cross entropy.
+ *   forward   N V / 16 bytes of statistics, a copy of hidden where rows are packed,
+ *             and 4 bytes per teacher entry
+ *   backward  logits' gradients of a piece of the vocabulary, at most 512 MB (or 256
+ *             columns); fp32 sums of dhidden, 4 N D bytes, twice that where rows are
+ *             packed; a copy of hidden; up to 160 MB of parts of split products */
 size_t lh_linear_loss_workspace_size(int N, int V, int D, int K, int backward);
 
 /* Bytes of `kept`, which the forward fills for the backward of the same problem.

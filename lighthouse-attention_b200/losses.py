@@ -4,11 +4,18 @@
 ``F.cross_entropy(hidden @ weight.T, target)`` and ``linear_distillation`` the
 divergence from a teacher's top logits, both with gradients for hidden and
 weight.  The logits live in tensor memory, tile by tile; the backward forms them
-again and goes over the vocabulary in pieces, so that beyond the inputs, the
-gradients and a copy of hidden it takes about half a gigabyte whatever the
-vocabulary is.  Between the two a reduced loss over at most 256 entries keeps 512
-bytes per position (the softmax less the targets); otherwise 20 bytes, and 8 per
-teacher entry.
+again and goes over the vocabulary in pieces.  Beyond the inputs and the gradients
+a call takes, while it runs,
+
+  forward   N V / 16 bytes of statistics (8 bytes per position and 128 entries)
+  backward  512 MB of logits' gradients at most (512 N from a million positions
+            on), 4 N D bytes of fp32 sums of dhidden, twice that where positions
+            are packed, and up to 160 MB of parts of products that are split
+  both      a copy of hidden's 2 N D bytes
+
+Between the two a reduced loss over at most 256 entries keeps 512 bytes per
+position (the softmax less the targets); otherwise 20 bytes, and 8 per teacher
+entry.
 
 hidden (..., D) and weight (V, D) are bf16 CUDA tensors, D a multiple of 8.
 Logits, softmax statistics and losses are fp32, gradients bf16.

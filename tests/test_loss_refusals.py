@@ -168,3 +168,16 @@ def test_one_graph_for_any_number_of_positions(lh, V, reduction):
         dh, dw = torch.autograd.grad(loss.sum(), (h, w))
         assert dh.shape == h.shape and dw.shape == w.shape
     assert len(compiled) == 1
+
+
+def test_workspace_is_what_the_documentation_says(lh):
+    size = lh._native.load().lh_linear_loss_workspace_size
+    for N in (1, 17, 64, 65, 1000, 2000, 4096, 20000, 37888, 65536, 262144, 1 << 22):
+        for V in (1, 256, 257, 5000, 50261, 131072, 1 << 20, 1 << 22):
+            tiles = (V + 255) // 256 * 256                     # a tile's statistics are whole
+            for D in (8, 512, 1024, 4096, 16384, 65536):
+                copy = 2 * max(N, 64) * D                      # up to 32 rows: two terms of 32
+                fwd = N * tiles // 16 + copy + 4 * N * 256 + 8 * N + (160 << 10)
+                assert size(N, V, D, 256, 0) <= fwd, (N, V, D)
+                sums = 8 * N * D + 160e6
+                assert size(N, V, D, 0, 1) <= max(512 << 20, 512 * max(N, 64)) + copy + sums, (N, V, D)
