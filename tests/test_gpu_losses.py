@@ -745,3 +745,34 @@ def test_compiled_with_any_number_of_positions(lh, cuda):
             loss = call(*ls, *args)
             res.append([x.detach() for x in loss] + list(torch.autograd.grad(loss[0] + loss[1], ls)))
         assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+# N x V x D in several pieces of the vocabulary, positions packed: 5000 x 120001 in three of 40192 columns, the last
+# one shorter; 40000 x 7001 in two of 3584, more row blocks than the table of parts has
+PIECES = [(5000, 120001, 64, 40192), (40000, 7001, 96, 3584)]
+
+
+@pytest.mark.parametrize("N,V,D,C", PIECES)
+@pytest.mark.parametrize("ignore", [0.4, 0.97])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_several_pieces_with_packed_positions(lh, cuda, N, V, D, C, ignore, reduction):
+    _run_xent(lh, cuda, N, V, D, reduction, seed=82, ignore=ignore)
+
+
+@pytest.mark.parametrize("N,V,D,C", PIECES)
+@pytest.mark.parametrize("empty", [0.0, 0.3, 0.97])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_distillation_over_several_pieces(lh, cuda, N, V, D, C, empty, reduction):
+    """Teacher entries on both sides of every border of the pieces, beside others."""
+    border = [i for b in range(C, V, C) for i in (b - 2, b - 1, b, b + 1)]
+
+    def edit(tv, ti):
+        some = ti[:, 0] >= 0
+        for k, i in enumerate(border):
+            rows = some.clone()
+            rows[k % 3::3] = False                       # not all of them in every row
+            taken = (ti == i).any(1)
+            ti[rows & ~taken, k] = i
+        ti[::5, 9] = torch.where(some[::5], ti[::5, 1], -1)      # the same entry twice
+
+    _run_distill(lh, cuda, N, V, D, 13, 2.0, reduction, seed=83, empty=empty, edit=edit)
