@@ -14,7 +14,8 @@
 // epilogue writing G (N, C) in bf16; then dH += G W_piece and dW_piece = G^T H.
 // G is rounded to bf16 once, as an operand of bf16 MMAs has to be; its relative
 // error of up to 2^-8 is that of the bf16 gradients it ends in (up to 32 rows: two
-// terms, 2^-16).  All sums are fp32.
+// terms, 2^-16; see kTwo).  Two terms everywhere would double the products of dH and
+// dW, half of a training call.  All sums are fp32.
 // Where the loss is reduced, c is the same for all rows: G / c is what is rounded, and
 // dH and dW are multiplied by c in fp32.  The targets' entries, the largest ones, are
 // then near -1, which bf16 holds, where G's would all be off by c's own rounding (434 x
@@ -74,11 +75,13 @@ enum Out { kOutBf16, kOutPlane, kOutPlaneAdd };
 // columns of dH) and its kFew columns are rows of hidden, so that the MMAs do an eighth
 // of the work and the stages hold weights, which are what has to be read.
 constexpr int kFew = 64;
-// Up to kTwo rows, G is the sum of two bf16 terms, the second one's rows kTwo behind: a gradient
-// that comes from a handful of entries would be off as a whole by the rounding of one (a row's
-// dH and dW by up to 2^-8), where over many rows the roundings differ and cancel.  The columns
-// of the MMAs and the rows of a K step are there anyway (16 x 32000 x 4096, forward and backward:
-// 243 us, 234 with one term; 32 x 128000 x 2048: 426, 421).
+// Up to kTwo rows, G is the sum of two bf16 terms, the second one's rows kTwo behind, off by 2^-16: the columns of
+// the MMAs and the rows of a K step are there anyway (16 x 32000 x 4096, forward and backward: 243 us, 234 with one
+// term; 32 x 128000 x 2048: 426, 421), and a gradient of so few positions is a handful of entries, whose roundings
+// do not cancel over it.  Beyond, one term: the whole of dH and dW is off by 0.0019 to 0.0024 of itself (0.0017 is
+// the rounding of the results), and a single row of dH, or one of dW that comes from one position, by up to 2^-8
+// from its largest entry of G besides its own rounding.  The rule looks at the rows that are there, not at those
+// that count, as the launches cannot know them.
 constexpr int kTwo = kFew / 2;
 // A stage holds two steps of 64: its eight MMAs are issued without a stop, as each wait for a
 // stage and each commit of one leaves the tensor pipe empty for about 100 cycles, whatever waits

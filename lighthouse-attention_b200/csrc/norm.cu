@@ -218,7 +218,7 @@ __device__ __forceinline__ void open8(const Raw8<float>& r, float (&f)[8]) {
 struct BwdArgs {
   const void *dy, *dh, *h, *w;
   const float* rstd;
-  void *dx, *dr;                 // dr NULL: no residual, or the same tensor as dx
+  void *dx, *dr;                 // dr NULL: no residual
   float* dw_part;                // (gridDim.x, D)
   long long N;
   int D;
