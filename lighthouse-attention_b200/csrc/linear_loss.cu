@@ -46,6 +46,7 @@
 #include <cudaTypedefs.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "lh_common.cuh"
 #include "sm100.cuh"
@@ -55,6 +56,7 @@ namespace lh {
 using namespace sm100;
 
 __device__ int g_loss_status;    // set to 1 when a bounded wait gave up
+// One thread of a block asks: 16000 warps that read one address take 3 us.
 __device__ __forceinline__ bool gave_up() { return *reinterpret_cast<volatile int*>(&g_loss_status) != 0; }
 
 namespace ll {
@@ -94,9 +96,9 @@ constexpr int kSubs = 2;
 // about 1e-9 D of itself, by twice that where its large products come first, by nothing where they come
 // last or the sum is exact: no factor takes that out.  So the forward sums a logit in parts of kPart steps,
 // which the epilogue adds in registers, rounding to nearest; what is lost no longer grows with D.  (65536 x
-// 256 x 1024, the mean's error and the forward: 2.7e-6 and 50 us in one part, 1.3e-6 and 50 in parts of 8
-// steps, 0.9e-6 and 51 of 6, 0.6e-6 and 54 of 4, whose accumulators the epilogue does not keep up with:
-// 1999 x 50261 x 768 takes 100, 100, 100, 113 us.)  The backward's logits are one sum: their exponentials
+// 256 x 1024, the mean's error, the forward alone and with the backward: 2.7e-6, 50 and 150 us in one part,
+// 1.3e-6, 50 and 152 in parts of 8 steps, 0.9e-6, 50 and 154 of 6, 0.6e-6, 54 and 162 of 4, whose accumulators
+// the epilogue does not keep up with: the forward of 1999 x 50261 x 768 takes 100, 98, 98 and 113 us.)  The backward's logits are one sum: their exponentials
 // are rounded to 2^-9.
 constexpr int kPart = 6;
 __host__ __device__ constexpr int stages(bool few) { return few ? 5 : 3; }
@@ -150,7 +152,7 @@ struct Args {
   const float *gout, *row_scale, *inv_count;       // gout NULL: c is row_scale (kGrad), or 1 (kDH, kDW)
   float cscale;
   int two;                        // few rows: G has two terms
-  void* result;                   // few rows: G (bf16, few_pitch), or the planes (fp32) of kDH; kOutBf16: dH, dW
+  void* result;                   // kDH, kDW: what the tiles go to (bf16, or fp32 planes); few rows, kGrad: G (few_pitch)
   long long few_pitch;
 };
 
@@ -308,10 +310,10 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     k1 = k0 + q + (split < rem ? 1 : 0);
   };
 
-  // A thread of the epilogue holds its half row of logits: registers of warps 0-3 go there (128 x 56 +
-  // 256 x 224 are the launch's 384 x 168).
+  // A thread of the epilogue holds its half row of logits: registers of warps 0-3 go there (128 x 40 +
+  // 256 x 232 are the launch's 384 x 168).
   if (warp < 4) {
-    if constexpr (kParts && !FEW) regs_shrink<56>();
+    if constexpr (kParts && !FEW) regs_shrink<40>();
     if (warp == 0 && *abort == 0) {
       // ---------------------------------------------------------- TMA producer
       // (The whole warp runs this role and the next one, one lane of it issues: with a single lane in a
@@ -419,7 +421,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       }
     }
   } else {
-    if constexpr (kParts && !FEW) regs_grow<224>();
+    if constexpr (kParts && !FEW) regs_grow<232>();
     if (*abort != 0) {
       // nothing to do
     } else if constexpr (FEW) {
@@ -579,24 +581,26 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int g0 = MODE == kGrad ? a.b_off + n0 : n0;
         const size_t kept0 = (size_t)orow * a.K;         // the row's place among the targets' values
         Window<int4, int> win;
-        Window<float4, float> val;                       // kGrad, kWhole: the targets' gval, prob
-        auto advance = [&]() {
+        Window<float4, float> val;                       // kGrad, kWhole (for G): the targets' gval, prob
+        using yes = std::true_type;
+        using no = std::false_type;
+        auto advance = [&](auto values) {
           ++cur;
           win.step(a.K, cur, kNone);
-          if (MODE == kGrad || MODE == kWhole) val.step(a.K, cur, 0.f);
+          if constexpr (decltype(values)::value) val.step(a.K, cur, 0.f);
           next = win.now.x == kNone ? kNone : win.now.x - g0;
         };
         float c = 0.f, lse2 = 0.f;
-        auto first = [&]() {                             // of the targets in this half
+        auto first = [&](auto values) {                  // of the targets in this half
           cur = lower_bound(a.idx + kept0, a.K, g0);
           win.open(a.idx + kept0, a.K, cur, kNone);
-          if (MODE == kGrad || MODE == kWhole) val.open((MODE == kGrad ? a.gval : a.prob) + kept0, a.K, cur, 0.f);
+          if constexpr (decltype(values)::value) val.open((MODE == kGrad ? a.gval : a.prob) + kept0, a.K, cur, 0.f);
           next = win.now.x == kNone ? kNone : win.now.x - g0;
         };
         auto targets = [&]() {
           if (live && cols > 0) {
             if constexpr (SPARSE) {
-              first();
+              first(std::integral_constant<bool, MODE == kGrad>());
               if (MODE == kWhole) c = a.row_scale[orow];
             } else {
               const long long tv = a.target[orow] - g0;
@@ -633,12 +637,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             for (int ch = 0; ch < 8; ++ch) put(stage, ch, 0, 0, 0, 0);
             return;
           }
+          auto two = [&](int e) { const float2 v = g(e); return pack_bf16(v.x, v.y); };
 #pragma unroll
-          for (int ch = 0; ch < 8; ++ch) {
-            const int e = 8 * ch;
-            put(stage, ch, pack_bf16(g(e), g(e + 1)), pack_bf16(g(e + 2), g(e + 3)), pack_bf16(g(e + 4), g(e + 5)),
-                pack_bf16(g(e + 6), g(e + 7)));
-          }
+          for (int ch = 0; ch < 8; ++ch) put(stage, ch, two(8 * ch), two(8 * ch + 2), two(8 * ch + 4), two(8 * ch + 6));
         };
         auto put_at = [&](int at, float v) {             // one of the 64 columns again
           *reinterpret_cast<__nv_bfloat16*>(stage + lane * 128 + (((at >> 3) ^ (lane & 7)) << 4) + (at & 7) * 2) =
@@ -655,10 +656,18 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         };
         if constexpr (kParts) {
           float s[kHalf];                                // logits of this row
+          bool ok = filled();
+          if (ok) {
+            uint32_t x[kHalf / 32][32];
 #pragma unroll
-          for (int e = 0; e < kHalf; ++e) s[e] = 0.f;
-          bool ok = true;
-          for (int k = 0; k < sched.kb; k += kPart) {
+            for (int c = 0; c < kHalf / 32; ++c) tmem_ld32(lane_base + (li & 1) * kTN + c * 32, x[c]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < kHalf; ++e) s[e] = __uint_as_float(x[e / 32][e % 32]);
+            release();
+            targets();                                   // their loads meet the wait for the next part
+          }
+          for (int k = kPart; ok && k < sched.kb; k += kPart) {
             if (!(ok = filled())) break;
 #pragma unroll
             for (int c0 = 0; c0 < kHalf; c0 += 32) {
@@ -666,10 +675,14 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               tmem_ld32(lane_base + (li & 1) * kTN + c0, x);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) s[c0 + e] += __uint_as_float(x[e]);
+              for (int e = 0; e < 32; e += 2) {
+                const float2 t = fadd2(make_float2(s[c0 + e], s[c0 + e + 1]),
+                                       make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+                s[c0 + e] = t.x;
+                s[c0 + e + 1] = t.y;
+              }
             }
             release();
-            if (k == 0) targets();                       // their loads meet the wait for the next part
           }
           if (MODE == kWhole) ok = pair_all(1 + quad, ok);      // the two warps of a row go on together or not at all
           if (!ok) break;
@@ -691,7 +704,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                 const int at = next - c0;
                 st = *reinterpret_cast<const float*>(stage + lane * 128 + (((at >> 2) ^ (lane & 7)) << 4) + (at & 3) * 4);
                 a.slog[kept0 + cur] = st;
-                if constexpr (SPARSE) advance();
+                if constexpr (SPARSE) advance(no());
                 else next = kNone;
               }
             }
@@ -733,7 +746,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             // c / sum of the exponentials; a half of -infinities only has none (NaN where the whole row has none)
             const float f = c * (mx == -INFINITY ? 0.f * lse2 : ex2(mb - lse2));
             if constexpr (SPARSE) {
-              if (live && cols > 0) first();
+              if (live && cols > 0) first(yes());
             } else if (live && cols > 0) {
               const long long tv = a.target[orow] - g0;
               next = tv >= 0 && tv < kHalf ? (int)tv : kNone;
@@ -743,14 +756,14 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               if (c0 >= cols || row0 >= min(a.n_rows, (M + 63) / 64 * 64)) continue;
               if (lane == 0) bulk_wait_read_all();
               __syncwarp();
-              g_rows(c != 0.f, [&](int e) { return f * s[c0 + e]; });
+              g_rows(c != 0.f, [&](int e) { return fmul2(make_float2(s[c0 + e], s[c0 + e + 1]), make_float2(f, f)); });
               while (c != 0.f && next < c0 + 64) {
                 const int at = next;
                 float p = 1.f;
                 if constexpr (SPARSE) {
                   st = a.slog[kept0 + cur];              // this thread's own
                   p = 0.f;
-                  do { p += val.now.x; advance(); } while (next == at);    // the same index adds up
+                  do { p += val.now.x; advance(yes()); } while (next == at);    // the same index adds up
                 } else {
                   next = kNone;
                 }
@@ -789,10 +802,15 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             if (lane == 0) bulk_wait_read_all();
             __syncwarp();
             if constexpr (MODE == kGrad) {
-              g_rows(c != 0.f, [&](int e) { return c * ex2(fmaf(__uint_as_float(e < 32 ? x[e] : y[e - 32]), a.a2, -lse2)); });
+              g_rows(c != 0.f, [&](int e) {
+                const uint32_t* u = e < 32 ? x + e : y + e - 32;
+                const float2 arg = ffma2(make_float2(__uint_as_float(u[0]), __uint_as_float(u[1])), make_float2(a.a2, a.a2),
+                                         make_float2(-lse2, -lse2));
+                return fmul2(make_float2(ex2(arg.x), ex2(arg.y)), make_float2(c, c));
+              });
               while (c != 0.f && next < c0 + 64) {       // the row's targets among these columns (the same one twice: twice alike)
                 put_at(next - c0, c * val.now.x);
-                if constexpr (SPARSE) advance();
+                if constexpr (SPARSE) advance(yes());
                 else next = kNone;
               }
             } else if (a.out == kOutBf16) {
@@ -823,15 +841,18 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   }
   if (threadIdx.x == 0 && sm->abort) atomicExch(&g_loss_status, 1);
   if constexpr (MODE == kDH || MODE == kDW) {
-    // this CTA's rows of its tiles (planes: planes_kernel's rows)
-    if (sm->abort && a.out == kOutBf16) {
-      __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.result);
+    // NaN in this CTA's rows of its tiles
+    if (sm->abort) {
+      const float nan = __int_as_float(0x7fc00000);
       for (int t = pair; t < total; t += n_pairs) {
         int m, n, k0, k1, split;
         decode(t, m, n, k0, k1, split);
         for (int i = threadIdx.x; i < 128 * kCols; i += kThreads) {
           const int r = m * kTM + rank * 128 + i / kCols, v = n * kCols + i % kCols;
-          if (r < M && v < a.N) out[FEW ? (size_t)v * a.M + r : (size_t)r * a.N + v] = __float2bfloat16_rn(__int_as_float(0x7fc00000));
+          if (r >= M || v >= a.N) continue;
+          const size_t at = FEW ? (size_t)v * a.M + r : (size_t)r * a.N + v;
+          if (a.out == kOutBf16) reinterpret_cast<__nv_bfloat16*>(a.result)[at] = __float2bfloat16_rn(nan);
+          else reinterpret_cast<float*>(a.result)[(size_t)split * (MODE == kDW ? a.M : a.n_rows) * (FEW ? a.M : a.N) + at] = nan;
         }
       }
     }
@@ -1035,8 +1056,7 @@ finish_kernel(const FinishArgs a) {
   after_previous();
   __shared__ float2 sh[1024];
   __shared__ double2 tot[32];
-  __shared__ bool last;
-  const bool lost = gave_up();                     // the statistics are not there: NaN
+  __shared__ bool last, lost;                      // lost: the statistics are not there, NaN
   const int tid = threadIdx.x, r = tid % RB, slot = tid / RB, N = a.N, K = a.K;
   const int j = blockIdx.x * RB + r;
   const bool live = j < (a.rows ? a.rows[0] : N);
@@ -1052,6 +1072,7 @@ finish_kernel(const FinishArgs a) {
     for (int t = slot; t < a.parts; t += a.slots) st = join(st, a.stats[(size_t)t * N + j]);
   }
   sh[tid] = st;
+  if (tid == 0) lost = gave_up();
   __syncthreads();
   for (int o = a.slots >> 1; o; o >>= 1) {
     if (slot < o) sh[tid] = join(sh[tid], sh[tid + o * RB]);
@@ -1174,7 +1195,6 @@ struct PlanesArgs {
 __global__ void __launch_bounds__(256)
 planes_kernel(const __grid_constant__ PlanesArgs a) {
   after_previous();
-  const bool lost = gave_up();
   const size_t plane = (size_t)a.n_rows * a.cols;
   const int chunks = a.cols / 8;
   int n = a.n;
@@ -1201,10 +1221,6 @@ planes_kernel(const __grid_constant__ PlanesArgs a) {
         plain16(p + k * plane + 4, u + 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += u[e];
-      }
-      if (lost) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __int_as_float(0x7fc00000);
       }
     }
     store16(a.out + i * 8, v);
@@ -1622,7 +1638,7 @@ static int backward(const Problem& q, int reduction, const Kept& kp, const float
     y.dirty = rows ? nullptr : kp.dirty;
     y.out = p.dw_splits > 1 ? kOutPlane : kOutBf16;
     char* dw_out = (char*)dweight + (size_t)v0 * D * 2;
-    y.result = dw_out;
+    y.result = p.dw_splits > 1 ? (void*)dw : dw_out;
     if ((rc = p.dw_splits > 1 ? map_store(&mdw, dw, true, p.dw_splits, cols, D, D)
                               : map_store(&mdw, dw_out, false, 1, cols, D, D)))
       return rc;
