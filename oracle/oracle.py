@@ -18,6 +18,7 @@ Reference citations (paths inside the reference project):
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import math
 import pathlib
 import unittest
@@ -33,16 +34,20 @@ _ref_cpu = {}
 _ref_gpu = {}
 
 
+def _build():
+    """oracle/build.py as a module."""
+    spec = importlib.util.spec_from_file_location("_lh_oracle_build", HERE / "build.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
 def _oracle_lib():
     global _lib
     if _lib is None:
         so = _REF / "liblh_oracle.so"
         if not so.exists():
-            import importlib.util
-            spec = importlib.util.spec_from_file_location("_lh_oracle_build", HERE / "build.py")
-            mod = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(mod)
-            mod.build_oracle()
+            _build().build_oracle()
         _lib = ctypes.CDLL(str(so))
         _lib.lho_select.restype = ctypes.c_int
         _lib.lho_sel_len.restype = ctypes.c_int
@@ -154,7 +159,10 @@ def ref_gpu_lib(p: int):
     if p not in _ref_gpu:
         so = _REF / f"libref_gpu_p{p}.so"
         if not so.exists():
-            # as for the kernel on host threads: a test that needs it skips where the reference tree is not there
+            # a test that needs it skips where the reference tree is not there, as for the kernel on host threads;
+            # with the tree, or half of what it is built into, a missing library is a build that failed
+            if _build().REFERENCE_CU.exists() or any(_REF.glob("libref_*.so")):
+                raise FileNotFoundError(f"{so} is missing: oracle/build.py build_ref did not finish")
             raise unittest.SkipTest(f"{so} not built (oracle/build.py build_ref needs the reference tree)")
         lib = ctypes.CDLL(str(so))
         lib.ref_gpu_topk.restype = ctypes.c_int

@@ -141,3 +141,22 @@ def test_gla_recurrence_equals_closed_form(O):
     A = torch.einsum("bthd,bshd->btsh", q, k) * dec * mask
     ref = 0.3 * torch.einsum("btsh,bshd->bthd", A, v)
     assert torch.allclose(o, ref, rtol=1e-5, atol=1e-5)
+
+
+def test_a_missing_reference_kernel_is_a_skip_only_where_nothing_was_built(O, monkeypatch, tmp_path):
+    """Without the reference tree its GPU kernel's tests skip; a build that did not finish fails them."""
+    import unittest
+    monkeypatch.setattr(O, "_REF", tmp_path)
+    monkeypatch.setattr(O, "_ref_gpu", {})
+    monkeypatch.setenv("LH_REFERENCE_ROOT", str(tmp_path / "none"))
+    with pytest.raises(unittest.SkipTest):
+        O.ref_gpu_lib(2)
+    (tmp_path / "libref_cpu_p2.so").touch()
+    with pytest.raises(FileNotFoundError, match="did not finish"):
+        O.ref_gpu_lib(2)
+    (tmp_path / "libref_cpu_p2.so").unlink()
+    (tmp_path / "tree" / "src").mkdir(parents=True)
+    (tmp_path / "tree" / "src" / "lighthouse_selection_cuda.py").touch()
+    monkeypatch.setenv("LH_REFERENCE_ROOT", str(tmp_path / "tree"))
+    with pytest.raises(FileNotFoundError, match="did not finish"):
+        O.ref_gpu_lib(2)
