@@ -251,7 +251,8 @@ int lh_rms_norm_bwd(const void* dy, int dy_dtype, const void* dh, const void* h,
 
 /* Losses of an output projection without its logits.  hidden (N, D) bf16,
  * weight (V, D) bf16, s = hidden weight^T (fp32, never stored).
- * Limits: D % 8 == 0, D <= 65536, N and V <= 2^22, K <= 256; hidden, weight,
+ * Limits: D % 8 == 0, D <= 65536, N and V <= 2^22, K <= 256, the temperature from
+ * 1e-18 to 1e18 (its square and inverse are fp32 numbers); hidden, weight,
  * kept and the gradients 16-byte aligned, the workspace 256-byte.
  *
  * Bytes of workspace that the forward (backward = 0) or the backward (1) of the

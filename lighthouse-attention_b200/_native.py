@@ -555,8 +555,8 @@ def linear_distill_fwd(hidden, weight, teacher_logits, teacher_indices, temperat
         raise LighthouseShapeError(f"linear_distill: K must be in [1, 256], got {K}")
     if teacher_logits.dtype not in LH_DTYPE or teacher_indices.dtype != torch.int64:
         raise ValueError("linear_distill: teacher logits must be bf16 or fp32, indices int64")
-    if not 0 < temperature < 1e30:
-        raise ValueError(f"linear_distill: temperature must be positive and finite, got {temperature}")
+    if not 1e-18 <= temperature <= 1e18:         # its square and inverse are fp32 numbers
+        raise ValueError(f"linear_distill: temperature must be in [1e-18, 1e18], got {temperature}")
     dev = _on_one_device("linear_distill", hidden, weight, teacher_logits, teacher_indices)
     loss = _loss_out(N, reduction, dev)
     kept = torch.empty(kept_size(N, V, K, reduction), dtype=torch.uint8, device=dev)

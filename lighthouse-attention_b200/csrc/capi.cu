@@ -336,7 +336,7 @@ static int loss_check(const char* what, const void* hidden, const void* weight, 
              "%s: N and V must be in [1, 2^22]", what);
   LH_REQUIRE(D % 8 == 0 && D <= (1 << 16), LH_ERR_SHAPE, "%s: D must be a multiple of 8 and at most 65536, got %d", what, D);
   LH_REQUIRE(K >= 0 && K <= 256, LH_ERR_SHAPE, "%s: K must be in [1, 256], got %d", what, K);
-  LH_REQUIRE(T > 0.f && T < 1e30f, LH_ERR_ARG, "%s: temperature must be positive and finite", what);
+  LH_REQUIRE(T >= 0.99e-18f && T <= 1.01e18f, LH_ERR_ARG, "%s: temperature must be in [1e-18, 1e18]", what);
   LH_REQUIRE(reduction >= LH_REDUCE_NONE && reduction <= LH_REDUCE_SUM, LH_ERR_ARG, "%s: bad reduction", what);
   LH_REQUIRE(!(((uintptr_t)hidden | (uintptr_t)weight | (uintptr_t)kept) & 15) && !((uintptr_t)ws & 255), LH_ERR_ARG,
              "%s: hidden, weight and kept must be 16-byte aligned, the workspace 256-byte", what);

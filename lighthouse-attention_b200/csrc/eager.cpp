@@ -287,7 +287,7 @@ py::object linear_distill(const Tensor& h, const Tensor& w, const Tensor& tl, co
                           int64_t reduction) {
   if (!loss_case(h, w, reduction) || !rows_case(tl, h, 2) || !rows_case(ti, h, 2) || ti.scalar_type() != at::kLong ||
       dtype_code(tl.scalar_type()) < 0 || tl.size(1) != ti.size(1) || tl.size(1) < 1 || tl.size(1) > 256 ||
-      !(temperature > 0 && temperature < 1e30))
+      !(temperature >= 1e-18 && temperature <= 1e18))
     return py::none();
   return py::cast(LossFn::apply(h, w, ti, std::optional<Tensor>(tl.detach()), temperature, 0, reduction, wants_grad(h, w)));
 }

@@ -103,8 +103,8 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logi
 
     teacher_logits (..., K) bf16 or fp32 and teacher_indices (..., K) int64 or
     int32, K at most 256, in any order; a negative index marks an absent entry.
-    With p = softmax(teacher_logits / T) over a position's entries,
-    loss = T^2 sum_k p_k (log p_k - log student_k).  A position without entries
+    With p = softmax(teacher_logits / T) over a position's entries, T within
+    [1e-18, 1e18], loss = T^2 sum_k p_k (log p_k - log student_k).  A position without entries
     has loss 0, no gradient and does not count in the mean.  Entries with the
     same index add up; an index >= V, or a logit that is NaN or +infinity, makes
     the position's loss NaN.  The teacher gets no gradient.  Returns fp32."""

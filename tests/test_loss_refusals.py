@@ -181,3 +181,17 @@ def test_workspace_is_what_the_documentation_says(lh):
                 assert size(N, V, D, 256, 0) <= fwd, (N, V, D)
                 sums = 8 * N * D + 160e6
                 assert size(N, V, D, 0, 1) <= max(512 << 20, 512 * max(N, 64)) + copy + sums, (N, V, D)
+
+
+def test_temperatures_whose_square_or_inverse_is_no_fp32_number(lh):
+    tv, ti = _z(4, 3, dtype=torch.float32), _z(4, 3, dtype=torch.int64)
+    for T in (1e-40, 1e-30, 1e19, 1e29):
+        with pytest.raises(ValueError, match="temperature"):
+            lh._native.linear_distill_fwd(_z(4, 64), _z(10, 64), tv, ti, T, "mean")
+        a = ctypes.c_void_p(4096)
+        lib = lh._native.load()
+        assert lib.lh_linear_distill_fwd(a, a, a, 1, a, 4, 10, 64, 3, T, 1, a, a, 1 << 40, a, 1 << 40, None) == 2
+        assert lib.lh_linear_distill_bwd(a, a, 4, 10, 64, 3, T, 1, a, 1 << 40, a, a, a, a, 1 << 40, None) == 2
+    for T in (1e-18, 1e18):                              # not refused for its temperature, only as a CPU tensor
+        with pytest.raises(ValueError, match="CUDA"):
+            lh._native.linear_distill_fwd(_z(4, 64), _z(10, 64), tv, ti, T, "mean")
