@@ -98,9 +98,12 @@ constexpr int kSubs = 2;
 // which the epilogue adds in registers, rounding to nearest; what is lost no longer grows with D.  (65536 x
 // 256 x 1024, the mean's error, the forward alone and with the backward: 2.7e-6, 50 and 150 us in one part,
 // 1.3e-6, 50 and 152 in parts of 8 steps, 0.9e-6, 50 and 154 of 6, 0.6e-6, 54 and 162 of 4, whose accumulators
-// the epilogue does not keep up with: the forward of 1999 x 50261 x 768 takes 100, 98, 98 and 113 us.)  The backward's logits are one sum: their exponentials
-// are rounded to 2^-9.
+// the epilogue does not keep up with: the forward of 1999 x 50261 x 768 takes 100, 98, 98 and 113 us.)  The
+// backward's logits are one sum: their exponentials are rounded to 2^-9.
 constexpr int kPart = 6;
+// Registers per thread of warps 0-3 and of the epilogue's in that forward; together the launch's 384 x 168 (a launch
+// with less would wait for ever: launch() asks how many the kernel was compiled to).
+constexpr int kRegsRoles = 40, kRegsEpilogue = 232;
 __host__ __device__ constexpr int stages(bool few) { return few ? 5 : 3; }
 __host__ __device__ constexpr int b_bytes(bool few) { return few ? kFew / 2 * 128 : kOpBytes; }
 constexpr int smem_bytes(bool few) {
@@ -310,10 +313,9 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     k1 = k0 + q + (split < rem ? 1 : 0);
   };
 
-  // A thread of the epilogue holds its half row of logits: registers of warps 0-3 go there (128 x 40 +
-  // 256 x 232 are the launch's 384 x 168).
+  // A thread of the epilogue holds its half row of logits: registers of warps 0-3 go there.
   if (warp < 4) {
-    if constexpr (kParts && !FEW) regs_shrink<40>();
+    if constexpr (kParts && !FEW) regs_shrink<kRegsRoles>();
     if (warp == 0 && *abort == 0) {
       // ---------------------------------------------------------- TMA producer
       // (The whole warp runs this role and the next one, one lane of it issues: with a single lane in a
@@ -421,7 +423,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       }
     }
   } else {
-    if constexpr (kParts && !FEW) regs_grow<232>();
+    if constexpr (kParts && !FEW) regs_grow<kRegsEpilogue>();
     if (*abort != 0) {
       // nothing to do
     } else if constexpr (FEW) {
@@ -1311,6 +1313,14 @@ static int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMa
   const uint64_t bit = 1ull << (dev & 63);
   if (e == cudaSuccess && (dev >= 64 || !(allowed.load() & bit))) {
     e = cudaFuncSetAttribute(loss_gemm_kernel<MODE, SPARSE, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(FEW));
+    if (e == cudaSuccess && (MODE == kStats || MODE == kWhole) && !FEW) {
+      cudaFuncAttributes fa;
+      e = cudaFuncGetAttributes(&fa, loss_gemm_kernel<MODE, SPARSE, FEW>);
+      if (e == cudaSuccess && fa.numRegs * kThreads < 128 * kRegsRoles + 256 * kRegsEpilogue) {
+        set_error("linear loss: the kernel was compiled to %d registers, too few to share out", fa.numRegs);
+        return LH_ERR_LAUNCH;
+      }
+    }
     if (e == cudaSuccess && dev < 64) allowed.fetch_or(bit);
   }
   if (e != cudaSuccess) { set_error("linear loss: %s", cudaGetErrorString(e)); return LH_ERR_LAUNCH; }
